@@ -101,6 +101,85 @@ void attn_flash_noalloc(const uint16_t *Q, const uint16_t *K, const uint16_t *V,
 int attn_flash_plan(int Hq, int Hkv, int Sq, int Sk, int D, int causal, int bk, int v_prepacked,
                     char *buf, size_t len);
 
+/* ---- The paged KV cache ------------------------------------------------------------------------
+ * No counterpart in the reference (one call there is one dense problem): a cache that grows token by
+ * token, shared by sequences of all lengths, and attention over it. Work is stream-ordered on the calling
+ * thread's stream like attn_flash's; nothing is allocated and no device memory is read on the host, so
+ * every call may be captured into a graph and replayed with other lengths, tables and rows.
+ *
+ * The cache holds `pages` pages of `page` tokens, K and V alike:
+ *   bits 16: bf16 [pages][Hkv][page][D], D % 16 == 0, 16 <= D <= 256
+ *   bits 4:  E2M1 codes [pages][Hkv][page][D/2] bytes, the even element in the low half, and one E8M0 scale
+ *            byte e per 32 elements, [pages][Hkv][page][D/32]: an element is its code's value (0, 0.5, 1,
+ *            1.5, 2, 3, 4, 6, the high bit negates) times 2^(e-127). D is 64, 128 or 256.
+ * Sequence b holds kv_len[b] tokens, token p in page table[b * table_cols + p / page]. The tokens of a call
+ * are rows of token tensors: sequence b's n_b = q_start[b+1] - q_start[b] of them are rows q_start[b] on,
+ * and the last n_b of its kv_len[b] tokens (row i is position kv_len[b] - n_b + i). Rows of no sequence are
+ * left as they are; kv_len counts a call's own tokens.
+ *
+ * table, kv_len and q_start lie in device memory and may hold anything: an entry of the table outside
+ * [0, pages) names no page (its keys are hidden from attention, its tokens are not appended, read back as
+ * zeros); a length is cut to what a row of the table holds, a start to [0, T] (starts fall nowhere).
+ * Pages may be shared between sequences that read them; a page that a call appends to belongs to one
+ * sequence, and no call of another stream reads it meanwhile.
+ *
+ * max_q and max_kv are the caller's bounds of n_b and kv_len[b]. They choose kernels and cut the work; a
+ * sequence that passes them is served all the same, only slower. */
+#define ATTN_KV_BF16 16
+#define ATTN_KV_FP4 4
+#define ATTN_KV_PAGE_MIN 16 /* a page is a power of two of tokens */
+#define ATTN_KV_PAGE_MAX 256
+
+struct attn_kv_cache {
+    void *k, *v;              /* device, 16-byte aligned */
+    void *k_scale, *v_scale;  /* bits 4: device, 16-byte aligned */
+    const int32_t *table;     /* device, [B][table_cols] */
+    const int32_t *kv_len;    /* device, [B] */
+    const int32_t *q_start;   /* device, [B + 1] */
+    int32_t B, table_cols;    /* table_cols * page <= 2^30 */
+    int32_t pages, page, Hkv, D, bits;
+};
+
+/* A token tensor [T][heads][D], bf16: 16-byte aligned, strides in elements, multiples of 8. */
+struct attn_rows {
+    void *data;
+    int64_t token, head;
+};
+
+/* What attn_paged does to scores: scale * q.k (scale 0: 1/sqrt(D)); then, with softcap > 0,
+ * softcap * tanh(score / softcap); then, with slopes (device, [Hq]), minus slopes[h] * |position - key|. */
+struct attn_scores {
+    float scale, softcap;
+    const float *slopes;
+};
+
+/* Writes a call's K and V rows into the cache, K with its position's rotation, and the rotated Q to q_out
+ * (q_out may be q; q and q_out may both be NULL). The first `rot` elements of a head turn (0: none), in
+ * pairs (i, i + rot/2), or with `pairs` (2i, 2i + 1): (x1, x2) -> (x1 c - x2 s, x2 c + x1 s) in fp32,
+ * rounded once to bf16, with c and s from row p of rope [rope_rows][rot], cosines in its first half, for
+ * position p. In 4 bits the rounded rows are quantised: a group's scale is the smallest power of two
+ * in [2^-126, 2^125] under which its largest element is at most 7, elements round to nearest, ties to even; a group with a
+ * NaN or an infinity reads as NaN. Tokens whose position is below 0 or has no row in rope are skipped. */
+void attn_kv_append(const struct attn_kv_cache *c, const struct attn_rows *q, const struct attn_rows *q_out,
+                    const struct attn_rows *k, const struct attn_rows *v, int T, int Hq, const float *rope,
+                    int rope_rows, int rot, int pairs, int max_q);
+
+/* The inverse: a call's rows of the cache to k and v, bf16 (with token = D and head = n D the dense layout
+ * that attn_flash takes). Reads every token of a sequence where n_b = kv_len[b]. */
+void attn_kv_read(const struct attn_kv_cache *c, const struct attn_rows *k, const struct attn_rows *v, int T,
+                  int max_q);
+
+/* Attention of a call's rows over their sequences' caches, o in bf16: row i of sequence b sees keys
+ * j < kv_len[b], and with causal j <= its position; kv = h / (Hq/Hkv). A row that sees none is written as
+ * zeros. P is rounded to bf16 before P.V, as in attn_flash. scores may be NULL (1/sqrt(D)). scratch is an
+ * attn_flash scratch of this D (attn_flash_scratch_bytes); calls that may overlap need one each. */
+void attn_paged(const struct attn_kv_cache *c, const struct attn_rows *q, const struct attn_rows *o, int T,
+                int Hq, int causal, const struct attn_scores *scores, int max_q, int max_kv, void *scratch);
+
+/* The kernels that call would launch, as attn_flash_plan gives them; nothing is launched or read. */
+int attn_paged_plan(const struct attn_kv_cache *c, int T, int Hq, int causal,
+                    const struct attn_scores *scores, int max_q, int max_kv, char *buf, size_t len);
+
 /* Stream selection for the calling thread (no counterpart in the reference, which has
  * no device). `stream` is a hipStream_t; NULL selects the null stream. */
 void attn_flash_set_stream(void *stream);

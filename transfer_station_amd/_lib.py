@@ -20,6 +20,12 @@ _SIGNATURES = {
     "attn_flash_noalloc": (None, [_c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_void_p] +
                            [_c.c_int] * 8),
     "attn_flash_plan": (_c.c_int, [_c.c_int] * 8 + [_c.c_char_p, _c.c_size_t]),
+    "attn_kv_append": (None, [_c.c_void_p] * 5 + [_c.c_int] * 2 + [_c.c_void_p] + [_c.c_int] * 4),
+    "attn_kv_read": (None, [_c.c_void_p] * 3 + [_c.c_int] * 2),
+    "attn_paged": (None, [_c.c_void_p] * 3 + [_c.c_int] * 3 + [_c.c_void_p] + [_c.c_int] * 2 +
+                   [_c.c_void_p]),
+    "attn_paged_plan": (_c.c_int, [_c.c_void_p] + [_c.c_int] * 3 + [_c.c_void_p] + [_c.c_int] * 2 +
+                        [_c.c_char_p, _c.c_size_t]),
     "attn_flash_set_stream": (None, [_c.c_void_p]),
     "attn_flash_get_stream": (_c.c_void_p, []),
     # include/attn_devutil.h

@@ -27,7 +27,7 @@ ROCM = os.environ.get("ROCM_PATH", "/opt/rocm")
 HIP_SOURCES = ["attn_kernels.hip"]
 # Standalone roofline microbenchmark (MFMA peak, HBM copy/read), built next to the library.
 TOOL_SOURCES = {"roofline_bench": "roofline_bench.hip"}
-C_SOURCES = ["attn_flash.c", "attn_devutil.c", "attn_synth.c"]
+C_SOURCES = ["attn_flash.c", "attn_paged.c", "attn_devutil.c", "attn_synth.c"]
 
 # Packed fp32 VALU forms are disabled for all device code on this platform.
 # IEEE mode off (with NaNs not honoured): fmaxf lowers to a bare v_max/v_max3 instead of

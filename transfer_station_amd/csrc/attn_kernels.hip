@@ -3752,3 +3752,6 @@ extern "C" int attn_hip_static_scratch(void **ptr, size_t *bytes) {
     *bytes = sizeof(scratch);
     return (int)hipSuccess;
 }
+
+// ---- the paged KV cache's kernels -------------------------------------------------------------
+#include "attn_paged_kernels.h"

@@ -1,0 +1,1091 @@
+// attn_paged_kernels.h -- gfx950 kernels of the paged KV cache: attention over it (attn_paged), appending
+// to it (attn_kv_append) and reading it back (attn_kv_read). Part of attn_kernels.hip.
+//
+// The cache: pages of 16 .. 256 tokens, K and V [pages][Hkv][page][D], in bf16, or in 4 bits as E2M1 codes
+// (two to a byte, the even element low) with one E8M0 scale byte per 32 elements of a row. A sequence's
+// pages are named by its row of the table. Every 16 keys that start at a multiple of 16 lie in one page,
+// back to back, so the kernels address the cache in such blocks: one page id, one buffer descriptor of at
+// most 16 rows whose range ends at the sequence's last key (keys past it arrive as zeros) and 32-bit
+// offsets inside it, however large the cache. A page id outside the cache gives an empty range, and its
+// keys are masked.
+//
+//   S = scale Q.K, optionally cap tanh(S / cap), minus slope |position - key|; softmax; O = P.V
+//
+// in fp32 but for the operands of the MFMAs: K, V, Q as they are (4-bit codes become bf16 exactly) and P
+// rounded to bf16, as in attn_flash; O is rounded once, to bf16.
+#ifndef ATTN_PAGED_KERNELS_H
+#define ATTN_PAGED_KERNELS_H
+
+#include "attn_device.h"
+#include "attn_launch.h"
+#include "attn_paged_cut.h"
+#include "attn_paged_rule.h"
+
+namespace {
+
+typedef __attribute__((ext_vector_type(2))) uint32_t u32x2;
+typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
+// Tables and lengths are read through the scalar cache: wave-uniform and not written by the kernel.
+typedef const __attribute__((address_space(4))) int32_t const_i32;
+__device__ __forceinline__ int scalar_i32(const int32_t *p, long i) {
+    return ((const_i32 *)(uintptr_t)p)[i];
+}
+
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
+// Eight 4-bit codes, times their scale, as eight bf16 values: exact, but for a scale so small or large
+// that bf16 has no such value.
+__device__ __forceinline__ u32x4 fp4_to_bf16(uint32_t w, float scale) {
+    const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 0);
+    const bf16x2 b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 1);
+    const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 2);
+    const bf16x2 d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 3);
+    return u32x4{__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b),
+                 __builtin_bit_cast(uint32_t, c), __builtin_bit_cast(uint32_t, d)};
+}
+__device__ __forceinline__ float e8m0(uint32_t e) { return __builtin_bit_cast(float, e << 23); }
+
+__device__ __forceinline__ uint32_t bf16_pair(float a, float b) {
+    const bf16x2 r = {(__bf16)a, (__bf16)b};
+    return __builtin_bit_cast(uint32_t, r);
+}
+
+// A score in units of log2, from the raw dot product: capped, then lowered by the distance.
+// cap tanh(x / cap) = cap (1 - 2 / (2^(2 log2(e) x / cap) + 1)) is off by a few 2^-24 of the cap,
+// which is below what P's rounding to bf16 does.
+__device__ __forceinline__ float score2(float s, float c, float cap_in, float cap_out, float slope,
+                                        int dist) {
+    float t = s * c;
+    if (cap_out != 0.f) {
+        const float y = fast_exp2(s * cap_in);
+        t = cap_out - 2.f * cap_out * __builtin_amdgcn_rcpf(y + 1.f);
+    }
+    return t - slope * (float)abs(dist);
+}
+
+// 16 keys of the cache from key kb (a multiple of 16): their rows' place, and how many of them there are
+// (0 where the page id is none, or past the sequence's end).
+struct kv_block {
+    int64_t row;
+    int n;
+};
+__device__ __forceinline__ kv_block block_at(const attn_paged_args &a, const int32_t *table, int u,
+                                             int kb, int kend) {
+    const int pg = scalar_i32(table, min(kb, kend - 1) >> a.lgp);
+    const bool ok = attn_page_ok(pg, a.pages);
+    return kv_block{attn_page_row(ok ? pg : 0, a.Hkv, u, kb, a.lgp), ok ? max(0, min(16, kend - kb)) : 0};
+}
+
+// b ? x : y of two values (of two array elements the operator itself would choose the address, and keep the
+// array in memory).
+__device__ __forceinline__ uint32_t pick(bool b, uint32_t x, uint32_t y) { return b ? x : y; }
+
+template <bool NT> __device__ __forceinline__ u32x4 buf16(__amdgpu_buffer_rsrc_t r, uint32_t off) {
+    return __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, NT ? kDmaNT : 0);
+}
+
+// ------------------------------------------------------------------------------------------
+// Few query rows per kv head. One workgroup per (sequence b, kv head u, part sp of its keys, tile of
+// 16 NRB rows); a sequence's rows are its tokens' heads of the group, token by token. The four waves take
+// interleaved tiles of 32 keys (two blocks of 16), each with a softmax of its own:
+//   S^T[key][row] = K . Q^T   (v_mfma_f32_16x16x32_bf16, K from memory straight into the operand)
+//   O^T[d][row]  += V^T . P^T (V through a wave-private LDS tile and the transposed read)
+// and merge in LDS at the end. Tiles past the grid's (a sequence with more rows than max_q says) follow
+// in the same workgroup, keys past the grid's in the last part.
+// ------------------------------------------------------------------------------------------
+template <int DP, bool F4, int NRB, bool MOD, bool NTL>
+__global__ __launch_bounds__(256, 2) void attn_paged_decode_kernel(const attn_paged_args a) {
+    constexpr int VSTR = DP + 16; // elements of a V row in LDS: the eight rows of a pass on other banks
+    constexpr int KN = DP / 32;   // MFMA steps along d
+    constexpr int NV = DP / 16;   // bf16: 16-byte pieces of a V tile per lane
+    // 4 bits: a lane's piece of a V row (PB bytes), lanes per row, rows per load, loads per tile
+    constexpr int PB = DP == 64 ? 8 : 16, LPR = DP / 2 / PB, RPL = 64 / LPR, NV4 = 32 / RPL;
+    constexpr int NSC = DP == 256 ? 2 : 1; // scales of a lane's share of a K row
+    constexpr int VTILE = 32 * VSTR;
+    __shared__ __attribute__((aligned(16))) uint16_t Vw[4 * VTILE];
+    __shared__ float red_m[NRB][4][16], red_l[NRB][4][16];
+    static_assert(4 * 16 * (DP + 4) * 4 <= 4 * VTILE * 2, "merge area must fit in the V tiles");
+
+    const int L = xcd_remap(wg_id_x(), a.B * a.Hkv * a.nsplit * a.tps);
+    const int t0 = L % a.tps, L1 = L / a.tps;
+    const int sp = L1 % a.nsplit, L2 = L1 / a.nsplit;
+    const int u = uniform(L2 % a.Hkv), b = uniform(L2 / a.Hkv);
+    const attn_seq sq = attn_seq_of(scalar_i32(a.q_start, b), scalar_i32(a.q_start, b + 1),
+                                    scalar_i32(a.kv_len, b), a.T, a.cols, a.lgp);
+    const int live = attn_live_parts(sq.kend, a.kps, a.nsplit);
+    if (sp >= live)
+        return;
+    const int k0 = attn_part_start(sq.kend, a.kps, sp), k1 = attn_part_end(sq.kend, a.kps, a.nsplit, sp);
+    const int32_t *table = a.table + (int64_t)b * a.cols;
+    const int tid = wi_id_x(), w = uniform(tid >> 6), lane = tid & 63;
+    const int r16 = lane & 15, grp = lane >> 4;
+    const int g = a.Hq / a.Hkv, R = sq.n * g, D = a.D;
+    const float c = MOD ? 1.f : a.c;
+    uint16_t *vt = &Vw[w * VTILE];
+
+    for (int tile = t0; (int64_t)tile * 16 * NRB < R; tile += a.tps) {
+        const int row0 = tile * 16 * NRB;
+        bf16x8 qb[NRB][KN];
+        int lim[NRB], pos[NRB];
+        float m_run[NRB], l_run[NRB], slope[NRB];
+        f32x4 o[NRB][DP / 16];
+#pragma unroll
+        for (int i = 0; i < NRB; ++i) {
+            const int row = row0 + 16 * i + r16;
+            const bool valid = row < R;
+            const int tok = valid ? row / g : 0, h = u * g + (valid ? row % g : 0);
+            const uint16_t *q = a.q + (sq.q0 + tok) * a.q_tok + h * a.q_head;
+#pragma unroll
+            for (int kk = 0; kk < KN; ++kk) {
+                const int col = F4 ? grp * (DP / 4) + kk * 8 : kk * 32 + grp * 8;
+                u32x4 x = zero4();
+                if (valid && col < D)
+                    x = *reinterpret_cast<const u32x4 *>(q + col);
+                qb[i][kk] = as_bf16x8(x);
+            }
+            pos[i] = sq.len - sq.n + tok;
+            lim[i] = a.causal ? min(pos[i], k1 - 1) : k1 - 1;
+            slope[i] = MOD && a.slopes ? a.slopes[h] * 1.44269504088896341f : 0.f;
+            m_run[i] = kNegInf;
+            l_run[i] = 0.f;
+#pragma unroll
+            for (int db = 0; db < DP / 16; ++db)
+                o[i][db] = f32x4{0.f, 0.f, 0.f, 0.f};
+        }
+        // Keys from the tile's last row's position on are hidden from it.
+        const int kstop = a.causal ? min(k1, sq.len - sq.n + (min(row0 + 16 * NRB, R) - 1) / g + 1) : k1;
+
+        struct frags {
+            u32x4 k[F4 ? 1 : 2 * KN], v[F4 ? 1 : NV];
+            uint32_t kw[F4 ? 2 * KN : 1], ksc[F4 ? 2 : 1];
+            uint32_t vw[F4 ? NV4 * PB / 4 : 1], vsc[F4 ? NV4 : 1];
+            int n0, n1;
+        };
+        // K and V of a tile, Q and O do not fit 256 registers at DP = 256 in bf16: V is loaded once the
+        // scores have freed K's.
+        constexpr bool kLate = DP == 256 && !F4;
+        auto load_v16 = [&](const kv_block &b0, const kv_block &b1, frags &f)
+            __attribute__((always_inline)) {
+            const uint32_t rb = (uint32_t)D * 2u;
+            const auto vr0 = make_rsrc(a.v + b0.row * rb, b0.n * rb);
+            const auto vr1 = make_rsrc(a.v + b1.row * rb, b1.n * rb);
+            const uint32_t v0 = (lane % (DP / 8)) * 8 < D
+                                    ? (lane / (DP / 8)) * rb + (lane % (DP / 8)) * 16
+                                    : 0x80000000u;
+#pragma unroll
+            for (int r = 0; r < NV; ++r)
+                f.v[r] = buf16<NTL>(r < NV / 2 ? vr0 : vr1, v0 + (r % (NV / 2)) * (512 / DP) * rb);
+        };
+        auto load = [&](int tb, frags &f) __attribute__((always_inline)) {
+            const kv_block b0 = block_at(a, table, u, tb, k1), b1 = block_at(a, table, u, tb + 16, k1);
+            f.n0 = b0.n;
+            f.n1 = b1.n;
+            if constexpr (!F4) {
+                const uint32_t rb = (uint32_t)D * 2u; // bytes of a row
+                const auto kr0 = make_rsrc(a.k + b0.row * rb, b0.n * rb);
+                const auto kr1 = make_rsrc(a.k + b1.row * rb, b1.n * rb);
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int kk = 0; kk < KN; ++kk) {
+                        const int col = kk * 32 + grp * 8;
+                        f.k[t * KN + kk] = buf16<NTL>(t ? kr1 : kr0,
+                                                     col < D ? r16 * rb + col * 2 : 0x80000000u);
+                    }
+                if (!kLate)
+                    load_v16(b0, b1, f);
+            } else {
+                constexpr int RB = DP / 2, SB = DP / 32; // bytes of a row's codes and scales
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    const kv_block &bl = t ? b1 : b0;
+                    const auto kr = make_rsrc(a.k + bl.row * RB, bl.n * RB);
+                    const auto sr = make_rsrc(a.ks + bl.row * SB, bl.n * SB);
+                    if constexpr (DP == 64) {
+                        const u32x2 x = __builtin_amdgcn_raw_buffer_load_b64(
+                            kr, r16 * RB + grp * (RB / 4), 0, NTL ? kDmaNT : 0);
+                        f.kw[t * KN] = x[0];
+                        f.kw[t * KN + 1] = x[1];
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < KN / 4; ++j) {
+                            const u32x4 x = buf16<NTL>(kr, r16 * RB + grp * (RB / 4) + 16 * j);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i)
+                                f.kw[t * KN + 4 * j + i] = x[i];
+                        }
+                    }
+                    if constexpr (NSC == 2)
+                        f.ksc[t] = __builtin_amdgcn_raw_buffer_load_b16(sr, r16 * SB + grp * 2, 0, 0);
+                    else
+                        f.ksc[t] = __builtin_amdgcn_raw_buffer_load_b8(sr, r16 * SB + grp * SB / 4, 0, 0);
+                }
+#pragma unroll
+                for (int r = 0; r < NV4; ++r) {
+                    const kv_block &bl = r < NV4 / 2 ? b0 : b1;
+                    const auto vr = make_rsrc(a.v + bl.row * RB, bl.n * RB);
+                    const auto sr = make_rsrc(a.vs + bl.row * SB, bl.n * SB);
+                    const int row = lane / LPR + r % (NV4 / 2) * RPL, piece = lane % LPR;
+                    if constexpr (DP == 64) {
+                        const u32x2 x = __builtin_amdgcn_raw_buffer_load_b64(
+                            vr, row * RB + piece * PB, 0, NTL ? kDmaNT : 0);
+                        f.vw[2 * r] = x[0];
+                        f.vw[2 * r + 1] = x[1];
+                    } else {
+                        const u32x4 x = buf16<NTL>(vr, row * RB + piece * PB);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            f.vw[4 * r + i] = x[i];
+                    }
+                    f.vsc[r] = __builtin_amdgcn_raw_buffer_load_b8(sr, row * SB + piece * SB / LPR, 0, 0);
+                }
+            }
+        };
+        auto put_v = [&](const frags &f) __attribute__((always_inline)) {
+            lds_wave_fence(); // the previous tile's transposed reads are complete
+            if constexpr (!F4) {
+#pragma unroll
+                for (int r = 0; r < NV; ++r) {
+                    const int at = lane + 64 * r;
+                    *reinterpret_cast<u32x4 *>(&vt[at / (DP / 8) * VSTR + at % (DP / 8) * 8]) = f.v[r];
+                }
+            } else {
+#pragma unroll
+                for (int r = 0; r < NV4; ++r) {
+                    const int row = lane / LPR + r * RPL, piece = lane % LPR;
+                    const float sc = e8m0(f.vsc[r]);
+#pragma unroll
+                    for (int j = 0; j < PB / 4; ++j)
+                        *reinterpret_cast<u32x4 *>(&vt[row * VSTR + piece * 2 * PB + 8 * j]) =
+                            fp4_to_bf16(f.vw[r * (PB / 4) + j], sc);
+                }
+            }
+        };
+        auto compute = [&](int tb, frags &f) __attribute__((always_inline)) {
+            bf16x8 kf[2][KN], pk[NRB];
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int kk = 0; kk < KN; ++kk) {
+                    if constexpr (F4)
+                        kf[t][kk] = as_bf16x8(fp4_to_bf16(
+                            f.kw[t * KN + kk],
+                            e8m0(NSC == 2 ? (f.ksc[t] >> (kk / 4 * 8)) & 0xff : f.ksc[t])));
+                    else
+                        kf[t][kk] = as_bf16x8(f.k[t * KN + kk]);
+                }
+#pragma unroll
+            for (int i = 0; i < NRB; ++i) {
+                f32x4 s[2];
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    s[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int kk = 0; kk < KN; ++kk)
+                        s[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[t][kk], qb[i][kk], s[t], 0, 0, 0);
+                }
+                if (kLate) { // NRB == 1
+                    __builtin_amdgcn_sched_barrier(0);
+                    load_v16(block_at(a, table, u, tb, k1), block_at(a, table, u, tb + 16, k1), f);
+                }
+                // Register (t, j) of this lane holds key tb + 16t + 4grp + j for row r16.
+                float mx = kNegInf;
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const int key = tb + 16 * t + 4 * grp + j;
+                        if (MOD)
+                            s[t][j] = score2(s[t][j], a.c, a.cap_in, a.cap_out, slope[i], pos[i] - key);
+                        if (key > lim[i] || (t ? f.n1 : f.n0) == 0)
+                            s[t][j] = kNegInf;
+                        mx = fmaxf(mx, s[t][j]);
+                    }
+                mx = max_xor32(max_xor16(mx));
+                const float mnew = fmaxf(m_run[i], mx);
+                const float muse = mnew == kNegInf ? 0.f : mnew;
+                const float alpha = fast_exp2((m_run[i] - muse) * c);
+                const float mc = muse * c;
+                float psum = 0.f;
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const float p = fast_exp2(fmaf(s[t][j], c, -mc));
+                        psum += p;
+                        pk[i][4 * t + j] = (__bf16)p;
+                    }
+                l_run[i] = alpha * l_run[i] + psum;
+                m_run[i] = mnew;
+#pragma unroll
+                for (int db = 0; db < DP / 16; ++db)
+                    o[i][db] *= alpha;
+            }
+            if (kLate)
+                put_v(f);
+            lds_wave_fence(); // this tile's V is in LDS before the transposed reads
+            const uint16_t *vb = &vt[(4 * grp + (r16 >> 2)) * VSTR + 4 * (r16 & 3)];
+#pragma unroll
+            for (int db = 0; db < DP / 16; ++db) {
+                const bf16x8 x = join_tr(lds_read_tr(vb + db * 16), lds_read_tr(vb + db * 16 + 16 * VSTR));
+#pragma unroll
+                for (int i = 0; i < NRB; ++i)
+                    o[i][db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, pk[i], o[i][db], 0, 0, 0);
+            }
+        };
+        for (int tb = k0 + 32 * w; tb < kstop; tb += 128) {
+            frags f;
+            load(tb, f);
+            if (!kLate)
+                put_v(f);
+            compute(tb, f);
+        }
+#pragma unroll
+        for (int i = 0; i < NRB; ++i)
+            l_run[i] = sum_xor32(sum_xor16(l_run[i]));
+
+        // Merge the waves: O^T register (db, j) of this lane holds d = 16db + 4grp + j of row r16.
+        float *om = reinterpret_cast<float *>(Vw); // [4][16][DP + 4]
+        if (grp == 0)
+#pragma unroll
+            for (int i = 0; i < NRB; ++i) {
+                red_m[i][w][r16] = m_run[i] * c; // in log2 units; -inf stays
+                red_l[i][w][r16] = l_run[i];
+            }
+#pragma unroll
+        for (int i = 0; i < NRB; ++i) {
+            __syncthreads();
+#pragma unroll
+            for (int db = 0; db < DP / 16; ++db)
+                *reinterpret_cast<f32x4 *>(&om[(w * 16 + r16) * (DP + 4) + db * 16 + 4 * grp]) = o[i][db];
+            __syncthreads();
+            const int rowb = row0 + 16 * i, nrow = min(16, R - rowb);
+            for (int idx = tid; idx < nrow * (DP / 4); idx += 256) {
+                const int r = idx / (DP / 4), d = 4 * (idx % (DP / 4));
+                if (d >= D)
+                    continue;
+                float mx = kNegInf;
+#pragma unroll
+                for (int ww = 0; ww < 4; ++ww)
+                    mx = fmaxf(mx, red_m[i][ww][r]);
+                const float muse = mx == kNegInf ? 0.f : mx;
+                f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+                float lsum = 0.f;
+#pragma unroll
+                for (int ww = 0; ww < 4; ++ww) {
+                    const float wgt = fast_exp2(red_m[i][ww][r] - muse);
+                    const f32x4 x = *reinterpret_cast<const f32x4 *>(&om[(ww * 16 + r) * (DP + 4) + d]);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        acc[j] += wgt * x[j];
+                    lsum += wgt * red_l[i][ww][r];
+                }
+                const int64_t tok = sq.q0 + (rowb + r) / g;
+                const int h = u * g + (rowb + r) % g;
+                if (live == 1) {
+                    const float inv = lsum > 0.f ? 1.0f / lsum : 0.f;
+                    *reinterpret_cast<u32x2 *>(a.o + tok * a.o_tok + h * a.o_head + d) =
+                        u32x2{bf16_pair(acc[0] * inv, acc[1] * inv), bf16_pair(acc[2] * inv, acc[3] * inv)};
+                } else {
+                    const int64_t slot = (tok * a.Hq + h) * a.nsplit + sp;
+                    if (d == 0) {
+                        a.pm[slot] = mx;
+                        a.pl[slot] = lsum;
+                    }
+                    *reinterpret_cast<f32x4 *>(a.pacc + slot * D + d) = acc;
+                }
+            }
+        }
+        __syncthreads(); // the merge area is V tiles again
+    }
+}
+
+// Joins the parts of each row: w_s = 2^(m_s - max m), O = sum w_s acc_s / sum w_s l_s. A workgroup takes
+// 256 / (LP SG) rows of one sequence at a time: LP lanes of four columns each, SG groups of parts. Rows
+// of sequences that one part covers were written by the attention kernel.
+constexpr int kPagedMaxSplit = ATTN_PAGED_MAX_PARTS;
+__global__ __launch_bounds__(256) void attn_paged_merge_kernel(const attn_paged_args a, int lglp,
+                                                               int lgsg, int tpm) {
+    __shared__ float wsh[kPagedMaxSplit]; // rows x parts: the launcher takes more than one row below 128
+    __shared__ __attribute__((aligned(16))) f32x4 red[256];
+    const int b = uniform(wg_id_x() / tpm), t0 = wg_id_x() % tpm;
+    const attn_seq sq = attn_seq_of(scalar_i32(a.q_start, b), scalar_i32(a.q_start, b + 1),
+                                    scalar_i32(a.kv_len, b), a.T, a.cols, a.lgp);
+    const int live = attn_live_parts(sq.kend, a.kps, a.nsplit);
+    if (live == 1)
+        return;
+    const int tid = wi_id_x(), lane = tid & 63, w = tid >> 6;
+    const int rpw = 256 >> (lglp + lgsg), R = sq.n * a.Hq;
+    const int rl = tid >> (lglp + lgsg), sg = (tid >> lglp) & ((1 << lgsg) - 1);
+    const int d = 4 * (tid & ((1 << lglp) - 1));
+    for (int r0 = t0 * rpw; r0 < R; r0 += tpm * rpw) {
+        for (int r = w; r < rpw; r += 4) {
+            const int64_t slot = ((int64_t)sq.q0 * a.Hq + min(r0 + r, R - 1)) * a.nsplit;
+            float m[kPagedMaxSplit / 64], l[kPagedMaxSplit / 64], mx = kNegInf;
+#pragma unroll
+            for (int i = 0; i < kPagedMaxSplit / 64; ++i) {
+                const int s = lane + 64 * i;
+                m[i] = s < live ? a.pm[slot + s] : kNegInf;
+                l[i] = s < live ? a.pl[slot + s] : 0.f;
+                mx = fmaxf(mx, m[i]);
+            }
+            mx = seg_all<true>(mx, true);
+            const float muse = mx == kNegInf ? 0.f : mx;
+            float sum = 0.f;
+#pragma unroll
+            for (int i = 0; i < kPagedMaxSplit / 64; ++i) {
+                m[i] = fast_exp2(m[i] - muse);
+                sum += m[i] * l[i];
+            }
+            sum = seg_all<false>(sum, true);
+            const float inv = sum > 0.f ? 1.0f / sum : 0.f;
+#pragma unroll
+            for (int i = 0; i < kPagedMaxSplit / 64; ++i)
+                if (lane + 64 * i < live)
+                    wsh[r * a.nsplit + lane + 64 * i] = m[i] * inv;
+        }
+        __syncthreads();
+        f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+        const int row = r0 + rl;
+        if (row < R && d < a.D) {
+            const float *p = a.pacc + ((int64_t)sq.q0 * a.Hq + row) * a.nsplit * a.D + d;
+#pragma unroll 8
+            for (int s = sg; s < live; s += 1 << lgsg) {
+                const f32x4 x = *reinterpret_cast<const f32x4 *>(p + (int64_t)s * a.D);
+                const float wgt = wsh[rl * a.nsplit + s];
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    acc[j] += wgt * x[j];
+            }
+        }
+        red[tid] = acc;
+        __syncthreads();
+        if (sg == 0 && row < R && d < a.D) {
+            for (int k = 1; k < 1 << lgsg; ++k) {
+                const f32x4 y = red[tid + (k << lglp)];
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    acc[j] += y[j];
+            }
+            const int64_t tok = sq.q0 + row / a.Hq;
+            *reinterpret_cast<u32x2 *>(a.o + tok * a.o_tok + row % a.Hq * a.o_head + d) =
+                u32x2{bf16_pair(acc[0], acc[1]), bf16_pair(acc[2], acc[3])};
+        }
+        __syncthreads();
+    }
+}
+
+// ------------------------------------------------------------------------------------------
+// Many query rows per kv head. One workgroup of four waves per (sequence, kv head, part, tile of 128
+// rows), 32 rows per wave; tiles of 64 keys, staged in LDS by the four waves (16 keys each) through
+// registers while the tile before is computed:
+//   S^T[key][row] = K . Q^T, O^T[d][row] += V^T . P^T   (v_mfma_f32_32x32x16_bf16)
+// with the LDS layouts of attn_prefill_fast_kernel. The running maximum is raised only where a tile's
+// is more than 2^8 above it, so that O is rarely rescaled: p stays below 2^8.
+// ------------------------------------------------------------------------------------------
+template <int DP, bool F4, bool MOD>
+__global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_paged_prefill_kernel(
+    const attn_paged_args a) {
+    constexpr int KT = 64, KN = DP / 16, PW = DP / 32; // PW: 16-byte pieces of a bf16 tile per lane
+    constexpr int KW = DP / 32, NSC = DP == 256 ? 2 : 1; // 4 bits: words and scales per lane
+    __shared__ __attribute__((aligned(1024))) uint16_t Ks[2][KT * DP];
+    __shared__ __attribute__((aligned(1024))) uint16_t Vs[2][KT * DP];
+
+    const int L = xcd_remap(wg_id_x(), a.B * a.Hkv * a.nsplit * a.tps);
+    const int L1 = L / a.tps, t0 = a.tps - 1 - L % a.tps; // heaviest first
+    const int sp = L1 % a.nsplit, L2 = L1 / a.nsplit;
+    const int u = uniform(L2 % a.Hkv), b = uniform(L2 / a.Hkv);
+    const attn_seq sq = attn_seq_of(scalar_i32(a.q_start, b), scalar_i32(a.q_start, b + 1),
+                                    scalar_i32(a.kv_len, b), a.T, a.cols, a.lgp);
+    const int live = attn_live_parts(sq.kend, a.kps, a.nsplit);
+    if (sp >= live)
+        return;
+    const int k0 = attn_part_start(sq.kend, a.kps, sp), k1 = attn_part_end(sq.kend, a.kps, a.nsplit, sp);
+    const int32_t *table = a.table + (int64_t)b * a.cols;
+    const int tid = wi_id_x(), w = uniform(tid >> 6), lane = tid & 63;
+    const int l32 = lane & 31, hi = lane >> 5, g16 = lane >> 4, i16 = lane & 15;
+    const int g = a.Hq / a.Hkv, R = sq.n * g, D = a.D;
+    const float c = MOD ? 1.f : a.c;
+    const float lift = 8.f / c; // how far a score may pass the running maximum
+
+    // Offsets of this lane's operand reads (elements): K row kperm, chunk 2kk + hi; V rows 8hi + i16 / 4
+    // (+ 4), columns 16 (g16 & 1) + 4 (i16 & 3).
+    const int kperm = (l32 & ~12) | ((l32 & 4) << 1) | ((l32 & 8) >> 1);
+    const int kfo = (kperm >> 3) * 8 * DP + (kperm & 7) * 16 + ((hi ^ ((kperm >> 3) & 1)) * 8);
+    const int vfo = hi * 8 * DP + (i16 >> 2) * 32 + (2 * (g16 & 1) + ((i16 & 3) >> 1)) * 8 + (i16 & 1) * 4;
+
+    // Staging: bf16 pieces in the order of the LDS layouts, byte (w PW + p) 1024 + 16 lane of the tile.
+    uint32_t kso[PW], vso[PW];
+#pragma unroll
+    for (int p = 0; p < PW; ++p) {
+        const int x = (w * PW + p) * 1024 + 16 * lane;
+        const int kg = x / (16 * DP), kw = x % (16 * DP);
+        const int kr = kg * 8 + (kw % 256) / 32 - 16 * w;
+        const int kc = 2 * (kw / 256) + (((kw % 32) / 16) ^ (kg & 1));
+        kso[p] = kc * 8 < D ? (uint32_t)(kr * D * 2 + kc * 16) : 0x80000000u;
+        const int vg = x / (8 * DP), vw = x % (8 * DP);
+        const int vr = vg * 4 + (vw % 256) / 64 - 16 * w;
+        const int vc = 4 * (vw / 256) + (vw % 64) / 16;
+        vso[p] = vc * 8 < D ? (uint32_t)(vr * D * 2 + vc * 16) : 0x80000000u;
+    }
+    struct stage {
+        u32x4 k[F4 ? 1 : PW], v[F4 ? 1 : PW];
+        uint32_t kw[F4 ? KW : 1], vw[F4 ? KW : 1], ksc, vsc;
+        bool whole; // every block of the tile has a page
+    };
+    auto load = [&](int kb, stage &f) __attribute__((always_inline)) {
+        const kv_block m = block_at(a, table, u, kb + 16 * w, k1);
+        f.whole = kb + KT <= k1;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            f.whole &= attn_page_ok(scalar_i32(table, min(kb + 16 * j, k1 - 1) >> a.lgp), a.pages) != 0;
+        if constexpr (!F4) {
+            const uint32_t rb = (uint32_t)D * 2u;
+            const auto kr = make_rsrc(a.k + m.row * rb, m.n * rb);
+            const auto vr = make_rsrc(a.v + m.row * rb, m.n * rb);
+#pragma unroll
+            for (int p = 0; p < PW; ++p)
+                f.k[p] = buf16<false>(kr, kso[p]);
+#pragma unroll
+            for (int p = 0; p < PW; ++p)
+                f.v[p] = buf16<false>(vr, vso[p]);
+        } else {
+            constexpr int RB = DP / 2, SB = DP / 32;
+            const auto kr = make_rsrc(a.k + m.row * RB, m.n * RB);
+            const auto vr = make_rsrc(a.v + m.row * RB, m.n * RB);
+            const auto ksr = make_rsrc(a.ks + m.row * SB, m.n * SB);
+            const auto vsr = make_rsrc(a.vs + m.row * SB, m.n * SB);
+            const uint32_t off = i16 * RB + g16 * (RB / 4);
+            if constexpr (DP == 64) {
+                const u32x2 x = __builtin_amdgcn_raw_buffer_load_b64(kr, off, 0, 0);
+                const u32x2 y = __builtin_amdgcn_raw_buffer_load_b64(vr, off, 0, 0);
+                f.kw[0] = x[0], f.kw[1] = x[1], f.vw[0] = y[0], f.vw[1] = y[1];
+            } else {
+#pragma unroll
+                for (int j = 0; j < KW / 4; ++j) {
+                    const u32x4 x = buf16<false>(kr, off + 16 * j), y = buf16<false>(vr, off + 16 * j);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        f.kw[4 * j + i] = x[i], f.vw[4 * j + i] = y[i];
+                }
+            }
+            if constexpr (NSC == 2) {
+                f.ksc = __builtin_amdgcn_raw_buffer_load_b16(ksr, i16 * SB + g16 * 2, 0, 0);
+                f.vsc = __builtin_amdgcn_raw_buffer_load_b16(vsr, i16 * SB + g16 * 2, 0, 0);
+            } else {
+                f.ksc = __builtin_amdgcn_raw_buffer_load_b8(ksr, i16 * SB + g16 * SB / 4, 0, 0);
+                f.vsc = __builtin_amdgcn_raw_buffer_load_b8(vsr, i16 * SB + g16 * SB / 4, 0, 0);
+            }
+        }
+    };
+    auto put = [&](const stage &f, int buf) __attribute__((always_inline)) {
+        if constexpr (!F4) {
+#pragma unroll
+            for (int p = 0; p < PW; ++p)
+                *reinterpret_cast<u32x4 *>(&Ks[buf][(w * PW + p) * 512 + lane * 8]) = f.k[p];
+#pragma unroll
+            for (int p = 0; p < PW; ++p)
+                *reinterpret_cast<u32x4 *>(&Vs[buf][(w * PW + p) * 512 + lane * 8]) = f.v[p];
+        } else {
+            // Row r of the tile, chunks of eight elements from c0 on. K: the 16 rows of a pass hit other
+            // banks. V: rows four apart would not, so each starts at another of its chunks.
+            const int r = 16 * w + i16, c0 = g16 * KW;
+#pragma unroll
+            for (int j = 0; j < KW; ++j) {
+                const int cc = c0 + j;
+                *reinterpret_cast<u32x4 *>(&Ks[buf][(r >> 3) * 8 * DP + (cc >> 1) * 128 + (r & 7) * 16 +
+                                                    ((cc & 1) ^ ((r >> 3) & 1)) * 8]) =
+                    fp4_to_bf16(f.kw[j], e8m0(NSC == 2 ? (f.ksc >> (j / 4 * 8)) & 0xff : f.ksc));
+            }
+            constexpr int RW = KW < 4 ? KW : 4;
+            const int rot = (i16 >> 2) & (RW - 1);
+#pragma unroll
+            for (int j0 = 0; j0 < KW; j0 += RW) {
+                const float sc = e8m0(NSC == 2 ? (f.vsc >> (j0 / 4 * 8)) & 0xff : f.vsc);
+                uint32_t x[RW], y[RW];
+#pragma unroll
+                for (int j = 0; j < RW; ++j)
+                    x[j] = pick(rot & 1, f.vw[j0 + (j + 1) % RW], f.vw[j0 + j]);
+#pragma unroll
+                for (int j = 0; j < RW; ++j)
+                    y[j] = pick(rot & 2, x[(j + 2) % RW], x[j]);
+#pragma unroll
+                for (int j = 0; j < RW; ++j) {
+                    const int cc = c0 + j0 + ((j + rot) & (RW - 1));
+                    *reinterpret_cast<u32x4 *>(&Vs[buf][(r >> 2) * 4 * DP + (cc >> 2) * 128 +
+                                                        (r & 3) * 32 + (cc & 3) * 8]) =
+                        fp4_to_bf16(y[j], sc);
+                }
+            }
+        }
+    };
+
+    for (int tile = t0; (int64_t)tile * 128 < R; tile += a.tps) {
+        const int row0 = tile * 128, row = row0 + 32 * w + l32;
+        const bool valid = row < R;
+        const int tok = valid ? row / g : 0, h = u * g + (valid ? row % g : 0);
+        const uint16_t *q = a.q + (sq.q0 + tok) * a.q_tok + h * a.q_head;
+        bf16x8 qb[KN];
+#pragma unroll
+        for (int kk = 0; kk < KN; ++kk) {
+            const int col = kk * 16 + hi * 8;
+            u32x4 x = zero4();
+            if (valid && col < D)
+                x = *reinterpret_cast<const u32x4 *>(q + col);
+            qb[kk] = as_bf16x8(x);
+        }
+        const int p0 = sq.len - sq.n; // position of the sequence's first row
+        const int pos = p0 + tok, lim = a.causal ? min(pos, k1 - 1) : k1 - 1;
+        const float slope = MOD && a.slopes ? a.slopes[h] * 1.44269504088896341f : 0.f;
+        // The wave's smallest and largest limits, and where the workgroup's tiles end.
+        const int wfirst = row0 + 32 * w, wlast = min(wfirst + 31, R - 1);
+        const int wmin = uniform(a.causal ? min(p0 + min(wfirst, R - 1) / g, k1 - 1) : k1 - 1);
+        const int wmax = uniform(wfirst >= R ? -1 : a.causal ? min(p0 + wlast / g, k1 - 1) : k1 - 1);
+        const int kstop = uniform(a.causal ? min(k1, p0 + min(row0 + 127, R - 1) / g + 1) : k1);
+
+        float m_run = kNegInf, l_run = 0.f;
+        f32x16 o[DP / 32];
+#pragma unroll
+        for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                o[db][i] = 0.f;
+
+        stage st;
+        bool whole = true;
+        if (k0 < kstop) {
+            load(k0, st);
+            whole = st.whole;
+            put(st, 0);
+        }
+        __syncthreads();
+        int buf = 0;
+        for (int kb = k0; kb < kstop; kb += KT, buf ^= 1) {
+            const bool more = kb + KT < kstop;
+            if (more)
+                load(kb + KT, st);
+            if (kb <= wmax) {
+                f32x16 s[2];
+                const uint16_t *kp = &Ks[buf][kfo];
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        s[t][i] = 0.f;
+#pragma unroll
+                    for (int kk = 0; kk < KN; ++kk)
+                        s[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+                            as_bf16x8(*reinterpret_cast<const u32x4 *>(kp + t * 32 * DP + kk * 128)),
+                            qb[kk], s[t], 0, 0, 0);
+                }
+                // Register i of sub-tile t: key kb + 32t + 16 (i / 8) + 8hi + i % 8.
+                if (MOD)
+#pragma unroll
+                    for (int t = 0; t < 2; ++t)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i)
+                            s[t][i] = score2(s[t][i], a.c, a.cap_in, a.cap_out, slope,
+                                             pos - (kb + 32 * t + 16 * (i >> 3) + 8 * hi + (i & 7)));
+                if (!whole || kb + KT - 1 > wmin) {
+                    // A block without a page hides its keys. The tile's blocks are looked up again
+                    // here: it is rare.
+                    uint32_t none = 0;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        none |= block_at(a, table, u, kb + 16 * j, k1).n == 0 ? 1u << j : 0u;
+#pragma unroll
+                    for (int t = 0; t < 2; ++t)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i)
+                            if (kb + 32 * t + 16 * (i >> 3) + 8 * hi + (i & 7) > lim ||
+                                (none >> (2 * t + (i >> 3)) & 1))
+                                s[t][i] = kNegInf;
+                }
+                float mx = kNegInf;
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int i = 0; i < 16; i += 2)
+                        mx = max3f(mx, s[t][i], s[t][i + 1]);
+                mx = max_xor32(mx);
+                if (__builtin_amdgcn_ballot_w64(mx > m_run + lift) != 0) {
+                    const float mnew = fmaxf(m_run, mx);
+                    const float alpha = fast_exp2((m_run - (mnew == kNegInf ? 0.f : mnew)) * c);
+                    m_run = mnew;
+                    l_run *= alpha;
+#pragma unroll
+                    for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i)
+                            o[db][i] *= alpha;
+                }
+                const float mc = m_run == kNegInf ? 0.f : m_run * c;
+                bf16x8 pk[4];
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const float p = fast_exp2(fmaf(s[t][i], c, -mc));
+                        l_run += p;
+                        pk[2 * t + (i >> 3)][i & 7] = (__bf16)p;
+                    }
+                const uint16_t *vp = &Vs[buf][vfo];
+#pragma unroll
+                for (int cc = 0; cc < 4; ++cc)
+#pragma unroll
+                    for (int db = 0; db < DP / 32; ++db) {
+                        const uint16_t *x = vp + cc * 16 * DP + db * 128;
+                        o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+                            join_tr(lds_read_tr(x), lds_read_tr(x + 4 * DP)), pk[cc], o[db], 0, 0, 0);
+                    }
+            }
+            if (more) {
+                put(st, buf ^ 1);
+                whole = st.whole;
+            }
+            __syncthreads();
+        }
+        l_run = sum_xor32(l_run);
+
+        if (valid) {
+            const int64_t at = sq.q0 + tok;
+            if (live == 1) {
+                const float inv = l_run > 0.f ? 1.0f / l_run : 0.f;
+                uint16_t *dst = a.o + at * a.o_tok + h * a.o_head;
+#pragma unroll
+                for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const int d = db * 32 + 8 * j + 4 * hi;
+                        if (d < D)
+                            *reinterpret_cast<u32x2 *>(dst + d) =
+                                u32x2{bf16_pair(o[db][4 * j] * inv, o[db][4 * j + 1] * inv),
+                                      bf16_pair(o[db][4 * j + 2] * inv, o[db][4 * j + 3] * inv)};
+                    }
+            } else {
+                const int64_t slot = (at * a.Hq + h) * a.nsplit + sp;
+                if (hi == 0) {
+                    a.pm[slot] = m_run * c;
+                    a.pl[slot] = l_run;
+                }
+                float *dst = a.pacc + slot * D;
+#pragma unroll
+                for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const int d = db * 32 + 8 * j + 4 * hi;
+                        if (d < D)
+                            *reinterpret_cast<f32x4 *>(dst + d) =
+                                f32x4{o[db][4 * j], o[db][4 * j + 1], o[db][4 * j + 2], o[db][4 * j + 3]};
+                    }
+            }
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------
+// Append. A workgroup takes 256 units of work of each of tpw tokens of one sequence, one unit per thread:
+// 16 elements of a head, the two eights that rotate with each other ((x1, x2) -> (x1 c - x2 s,
+// x2 c + x1 s), in fp32, products and sums rounded apart, the result once to bf16), or for the 4-bit
+// cache eight elements of a K or V row. HBM-bound: each element is read and written once, and the rope
+// row is shared by a token's heads through the L1 cache.
+// ------------------------------------------------------------------------------------------
+__device__ __forceinline__ float lo_bf16(uint32_t x) { return __builtin_bit_cast(float, x << 16); }
+__device__ __forceinline__ float hi_bf16(uint32_t x) {
+    return __builtin_bit_cast(float, x & 0xffff0000u);
+}
+__device__ __forceinline__ void to_f32(u32x4 v, float *x) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        x[2 * i] = lo_bf16(v[i]);
+        x[2 * i + 1] = hi_bf16(v[i]);
+    }
+}
+__device__ __forceinline__ u32x4 to_bf16(const float *x) {
+    return u32x4{bf16_pair(x[0], x[1]), bf16_pair(x[2], x[3]), bf16_pair(x[4], x[5]),
+                 bf16_pair(x[6], x[7])};
+}
+
+// max over each four consecutive lanes, in every one of them
+__device__ __forceinline__ uint32_t quad_max(uint32_t x) {
+    x = max(x, (uint32_t)__builtin_amdgcn_update_dpp((int)x, (int)x, 0xB1, 0xf, 0xf, false)); // 1,0,3,2
+    return max(x, (uint32_t)__builtin_amdgcn_update_dpp((int)x, (int)x, 0x4E, 0xf, 0xf, false)); // 2,3,0,1
+}
+
+// Scale byte of a group whose largest magnitude has the fp32 bits amax: the smallest power of two 2^(e-127)
+// under which that is at most 7, so that no element is further off than half of E2M1's widest step
+// (between 4 and 6; 7 is held as 6), but within 2^-126 .. 2^125, so that scale and values are normal
+// numbers (8 2^125 is no bf16 value). 255, E8M0's NaN, where the group is not finite.
+__device__ __forceinline__ uint32_t e8m0_of(uint32_t amax) {
+    if (amax >= 0x7f800000u)
+        return 255u;
+    const int e = (int)(amax >> 23) - 2 + ((amax & 0x7fffffu) > 0x600000u ? 1 : 0);
+    return (uint32_t)min(max(e, 1), 252);
+}
+
+template <bool F4, bool PAIRS>
+__global__ __launch_bounds__(256) void attn_kv_append_kernel(const attn_kv_args a) {
+#pragma clang fp contract(off)
+    const int per = a.tblk * a.ublk;
+    const int b = uniform(wg_id_x() / per), L = wg_id_x() % per;
+    const int ub = uniform(L % a.ublk), tb = uniform(L / a.ublk);
+    const attn_seq sq = attn_seq_of(scalar_i32(a.q_start, b), scalar_i32(a.q_start, b + 1),
+                                    scalar_i32(a.kv_len, b), a.T, a.cols, a.lgp);
+    const int unit = ub * 256 + wi_id_x(), D = a.D, half = a.rot / 2;
+    // This thread's unit: which tensor (0 q, 1 k, 2 v), head and part of the head.
+    const int uh = D / 16, uh4 = D / 8;
+    const int nq = F4 ? (a.Hq * uh + 3) / 4 * 4 : a.Hq * uh, nk = a.Hkv * (F4 ? uh4 : uh);
+    int what = 0, x = unit;
+    if (unit >= nq) {
+        what = unit >= nq + nk ? 2 : 1;
+        x = unit - nq - (what == 2 ? nk : 0);
+    }
+    const bool mine = what == 0 ? unit < a.Hq * uh : x < nk;
+    const bool eight = F4 && what != 0;
+    const int n = eight ? uh4 : uh, head = x / n, j = x % n;
+    const bool turn = what != 2 && (eight ? j * 8 < a.rot : j * 16 < a.rot);
+    // Columns of the two eights, and of the cosines of the first one's elements (or pairs).
+    int c0, c1, rc;
+    if (eight) { // c0: this unit's own; c1: its partner (PAIRS: none)
+        c0 = 8 * j;
+        c1 = !turn || PAIRS ? c0 : c0 < half ? c0 + half : c0 - half;
+        rc = PAIRS ? 4 * j : c0 < half ? c0 : c0 - half;
+    } else {
+        c0 = turn && !PAIRS ? 8 * j : 16 * j;
+        c1 = turn && !PAIRS ? half + 8 * j : 16 * j + 8;
+        rc = 8 * j;
+    }
+    const int64_t tok_s = what == 0 ? a.q_tok : what == 1 ? a.k_tok : a.v_tok;
+    const uint16_t *src = (what == 0   ? a.q + head * a.q_head
+                           : what == 1 ? a.k + head * a.k_head
+                                       : a.v + head * a.v_head);
+    const int32_t *table = a.table + (int64_t)b * a.cols;
+
+    for (int i0 = tb * a.tpw; i0 < sq.n; i0 += a.tblk * a.tpw)
+        for (int i = i0; i < min(i0 + a.tpw, sq.n); ++i) {
+            const int pos = sq.len - sq.n + i;
+            const bool placed = pos >= 0 && (a.rot == 0 || pos < a.rope_rows);
+            bool kept = placed && pos < sq.kend;
+            int pg = 0;
+            if (kept) {
+                pg = scalar_i32(table, pos >> a.lgp);
+                kept = attn_page_ok(pg, a.pages);
+            }
+            if (!mine || !(what == 0 ? placed || a.rot == 0 : kept))
+                continue;
+            const uint16_t *s = src + (sq.q0 + i) * tok_s;
+            const u32x4 v0 = *reinterpret_cast<const u32x4 *>(s + c0);
+            const u32x4 v1 = *reinterpret_cast<const u32x4 *>(s + c1);
+            u32x4 y0 = v0, y1 = v1;
+            if (turn) {
+                const float *cr = a.rope + (int64_t)pos * a.rot + rc, *sr = cr + half;
+                float p[8], q[8], cs[8], sn[8], r0[8], r1[8];
+                to_f32(v0, p);
+                to_f32(v1, q);
+#pragma unroll
+                for (int e = 0; e < 8; e += 4) {
+                    if (PAIRS && eight && e == 4) // eight elements are four pairs
+                        break;
+                    const f32x4 x0 = *reinterpret_cast<const f32x4 *>(cr + e);
+                    const f32x4 x1 = *reinterpret_cast<const f32x4 *>(sr + e);
+#pragma unroll
+                    for (int f = 0; f < 4; ++f)
+                        cs[e + f] = x0[f], sn[e + f] = x1[f];
+                }
+                if (PAIRS) {
+                    // elements (2e, 2e + 1) turn together; eight pairs in sixteen elements
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        r0[2 * e] = p[2 * e] * cs[e] - p[2 * e + 1] * sn[e];
+                        r0[2 * e + 1] = p[2 * e + 1] * cs[e] + p[2 * e] * sn[e];
+                    }
+                    if (!eight)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            r1[2 * e] = q[2 * e] * cs[4 + e] - q[2 * e + 1] * sn[4 + e];
+                            r1[2 * e + 1] = q[2 * e + 1] * cs[4 + e] + q[2 * e] * sn[4 + e];
+                        }
+                } else if (eight && c0 >= half) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        r0[e] = p[e] * cs[e] + q[e] * sn[e];
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        r0[e] = p[e] * cs[e] - q[e] * sn[e];
+                        if (!eight)
+                            r1[e] = q[e] * cs[e] + p[e] * sn[e];
+                    }
+                }
+                y0 = to_bf16(r0);
+                if (!eight)
+                    y1 = to_bf16(r1);
+            }
+            if (what == 0) {
+                uint16_t *d = a.q_out + (sq.q0 + i) * a.qo_tok + head * a.qo_head;
+                *reinterpret_cast<u32x4 *>(d + c0) = y0;
+                *reinterpret_cast<u32x4 *>(d + c1) = y1;
+                continue;
+            }
+            const int64_t row = attn_page_row(pg, a.Hkv, head, pos, a.lgp);
+            if constexpr (!F4) {
+                uint16_t *d = reinterpret_cast<uint16_t *>(what == 1 ? a.ck : a.cv) + row * D;
+                *reinterpret_cast<u32x4 *>(d + c0) = y0;
+                *reinterpret_cast<u32x4 *>(d + c1) = y1;
+            } else {
+                uint32_t am = 0;
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    am = max(am, max(y0[e] << 16 & 0x7fff0000u, y0[e] & 0x7fff0000u));
+                const uint32_t e8 = e8m0_of(quad_max(am));
+                const float sc = e8m0(e8);
+                uint32_t code = 0;
+                if (e8 != 255) {
+                    code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, lo_bf16(y0[0]), hi_bf16(y0[0]), sc, 0);
+                    code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, lo_bf16(y0[1]), hi_bf16(y0[1]), sc, 1);
+                    code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, lo_bf16(y0[2]), hi_bf16(y0[2]), sc, 2);
+                    code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, lo_bf16(y0[3]), hi_bf16(y0[3]), sc, 3);
+                }
+                *reinterpret_cast<uint32_t *>((what == 1 ? a.ck : a.cv) + row * (D / 2) + 4 * j) = code;
+                if (j % 4 == 0)
+                    (what == 1 ? a.cks : a.cvs)[row * (D / 32) + j / 4] = (uint8_t)e8;
+            }
+        }
+}
+
+// Read back: eight elements of a K or V row per thread and token. A token without a place in the cache
+// gives zeros.
+template <bool F4>
+__global__ __launch_bounds__(256) void attn_kv_read_kernel(const attn_kv_args a) {
+    const int per = a.tblk * a.ublk;
+    const int b = uniform(wg_id_x() / per), L = wg_id_x() % per;
+    const int ub = uniform(L % a.ublk), tb = uniform(L / a.ublk);
+    const attn_seq sq = attn_seq_of(scalar_i32(a.q_start, b), scalar_i32(a.q_start, b + 1),
+                                    scalar_i32(a.kv_len, b), a.T, a.cols, a.lgp);
+    const int unit = ub * 256 + wi_id_x(), D = a.D, n = D / 8;
+    const bool isv = unit >= a.Hkv * n;
+    const int x = unit - (isv ? a.Hkv * n : 0), head = x / n, j = x % n;
+    if (x >= a.Hkv * n)
+        return;
+    const int32_t *table = a.table + (int64_t)b * a.cols;
+    const uint8_t *pages = isv ? a.cv : a.ck, *scales = isv ? a.cvs : a.cks;
+    uint16_t *dst = (isv ? a.v_out + head * a.v_head : a.k_out + head * a.k_head) + 8 * j;
+    const int64_t tok_s = isv ? a.v_tok : a.k_tok;
+    for (int i0 = tb * a.tpw; i0 < sq.n; i0 += a.tblk * a.tpw)
+        for (int i = i0; i < min(i0 + a.tpw, sq.n); ++i) {
+            const int pos = sq.len - sq.n + i;
+            const int pg = pos >= 0 && pos < sq.kend ? scalar_i32(table, pos >> a.lgp) : -1;
+            u32x4 y = zero4();
+            if (attn_page_ok(pg, a.pages)) {
+                const int64_t row = attn_page_row(pg, a.Hkv, head, pos, a.lgp);
+                if constexpr (F4)
+                    y = fp4_to_bf16(*reinterpret_cast<const uint32_t *>(pages + row * (D / 2) + 4 * j),
+                                    e8m0(scales[row * (D / 32) + j / 4]));
+                else
+                    y = *reinterpret_cast<const u32x4 *>(pages + row * D * 2 + 16 * j);
+            }
+            *reinterpret_cast<u32x4 *>(dst + (sq.q0 + i) * tok_s) = y;
+        }
+}
+
+// ---- launchers -------------------------------------------------------------------------------
+template <int DP, bool F4> hipError_t launch_paged_d(const attn_paged_args &a, int rows16, hipStream_t st) {
+    const unsigned grid = (unsigned)(a.B * (long)a.Hkv * a.nsplit * a.tps);
+    const bool mod = a.cap_out != 0.f || a.slopes;
+    return with_flag(mod, [&](auto M) {
+        constexpr bool kM = decltype(M)::value;
+        auto decode = [&](auto NB, auto NT) {
+            constexpr int kN = decltype(NB)::value;
+            constexpr bool kT = decltype(NT)::value;
+            if (t_plan)
+                plan_note(dim3(grid), dim3(256),
+                          "attn_paged_decode_kernel<%d, %d, %d, %s, %s> parts=%d keys=%d", DP, F4 ? 4 : 16,
+                          kN, tf(kM), tf(kT), a.nsplit, a.kps);
+            else
+                hipLaunchKernelGGL((attn_paged_decode_kernel<DP, F4, kN, kM, kT>), dim3(grid), dim3(256), 0,
+                                   st, a);
+            return hipGetLastError();
+        };
+        if (rows16 == 1)
+            return with_flag(a.tps == 1, [&](auto NT) {
+                return decode(std::integral_constant<int, 1>{}, NT);
+            });
+        if constexpr (DP <= 128)
+            if (rows16 == 2)
+                return decode(std::integral_constant<int, 2>{}, std::false_type{});
+        if (t_plan)
+            plan_note(dim3(grid), dim3(256), "attn_paged_prefill_kernel<%d, %d, %s> parts=%d keys=%d", DP,
+                      F4 ? 4 : 16, tf(kM), a.nsplit, a.kps);
+        else
+            hipLaunchKernelGGL((attn_paged_prefill_kernel<DP, F4, kM>), dim3(grid), dim3(256), 0, st, a);
+        return hipGetLastError();
+    });
+}
+
+} // namespace
+
+// rows16: 1 or 2 row blocks of 16 per workgroup (decode), or 8 (prefill). Joins the parts where the call
+// has more than one; max_q bounds the merge's grid.
+extern "C" int attn_hip_launch_paged(const struct attn_paged_args *ap, int bits, int rows16, int max_q,
+                                     void *stream) {
+    const attn_paged_args &a = *ap;
+    const hipStream_t st = (hipStream_t)stream;
+    const long grid = (long)a.B * a.Hkv * a.nsplit * a.tps;
+    if (grid <= 0 || grid > ATTN_PAGED_MAX_GRID || a.nsplit > kPagedMaxSplit)
+        return (int)hipErrorInvalidValue;
+    hipError_t e;
+    if (bits == 4)
+        e = a.D == 64    ? launch_paged_d<64, true>(a, rows16, st)
+            : a.D == 128 ? launch_paged_d<128, true>(a, rows16, st)
+                         : launch_paged_d<256, true>(a, rows16, st);
+    else
+        e = a.D <= 64    ? launch_paged_d<64, false>(a, rows16, st)
+            : a.D <= 128 ? launch_paged_d<128, false>(a, rows16, st)
+                         : launch_paged_d<256, false>(a, rows16, st);
+    if (e != hipSuccess || a.nsplit == 1)
+        return (int)e;
+    // LP lanes of four columns, SG groups of parts: 8 loads or fewer per thread where there are parts
+    // for it.
+    int lglp = 3, lgsg = 0;
+    while ((4 << lglp) < a.D)
+        ++lglp;
+    while (lglp + lgsg < 8 && (4 << lgsg) < a.nsplit)
+        ++lgsg;
+    const int rpw = 256 >> (lglp + lgsg);
+    const long tiles = ((long)max_q * a.Hq + rpw - 1) / rpw;
+    const long tpm = std::max(1L, std::min(tiles, ATTN_PAGED_MAX_GRID / a.B));
+    if (t_plan)
+        plan_note(dim3((unsigned)(a.B * tpm)), dim3(256), "attn_paged_merge_kernel rows=%d", rpw);
+    else
+        hipLaunchKernelGGL(attn_paged_merge_kernel, dim3((unsigned)(a.B * tpm)), dim3(256), 0, st, a, lglp,
+                           lgsg, (int)tpm);
+    return (int)hipGetLastError();
+}
+
+extern "C" int attn_hip_launch_kv_append(const struct attn_kv_args *ap, int bits, int pairs, void *stream) {
+    const attn_kv_args &a = *ap;
+    const long grid = (long)a.B * a.tblk * a.ublk;
+    if (grid <= 0 || grid > ATTN_PAGED_MAX_GRID)
+        return (int)hipErrorInvalidValue;
+    return (int)with_flag(bits == 4, [&](auto F) {
+        return with_flag(pairs != 0, [&](auto P) {
+            hipLaunchKernelGGL((attn_kv_append_kernel<decltype(F)::value, decltype(P)::value>),
+                               dim3((unsigned)grid), dim3(256), 0, (hipStream_t)stream, a);
+            return hipGetLastError();
+        });
+    });
+}
+
+extern "C" int attn_hip_launch_kv_read(const struct attn_kv_args *ap, int bits, void *stream) {
+    const attn_kv_args &a = *ap;
+    const long grid = (long)a.B * a.tblk * a.ublk;
+    if (grid <= 0 || grid > ATTN_PAGED_MAX_GRID)
+        return (int)hipErrorInvalidValue;
+    return (int)with_flag(bits == 4, [&](auto F) {
+        hipLaunchKernelGGL((attn_kv_read_kernel<decltype(F)::value>), dim3((unsigned)grid), dim3(256), 0,
+                           (hipStream_t)stream, a);
+        return hipGetLastError();
+    });
+}
+
+#endif
