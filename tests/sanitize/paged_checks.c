@@ -67,14 +67,38 @@ static void touch_slot(const struct attn_paged_args *a, int64_t slot, char *seen
  * the table entries they read, the blocks of 16 keys they address. */
 static char *token_seen; /* [T], or NULL: only the cut is checked */
 static char *cache_rows; /* [pages * Hkv * page] */
-int attn_hip_launch_paged(const struct attn_paged_args *a, int bits, int rows16, int max_q, void *stream) {
-    CHECK(stream == &stream_token && (bits == 4 || bits == 16) && max_q >= 1, "launch");
-    CHECK(rows16 == 1 || rows16 == 2 || rows16 == 8, "rows16 %d", rows16);
-    CHECK(a->D <= 128 || rows16 != 2, "two row blocks at D = %d", a->D);
+static void touch_keys(const struct attn_paged_args *a, int b, int u, int k0, int k1) {
+    for (int kb = k0; kb < k1; kb += 16) {
+        const int pg = a->table[(int64_t)b * a->cols + ((kb < k1 - 1 ? kb : k1 - 1) >> a->lgp)];
+        if (!attn_page_ok(pg, a->pages))
+            continue;
+        const int64_t row = attn_page_row(pg, a->Hkv, u, kb, a->lgp);
+        const int n = k1 - kb < 16 ? k1 - kb : 16;
+        for (int i = 0; i < n; ++i)
+            cache_rows[row + i] = 1;
+    }
+}
+
+static struct attn_seq seq_of(const struct attn_paged_args *a, int b) {
+    return attn_seq_of(a->q_start[b], a->q_start[b + 1], a->kv_len[b], a->T, a->cols, a->lgp);
+}
+
+int attn_hip_launch_paged(const struct attn_paged_args *a, const struct attn_paged_cut *cut, int bits,
+                          void *stream) {
+    const int rows16 = cut->rows16;
+    const int64_t seqs = (int64_t)a->B * a->Hkv;
+    CHECK(stream == &stream_token && (bits == 4 || bits == 16), "launch");
+    CHECK(rows16 == 1 || rows16 == 2 || rows16 == 4 || rows16 == 8, "rows16 %d", rows16);
+    CHECK(a->D <= 128 || rows16 == 1 || rows16 == 8, "%d row blocks at D = %d", rows16, a->D);
     CHECK(a->tps >= 1 && a->nsplit >= 1 && a->nsplit <= ATTN_PAGED_MAX_PARTS, "cut");
-    CHECK(a->kps >= 128 && a->kps % 128 == 0, "kps %d", a->kps);
-    CHECK((int64_t)a->B * a->Hkv * a->nsplit * a->tps <= ATTN_PAGED_MAX_GRID, "grid");
+    CHECK(cut->grid >= 1 && cut->grid <= ATTN_PAGED_MAX_GRID, "grid %lld", (long long)cut->grid);
     CHECK(a->nsplit == 1 || (int64_t)a->T * a->Hq * a->nsplit <= ATTN_SLOTS, "slots");
+    CHECK(a->teams == 0 || a->nsplit >= 2, "teams without parts");
+    if (a->nsplit > 1) {
+        CHECK((256 >> (cut->lglp + cut->lgsg)) * a->nsplit <= ATTN_PAGED_MERGE_WEIGHTS, "merge weights");
+        CHECK(cut->lglp + cut->lgsg <= 8 && 4 << cut->lglp >= a->D, "merge lanes");
+        CHECK(cut->merge_tiles >= 1 && seqs * cut->merge_tiles <= ATTN_PAGED_MAX_GRID, "merge grid");
+    }
     if (a->nsplit > 1 && scratch_base)
         touch_slot(a, (int64_t)a->T * a->Hq * a->nsplit - 1, NULL);
     if (!token_seen)
@@ -82,35 +106,102 @@ int attn_hip_launch_paged(const struct attn_paged_args *a, int bits, int rows16,
     const int g = a->Hq / a->Hkv;
     int64_t keys_seen = 0, keys_want = 0;
     for (int b = 0; b < a->B; ++b) {
-        const struct attn_seq s =
-            attn_seq_of(a->q_start[b], a->q_start[b + 1], a->kv_len[b], a->T, a->cols, a->lgp);
+        const struct attn_seq s = seq_of(a, b);
         CHECK(s.q0 >= 0 && s.n >= 0 && s.q0 + s.n <= a->T && s.len >= 0, "sequence");
         CHECK(s.kend >= 0 && s.kend <= (int64_t)a->cols << a->lgp && s.kend <= s.len, "kend");
-        const int live = attn_live_parts(s.kend, a->kps, a->nsplit);
-        CHECK(live >= 1 && live <= a->nsplit, "live");
-        keys_want += s.kend;
-        for (int sp = 0; sp < live; ++sp) {
-            const int k0 = attn_part_start(s.kend, a->kps, sp);
-            const int k1 = attn_part_end(s.kend, a->kps, a->nsplit, sp);
-            CHECK(k0 % 16 == 0 && k0 <= k1 && k1 <= s.kend, "part %d: %d %d", sp, k0, k1);
-            CHECK(sp + 1 < live || k1 == s.kend, "last part");
-            keys_seen += k1 - k0;
-            for (int kb = k0; kb < k1; kb += 16) {
-                const int pg = a->table[(int64_t)b * a->cols + ((kb < k1 - 1 ? kb : k1 - 1) >> a->lgp)];
-                if (!attn_page_ok(pg, a->pages))
-                    continue;
-                for (int u = 0; u < a->Hkv; ++u) {
-                    const int64_t row = attn_page_row(pg, a->Hkv, u, kb, a->lgp);
-                    const int n = k1 - kb < 16 ? k1 - kb : 16;
-                    for (int i = 0; i < n; ++i)
-                        cache_rows[row + i] = 1;
-                }
-            }
-        }
+        if (s.n > 0)
+            keys_want += (int64_t)s.kend * a->Hkv;
         for (int t0 = 0; t0 < a->tps; ++t0)
             for (int tile = t0; (int64_t)tile * 16 * rows16 < s.n * g; tile += a->tps)
                 for (int r = tile * 16 * rows16; r < (tile + 1) * 16 * rows16 && r < s.n * g; ++r)
                     token_seen[s.q0 + r / g]++;
+    }
+    if (rows16 >= 4) {
+        const int64_t groups = seqs * a->nsplit;
+        CHECK(a->share >= 128 && cut->grid >= groups * a->tps, "prefill grid");
+        char *placed = calloc((size_t)(groups * a->tps), 1);
+        for (int wg = 0; wg < cut->grid; ++wg) {
+            const struct attn_place p = attn_place_of(wg, (int)groups, a->tps, a->deal);
+            if (p.group >= 0)
+                placed[(int64_t)p.group * a->tps + p.tile]++;
+        }
+        for (int64_t i = 0; i < groups * a->tps; ++i)
+            CHECK(placed[i] == 1, "tile %lld placed %d times", (long long)i, placed[i]);
+        free(placed);
+        for (int b = 0; b < a->B; ++b) {
+            const struct attn_seq s = seq_of(a, b);
+            const struct attn_parts parts = attn_parts_of(s.kend, a->share, a->nsplit);
+            CHECK(parts.live >= 1 && parts.live <= a->nsplit, "live");
+            for (int sp = 0; sp < parts.live; ++sp) {
+                const int k0 = attn_part_start(s.kend, parts.kps, sp);
+                const int k1 = attn_part_start(s.kend, parts.kps, sp + 1);
+                CHECK(k0 % 128 == 0 && k0 <= k1 && k1 <= s.kend, "part %d: %d %d", sp, k0, k1);
+                CHECK(sp + 1 < parts.live || k1 == s.kend, "last part");
+                if (s.n > 0)
+                    keys_seen += (int64_t)(k1 - k0) * a->Hkv;
+                for (int u = 0; u < a->Hkv; ++u)
+                    touch_keys(a, b, u, k0, k1);
+            }
+        }
+    } else if (a->teams == 0) {
+        CHECK(cut->grid == seqs * a->tps, "whole grid");
+        keys_seen = keys_want;
+    } else {
+        CHECK(cut->grid == (int64_t)a->teams * a->tps, "team grid");
+        int total = 0, most = 0;
+        for (int b = 0; b < a->B; ++b) {
+            const struct attn_seq s = seq_of(a, b);
+            const int n = attn_units(s.n, s.kend);
+            total += n;
+            most = n > most ? n : most;
+        }
+        const int q = attn_quota(total, most, a->Hkv, a->teams, a->nsplit);
+        CHECK((int64_t)q * a->teams >= (int64_t)total * a->Hkv, "the teams cover the line");
+        int *part_seen = calloc((size_t)seqs * a->nsplit, sizeof(int));
+        for (int team = 0; team < a->teams; ++team) {
+            if ((int64_t)team * q >= (int64_t)total * a->Hkv)
+                continue;
+            int pos = team * q, left = q < total * a->Hkv - pos ? q : total * a->Hkv - pos;
+            int u = pos / total, b = 0, off = pos - u * total;
+            for (;; ++b) {
+                const struct attn_seq s = seq_of(a, b);
+                const int n = attn_units(s.n, s.kend);
+                if (off < n)
+                    break;
+                off -= n;
+            }
+            while (left > 0 && u < a->Hkv) {
+                const struct attn_seq s = seq_of(a, b);
+                const int units = attn_units(s.n, s.kend), take = left < units - off ? left : units - off;
+                if (take > 0) {
+                    const struct attn_cover c = attn_cover_of(pos - off, units, q);
+                    const int sp = team - c.first;
+                    CHECK(c.live <= a->nsplit && sp >= 0 && sp < c.live, "part %d of %d (%d)", sp, c.live,
+                          a->nsplit);
+                    part_seen[((int64_t)b * a->Hkv + u) * a->nsplit + sp]++;
+                    const int k0 = off * 128 < s.kend ? off * 128 : s.kend;
+                    const int k1 = (off + take) * 128 < s.kend ? (off + take) * 128 : s.kend;
+                    keys_seen += k1 - k0;
+                    touch_keys(a, b, u, k0, k1);
+                }
+                left -= take, pos += take, off = 0;
+                if (++b == a->B)
+                    b = 0, ++u;
+            }
+            CHECK(left == 0, "the line ends before the quota");
+        }
+        for (int b = 0, before = 0; b < a->B; ++b) { /* what the merge will read */
+            const struct attn_seq s = seq_of(a, b);
+            const int units = attn_units(s.n, s.kend);
+            for (int u = 0; u < a->Hkv && units; ++u) {
+                const struct attn_cover c = attn_cover_of(u * total + before, units, q);
+                for (int sp = 0; sp < a->nsplit; ++sp)
+                    CHECK(part_seen[((int64_t)b * a->Hkv + u) * a->nsplit + sp] == (sp < c.live),
+                          "part %d of sequence %d head %d", sp, b, u);
+            }
+            before += units;
+        }
+        free(part_seen);
     }
     CHECK(keys_seen == keys_want, "every key once: %lld %lld", (long long)keys_seen, (long long)keys_want);
     return 0;
@@ -217,6 +308,15 @@ static void walk(void) {
 
 /* The cut at the ends of its ranges: only its own invariants. */
 static void cuts(void) {
+    const int kends[] = {0, 1, 127, 128, 129, 5000, 1 << 20, (1 << 30) - 1, 1 << 30};
+    for (int i = 0; i < 9; ++i)
+        for (int sh = 128; sh > 0 && sh <= 1 << 29; sh *= 2)
+            for (int ns = 1; ns <= ATTN_PAGED_MAX_PARTS; ns = ns * 3 / 2 + 1) {
+                const struct attn_parts p = attn_parts_of(kends[i], sh, ns);
+                CHECK(p.live >= 1 && p.live <= ns && p.kps % 128 == 0 && p.kps > 0, "parts");
+                CHECK(attn_part_start(kends[i], p.kps, p.live) == kends[i], "parts cover");
+                CHECK(p.live == 1 || attn_part_start(kends[i], p.kps, p.live - 1) < kends[i], "no empty part");
+            }
     static int32_t one[2];
     const int bs[] = {1, 3, 64, 8192}, ts[] = {1, 64, 4096, 1 << 20, 1 << 30};
     const int qs[] = {1, 2, 17, 4096, INT_MAX}, ks[] = {1, 127, 129, 8192, 1 << 20, INT_MAX};
@@ -228,7 +328,7 @@ static void cuts(void) {
         if ((int64_t)T * Hkv * g > 1 << 30)
             continue;
         struct attn_kv_cache c = {(void *)4096, (void *)4096, NULL, NULL, one, one, one, B,
-                                  1 << 22,      1000,         256,  Hkv,  D,   ATTN_KV_BF16};
+                                  1 << 9,       1000,         256,  Hkv,  D,   ATTN_KV_BF16};
         const struct attn_rows r = {(void *)4096, 8, 8};
         char buf[64];
         attn_paged_plan(&c, T, g * Hkv, 1, NULL, q, k, buf, sizeof buf);

@@ -214,6 +214,17 @@ ATTEND = [
     (16, 256, 16, 8, 2, [(8, 70)], 1, 0, 0, None, None),
     (4, 128, 16, 8, 1, [(8, 257), (2, 31)], 1, 20.0, 0, None, None),
     (4, 256, 16, 4, 1, [(9, 90)], 1, 0, 0, None, None),
+    # 33 to 64 rows of a kv head: key halves
+    (16, 128, 32, 16, 2, [(8, 900), (5, 70), (4, 2)], 1, 0, 1, None, None),
+    (16, 64, 16, 8, 1, [(8, 300), (0, 9), (6, 6)], 0, 0, 0, None, None),
+    (16, 48, 64, 10, 1, [(5, 333), (4, 40)], 1, 9.0, 0, None, None),
+    (4, 128, 64, 16, 2, [(7, 500), (8, 33)], 1, 0, 0, None, None),
+    (4, 64, 16, 6, 1, [(9, 65), (10, 200)], 1, 30.0, 1, None, None),
+    # many sequences, some without rows or keys: the decode line is read 64 sequences at a time
+    (16, 64, 16, 4, 2, [(int(i % 7 != 3), i * 37 % 400) for i in range(70)], 1, 0, 0, None, None),
+    (4, 64, 16, 2, 1, [(1 + i % 2, i * 53 % 290) for i in range(150)], 1, 0, 0, None, None),
+    (16, 32, 16, 2, 2, [(0, 30)] * 65 + [(1, 700), (1, 20)] + [(0, 0)] * 70 + [(2, 300)], 1, 0, 0, None, None),
+    (16, 16, 16, 8, 8, [(16, 20)] * 300, 1, 0, 0, 1, None),       # more rows than partial slots
     # prompts
     (16, 128, 64, 4, 2, [(130, 130), (40, 100), (1, 5)], 1, 0, 0, None, None),
     (16, 128, 16, 8, 1, [(33, 20), (17, 300)], 1, 0, 0, None, None),

@@ -76,6 +76,7 @@ REFUSED = [
     (attend("cache(pages=0)"), "need B >= 1"),
     (attend("cache(table_cols=0)"), "need B >= 1"),
     (attend("cache(table_cols=2**27)"), "at most 2^30 tokens"),
+    (attend("cache(B=2**10, table_cols=2**25, Hkv=2**10)"), "at most 2^38 tokens"),
     (attend("cache(k=None)"), "k and v must be"),
     (attend("cache(v=4104)"), "k and v must be"),
     (attend("cache(bits=4)"), "k_scale and v_scale"),

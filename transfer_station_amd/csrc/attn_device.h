@@ -258,6 +258,10 @@ __device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t r, uint16_t *lds, u
                                              voff, 0, IMM, AUX);
 }
 
+// s_waitcnt operand (gfx9 encoding) that waits until at most n vector memory operations of
+// the wave are in flight, with no wait on expcnt or lgkmcnt.
+constexpr int waitcnt_vm(int n) { return 0x0F70 | (n & 15) | ((n >> 4) << 14); }
+
 // max or sum over each 16 (all: 64) lanes of the wave, in every lane, on the VALU.
 template <bool MAX> __device__ __forceinline__ float seg_all(float x, bool all) {
     auto op = [](float a, float b) { return MAX ? fmaxf(a, b) : a + b; };

@@ -1312,11 +1312,6 @@ __global__ __launch_bounds__(NW * 64, prefill_wg_per_cu(DP, KT, NW)) void attn_p
 // columns. A pair's key-tile counts add up to an odd number, so the item of even count runs
 // first: the buffer order stays a compile-time constant without a padding tile.
 // ------------------------------------------------------------------------------------------
-// s_waitcnt operand (gfx9 encoding) that waits until at most n vector memory operations of
-// the wave are in flight, with no wait on expcnt or lgkmcnt.
-constexpr int waitcnt_vm(int n) { return 0x0F70 | (n & 15) | ((n >> 4) << 14); }
-
-
 template <int DP, bool CAUSAL, bool KH>
 __global__ __launch_bounds__(512, 1) void attn_prefill_persist_kernel(
     const uint16_t *__restrict__ Q, const uint16_t *__restrict__ K,

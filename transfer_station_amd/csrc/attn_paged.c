@@ -17,7 +17,8 @@
 #include <stdlib.h>
 #include <string.h>
 
-int attn_hip_launch_paged(const struct attn_paged_args *a, int bits, int rows16, int max_q, void *stream);
+int attn_hip_launch_paged(const struct attn_paged_args *a, const struct attn_paged_cut *cut, int bits,
+                          void *stream);
 int attn_hip_launch_kv_append(const struct attn_kv_args *a, int bits, int pairs, void *stream);
 int attn_hip_launch_kv_read(const struct attn_kv_args *a, int bits, void *stream);
 void attn_hip_plan_begin(char *buf, size_t len);
@@ -55,6 +56,8 @@ static int paged_check_cache(const char *who, const struct attn_kv_cache *c, int
         paged_fail(who, "need B * Hkv <= 2^20");
     if ((int64_t)c->table_cols * c->page > 1 << 30)
         paged_fail(who, "a table row holds at most 2^30 tokens");
+    if (((int64_t)c->table_cols * c->page + 127) / 128 * c->B * c->Hkv > 0x7fffffff)
+        paged_fail(who, "B * Hkv table rows hold at most 2^38 tokens");
     if (T < 1 || T > 1 << 30)
         paged_fail(who, "need T in [1, 2^30]");
     if (misaligned(c->k, 16) || misaligned(c->v, 16))
@@ -130,12 +133,12 @@ static void paged_run(const char *who, const struct attn_kv_cache *c, const stru
         max_kv = c->table_cols * c->page;
     const struct attn_paged_cut cut =
         attn_paged_cut_of(c->B, c->Hkv, Hq / c->Hkv, T, max_q, max_kv, c->D);
-    a.tps = cut.tps, a.nsplit = cut.nsplit, a.kps = cut.kps;
+    a.tps = cut.tps, a.nsplit = cut.nsplit, a.teams = cut.teams, a.deal = cut.deal, a.share = cut.share;
     /* the scratch of attn_flash: m, l and acc[D] of ATTN_SLOTS partials, each on 256 bytes */
     a.pm = (float *)scratch;
     a.pl = a.pm + ATTN_SLOTS;
     a.pacc = a.pl + ATTN_SLOTS;
-    paged_hip_check(attn_hip_launch_paged(&a, c->bits, cut.rows16, max_q, attn_flash_get_stream()), who);
+    paged_hip_check(attn_hip_launch_paged(&a, &cut, c->bits, attn_flash_get_stream()), who);
 }
 
 void attn_paged(const struct attn_kv_cache *c, const struct attn_rows *q, const struct attn_rows *o, int T,

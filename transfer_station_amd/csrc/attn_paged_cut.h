@@ -7,6 +7,7 @@
 #include <stdint.h>
 
 #include "attn_decode_rule.h"
+#include "attn_paged_rule.h"
 
 /* What the attention kernels are given. */
 struct attn_paged_args {
@@ -20,7 +21,9 @@ struct attn_paged_args {
     int32_t B, T, Hq, Hkv, D, cols, pages, lgp, causal;
     float c;                  /* scale log2(e) */
     float cap_in, cap_out;    /* softcap: 2 log2(e) scale / cap and cap log2(e); cap_out = 0 without */
-    int32_t tps, nsplit, kps; /* row tiles per sequence, parts, keys per part */
+    int32_t tps, nsplit; /* row tiles per sequence, parts of a sequence at most */
+    int32_t teams;       /* decode: see attn_quota; 0: a workgroup takes a whole sequence */
+    int32_t deal, share; /* prefill: see attn_place_of, attn_parts_of */
 };
 
 /* What the append and read kernels are given. */
@@ -35,12 +38,18 @@ struct attn_kv_args {
     int32_t tblk, ublk, tpw; /* token blocks per sequence, blocks of 256 units, tokens per block */
 };
 
+#define ATTN_PAGED_DECODE_WG 512 /* workgroups of a decode call: two per CU */
 #define ATTN_PAGED_MAX_PARTS 256
 #define ATTN_PAGED_MAX_GRID 0xffffffL
+#define ATTN_PAGED_MERGE_WEIGHTS 2048 /* rows x parts that a workgroup of the merge holds the weights of */
 
-/* rows16: row blocks of 16 per workgroup, 1 or 2 (the decode kernel) or 8 (the prefill kernel). */
+/* rows16: row blocks of 16 per workgroup, 1 or 2 (the decode kernel), 4 or 8 (the prefill kernel); rpw: rows
+ * that a workgroup of the merge takes at a time, 0 without one (lglp, lgsg: log2 of its lanes per row and
+ * of its groups of parts). */
 struct attn_paged_cut {
-    int rows16, tps, nsplit, kps;
+    int rows16, tps, nsplit, teams, deal, share;
+    int64_t grid;
+    int lglp, lgsg, merge_tiles, merge_loads;
 };
 
 static inline struct attn_paged_cut attn_paged_cut_of(int B, int Hkv, int g, int T, int max_q, int max_kv,
@@ -48,26 +57,60 @@ static inline struct attn_paged_cut attn_paged_cut_of(int B, int Hkv, int g, int
     if (max_kv > 1 << 30) /* what a row of the table can hold */
         max_kv = 1 << 30;
     const int64_t rows = (int64_t)(max_q < T ? max_q : T) * g;
-    const int rows16 = rows <= 16 ? 1 : rows > 64 ? 8 : D <= 128 ? 2 : 1;
-    int64_t tps = (rows + 16 * rows16 - 1) / (16 * rows16);
+    const int rows16 = rows <= 16 ? 1 : rows > 64 ? 8 : D > 128 ? 1 : rows <= 32 ? 2 : 4;
     const int64_t seqs = (int64_t)B * Hkv;
-    if (tps * seqs > ATTN_PAGED_MAX_GRID) /* workgroups go on to further tiles */
-        tps = ATTN_PAGED_MAX_GRID / seqs > 1 ? ATTN_PAGED_MAX_GRID / seqs : 1;
-    const int64_t wgs = seqs * tps;
+    int64_t tps = (rows + 16 * rows16 - 1) / (16 * rows16);
+    if (tps * seqs > ATTN_PAGED_MAX_GRID / 16) /* workgroups go on to further tiles */
+        tps = ATTN_PAGED_MAX_GRID / 16 / seqs > 1 ? ATTN_PAGED_MAX_GRID / 16 / seqs : 1;
     const int64_t cap = ATTN_SLOTS / ((int64_t)T * Hkv * g);
-    const int64_t by_len = ((int64_t)max_kv + 127) / 128;
-    int64_t ns = (ATTN_DECODE_TARGET_WG + wgs - 1) / wgs;
-    if (ns > by_len)
-        ns = by_len;
-    if (ns > cap)
-        ns = cap;
-    if (ns > ATTN_PAGED_MAX_PARTS)
-        ns = ATTN_PAGED_MAX_PARTS;
-    if (ns < 2)
-        ns = 1;
-    int64_t kps = ((int64_t)max_kv + ns - 1) / ns;
-    kps = (kps + 127) / 128 * 128;
-    struct attn_paged_cut c = {rows16, (int)tps, (int)(((int64_t)max_kv + kps - 1) / kps), (int)kps};
+    const int64_t units = ((int64_t)max_kv + 127) / 128;
+    struct attn_paged_cut c = {rows16, (int)tps, 1, 0, 1, 1 << 30, 0, 0, 0, 0, 8};
+    int64_t likely = 1; /* parts of a sequence */
+    if (rows16 <= 2) {
+        int64_t teams = (ATTN_PAGED_DECODE_WG + tps - 1) / tps;
+        if (teams > seqs * units)
+            teams = seqs * units;
+        if (cap >= 2) {
+            c.teams = (int)teams;
+            const int64_t most = units + 1 > ATTN_PAGED_MAX_PARTS ? ATTN_PAGED_MAX_PARTS : units + 1;
+            c.nsplit = (int)(cap > most ? most : cap);
+            likely = teams / seqs + 1;
+        }
+        c.grid = (c.teams ? c.teams : seqs) * tps;
+    } else {
+        int64_t ns = (512 + seqs * tps - 1) / (seqs * tps);
+        ns = ns > units ? units : ns;
+        ns = ns > cap ? cap : ns;
+        ns = ns > ATTN_PAGED_MAX_PARTS ? ATTN_PAGED_MAX_PARTS : ns;
+        if (ns >= 2) {
+            c.nsplit = (int)ns;
+            c.share = (int)((((int64_t)max_kv + ns - 1) / ns + 127) / 128 * 128);
+        }
+        const int64_t groups = seqs * c.nsplit;
+        while (c.deal < 8 && c.deal < tps && groups < 64 && groups * c.deal % 8 != 0)
+            c.deal *= 2;
+        c.grid = attn_place_grid(groups, c.tps, c.deal);
+        likely = c.nsplit;
+    }
+    if (c.nsplit > 1) {
+        /* Lanes of four columns each; groups of parts until a thread has eight loads or fewer, or the
+         * workgroup is one row's. */
+        c.lglp = 3;
+        while ((4 << c.lglp) < D)
+            ++c.lglp;
+        while (c.lglp + c.lgsg < 8 && (8 << c.lgsg) < likely)
+            ++c.lgsg;
+        while (c.lglp + c.lgsg < 8 && (2 << c.lgsg) <= likely && seqs * rows << (c.lglp + c.lgsg) < 65536)
+            ++c.lgsg;
+        c.merge_loads = likely <= 3 << c.lgsg ? 2 : 8;
+        const int64_t rpw = 256 >> (c.lglp + c.lgsg);
+        if (c.nsplit > ATTN_PAGED_MERGE_WEIGHTS / rpw)
+            c.nsplit = (int)(ATTN_PAGED_MERGE_WEIGHTS / rpw);
+        int64_t tiles = (rows + rpw - 1) / rpw;
+        if (tiles * seqs > ATTN_PAGED_MAX_GRID)
+            tiles = ATTN_PAGED_MAX_GRID / seqs;
+        c.merge_tiles = (int)tiles;
+    }
     return c;
 }
 

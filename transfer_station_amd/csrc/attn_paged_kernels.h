@@ -63,17 +63,102 @@ __device__ __forceinline__ float score2(float s, float c, float cap_in, float ca
     return t - slope * (float)abs(dist);
 }
 
-// 16 keys of the cache from key kb (a multiple of 16): their rows' place, and how many of them there are
+__device__ __forceinline__ attn_seq seq_at(const attn_paged_args &a, int b) {
+    return attn_seq_of(scalar_i32(a.q_start, b), scalar_i32(a.q_start, b + 1), scalar_i32(a.kv_len, b), a.T,
+                       a.cols, a.lgp);
+}
+
+// Sum or maximum over the wave, in every lane.
+template <bool MAX> __device__ __forceinline__ int wave_all(int x) {
+    auto op = [](int p, int q) { return MAX ? max(p, q) : p + q; };
+    x = op(x, __builtin_amdgcn_update_dpp(x, x, 0x128, 0xf, 0xf, false)); // row_ror:8, 4, 2, 1
+    x = op(x, __builtin_amdgcn_update_dpp(x, x, 0x124, 0xf, 0xf, false));
+    x = op(x, __builtin_amdgcn_update_dpp(x, x, 0x122, 0xf, 0xf, false));
+    x = op(x, __builtin_amdgcn_update_dpp(x, x, 0x121, 0xf, 0xf, false));
+    const auto p = __builtin_amdgcn_permlane16_swap((unsigned)x, (unsigned)x, false, false);
+    x = op((int)p[0], (int)p[1]);
+    const auto r = __builtin_amdgcn_permlane32_swap((unsigned)x, (unsigned)x, false, false);
+    return op((int)r[0], (int)r[1]);
+}
+
+// x plus those of the lanes below (DPP row shifts, then the rows' last lanes broadcast to the rows behind).
+__device__ __forceinline__ int wave_scan(int x) {
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, true); // row_shr:1, 2, 4, 8
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, true);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, true);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, true);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false); // row_bcast:15 into rows 1 and 3
+    return x + __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false); // row_bcast:31 into rows 2 and 3
+}
+
+// The decode line (attn_quota) as a wave sees it, 64 sequences at a time: a kv head's units and the quota.
+// One sequence needs no sum, and up to 64 are read once.
+struct line {
+    int total, quota;
+    int n, sum; // of sequence `lane`: units, and units up to and with it
+};
+__device__ __forceinline__ int units_at(const attn_paged_args &a, int i) {
+    if (i >= a.B)
+        return 0;
+    const attn_seq s = attn_seq_of(a.q_start[i], a.q_start[i + 1], a.kv_len[i], a.T, a.cols, a.lgp);
+    return attn_units(s.n, s.kend);
+}
+__device__ __forceinline__ line line_at(const attn_paged_args &a, int lane) {
+    line l;
+    int most;
+    if (a.B == 1) {
+        const attn_seq s = seq_at(a, 0);
+        l.n = l.sum = l.total = most = attn_units(s.n, s.kend);
+    } else {
+        l.n = units_at(a, lane);
+        l.sum = wave_scan(l.n);
+        l.total = __builtin_amdgcn_readlane(l.sum, 63);
+        int m = l.n;
+        for (int i0 = 64; i0 < a.B; i0 += 64) {
+            const int n = units_at(a, i0 + lane);
+            m = max(m, n);
+            l.total += __builtin_amdgcn_readlane(wave_scan(n), 63);
+        }
+        most = uniform(wave_all<true>(m));
+    }
+    l.quota = uniform(attn_quota(l.total, most, a.Hkv, a.teams, a.nsplit));
+    return l;
+}
+// The sequence that unit `at` of a kv head's line belongs to, and the units before that.
+__device__ __forceinline__ int seq_of_unit(const attn_paged_args &a, const line &l, int lane, int at,
+                                           int &before) {
+    before = 0;
+    if (a.B == 1)
+        return 0;
+    int n = l.n, sum = l.sum, base = 0;
+    for (int i0 = 0;;) {
+        const uint64_t past = __builtin_amdgcn_ballot_w64(base + sum > at);
+        if (past != 0) {
+            const int k = __builtin_ctzll(past);
+            before = base + __builtin_amdgcn_readlane(sum - n, k);
+            return i0 + k;
+        }
+        base += __builtin_amdgcn_readlane(sum, 63);
+        i0 += 64;
+        if (i0 >= a.B) // not reached for a unit of the line
+            return 0;
+        n = units_at(a, i0 + lane);
+        sum = wave_scan(n);
+    }
+}
+
+// 16 keys of the cache from key kb (a multiple of 16; or N from a multiple of N): their rows' place, and how many of them there are
 // (0 where the page id is none, or past the sequence's end).
 struct kv_block {
     int64_t row;
     int n;
 };
+template <int N = 16>
 __device__ __forceinline__ kv_block block_at(const attn_paged_args &a, const int32_t *table, int u,
                                              int kb, int kend) {
     const int pg = scalar_i32(table, min(kb, kend - 1) >> a.lgp);
     const bool ok = attn_page_ok(pg, a.pages);
-    return kv_block{attn_page_row(ok ? pg : 0, a.Hkv, u, kb, a.lgp), ok ? max(0, min(16, kend - kb)) : 0};
+    return kv_block{attn_page_row(ok ? pg : 0, a.Hkv, u, kb, a.lgp), ok ? max(0, min(N, kend - kb)) : 0};
 }
 
 // b ? x : y of two values (of two array elements the operator itself would choose the address, and keep the
@@ -106,24 +191,46 @@ __global__ __launch_bounds__(256, 2) void attn_paged_decode_kernel(const attn_pa
     __shared__ float red_m[NRB][4][16], red_l[NRB][4][16];
     static_assert(4 * 16 * (DP + 4) * 4 <= 4 * VTILE * 2, "merge area must fit in the V tiles");
 
-    const int L = xcd_remap(wg_id_x(), a.B * a.Hkv * a.nsplit * a.tps);
-    const int t0 = L % a.tps, L1 = L / a.tps;
-    const int sp = L1 % a.nsplit, L2 = L1 / a.nsplit;
-    const int u = uniform(L2 % a.Hkv), b = uniform(L2 / a.Hkv);
-    const attn_seq sq = attn_seq_of(scalar_i32(a.q_start, b), scalar_i32(a.q_start, b + 1),
-                                    scalar_i32(a.kv_len, b), a.T, a.cols, a.lgp);
-    const int live = attn_live_parts(sq.kend, a.kps, a.nsplit);
-    if (sp >= live)
-        return;
-    const int k0 = attn_part_start(sq.kend, a.kps, sp), k1 = attn_part_end(sq.kend, a.kps, a.nsplit, sp);
-    const int32_t *table = a.table + (int64_t)b * a.cols;
     const int tid = wi_id_x(), w = uniform(tid >> 6), lane = tid & 63;
     const int r16 = lane & 15, grp = lane >> 4;
-    const int g = a.Hq / a.Hkv, R = sq.n * g, D = a.D;
+    const int g = a.Hq / a.Hkv, D = a.D;
     const float c = MOD ? 1.f : a.c;
+    const float lift = 8.f / c; // how far a score may pass the running maximum
+    // This workgroup's row tile t0 and its place on the line: sequence b, kv head u, first unit `off` of the
+    // sequence, `left` units in all. The workgroups of a team, and of neighbouring ones, share an XCD.
+    const int L = uniform(xcd_remap(wg_id_x(), (a.teams ? a.teams : a.B * a.Hkv) * a.tps));
+    const int team = uniform(L / a.tps), t0 = L - team * a.tps;
+    int u, b, off = 0, left = 1, pos0 = 0;
+    line ln = {0, 1, 0, 0};
+    if (a.teams) {
+        ln = line_at(a, lane);
+        if ((int64_t)team * ln.quota >= (int64_t)ln.total * a.Hkv)
+            return;
+        pos0 = team * ln.quota;
+        left = min(ln.quota, ln.total * a.Hkv - pos0);
+        u = uniform(pos0 / ln.total);
+        int before;
+        b = uniform(seq_of_unit(a, ln, lane, pos0 - u * ln.total, before));
+        off = pos0 - u * ln.total - before;
+    } else {
+        u = uniform(team / a.B);
+        b = team - u * a.B;
+    }
     uint16_t *vt = &Vw[w * VTILE];
 
-    for (int tile = t0; (int64_t)tile * 16 * NRB < R; tile += a.tps) {
+    while (left > 0 && u < a.Hkv) {
+    const attn_seq sq = seq_at(a, b);
+    const int units = attn_units(sq.n, sq.kend), R = sq.n * g;
+    const int take = a.teams ? min(left, units - off) : 1;
+    attn_cover cover = {0, 1};
+    if (a.teams) {
+        cover = attn_cover_of(pos0 - off, max(units, 1), ln.quota);
+        cover = attn_cover{uniform(cover.first), uniform(cover.live)};
+    }
+    const int live = cover.live, sp = team - cover.first;
+    const int k0 = min(off * 128, sq.kend), k1 = a.teams ? min((off + take) * 128, sq.kend) : sq.kend;
+    const int32_t *table = a.table + (int64_t)b * a.cols;
+    for (int tile = t0; take > 0 && (int64_t)tile * 16 * NRB < R; tile += a.tps) {
         const int row0 = tile * 16 * NRB;
         bf16x8 qb[NRB][KN];
         int lim[NRB], pos[NRB];
@@ -159,46 +266,25 @@ __global__ __launch_bounds__(256, 2) void attn_paged_decode_kernel(const attn_pa
             u32x4 k[F4 ? 1 : 2 * KN], v[F4 ? 1 : NV];
             uint32_t kw[F4 ? 2 * KN : 1], ksc[F4 ? 2 : 1];
             uint32_t vw[F4 ? NV4 * PB / 4 : 1], vsc[F4 ? NV4 : 1];
-            int n0, n1;
         };
-        // K and V of a tile, Q and O do not fit 256 registers at DP = 256 in bf16: V is loaded once the
-        // scores have freed K's.
+        // The loads of the next tile are issued as soon as this one's have been used: V's once it is in LDS,
+        // K's once the scores are there. K and V of a tile, Q and O do not fit 256 registers at DP = 256 in
+        // bf16: there a tile's K is loaded at its start, and V once the scores have freed K's registers.
         constexpr bool kLate = DP == 256 && !F4;
-        auto load_v16 = [&](const kv_block &b0, const kv_block &b1, frags &f)
-            __attribute__((always_inline)) {
-            const uint32_t rb = (uint32_t)D * 2u;
-            const auto vr0 = make_rsrc(a.v + b0.row * rb, b0.n * rb);
-            const auto vr1 = make_rsrc(a.v + b1.row * rb, b1.n * rb);
-            const uint32_t v0 = (lane % (DP / 8)) * 8 < D
-                                    ? (lane / (DP / 8)) * rb + (lane % (DP / 8)) * 16
-                                    : 0x80000000u;
+        auto load_k = [&](const kv_block &b0, const kv_block &b1, frags &f) __attribute__((always_inline)) {
 #pragma unroll
-            for (int r = 0; r < NV; ++r)
-                f.v[r] = buf16<NTL>(r < NV / 2 ? vr0 : vr1, v0 + (r % (NV / 2)) * (512 / DP) * rb);
-        };
-        auto load = [&](int tb, frags &f) __attribute__((always_inline)) {
-            const kv_block b0 = block_at(a, table, u, tb, k1), b1 = block_at(a, table, u, tb + 16, k1);
-            f.n0 = b0.n;
-            f.n1 = b1.n;
-            if constexpr (!F4) {
-                const uint32_t rb = (uint32_t)D * 2u; // bytes of a row
-                const auto kr0 = make_rsrc(a.k + b0.row * rb, b0.n * rb);
-                const auto kr1 = make_rsrc(a.k + b1.row * rb, b1.n * rb);
-#pragma unroll
-                for (int t = 0; t < 2; ++t)
+            for (int t = 0; t < 2; ++t) {
+                const kv_block &bl = t ? b1 : b0;
+                if constexpr (!F4) {
+                    const uint32_t rb = (uint32_t)D * 2u; // bytes of a row
+                    const auto kr = make_rsrc(a.k + bl.row * rb, bl.n * rb);
 #pragma unroll
                     for (int kk = 0; kk < KN; ++kk) {
                         const int col = kk * 32 + grp * 8;
-                        f.k[t * KN + kk] = buf16<NTL>(t ? kr1 : kr0,
-                                                     col < D ? r16 * rb + col * 2 : 0x80000000u);
+                        f.k[t * KN + kk] = buf16<NTL>(kr, col < D ? r16 * rb + col * 2 : 0x80000000u);
                     }
-                if (!kLate)
-                    load_v16(b0, b1, f);
-            } else {
-                constexpr int RB = DP / 2, SB = DP / 32; // bytes of a row's codes and scales
-#pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    const kv_block &bl = t ? b1 : b0;
+                } else {
+                    constexpr int RB = DP / 2, SB = DP / 32; // bytes of a row's codes and scales
                     const auto kr = make_rsrc(a.k + bl.row * RB, bl.n * RB);
                     const auto sr = make_rsrc(a.ks + bl.row * SB, bl.n * SB);
                     if constexpr (DP == 64) {
@@ -220,6 +306,21 @@ __global__ __launch_bounds__(256, 2) void attn_paged_decode_kernel(const attn_pa
                     else
                         f.ksc[t] = __builtin_amdgcn_raw_buffer_load_b8(sr, r16 * SB + grp * SB / 4, 0, 0);
                 }
+            }
+        };
+        auto load_v = [&](const kv_block &b0, const kv_block &b1, frags &f) __attribute__((always_inline)) {
+            if constexpr (!F4) {
+                const uint32_t rb = (uint32_t)D * 2u;
+                const auto vr0 = make_rsrc(a.v + b0.row * rb, b0.n * rb);
+                const auto vr1 = make_rsrc(a.v + b1.row * rb, b1.n * rb);
+                const uint32_t v0 = (lane % (DP / 8)) * 8 < D
+                                        ? (lane / (DP / 8)) * rb + (lane % (DP / 8)) * 16
+                                        : 0x80000000u;
+#pragma unroll
+                for (int r = 0; r < NV; ++r)
+                    f.v[r] = buf16<NTL>(r < NV / 2 ? vr0 : vr1, v0 + (r % (NV / 2)) * (512 / DP) * rb);
+            } else {
+                constexpr int RB = DP / 2, SB = DP / 32;
 #pragma unroll
                 for (int r = 0; r < NV4; ++r) {
                     const kv_block &bl = r < NV4 / 2 ? b0 : b1;
@@ -261,8 +362,10 @@ __global__ __launch_bounds__(256, 2) void attn_paged_decode_kernel(const attn_pa
                 }
             }
         };
-        auto compute = [&](int tb, frags &f) __attribute__((always_inline)) {
+        auto compute = [&](int tb, int tn, const kv_block &b0, const kv_block &b1, const kv_block &n0,
+                           const kv_block &n1, frags &f) __attribute__((always_inline)) {
             bf16x8 kf[2][KN], pk[NRB];
+            f32x4 s[NRB][2];
 #pragma unroll
             for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -275,19 +378,21 @@ __global__ __launch_bounds__(256, 2) void attn_paged_decode_kernel(const attn_pa
                         kf[t][kk] = as_bf16x8(f.k[t * KN + kk]);
                 }
 #pragma unroll
-            for (int i = 0; i < NRB; ++i) {
-                f32x4 s[2];
+            for (int i = 0; i < NRB; ++i)
 #pragma unroll
                 for (int t = 0; t < 2; ++t) {
-                    s[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+                    s[i][t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                     for (int kk = 0; kk < KN; ++kk)
-                        s[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[t][kk], qb[i][kk], s[t], 0, 0, 0);
+                        s[i][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[t][kk], qb[i][kk], s[i][t], 0, 0, 0);
                 }
-                if (kLate) { // NRB == 1
-                    __builtin_amdgcn_sched_barrier(0);
-                    load_v16(block_at(a, table, u, tb, k1), block_at(a, table, u, tb + 16, k1), f);
-                }
+            __builtin_amdgcn_sched_barrier(0);
+            if (kLate)
+                load_v(b0, b1, f);
+            else if (tn < kstop)
+                load_k(n0, n1, f);
+#pragma unroll
+            for (int i = 0; i < NRB; ++i) {
                 // Register (t, j) of this lane holds key tb + 16t + 4grp + j for row r16.
                 float mx = kNegInf;
 #pragma unroll
@@ -296,30 +401,32 @@ __global__ __launch_bounds__(256, 2) void attn_paged_decode_kernel(const attn_pa
                     for (int j = 0; j < 4; ++j) {
                         const int key = tb + 16 * t + 4 * grp + j;
                         if (MOD)
-                            s[t][j] = score2(s[t][j], a.c, a.cap_in, a.cap_out, slope[i], pos[i] - key);
-                        if (key > lim[i] || (t ? f.n1 : f.n0) == 0)
-                            s[t][j] = kNegInf;
-                        mx = fmaxf(mx, s[t][j]);
+                            s[i][t][j] = score2(s[i][t][j], a.c, a.cap_in, a.cap_out, slope[i], pos[i] - key);
+                        if (key > lim[i] || (t ? b1.n : b0.n) == 0)
+                            s[i][t][j] = kNegInf;
+                        mx = fmaxf(mx, s[i][t][j]);
                     }
                 mx = max_xor32(max_xor16(mx));
-                const float mnew = fmaxf(m_run[i], mx);
-                const float muse = mnew == kNegInf ? 0.f : mnew;
-                const float alpha = fast_exp2((m_run[i] - muse) * c);
-                const float mc = muse * c;
+                if (__builtin_amdgcn_ballot_w64(mx > m_run[i] + lift) != 0) {
+                    const float mnew = fmaxf(m_run[i], mx);
+                    const float alpha = fast_exp2((m_run[i] - (mnew == kNegInf ? 0.f : mnew)) * c);
+                    m_run[i] = mnew;
+                    l_run[i] *= alpha;
+#pragma unroll
+                    for (int db = 0; db < DP / 16; ++db)
+                        o[i][db] *= alpha;
+                }
+                const float mc = m_run[i] == kNegInf ? 0.f : m_run[i] * c;
                 float psum = 0.f;
 #pragma unroll
                 for (int t = 0; t < 2; ++t)
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        const float p = fast_exp2(fmaf(s[t][j], c, -mc));
+                        const float p = fast_exp2(fmaf(s[i][t][j], c, -mc));
                         psum += p;
                         pk[i][4 * t + j] = (__bf16)p;
                     }
-                l_run[i] = alpha * l_run[i] + psum;
-                m_run[i] = mnew;
-#pragma unroll
-                for (int db = 0; db < DP / 16; ++db)
-                    o[i][db] *= alpha;
+                l_run[i] += psum;
             }
             if (kLate)
                 put_v(f);
@@ -333,12 +440,42 @@ __global__ __launch_bounds__(256, 2) void attn_paged_decode_kernel(const attn_pa
                     o[i][db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, pk[i], o[i][db], 0, 0, 0);
             }
         };
-        for (int tb = k0 + 32 * w; tb < kstop; tb += 128) {
-            frags f;
-            load(tb, f);
-            if (!kLate)
-                put_v(f);
-            compute(tb, f);
+        // Tiles in flight per wave: one and a half ahead of the one at work, or, with 4-bit rows, which are
+        // short, two and a half.
+        constexpr int AHEAD = F4 ? 2 : 1;
+        int tb = k0 + 32 * w;
+        if (tb < kstop) {
+            frags f[AHEAD];
+            kv_block b0[AHEAD + 1], b1[AHEAD + 1];
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i) {
+                b0[i] = block_at(a, table, u, tb + 128 * i, k1);
+                b1[i] = block_at(a, table, u, tb + 128 * i + 16, k1);
+                if (!kLate && tb + 128 * i < kstop) {
+                    load_v(b0[i], b1[i], f[i]);
+                    load_k(b0[i], b1[i], f[i]);
+                }
+            }
+            for (; tb < kstop; tb += 128 * AHEAD)
+#pragma unroll
+                for (int i = 0; i < AHEAD; ++i) {
+                    const int t = tb + 128 * i, tn = t + 128 * AHEAD;
+                    if (i > 0 && t >= kstop)
+                        break;
+                    const kv_block n0 = block_at(a, table, u, tn, k1);
+                    const kv_block n1 = block_at(a, table, u, tn + 16, k1);
+                    if (kLate) {
+                        load_k(b0[i], b1[i], f[i]);
+                    } else {
+                        put_v(f[i]);
+                        __builtin_amdgcn_sched_barrier(0);
+                        if (tn < kstop)
+                            load_v(n0, n1, f[i]);
+                    }
+                    compute(t, tn, b0[i], b1[i], n0, n1, f[i]);
+                    b0[i] = n0;
+                    b1[i] = n1;
+                }
         }
 #pragma unroll
         for (int i = 0; i < NRB; ++i)
@@ -382,93 +519,152 @@ __global__ __launch_bounds__(256, 2) void attn_paged_decode_kernel(const attn_pa
                 }
                 const int64_t tok = sq.q0 + (rowb + r) / g;
                 const int h = u * g + (rowb + r) % g;
+                const int64_t slot = (tok * a.Hq + h) * a.nsplit;
                 if (live == 1) {
                     const float inv = lsum > 0.f ? 1.0f / lsum : 0.f;
                     *reinterpret_cast<u32x2 *>(a.o + tok * a.o_tok + h * a.o_head + d) =
                         u32x2{bf16_pair(acc[0] * inv, acc[1] * inv), bf16_pair(acc[2] * inv, acc[3] * inv)};
+                    if (d == 0 && a.nsplit > 1)
+                        a.pm[slot] = -kNegInf; // the row is written
                 } else {
-                    const int64_t slot = (tok * a.Hq + h) * a.nsplit + sp;
                     if (d == 0) {
-                        a.pm[slot] = mx;
-                        a.pl[slot] = lsum;
+                        a.pm[slot + sp] = mx;
+                        a.pl[slot + sp] = lsum;
                     }
-                    *reinterpret_cast<f32x4 *>(a.pacc + slot * D + d) = acc;
+                    *reinterpret_cast<f32x4 *>(a.pacc + (slot + sp) * D + d) = acc;
+                    if (sp == live - 1) // no parts behind the last
+                        for (int s = live + d / 4; s < a.nsplit; s += D / 4)
+                            a.pm[slot + s] = kNegInf;
                 }
             }
         }
         __syncthreads(); // the merge area is V tiles again
     }
+    left -= take;
+    pos0 += take;
+    off = 0;
+    if (++b == a.B) {
+        b = 0;
+        ++u;
+    }
+    }
 }
 
 // Joins the parts of each row: w_s = 2^(m_s - max m), O = sum w_s acc_s / sum w_s l_s. A workgroup takes
-// 256 / (LP SG) rows of one sequence at a time: LP lanes of four columns each, SG groups of parts. Rows
-// of sequences that one part covers were written by the attention kernel.
+// 256 / (LP SG) rows of one sequence and kv head at a time: LP lanes of four columns each, SG groups of
+// parts, NL loads of each thread on their way before the weights are known. The attention kernel says what
+// a row has: +inf as the first m where it wrote the row itself, -inf behind the last part (whose acc is
+// whatever it was: it gets no weight and is not multiplied). What bounds it is latency: the maxima, sums
+// and columns of a row are all asked for at once, right behind the sequence's start.
 constexpr int kPagedMaxSplit = ATTN_PAGED_MAX_PARTS;
-__global__ __launch_bounds__(256) void attn_paged_merge_kernel(const attn_paged_args a, int lglp,
-                                                               int lgsg, int tpm) {
-    __shared__ float wsh[kPagedMaxSplit]; // rows x parts: the launcher takes more than one row below 128
+template <int NL>
+__global__ __launch_bounds__(256) void attn_paged_merge_kernel(const attn_paged_args a, int lglp, int lgsg,
+                                                               int tpm) {
+    __shared__ float wsh[ATTN_PAGED_MERGE_WEIGHTS]; // [rows][parts]
+    __shared__ int nsh[32];                         // parts of each row; -1: written already
     __shared__ __attribute__((aligned(16))) f32x4 red[256];
-    const int b = uniform(wg_id_x() / tpm), t0 = wg_id_x() % tpm;
-    const attn_seq sq = attn_seq_of(scalar_i32(a.q_start, b), scalar_i32(a.q_start, b + 1),
-                                    scalar_i32(a.kv_len, b), a.T, a.cols, a.lgp);
-    const int live = attn_live_parts(sq.kend, a.kps, a.nsplit);
-    if (live == 1)
-        return;
-    const int tid = wi_id_x(), lane = tid & 63, w = tid >> 6;
-    const int rpw = 256 >> (lglp + lgsg), R = sq.n * a.Hq;
+    const int bu = uniform(wg_id_x() / tpm), t0 = wg_id_x() - bu * tpm;
+    const int b = uniform(bu / a.Hkv), u = bu - b * a.Hkv;
+    const int tid = wi_id_x(), lane = tid & 63;
+    const attn_seq sq = seq_at(a, b);
+    const int g = a.Hq / a.Hkv, rpw = 256 >> (lglp + lgsg), R = sq.n * g;
+    auto slot_of = [&](int r) { // the first partial of row r
+        return ((int64_t)(sq.q0 + r / g) * a.Hq + u * g + r % g) * a.nsplit;
+    };
     const int rl = tid >> (lglp + lgsg), sg = (tid >> lglp) & ((1 << lgsg) - 1);
     const int d = 4 * (tid & ((1 << lglp) - 1));
     for (int r0 = t0 * rpw; r0 < R; r0 += tpm * rpw) {
-        for (int r = w; r < rpw; r += 4) {
-            const int64_t slot = ((int64_t)sq.q0 * a.Hq + min(r0 + r, R - 1)) * a.nsplit;
-            float m[kPagedMaxSplit / 64], l[kPagedMaxSplit / 64], mx = kNegInf;
-#pragma unroll
-            for (int i = 0; i < kPagedMaxSplit / 64; ++i) {
-                const int s = lane + 64 * i;
-                m[i] = s < live ? a.pm[slot + s] : kNegInf;
-                l[i] = s < live ? a.pl[slot + s] : 0.f;
-                mx = fmaxf(mx, m[i]);
-            }
-            mx = seg_all<true>(mx, true);
-            const float muse = mx == kNegInf ? 0.f : mx;
-            float sum = 0.f;
-#pragma unroll
-            for (int i = 0; i < kPagedMaxSplit / 64; ++i) {
-                m[i] = fast_exp2(m[i] - muse);
-                sum += m[i] * l[i];
-            }
-            sum = seg_all<false>(sum, true);
-            const float inv = sum > 0.f ? 1.0f / sum : 0.f;
-#pragma unroll
-            for (int i = 0; i < kPagedMaxSplit / 64; ++i)
-                if (lane + 64 * i < live)
-                    wsh[r * a.nsplit + lane + 64 * i] = m[i] * inv;
-        }
-        __syncthreads();
-        f32x4 acc = {0.f, 0.f, 0.f, 0.f};
         const int row = r0 + rl;
-        if (row < R && d < a.D) {
-            const float *p = a.pacc + ((int64_t)sq.q0 * a.Hq + row) * a.nsplit * a.D + d;
-#pragma unroll 8
-            for (int s = sg; s < live; s += 1 << lgsg) {
-                const f32x4 x = *reinterpret_cast<const f32x4 *>(p + (int64_t)s * a.D);
-                const float wgt = wsh[rl * a.nsplit + s];
+        const float *p = a.pacc + slot_of(min(row, R - 1)) * a.D + min(d, a.D - 4);
+        f32x4 x[NL];
+        auto load = [&](int s0) __attribute__((always_inline)) {
+#pragma unroll
+            for (int i = 0; i < NL; ++i)
+                x[i] = *reinterpret_cast<const f32x4 *>(
+                    p + (int64_t)min(s0 + sg + (i << lgsg), a.nsplit - 1) * a.D);
+        };
+        load(0);
+        // Weights: 16 lanes per row up to 16 parts, else a wave per row, which has NI parts per lane.
+        auto weights = [&](auto N, bool all) __attribute__((always_inline)) {
+            constexpr int NI = decltype(N)::value;
+            const int lgs = all ? 6 : 4, sl = lane & ((1 << lgs) - 1);
+            for (int r = tid >> lgs; r < rpw; r += 256 >> lgs) {
+                const int64_t slot = slot_of(min(r0 + r, R - 1));
+                float m[NI], l[NI], mx = kNegInf;
+                int last = 0;
+#pragma unroll
+                for (int i = 0; i < NI; ++i) {
+                    const int s = min(sl + 64 * i, a.nsplit - 1);
+                    m[i] = a.pm[slot + s];
+                    l[i] = a.pl[slot + s];
+                }
+                const float first = __builtin_bit_cast(
+                    float, __builtin_amdgcn_ds_bpermute((lane & ~((1 << lgs) - 1)) * 4,
+                                                        __builtin_bit_cast(int, m[0])));
+#pragma unroll
+                for (int i = 0; i < NI; ++i) {
+                    if (sl + 64 * i >= a.nsplit)
+                        m[i] = kNegInf;
+                    if (m[i] > kNegInf)
+                        last = sl + 64 * i + 1;
+                    mx = fmaxf(mx, m[i]);
+                }
+                mx = seg_all<true>(mx, all);
+                const float fl = seg_all<true>((float)last, all);
+                const float muse = mx == kNegInf ? 0.f : mx;
+                float sum = 0.f;
+#pragma unroll
+                for (int i = 0; i < NI; ++i) {
+                    const bool none = m[i] == kNegInf;
+                    m[i] = none ? 0.f : fast_exp2(m[i] - muse);
+                    sum += none ? 0.f : m[i] * l[i];
+                }
+                sum = seg_all<false>(sum, all);
+                const float inv = sum > 0.f ? 1.0f / sum : 0.f;
+#pragma unroll
+                for (int i = 0; i < NI; ++i)
+                    if (sl + 64 * i < a.nsplit)
+                        wsh[r * a.nsplit + sl + 64 * i] = m[i] * inv;
+                if (sl == 0)
+                    nsh[r] = first == -kNegInf ? -1 : (int)fl;
+            }
+        };
+        if (a.nsplit <= 16)
+            weights(std::integral_constant<int, 1>{}, false);
+        else if (a.nsplit <= 64)
+            weights(std::integral_constant<int, 1>{}, true);
+        else
+            weights(std::integral_constant<int, kPagedMaxSplit / 64>{}, true);
+        __syncthreads();
+        const int parts = nsh[rl];
+        f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+        for (int s0 = 0;;) {
+#pragma unroll
+            for (int i = 0; i < NL; ++i) {
+                const int s = s0 + sg + (i << lgsg);
+                const float wgt = s < parts ? wsh[rl * a.nsplit + s] : 0.f;
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
-                    acc[j] += wgt * x[j];
+                    acc[j] += s < parts ? wgt * x[i][j] : 0.f;
             }
+            s0 += NL << lgsg;
+            if (s0 >= parts)
+                break;
+            load(s0);
         }
-        red[tid] = acc;
-        __syncthreads();
-        if (sg == 0 && row < R && d < a.D) {
+        if (lgsg > 0) {
+            red[tid] = acc;
+            __syncthreads();
+        }
+        if (sg == 0 && row < R && d < a.D && parts >= 0) {
             for (int k = 1; k < 1 << lgsg; ++k) {
                 const f32x4 y = red[tid + (k << lglp)];
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
                     acc[j] += y[j];
             }
-            const int64_t tok = sq.q0 + row / a.Hq;
-            *reinterpret_cast<u32x2 *>(a.o + tok * a.o_tok + row % a.Hq * a.o_head + d) =
+            *reinterpret_cast<u32x2 *>(a.o + (int64_t)(sq.q0 + row / g) * a.o_tok +
+                                       (u * g + row % g) * a.o_head + d) =
                 u32x2{bf16_pair(acc[0], acc[1]), bf16_pair(acc[2], acc[3])};
         }
         __syncthreads();
@@ -476,152 +672,156 @@ __global__ __launch_bounds__(256) void attn_paged_merge_kernel(const attn_paged_
 }
 
 // ------------------------------------------------------------------------------------------
-// Many query rows per kv head. One workgroup of four waves per (sequence, kv head, part, tile of 128
-// rows), 32 rows per wave; tiles of 64 keys, staged in LDS by the four waves (16 keys each) through
-// registers while the tile before is computed:
+// Many query rows per kv head. One workgroup of four waves per (sequence, kv head, part, tile of 128 rows, or
+// 64 with KH = 2), tiles of KT keys staged in LDS, two of them: the next one's loads run beside this one's
 //   S^T[key][row] = K . Q^T, O^T[d][row] += V^T . P^T   (v_mfma_f32_32x32x16_bf16)
-// with the LDS layouts of attn_prefill_fast_kernel. The running maximum is raised only where a tile's
-// is more than 2^8 above it, so that O is rarely rescaled: p stays below 2^8.
+// with the LDS layouts of attn_prefill_fast_kernel. KH = 1: a wave takes 32 rows and all keys of a tile;
+// KH = 2: waves w and w + 2 take the same 32 rows and a half of each tile, joined through LDS at the end.
+//   * bf16: LDS-DMA, a wave KT / 4 keys of each tile, block by block of 16 (or 8) with a descriptor each.
+//   * 4 bits: a lane loads 32 codes of a row and their scale a tile and a half ahead, and puts them into LDS
+//     as bf16 at the end of the tile before.
+// The running maximum is raised only where a tile's is more than 2^8 above it, so that O is rarely rescaled;
+// p stays below 2^8.
 // ------------------------------------------------------------------------------------------
-template <int DP, bool F4, bool MOD>
-__global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_paged_prefill_kernel(
-    const attn_paged_args a) {
-    constexpr int KT = 64, KN = DP / 16, PW = DP / 32; // PW: 16-byte pieces of a bf16 tile per lane
-    constexpr int KW = DP / 32, NSC = DP == 256 ? 2 : 1; // 4 bits: words and scales per lane
-    __shared__ __attribute__((aligned(1024))) uint16_t Ks[2][KT * DP];
-    __shared__ __attribute__((aligned(1024))) uint16_t Vs[2][KT * DP];
+constexpr int paged_tile_keys(int DP, bool F4) { return DP == 64 ? (F4 ? 64 : 128) : DP == 128 ? 64 : 32; }
 
-    const int L = xcd_remap(wg_id_x(), a.B * a.Hkv * a.nsplit * a.tps);
-    const int L1 = L / a.tps, t0 = a.tps - 1 - L % a.tps; // heaviest first
-    const int sp = L1 % a.nsplit, L2 = L1 / a.nsplit;
-    const int u = uniform(L2 % a.Hkv), b = uniform(L2 / a.Hkv);
-    const attn_seq sq = attn_seq_of(scalar_i32(a.q_start, b), scalar_i32(a.q_start, b + 1),
-                                    scalar_i32(a.kv_len, b), a.T, a.cols, a.lgp);
-    const int live = attn_live_parts(sq.kend, a.kps, a.nsplit);
+template <int DP, bool F4, bool MOD, int KH>
+__global__ __launch_bounds__(256, 2) void attn_paged_prefill_kernel(const attn_paged_args a) {
+    constexpr int KT = paged_tile_keys(DP, F4), KN = DP / 16, RWV = KT / 4; // rows a wave stages
+    constexpr int PW = KT * DP / 2048;                    // 1 KB blocks of a bf16 tile per wave
+    constexpr int NBK = RWV <= 16 ? 1 : RWV / 16;         // blocks of 16 keys per wave
+    constexpr int NR = 4 / KH, BQ = 32 * NR, KW = KT / KH, NT = KW / 32; // rows, keys of a wave
+    constexpr int LB = RWV * DP / 2 / 64; // 4 bits: bytes of codes per lane (16, or 8 at DP = 64)
+    static_assert(NT >= 1 && PW % NBK == 0 && (!F4 || (NBK == 1 && LB * 2 % 16 == 0)), "tile shape");
+    // Each buffer is a variable of its own: the compiler tells LDS accesses apart by variable.
+    __shared__ __attribute__((aligned(1024))) uint16_t Ks0[KT * DP], Ks1[KT * DP];
+    __shared__ __attribute__((aligned(1024))) uint16_t Vs0[KT * DP], Vs1[KT * DP];
+    __shared__ float kh_ml[KH > 1 ? 2 * NR * 64 : 1];
+
+    const attn_place at = attn_place_of(wg_id_x(), a.B * a.Hkv * a.nsplit, a.tps, a.deal);
+    if (at.group < 0)
+        return;
+    const int t0 = uniform(a.tps - 1 - at.tile); // heaviest first
+    const int sp = uniform(at.group / (a.B * a.Hkv)), bu = at.group - sp * (a.B * a.Hkv);
+    const int u = uniform(bu % a.Hkv), b = uniform(bu / a.Hkv);
+    const int tid = wi_id_x(), w = uniform(tid >> 6), lane = tid & 63;
+    const attn_seq sq = seq_at(a, b);
+    // The divisions run on the vector unit: back into scalar registers, with all that follows from them.
+    const attn_parts parts = attn_parts_of(sq.kend, a.share, a.nsplit);
+    const int live = uniform(parts.live), kps = uniform(parts.kps);
     if (sp >= live)
         return;
-    const int k0 = attn_part_start(sq.kend, a.kps, sp), k1 = attn_part_end(sq.kend, a.kps, a.nsplit, sp);
+    const int k0 = attn_part_start(sq.kend, kps, sp), k1 = attn_part_start(sq.kend, kps, sp + 1);
     const int32_t *table = a.table + (int64_t)b * a.cols;
-    const int tid = wi_id_x(), w = uniform(tid >> 6), lane = tid & 63;
     const int l32 = lane & 31, hi = lane >> 5, g16 = lane >> 4, i16 = lane & 15;
+    const int wr = KH > 1 ? w % NR : w, kh = KH > 1 ? w / NR : 0;
     const int g = a.Hq / a.Hkv, R = sq.n * g, D = a.D;
     const float c = MOD ? 1.f : a.c;
     const float lift = 8.f / c; // how far a score may pass the running maximum
 
     // Offsets of this lane's operand reads (elements): K row kperm, chunk 2kk + hi; V rows 8hi + i16 / 4
-    // (+ 4), columns 16 (g16 & 1) + 4 (i16 & 3).
+    // (+ 4), columns 16 (g16 & 1) + 4 (i16 & 3); and the wave's keys of the tile.
     const int kperm = (l32 & ~12) | ((l32 & 4) << 1) | ((l32 & 8) >> 1);
-    const int kfo = (kperm >> 3) * 8 * DP + (kperm & 7) * 16 + ((hi ^ ((kperm >> 3) & 1)) * 8);
-    const int vfo = hi * 8 * DP + (i16 >> 2) * 32 + (2 * (g16 & 1) + ((i16 & 3) >> 1)) * 8 + (i16 & 1) * 4;
+    const int kfo = (kperm >> 3) * 8 * DP + (kperm & 7) * 16 + ((hi ^ ((kperm >> 3) & 1)) * 8) + kh * KW * DP;
+    const int vfo = hi * 8 * DP + (i16 >> 2) * 32 + (2 * (g16 & 1) + ((i16 & 3) >> 1)) * 8 + (i16 & 1) * 4 +
+                    kh * KW * DP;
 
-    // Staging: bf16 pieces in the order of the LDS layouts, byte (w PW + p) 1024 + 16 lane of the tile.
+    // bf16: byte (w PW + p) 1024 + 16 lane of the tile's layout is row kr of the wave's rows.
     uint32_t kso[PW], vso[PW];
+    if constexpr (!F4)
 #pragma unroll
-    for (int p = 0; p < PW; ++p) {
-        const int x = (w * PW + p) * 1024 + 16 * lane;
-        const int kg = x / (16 * DP), kw = x % (16 * DP);
-        const int kr = kg * 8 + (kw % 256) / 32 - 16 * w;
-        const int kc = 2 * (kw / 256) + (((kw % 32) / 16) ^ (kg & 1));
-        kso[p] = kc * 8 < D ? (uint32_t)(kr * D * 2 + kc * 16) : 0x80000000u;
-        const int vg = x / (8 * DP), vw = x % (8 * DP);
-        const int vr = vg * 4 + (vw % 256) / 64 - 16 * w;
-        const int vc = 4 * (vw / 256) + (vw % 64) / 16;
-        vso[p] = vc * 8 < D ? (uint32_t)(vr * D * 2 + vc * 16) : 0x80000000u;
-    }
+        for (int p = 0; p < PW; ++p) {
+            const int x = (w * PW + p) * 1024 + 16 * lane;
+            const int kg = x / (16 * DP), kw = x % (16 * DP);
+            const int kr = kg * 8 + (kw % 256) / 32 - RWV * w;
+            const int kc = 2 * (kw / 256) + (((kw % 32) / 16) ^ (kg & 1));
+            kso[p] = kc * 8 < D ? (uint32_t)((kr & 15) * D * 2 + kc * 16) : 0x80000000u;
+            const int vg = x / (8 * DP), vw = x % (8 * DP);
+            const int vr = vg * 4 + (vw % 256) / 64 - RWV * w;
+            const int vc = 4 * (vw / 256) + (vw % 64) / 16;
+            vso[p] = vc * 8 < D ? (uint32_t)((vr & 15) * D * 2 + vc * 16) : 0x80000000u;
+        }
+    // Row and group of 32 (DP = 64: 16) codes that this lane loads of a 4-bit tile.
+    const int srow = lane % RWV, sgrp = lane / RWV;
     struct stage {
-        u32x4 k[F4 ? 1 : PW], v[F4 ? 1 : PW];
-        uint32_t kw[F4 ? KW : 1], vw[F4 ? KW : 1], ksc, vsc;
-        bool whole; // every block of the tile has a page
+        uint32_t k[F4 ? LB / 4 : 1], v[F4 ? LB / 4 : 1], ks, vs;
     };
-    auto load = [&](int kb, stage &f) __attribute__((always_inline)) {
-        const kv_block m = block_at(a, table, u, kb + 16 * w, k1);
-        f.whole = kb + KT <= k1;
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            f.whole &= attn_page_ok(scalar_i32(table, min(kb + 16 * j, k1 - 1) >> a.lgp), a.pages) != 0;
+    constexpr int RB = DP / 2, SB = DP / 32; // bytes of a row's codes and scales
+    // The wave's rows of the tile from key kb: into LDS, or (4 bits) into registers.
+    auto load = [&](int kb, [[maybe_unused]] uint16_t *Kd, [[maybe_unused]] uint16_t *Vd,
+                    [[maybe_unused]] stage &f) __attribute__((always_inline)) {
         if constexpr (!F4) {
             const uint32_t rb = (uint32_t)D * 2u;
-            const auto kr = make_rsrc(a.k + m.row * rb, m.n * rb);
-            const auto vr = make_rsrc(a.v + m.row * rb, m.n * rb);
 #pragma unroll
-            for (int p = 0; p < PW; ++p)
-                f.k[p] = buf16<false>(kr, kso[p]);
+            for (int h = 0; h < NBK; ++h) {
+                const kv_block m = block_at<(RWV < 16 ? RWV : 16)>(a, table, u, kb + RWV * w + 16 * h, k1);
+                const auto kr = make_rsrc(a.k + m.row * rb, m.n * rb);
+                const auto vr = make_rsrc(a.v + m.row * rb, m.n * rb);
 #pragma unroll
-            for (int p = 0; p < PW; ++p)
-                f.v[p] = buf16<false>(vr, vso[p]);
+                for (int p = h * PW / NBK; p < (h + 1) * PW / NBK; ++p)
+                    dma16<0>(kr, Kd + (w * PW + p) * 512, kso[p]);
+#pragma unroll
+                for (int p = h * PW / NBK; p < (h + 1) * PW / NBK; ++p)
+                    dma16<0>(vr, Vd + (w * PW + p) * 512, vso[p]);
+            }
         } else {
-            constexpr int RB = DP / 2, SB = DP / 32;
-            const auto kr = make_rsrc(a.k + m.row * RB, m.n * RB);
-            const auto vr = make_rsrc(a.v + m.row * RB, m.n * RB);
+            const kv_block m = block_at<(RWV < 16 ? RWV : 16)>(a, table, u, kb + RWV * w, k1);
+            const auto kr = make_rsrc(a.k + m.row * RB, m.n * RB), vr = make_rsrc(a.v + m.row * RB, m.n * RB);
             const auto ksr = make_rsrc(a.ks + m.row * SB, m.n * SB);
             const auto vsr = make_rsrc(a.vs + m.row * SB, m.n * SB);
-            const uint32_t off = i16 * RB + g16 * (RB / 4);
-            if constexpr (DP == 64) {
+            const uint32_t off = srow * RB + sgrp * LB, soff = srow * SB + sgrp * LB / 16;
+            if constexpr (LB == 8) {
                 const u32x2 x = __builtin_amdgcn_raw_buffer_load_b64(kr, off, 0, 0);
                 const u32x2 y = __builtin_amdgcn_raw_buffer_load_b64(vr, off, 0, 0);
-                f.kw[0] = x[0], f.kw[1] = x[1], f.vw[0] = y[0], f.vw[1] = y[1];
+                f.k[0] = x[0], f.k[1] = x[1], f.v[0] = y[0], f.v[1] = y[1];
             } else {
+                const u32x4 x = buf16<false>(kr, off), y = buf16<false>(vr, off);
 #pragma unroll
-                for (int j = 0; j < KW / 4; ++j) {
-                    const u32x4 x = buf16<false>(kr, off + 16 * j), y = buf16<false>(vr, off + 16 * j);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        f.kw[4 * j + i] = x[i], f.vw[4 * j + i] = y[i];
-                }
+                for (int i = 0; i < 4; ++i)
+                    f.k[i] = x[i], f.v[i] = y[i];
             }
-            if constexpr (NSC == 2) {
-                f.ksc = __builtin_amdgcn_raw_buffer_load_b16(ksr, i16 * SB + g16 * 2, 0, 0);
-                f.vsc = __builtin_amdgcn_raw_buffer_load_b16(vsr, i16 * SB + g16 * 2, 0, 0);
-            } else {
-                f.ksc = __builtin_amdgcn_raw_buffer_load_b8(ksr, i16 * SB + g16 * SB / 4, 0, 0);
-                f.vsc = __builtin_amdgcn_raw_buffer_load_b8(vsr, i16 * SB + g16 * SB / 4, 0, 0);
-            }
+            f.ks = __builtin_amdgcn_raw_buffer_load_b8(ksr, soff, 0, 0);
+            f.vs = __builtin_amdgcn_raw_buffer_load_b8(vsr, soff, 0, 0);
         }
     };
-    auto put = [&](const stage &f, int buf) __attribute__((always_inline)) {
-        if constexpr (!F4) {
+    // 4 bits: the lane's chunks of eight elements into the tile's layouts. K: the rows of a 16-lane pass hit
+    // other banks. V: rows four apart would not, so each starts at another of its chunks.
+    auto put = [&](const stage &f, uint16_t *Kd, uint16_t *Vd) __attribute__((always_inline)) {
+        constexpr int NC = LB / 4;
+        const int r = RWV * w + srow, c0 = sgrp * NC;
+        const float ksc = e8m0(f.ks), vsc = e8m0(f.vs);
 #pragma unroll
-            for (int p = 0; p < PW; ++p)
-                *reinterpret_cast<u32x4 *>(&Ks[buf][(w * PW + p) * 512 + lane * 8]) = f.k[p];
-#pragma unroll
-            for (int p = 0; p < PW; ++p)
-                *reinterpret_cast<u32x4 *>(&Vs[buf][(w * PW + p) * 512 + lane * 8]) = f.v[p];
-        } else {
-            // Row r of the tile, chunks of eight elements from c0 on. K: the 16 rows of a pass hit other
-            // banks. V: rows four apart would not, so each starts at another of its chunks.
-            const int r = 16 * w + i16, c0 = g16 * KW;
-#pragma unroll
-            for (int j = 0; j < KW; ++j) {
-                const int cc = c0 + j;
-                *reinterpret_cast<u32x4 *>(&Ks[buf][(r >> 3) * 8 * DP + (cc >> 1) * 128 + (r & 7) * 16 +
-                                                    ((cc & 1) ^ ((r >> 3) & 1)) * 8]) =
-                    fp4_to_bf16(f.kw[j], e8m0(NSC == 2 ? (f.ksc >> (j / 4 * 8)) & 0xff : f.ksc));
-            }
-            constexpr int RW = KW < 4 ? KW : 4;
-            const int rot = (i16 >> 2) & (RW - 1);
-#pragma unroll
-            for (int j0 = 0; j0 < KW; j0 += RW) {
-                const float sc = e8m0(NSC == 2 ? (f.vsc >> (j0 / 4 * 8)) & 0xff : f.vsc);
-                uint32_t x[RW], y[RW];
-#pragma unroll
-                for (int j = 0; j < RW; ++j)
-                    x[j] = pick(rot & 1, f.vw[j0 + (j + 1) % RW], f.vw[j0 + j]);
-#pragma unroll
-                for (int j = 0; j < RW; ++j)
-                    y[j] = pick(rot & 2, x[(j + 2) % RW], x[j]);
-#pragma unroll
-                for (int j = 0; j < RW; ++j) {
-                    const int cc = c0 + j0 + ((j + rot) & (RW - 1));
-                    *reinterpret_cast<u32x4 *>(&Vs[buf][(r >> 2) * 4 * DP + (cc >> 2) * 128 +
-                                                        (r & 3) * 32 + (cc & 3) * 8]) =
-                        fp4_to_bf16(y[j], sc);
-                }
-            }
+        for (int j = 0; j < NC; ++j) {
+            const int cc = c0 + j;
+            *reinterpret_cast<u32x4 *>(&Kd[(r >> 3) * 8 * DP + (cc >> 1) * 128 + (r & 7) * 16 +
+                                           ((cc & 1) ^ ((r >> 3) & 1)) * 8]) = fp4_to_bf16(f.k[j], ksc);
         }
+        const int rot = (srow >> 2) & (NC - 1);
+        uint32_t x[NC], y[NC];
+#pragma unroll
+        for (int j = 0; j < NC; ++j)
+            x[j] = pick(rot & 1, f.v[(j + 1) % NC], f.v[j]);
+#pragma unroll
+        for (int j = 0; j < NC; ++j)
+            y[j] = pick(rot & 2, x[(j + 2) % NC], x[j]);
+#pragma unroll
+        for (int j = 0; j < NC; ++j) {
+            const int cc = c0 + ((j + rot) & (NC - 1));
+            *reinterpret_cast<u32x4 *>(&Vd[(r >> 2) * 4 * DP + (cc >> 2) * 128 + (r & 3) * 32 + (cc & 3) * 8]) =
+                fp4_to_bf16(y[j], vsc);
+        }
+    };
+    // Every 16 keys of the tile from kb have a page, and the part reaches past them.
+    auto whole = [&](int kb) __attribute__((always_inline)) {
+        bool ok = kb + KT <= k1;
+#pragma unroll
+        for (int j = 0; j < KT; j += 16)
+            ok &= attn_page_ok(scalar_i32(table, min(kb + j, k1 - 1) >> a.lgp), a.pages) != 0;
+        return ok;
     };
 
-    for (int tile = t0; (int64_t)tile * 128 < R; tile += a.tps) {
-        const int row0 = tile * 128, row = row0 + 32 * w + l32;
+    for (int tile = t0; (int64_t)tile * BQ < R; tile += a.tps) {
+        const int row0 = tile * BQ, row = row0 + 32 * wr + l32;
         const bool valid = row < R;
         const int tok = valid ? row / g : 0, h = u * g + (valid ? row % g : 0);
         const uint16_t *q = a.q + (sq.q0 + tok) * a.q_tok + h * a.q_head;
@@ -638,10 +838,10 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_paged_prefill_ker
         const int pos = p0 + tok, lim = a.causal ? min(pos, k1 - 1) : k1 - 1;
         const float slope = MOD && a.slopes ? a.slopes[h] * 1.44269504088896341f : 0.f;
         // The wave's smallest and largest limits, and where the workgroup's tiles end.
-        const int wfirst = row0 + 32 * w, wlast = min(wfirst + 31, R - 1);
+        const int wfirst = row0 + 32 * wr, wlast = min(wfirst + 31, R - 1);
         const int wmin = uniform(a.causal ? min(p0 + min(wfirst, R - 1) / g, k1 - 1) : k1 - 1);
         const int wmax = uniform(wfirst >= R ? -1 : a.causal ? min(p0 + wlast / g, k1 - 1) : k1 - 1);
-        const int kstop = uniform(a.causal ? min(k1, p0 + min(row0 + 127, R - 1) / g + 1) : k1);
+        const int kstop = uniform(a.causal ? min(k1, p0 + min(row0 + BQ - 1, R - 1) / g + 1) : k1);
 
         float m_run = kNegInf, l_run = 0.f;
         f32x16 o[DP / 32];
@@ -651,107 +851,180 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_paged_prefill_ker
             for (int i = 0; i < 16; ++i)
                 o[db][i] = 0.f;
 
-        stage st;
-        bool whole = true;
-        if (k0 < kstop) {
-            load(k0, st);
-            whole = st.whole;
-            put(st, 0);
-        }
-        __syncthreads();
-        int buf = 0;
-        for (int kb = k0; kb < kstop; kb += KT, buf ^= 1) {
-            const bool more = kb + KT < kstop;
-            if (more)
-                load(kb + KT, st);
-            if (kb <= wmax) {
-                f32x16 s[2];
-                const uint16_t *kp = &Ks[buf][kfo];
+        // One tile from key kb, in the buffers Kb and Vb.
+        auto compute = [&](int kb, bool all, const uint16_t *Kb, const uint16_t *Vb)
+            __attribute__((always_inline)) {
+            const int kw = kb + kh * KW; // the wave's first key
+            if (kw > wmax)
+                return;
+            f32x16 s[NT];
+            bf16x8 ka[2][KN];
+            const uint16_t *kp = Kb + kfo;
 #pragma unroll
-                for (int t = 0; t < 2; ++t) {
+            for (int kk = 0; kk < KN; ++kk)
+                ka[0][kk] = as_bf16x8(*reinterpret_cast<const u32x4 *>(kp + kk * 128));
+            __builtin_amdgcn_sched_group_barrier(0x100, KN, 0);
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    s[t][i] = 0.f;
+#pragma unroll
+                for (int kk = 0; kk < KN; ++kk) {
+                    s[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ka[t & 1][kk], qb[kk], s[t], 0, 0, 0);
+                    if (t + 1 < NT)
+                        ka[(t + 1) & 1][kk] = as_bf16x8(
+                            *reinterpret_cast<const u32x4 *>(kp + (t + 1) * 32 * DP + kk * 128));
+                }
+#pragma unroll
+                for (int kk = 0; kk < KN; ++kk) {
+                    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                    if (t + 1 < NT)
+                        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+                }
+            }
+            // Register i of sub-tile t: key kw + 32t + 16 (i / 8) + 8hi + i % 8.
+            if (MOD)
+#pragma unroll
+                for (int t = 0; t < NT; ++t)
 #pragma unroll
                     for (int i = 0; i < 16; ++i)
-                        s[t][i] = 0.f;
+                        s[t][i] = score2(s[t][i], a.c, a.cap_in, a.cap_out, slope,
+                                         pos - (kw + 32 * t + 16 * (i >> 3) + 8 * hi + (i & 7)));
+            if (!all || kw + KW - 1 > wmin) {
+                // A block without a page hides its keys: looked up again here, where it is rare.
+                uint32_t none = 0;
 #pragma unroll
-                    for (int kk = 0; kk < KN; ++kk)
-                        s[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-                            as_bf16x8(*reinterpret_cast<const u32x4 *>(kp + t * 32 * DP + kk * 128)),
-                            qb[kk], s[t], 0, 0, 0);
-                }
-                // Register i of sub-tile t: key kb + 32t + 16 (i / 8) + 8hi + i % 8.
-                if (MOD)
+                for (int j = 0; j < KW / 16; ++j)
+                    none |= attn_page_ok(scalar_i32(table, min(kw + 16 * j, k1 - 1) >> a.lgp), a.pages) ? 0u : 1u << j;
 #pragma unroll
-                    for (int t = 0; t < 2; ++t)
+                for (int t = 0; t < NT; ++t)
 #pragma unroll
-                        for (int i = 0; i < 16; ++i)
-                            s[t][i] = score2(s[t][i], a.c, a.cap_in, a.cap_out, slope,
-                                             pos - (kb + 32 * t + 16 * (i >> 3) + 8 * hi + (i & 7)));
-                if (!whole || kb + KT - 1 > wmin) {
-                    // A block without a page hides its keys. The tile's blocks are looked up again
-                    // here: it is rare.
-                    uint32_t none = 0;
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        none |= block_at(a, table, u, kb + 16 * j, k1).n == 0 ? 1u << j : 0u;
-#pragma unroll
-                    for (int t = 0; t < 2; ++t)
-#pragma unroll
-                        for (int i = 0; i < 16; ++i)
-                            if (kb + 32 * t + 16 * (i >> 3) + 8 * hi + (i & 7) > lim ||
-                                (none >> (2 * t + (i >> 3)) & 1))
-                                s[t][i] = kNegInf;
-                }
-                float mx = kNegInf;
-#pragma unroll
-                for (int t = 0; t < 2; ++t)
-#pragma unroll
-                    for (int i = 0; i < 16; i += 2)
-                        mx = max3f(mx, s[t][i], s[t][i + 1]);
-                mx = max_xor32(mx);
-                if (__builtin_amdgcn_ballot_w64(mx > m_run + lift) != 0) {
-                    const float mnew = fmaxf(m_run, mx);
-                    const float alpha = fast_exp2((m_run - (mnew == kNegInf ? 0.f : mnew)) * c);
-                    m_run = mnew;
-                    l_run *= alpha;
-#pragma unroll
-                    for (int db = 0; db < DP / 32; ++db)
-#pragma unroll
-                        for (int i = 0; i < 16; ++i)
-                            o[db][i] *= alpha;
-                }
-                const float mc = m_run == kNegInf ? 0.f : m_run * c;
-                bf16x8 pk[4];
-#pragma unroll
-                for (int t = 0; t < 2; ++t)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const float p = fast_exp2(fmaf(s[t][i], c, -mc));
-                        l_run += p;
-                        pk[2 * t + (i >> 3)][i & 7] = (__bf16)p;
-                    }
-                const uint16_t *vp = &Vs[buf][vfo];
-#pragma unroll
-                for (int cc = 0; cc < 4; ++cc)
-#pragma unroll
-                    for (int db = 0; db < DP / 32; ++db) {
-                        const uint16_t *x = vp + cc * 16 * DP + db * 128;
-                        o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-                            join_tr(lds_read_tr(x), lds_read_tr(x + 4 * DP)), pk[cc], o[db], 0, 0, 0);
-                    }
+                    for (int i = 0; i < 16; ++i)
+                        if (kw + 32 * t + 16 * (i >> 3) + 8 * hi + (i & 7) > lim ||
+                            (none >> (2 * t + (i >> 3)) & 1))
+                            s[t][i] = kNegInf;
             }
-            if (more) {
-                put(st, buf ^ 1);
-                whole = st.whole;
+            float mx = kNegInf;
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int i = 0; i < 16; i += 2)
+                    mx = max3f(mx, s[t][i], s[t][i + 1]);
+            mx = max_xor32(mx);
+            if (__builtin_amdgcn_ballot_w64(mx > m_run + lift) != 0) {
+                const float mnew = fmaxf(m_run, mx);
+                const float alpha = fast_exp2((m_run - (mnew == kNegInf ? 0.f : mnew)) * c);
+                m_run = mnew;
+                l_run *= alpha;
+#pragma unroll
+                for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        o[db][i] *= alpha;
+            }
+            const float mc = m_run == kNegInf ? 0.f : m_run * c;
+            bf16x8 pk[2 * NT];
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const float p = fast_exp2(fmaf(s[t][i], c, -mc));
+                    l_run += p;
+                    pk[2 * t + (i >> 3)][i & 7] = (__bf16)p;
+                }
+            const uint16_t *vp = Vb + vfo;
+#pragma unroll
+            for (int cc = 0; cc < 2 * NT; ++cc)
+#pragma unroll
+                for (int db = 0; db < DP / 32; ++db) {
+                    const uint16_t *x = vp + cc * 16 * DP + db * 128;
+                    o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+                        join_tr(lds_read_tr(x), lds_read_tr(x + 4 * DP)), pk[cc], o[db], 0, 0, 0);
+                }
+        };
+        auto wait_loads = [] { __builtin_amdgcn_s_waitcnt(waitcnt_vm(0)); };
+
+        stage st[2];
+        bool all = true;
+        if (k0 < kstop) {
+            load(k0, Ks0, Vs0, st[0]);
+            all = whole(k0);
+            if constexpr (F4) {
+                if (k0 + KT < kstop)
+                    load(k0 + KT, Ks1, Vs1, st[1]);
+                put(st[0], Ks0, Vs0);
+            } else {
+                wait_loads();
+            }
+        }
+        __syncthreads();
+        // Tile i (0 or 1, in buffer i); f: the registers of the tile after it (4 bits).
+        auto step = [&](int kb, const uint16_t *Kb, const uint16_t *Vb, uint16_t *Kn, uint16_t *Vn, stage &f,
+                        stage &f2) __attribute__((always_inline)) {
+            const bool more = kb + KT < kstop, more2 = kb + 2 * KT < kstop;
+            if constexpr (F4) {
+                if (more2)
+                    load(kb + 2 * KT, nullptr, nullptr, f2);
+            } else if (more) {
+                load(kb + KT, Kn, Vn, f);
+            }
+            const bool now = all;
+            all = more && whole(kb + KT);
+            compute(kb, now, Kb, Vb);
+            if constexpr (F4) {
+                if (more)
+                    put(f, Kn, Vn);
+            } else {
+                wait_loads(); // this wave's part of the next tile has arrived
             }
             __syncthreads();
+        };
+        for (int kb = k0; kb < kstop; kb += 2 * KT) {
+            step(kb, Ks0, Vs0, Ks1, Vs1, st[1], st[0]);
+            if (kb + KT < kstop)
+                step(kb + KT, Ks1, Vs1, Ks0, Vs0, st[0], st[1]);
         }
         l_run = sum_xor32(l_run);
 
-        if (valid) {
-            const int64_t at = sq.q0 + tok;
+        bool writes = valid;
+        if constexpr (KH > 1) {
+            // Join the halves of the tiles: the second half's waves leave (m, l) and O in LDS.
+            static_assert(KT >= 64, "a wave's O fits a buffer");
+            float *kho = reinterpret_cast<float *>(wr == 0 ? Ks0 : Vs0) + lane;
+            if (kh == 1) {
+                kh_ml[wr * 64 + lane] = m_run * c;
+                kh_ml[NR * 64 + wr * 64 + lane] = l_run;
+#pragma unroll
+                for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        kho[(db * 16 + i) * 64] = o[db][i];
+            }
+            __syncthreads();
+            if (kh == 0) {
+                const float m1 = kh_ml[wr * 64 + lane], l1 = kh_ml[NR * 64 + wr * 64 + lane];
+                const float mm = fmaxf(m_run * c, m1), mu = mm == kNegInf ? 0.f : mm;
+                const float w0 = fast_exp2(m_run * c - mu), w1 = fast_exp2(m1 - mu);
+                l_run = w0 * l_run + w1 * l1;
+                m_run = mm / c;
+#pragma unroll
+                for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        o[db][i] = w0 * o[db][i] + w1 * kho[(db * 16 + i) * 64];
+            }
+            __syncthreads();
+            writes = valid && kh == 0;
+        }
+        if (writes) {
+            const int64_t orow = sq.q0 + tok;
+            const int64_t slot = (orow * a.Hq + h) * a.nsplit;
             if (live == 1) {
                 const float inv = l_run > 0.f ? 1.0f / l_run : 0.f;
-                uint16_t *dst = a.o + at * a.o_tok + h * a.o_head;
+                if (hi == 0 && a.nsplit > 1)
+                    a.pm[slot] = -kNegInf; // the row is written
+                uint16_t *dst = a.o + orow * a.o_tok + h * a.o_head;
 #pragma unroll
                 for (int db = 0; db < DP / 32; ++db)
 #pragma unroll
@@ -763,12 +1036,14 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_paged_prefill_ker
                                       bf16_pair(o[db][4 * j + 2] * inv, o[db][4 * j + 3] * inv)};
                     }
             } else {
-                const int64_t slot = (at * a.Hq + h) * a.nsplit + sp;
                 if (hi == 0) {
-                    a.pm[slot] = m_run * c;
-                    a.pl[slot] = l_run;
+                    a.pm[slot + sp] = m_run * c;
+                    a.pl[slot + sp] = l_run;
+                    if (sp == live - 1) // no parts behind the last
+                        for (int s = live; s < a.nsplit; ++s)
+                            a.pm[slot + s] = kNegInf;
                 }
-                float *dst = a.pacc + slot * D;
+                float *dst = a.pacc + (slot + sp) * D;
 #pragma unroll
                 for (int db = 0; db < DP / 32; ++db)
 #pragma unroll
@@ -989,8 +1264,9 @@ __global__ __launch_bounds__(256) void attn_kv_read_kernel(const attn_kv_args a)
 }
 
 // ---- launchers -------------------------------------------------------------------------------
-template <int DP, bool F4> hipError_t launch_paged_d(const attn_paged_args &a, int rows16, hipStream_t st) {
-    const unsigned grid = (unsigned)(a.B * (long)a.Hkv * a.nsplit * a.tps);
+template <int DP, bool F4>
+hipError_t launch_paged_d(const attn_paged_args &a, const attn_paged_cut &cut, hipStream_t st) {
+    const dim3 grid((unsigned)cut.grid), block(256);
     const bool mod = a.cap_out != 0.f || a.slopes;
     return with_flag(mod, [&](auto M) {
         constexpr bool kM = decltype(M)::value;
@@ -998,67 +1274,67 @@ template <int DP, bool F4> hipError_t launch_paged_d(const attn_paged_args &a, i
             constexpr int kN = decltype(NB)::value;
             constexpr bool kT = decltype(NT)::value;
             if (t_plan)
-                plan_note(dim3(grid), dim3(256),
-                          "attn_paged_decode_kernel<%d, %d, %d, %s, %s> parts=%d keys=%d", DP, F4 ? 4 : 16,
-                          kN, tf(kM), tf(kT), a.nsplit, a.kps);
+                plan_note(grid, block, "attn_paged_decode_kernel<%d, %d, %d, %s, %s> teams=%d parts=%d", DP,
+                          F4 ? 4 : 16, kN, tf(kM), tf(kT), a.teams, a.nsplit);
             else
-                hipLaunchKernelGGL((attn_paged_decode_kernel<DP, F4, kN, kM, kT>), dim3(grid), dim3(256), 0,
-                                   st, a);
+                hipLaunchKernelGGL((attn_paged_decode_kernel<DP, F4, kN, kM, kT>), grid, block, 0, st, a);
             return hipGetLastError();
         };
-        if (rows16 == 1)
+        if (cut.rows16 == 1)
             return with_flag(a.tps == 1, [&](auto NT) {
                 return decode(std::integral_constant<int, 1>{}, NT);
             });
         if constexpr (DP <= 128)
-            if (rows16 == 2)
-                return decode(std::integral_constant<int, 2>{}, std::false_type{});
-        if (t_plan)
-            plan_note(dim3(grid), dim3(256), "attn_paged_prefill_kernel<%d, %d, %s> parts=%d keys=%d", DP,
-                      F4 ? 4 : 16, tf(kM), a.nsplit, a.kps);
-        else
-            hipLaunchKernelGGL((attn_paged_prefill_kernel<DP, F4, kM>), dim3(grid), dim3(256), 0, st, a);
-        return hipGetLastError();
+            if (cut.rows16 == 2)
+                return with_flag(a.tps == 1, [&](auto NT) {
+                    return decode(std::integral_constant<int, 2>{}, NT);
+                });
+        auto prefill = [&](auto KHF) {
+            constexpr int kK = decltype(KHF)::value;
+            if (t_plan)
+                plan_note(grid, block, "attn_paged_prefill_kernel<%d, %d, %s, %d> parts=%d share=%d", DP,
+                          F4 ? 4 : 16, tf(kM), kK, a.nsplit, a.share);
+            else
+                hipLaunchKernelGGL((attn_paged_prefill_kernel<DP, F4, kM, kK>), grid, block, 0, st, a);
+            return hipGetLastError();
+        };
+        if constexpr (DP <= 128)
+            if (cut.rows16 == 4)
+                return prefill(std::integral_constant<int, 2>{});
+        return prefill(std::integral_constant<int, 1>{});
     });
 }
 
 } // namespace
 
-// rows16: 1 or 2 row blocks of 16 per workgroup (decode), or 8 (prefill). Joins the parts where the call
-// has more than one; max_q bounds the merge's grid.
-extern "C" int attn_hip_launch_paged(const struct attn_paged_args *ap, int bits, int rows16, int max_q,
+// The attention kernel that the cut names and, where it may leave parts, the merge.
+extern "C" int attn_hip_launch_paged(const struct attn_paged_args *ap, const struct attn_paged_cut *cut, int bits,
                                      void *stream) {
     const attn_paged_args &a = *ap;
     const hipStream_t st = (hipStream_t)stream;
-    const long grid = (long)a.B * a.Hkv * a.nsplit * a.tps;
-    if (grid <= 0 || grid > ATTN_PAGED_MAX_GRID || a.nsplit > kPagedMaxSplit)
+    if (cut->grid <= 0 || cut->grid > ATTN_PAGED_MAX_GRID || a.nsplit > kPagedMaxSplit ||
+        (a.nsplit > 1 && (256 >> (cut->lglp + cut->lgsg)) * a.nsplit > ATTN_PAGED_MERGE_WEIGHTS))
         return (int)hipErrorInvalidValue;
     hipError_t e;
     if (bits == 4)
-        e = a.D == 64    ? launch_paged_d<64, true>(a, rows16, st)
-            : a.D == 128 ? launch_paged_d<128, true>(a, rows16, st)
-                         : launch_paged_d<256, true>(a, rows16, st);
+        e = a.D == 64    ? launch_paged_d<64, true>(a, *cut, st)
+            : a.D == 128 ? launch_paged_d<128, true>(a, *cut, st)
+                         : launch_paged_d<256, true>(a, *cut, st);
     else
-        e = a.D <= 64    ? launch_paged_d<64, false>(a, rows16, st)
-            : a.D <= 128 ? launch_paged_d<128, false>(a, rows16, st)
-                         : launch_paged_d<256, false>(a, rows16, st);
+        e = a.D <= 64    ? launch_paged_d<64, false>(a, *cut, st)
+            : a.D <= 128 ? launch_paged_d<128, false>(a, *cut, st)
+                         : launch_paged_d<256, false>(a, *cut, st);
     if (e != hipSuccess || a.nsplit == 1)
         return (int)e;
-    // LP lanes of four columns, SG groups of parts: 8 loads or fewer per thread where there are parts
-    // for it.
-    int lglp = 3, lgsg = 0;
-    while ((4 << lglp) < a.D)
-        ++lglp;
-    while (lglp + lgsg < 8 && (4 << lgsg) < a.nsplit)
-        ++lgsg;
-    const int rpw = 256 >> (lglp + lgsg);
-    const long tiles = ((long)max_q * a.Hq + rpw - 1) / rpw;
-    const long tpm = std::max(1L, std::min(tiles, ATTN_PAGED_MAX_GRID / a.B));
+    const dim3 grid((unsigned)((long)a.B * a.Hkv * cut->merge_tiles));
     if (t_plan)
-        plan_note(dim3((unsigned)(a.B * tpm)), dim3(256), "attn_paged_merge_kernel rows=%d", rpw);
+        plan_note(grid, dim3(256), "attn_paged_merge_kernel rows=%d", 256 >> (cut->lglp + cut->lgsg));
     else
-        hipLaunchKernelGGL(attn_paged_merge_kernel, dim3((unsigned)(a.B * tpm)), dim3(256), 0, st, a, lglp,
-                           lgsg, (int)tpm);
+        with_flag(cut->merge_loads == 2, [&](auto FEW) {
+            hipLaunchKernelGGL((attn_paged_merge_kernel<decltype(FEW)::value ? 2 : 8>), grid, dim3(256), 0, st,
+                               a, cut->lglp, cut->lgsg, cut->merge_tiles);
+            return hipSuccess;
+        });
     return (int)hipGetLastError();
 }
 
