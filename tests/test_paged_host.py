@@ -45,6 +45,8 @@ def cache(**k):
     a.update(k)
     return ts.KvCache(**a)
 r = ts.Rows(4096, 1024, 128)
+class none:  # NULL
+    _at = None
 """
 FOUR = "bits=4, k_scale=4096, v_scale=4096"
 ATTEND = "ts.attn_paged(%s, %s, %s, %s, %s, 1, %s, %s, %s, %s)"
@@ -62,7 +64,7 @@ def append(c="cache()", q="r", qo="r", k="r", v="r", T=4, Hq=8, rope=4096, rows=
 
 
 REFUSED = [
-    (attend("None"), "attn_paged: the cache must be non-NULL"),
+    (attend("none"), "attn_paged: the cache must be non-NULL"),
     (attend("cache(bits=8)"), "bits must be"),
     (attend("cache(D=24)"), "D % 16 == 0"),
     (attend("cache(D=0)"), "D % 16 == 0"),
@@ -91,7 +93,7 @@ REFUSED = [
     (attend(T=2 ** 28, Hq=8), "T * Hq <= 2^30"),
     (attend(mq=0), "max_q >= 1"),
     (attend(mk=0), "max_kv >= 1"),
-    (attend(q="None"), "q needs a 16-byte aligned"),
+    (attend(q="none"), "q needs a 16-byte aligned"),
     (attend(q="ts.Rows(4100, 1024, 128)"), "q needs a 16-byte aligned"),
     (attend(o="ts.Rows(4096, 1020, 128)"), "o needs a 16-byte aligned"),
     (attend(o="ts.Rows(4096, 1024, -128)"), "o needs a 16-byte aligned"),
@@ -103,11 +105,11 @@ REFUSED = [
     (attend(sc="ts.Scores(0.0, 0.0, 4097)"), "slopes must be"),
     (attend(s="None"), "scratch must be"),
     (attend(s=4128), "scratch must be"),
-    (append("None"), "attn_kv_append: the cache must be non-NULL"),
+    (append("none"), "attn_kv_append: the cache must be non-NULL"),
     (append(Hq=5), "Hq % Hkv"),
     (append(q="None"), "q_out without q"),
     (append(qo="None"), "q_out needs"),
-    (append(k="None"), "k needs"),
+    (append(k="none"), "k needs"),
     (append(v="ts.Rows(4096, 4, 8)"), "v needs"),
     (append(rot=136), "rot must be"),
     (append(rot=144), "rot must be"),
@@ -116,10 +118,9 @@ REFUSED = [
     (append(rope=4100), "rope must be"),
     (append(rows=0), "rope must be"),
     (append(mq=0), "max_q >= 1"),
-    (append("cache(Hkv=2**18)", q="None", qo="None"), "too many sequences and heads"),
     (attend("cache(B=2**17, Hkv=16)"), "B * Hkv <= 2^20"),
     ("ts.attn_kv_read(cache(D=40), r, r, 4, 1)", "attn_kv_read: a bf16 cache"),
-    ("ts.attn_kv_read(cache(), None, r, 4, 1)", "k needs"),
+    ("ts.attn_kv_read(cache(), none, r, 4, 1)", "k needs"),
     ("ts.attn_kv_read(cache(), r, ts.Rows(4096, 8, 9), 4, 1)", "v needs"),
     ("ts.attn_kv_read(cache(), r, r, 4, 0)", "max_q >= 1"),
     ("ts.attn_paged_plan(cache(page=20), 4, 8, 1, None, 1, 1)", "attn_paged_plan: page must be"),

@@ -165,8 +165,8 @@ int attn_paged_plan(const struct attn_kv_cache *c, int T, int Hq, int causal, co
     return n < 0 || n > 0x7fffffffL ? -1 : (int)n;
 }
 
-/* What append and read share; units: pieces of work per token, one per thread. */
-static struct attn_kv_args kv_args(const struct attn_kv_cache *c, int lgp, int T, int max_q, int64_t units,
+/* What append and read share. */
+static struct attn_kv_args kv_args(const struct attn_kv_cache *c, int lgp, int T, int max_q, int tpw,
                                    const struct attn_rows *k, const struct attn_rows *v) {
     struct attn_kv_args a;
     memset(&a, 0, sizeof a);
@@ -175,8 +175,7 @@ static struct attn_kv_args kv_args(const struct attn_kv_cache *c, int lgp, int T
     a.table = c->table, a.kv_len = c->kv_len, a.q_start = c->q_start;
     a.B = c->B, a.T = T, a.Hkv = c->Hkv, a.D = c->D;
     a.cols = c->table_cols, a.pages = c->pages, a.lgp = lgp;
-    const struct attn_kv_cut cut = attn_kv_cut_of(c->B, T, max_q, units);
-    a.tblk = cut.tblk, a.ublk = cut.ublk, a.tpw = cut.tpw;
+    a.tblk = attn_kv_blocks(c->B, T, max_q, tpw);
     return a;
 }
 
@@ -200,11 +199,7 @@ void attn_kv_append(const struct attn_kv_cache *c, const struct attn_rows *q, co
         paged_fail(who, "rope must be a 16-byte aligned device pointer to rope_rows >= 1 rows");
     if (max_q < 1)
         paged_fail(who, "need max_q >= 1");
-    const int64_t uq = q ? (int64_t)Hq * (c->D / 16) : 0, uk = (int64_t)c->Hkv * (c->D / 16);
-    const int64_t units = c->bits == ATTN_KV_FP4 ? (uq + 3) / 4 * 4 + 4 * uk : uq + 2 * uk;
-    if (units > 1 << 20 || units / 256 * c->B > ATTN_PAGED_MAX_GRID / 2)
-        paged_fail(who, "too many sequences and heads");
-    struct attn_kv_args a = kv_args(c, lgp, T, max_q, units, k, v);
+    struct attn_kv_args a = kv_args(c, lgp, T, max_q, 1, k, v);
     if (q) {
         a.q = (const uint16_t *)q->data, a.q_out = (uint16_t *)q_out->data;
         a.q_tok = q->token, a.q_head = q->head, a.qo_tok = q_out->token, a.qo_head = q_out->head;
@@ -223,10 +218,7 @@ void attn_kv_read(const struct attn_kv_cache *c, const struct attn_rows *k, cons
     paged_check_rows(who, "v", v);
     if (max_q < 1)
         paged_fail(who, "need max_q >= 1");
-    const int64_t units = 2 * (int64_t)c->Hkv * (c->D / 8);
-    if (units > 1 << 20 || units / 256 * c->B > ATTN_PAGED_MAX_GRID / 2)
-        paged_fail(who, "too many sequences and heads");
-    struct attn_kv_args a = kv_args(c, lgp, T, max_q, units, k, v);
+    struct attn_kv_args a = kv_args(c, lgp, T, max_q, 4, k, v);
     a.k_out = (uint16_t *)k->data, a.v_out = (uint16_t *)v->data;
     paged_hip_check(attn_hip_launch_kv_read(&a, c->bits, attn_flash_get_stream()), who);
 }

@@ -35,7 +35,7 @@ struct attn_kv_args {
     const int32_t *table, *kv_len, *q_start;
     const float *rope;
     int32_t B, T, Hq, Hkv, D, cols, pages, lgp, rope_rows, rot;
-    int32_t tblk, ublk, tpw; /* token blocks per sequence, blocks of 256 units, tokens per block */
+    int32_t tblk; /* workgroups per sequence */
 };
 
 #define ATTN_PAGED_DECODE_WG 512 /* workgroups of a decode call: two per CU */
@@ -114,22 +114,10 @@ static inline struct attn_paged_cut attn_paged_cut_of(int B, int Hkv, int g, int
     return c;
 }
 
-struct attn_kv_cut {
-    int tblk, ublk, tpw;
-};
-
-/* Tokens per workgroup: one while that leaves a grid of at most 2048 workgroups, else up to 8. */
-static inline struct attn_kv_cut attn_kv_cut_of(int B, int T, int max_q, int64_t units) {
-    const int64_t ublk = (units + 255) / 256;
-    const int64_t mq = max_q < T ? max_q : T;
-    int64_t tpw = 1;
-    while (tpw < 8 && (mq + tpw - 1) / tpw * ublk * B > 2048)
-        tpw *= 2;
-    int64_t tblk = (mq + tpw - 1) / tpw;
-    if (tblk * ublk * B > ATTN_PAGED_MAX_GRID)
-        tblk = ATTN_PAGED_MAX_GRID / (ublk * B) > 1 ? ATTN_PAGED_MAX_GRID / (ublk * B) : 1;
-    struct attn_kv_cut c = {(int)tblk, (int)ublk, (int)tpw};
-    return c;
+/* Append and read: workgroups per sequence, of tpw tokens each (append one, read one per wave). */
+static inline int attn_kv_blocks(int B, int T, int max_q, int tpw) {
+    const int64_t n = ((int64_t)(max_q < T ? max_q : T) + tpw - 1) / tpw;
+    return (int)(n * B > ATTN_PAGED_MAX_GRID ? ATTN_PAGED_MAX_GRID / B : n);
 }
 
 #endif

@@ -1059,11 +1059,12 @@ __global__ __launch_bounds__(256, 2) void attn_paged_prefill_kernel(const attn_p
 }
 
 // ------------------------------------------------------------------------------------------
-// Append. A workgroup takes 256 units of work of each of tpw tokens of one sequence, one unit per thread:
-// 16 elements of a head, the two eights that rotate with each other ((x1, x2) -> (x1 c - x2 s,
-// x2 c + x1 s), in fp32, products and sums rounded apart, the result once to bf16), or for the 4-bit
-// cache eight elements of a K or V row. HBM-bound: each element is read and written once, and the rope
-// row is shared by a token's heads through the L1 cache.
+// Append. A workgroup takes one token at a time, its four waves two halves of q's heads, k and v. A lane holds
+// the two eights of a head that rotate with each other ((x1, x2) -> (x1 c - x2 s, x2 c + x1 s), in fp32,
+// products and sums rounded apart, the result once to bf16), the wave's lanes lie across several heads, and
+// four of a lane's heads are in flight, so that the cosines and sines are read once per wave. K and V of the
+// 4-bit cache go eight elements to a lane, four lanes to a group. HBM-bound: each element is read and
+// written once, past the L2, whose copies the attention on other XCDs could not use.
 // ------------------------------------------------------------------------------------------
 __device__ __forceinline__ float lo_bf16(uint32_t x) { return __builtin_bit_cast(float, x << 16); }
 __device__ __forceinline__ float hi_bf16(uint32_t x) {
@@ -1101,166 +1102,193 @@ __device__ __forceinline__ uint32_t e8m0_of(uint32_t amax) {
 template <bool F4, bool PAIRS>
 __global__ __launch_bounds__(256) void attn_kv_append_kernel(const attn_kv_args a) {
 #pragma clang fp contract(off)
-    const int per = a.tblk * a.ublk;
-    const int b = uniform(wg_id_x() / per), L = wg_id_x() % per;
-    const int ub = uniform(L % a.ublk), tb = uniform(L / a.ublk);
+    const int b = uniform(wg_id_x() / a.tblk), tb = wg_id_x() - b * a.tblk;
     const attn_seq sq = attn_seq_of(scalar_i32(a.q_start, b), scalar_i32(a.q_start, b + 1),
                                     scalar_i32(a.kv_len, b), a.T, a.cols, a.lgp);
-    const int unit = ub * 256 + wi_id_x(), D = a.D, half = a.rot / 2;
-    // This thread's unit: which tensor (0 q, 1 k, 2 v), head and part of the head.
-    const int uh = D / 16, uh4 = D / 8;
-    const int nq = F4 ? (a.Hq * uh + 3) / 4 * 4 : a.Hq * uh, nk = a.Hkv * (F4 ? uh4 : uh);
-    int what = 0, x = unit;
-    if (unit >= nq) {
-        what = unit >= nq + nk ? 2 : 1;
-        x = unit - nq - (what == 2 ? nk : 0);
-    }
-    const bool mine = what == 0 ? unit < a.Hq * uh : x < nk;
-    const bool eight = F4 && what != 0;
-    const int n = eight ? uh4 : uh, head = x / n, j = x % n;
-    const bool turn = what != 2 && (eight ? j * 8 < a.rot : j * 16 < a.rot);
-    // Columns of the two eights, and of the cosines of the first one's elements (or pairs).
-    int c0, c1, rc;
-    if (eight) { // c0: this unit's own; c1: its partner (PAIRS: none)
-        c0 = 8 * j;
-        c1 = !turn || PAIRS ? c0 : c0 < half ? c0 + half : c0 - half;
-        rc = PAIRS ? 4 * j : c0 < half ? c0 : c0 - half;
-    } else {
-        c0 = turn && !PAIRS ? 8 * j : 16 * j;
-        c1 = turn && !PAIRS ? half + 8 * j : 16 * j + 8;
-        rc = 8 * j;
-    }
-    const int64_t tok_s = what == 0 ? a.q_tok : what == 1 ? a.k_tok : a.v_tok;
-    const uint16_t *src = (what == 0   ? a.q + head * a.q_head
-                           : what == 1 ? a.k + head * a.k_head
-                                       : a.v + head * a.v_head);
+    const int lane = wi_id_x() & 63, w = uniform(wi_id_x() >> 6), D = a.D, half = a.rot / 2;
     const int32_t *table = a.table + (int64_t)b * a.cols;
+    constexpr int U = 2; // heads of a lane in flight
 
-    for (int i0 = tb * a.tpw; i0 < sq.n; i0 += a.tblk * a.tpw)
-        for (int i = i0; i < min(i0 + a.tpw, sq.n); ++i) {
-            const int pos = sq.len - sq.n + i;
-            const bool placed = pos >= 0 && (a.rot == 0 || pos < a.rope_rows);
-            bool kept = placed && pos < sq.kend;
-            int pg = 0;
-            if (kept) {
-                pg = scalar_i32(table, pos >> a.lgp);
-                kept = attn_page_ok(pg, a.pages);
-            }
-            if (!mine || !(what == 0 ? placed || a.rot == 0 : kept))
-                continue;
-            const uint16_t *s = src + (sq.q0 + i) * tok_s;
-            const u32x4 v0 = *reinterpret_cast<const u32x4 *>(s + c0);
-            const u32x4 v1 = *reinterpret_cast<const u32x4 *>(s + c1);
-            u32x4 y0 = v0, y1 = v1;
-            if (turn) {
-                const float *cr = a.rope + (int64_t)pos * a.rot + rc, *sr = cr + half;
-                float p[8], q[8], cs[8], sn[8], r0[8], r1[8];
-                to_f32(v0, p);
-                to_f32(v1, q);
+    // This wave's heads: of q (waves 0 and 1), k (2) or v (3).
+    const int h0 = w == 1 ? (a.Hq + 1) / 2 : 0;
+    const int heads = w > 1 ? a.Hkv : w == 1 ? a.Hq - h0 : (a.Hq + 1) / 2;
+    const int64_t tok_s = w < 2 ? a.q_tok : w == 2 ? a.k_tok : a.v_tok;
+    const int64_t head_s = w < 2 ? a.q_head : w == 2 ? a.k_head : a.v_head;
+    const uint16_t *src = w < 2 ? a.q : w == 2 ? a.k : a.v;
+    uint8_t *const cache = w == 2 ? a.ck : a.cv, *const scales = w == 2 ? a.cks : a.cvs;
+    if (heads == 0)
+        return;
+
+    // Sixteen elements of a head per lane: columns c0 .. + 7 and c1 .. + 7, which turn by the angles from r on;
+    // or eight (k and v in 4 bits), columns c0 .. + 7, and the columns c1 .. + 7 that they turn with.
+    const bool eight = F4 && w > 1;
+    const int n = eight ? D / 8 : D / 16, hp = 64 / n, hl = lane / n, j = lane % n;
+    const bool turn = w < 3 && (eight ? 8 : 16) * j < a.rot;
+    int c0 = 16 * j, c1 = 16 * j + 8, r = 8 * j;
+    bool low = true;
+    if (eight) {
+        low = PAIRS || 8 * j < half;
+        c0 = 8 * j;
+        c1 = !turn || PAIRS ? c0 : low ? c0 + half : c0 - half;
+        r = PAIRS ? 4 * j : low ? c0 : c0 - half;
+    } else if (turn && !PAIRS) {
+        c0 = 8 * j;
+        c1 = half + 8 * j;
+    }
+
+    for (int i = tb; i < sq.n; i += a.tblk) {
+        // The rows are asked for before their place is known; a token without one is not stored.
+        const int pos = sq.len - sq.n + i;
+        const uint16_t *s = src + (sq.q0 + i) * tok_s + h0 * head_s;
+        u32x4 x0[U], x1[U];
+        auto load = [&](int h) __attribute__((always_inline)) {
 #pragma unroll
-                for (int e = 0; e < 8; e += 4) {
-                    if (PAIRS && eight && e == 4) // eight elements are four pairs
-                        break;
-                    const f32x4 x0 = *reinterpret_cast<const f32x4 *>(cr + e);
-                    const f32x4 x1 = *reinterpret_cast<const f32x4 *>(sr + e);
+            for (int e = 0; e < U; ++e) {
+                const uint16_t *t = s + min(h + e * hp + hl, heads - 1) * head_s;
+                x0[e] = *reinterpret_cast<const u32x4 *>(t + c0);
+                x1[e] = *reinterpret_cast<const u32x4 *>(t + c1);
+            }
+        };
+        load(0);
+        const bool placed = pos >= 0 && (a.rot == 0 || pos < a.rope_rows);
+        const int pg = scalar_i32(table, max(0, min(pos, sq.kend - 1)) >> a.lgp);
+        float cs[8], sn[8];
+        if (turn) {
+            const float *cr = a.rope + (int64_t)(placed ? pos : 0) * a.rot + r;
+#pragma unroll
+            for (int e = 0; e < 8; e += 4) {
+                if (PAIRS && eight && e == 4) // eight elements are four pairs
+                    break;
+                const f32x4 y0 = *reinterpret_cast<const f32x4 *>(cr + e);
+                const f32x4 y1 = *reinterpret_cast<const f32x4 *>(cr + half + e);
+#pragma unroll
+                for (int f = 0; f < 4; ++f)
+                    cs[e + f] = y0[f], sn[e + f] = y1[f];
+            }
+        }
+        if (w < 2 ? !placed && a.rot != 0
+                  : !placed || pos >= sq.kend || !attn_page_ok(pg, a.pages))
+            continue;
+        const int64_t row = attn_page_row(pg, a.Hkv, 0, max(pos, 0), a.lgp);
+        for (int h = 0;;) {
+#pragma unroll
+            for (int e = 0; e < U; ++e) {
+                if (h + e * hp >= heads)
+                    break;
+                if (turn) {
+                    float p[8], q[8], y0[8], y1[8];
+                    to_f32(x0[e], p);
+                    to_f32(x1[e], q);
+                    if (PAIRS) { // neighbours; of sixteen elements eight pairs
+#pragma unroll
+                        for (int f = 0; f < 4; ++f) {
+                            y0[2 * f] = p[2 * f] * cs[f] - p[2 * f + 1] * sn[f];
+                            y0[2 * f + 1] = p[2 * f + 1] * cs[f] + p[2 * f] * sn[f];
+                            if (!eight) {
+                                y1[2 * f] = q[2 * f] * cs[4 + f] - q[2 * f + 1] * sn[4 + f];
+                                y1[2 * f + 1] = q[2 * f + 1] * cs[4 + f] + q[2 * f] * sn[4 + f];
+                            }
+                        }
+                    } else {
+#pragma unroll
+                        for (int f = 0; f < 8; ++f) {
+                            const float m = q[f] * sn[f];
+                            y0[f] = low ? p[f] * cs[f] - m : p[f] * cs[f] + m;
+                            if (!eight)
+                                y1[f] = q[f] * cs[f] + p[f] * sn[f];
+                        }
+                    }
+                    x0[e] = to_bf16(y0);
+                    if (!eight)
+                        x1[e] = to_bf16(y1);
+                }
+                const int hh = h + e * hp + hl;
+                if (eight) {
+                    uint32_t am = 0;
 #pragma unroll
                     for (int f = 0; f < 4; ++f)
-                        cs[e + f] = x0[f], sn[e + f] = x1[f];
-                }
-                if (PAIRS) {
-                    // elements (2e, 2e + 1) turn together; eight pairs in sixteen elements
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        r0[2 * e] = p[2 * e] * cs[e] - p[2 * e + 1] * sn[e];
-                        r0[2 * e + 1] = p[2 * e + 1] * cs[e] + p[2 * e] * sn[e];
+                        am = max(am, max(x0[e][f] << 16 & 0x7fff0000u, x0[e][f] & 0x7fff0000u));
+                    const uint32_t e8 = e8m0_of(quad_max(am));
+                    const float sc = e8m0(e8);
+                    uint32_t c = 0;
+                    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, lo_bf16(x0[e][0]), hi_bf16(x0[e][0]), sc, 0);
+                    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, lo_bf16(x0[e][1]), hi_bf16(x0[e][1]), sc, 1);
+                    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, lo_bf16(x0[e][2]), hi_bf16(x0[e][2]), sc, 2);
+                    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, lo_bf16(x0[e][3]), hi_bf16(x0[e][3]), sc, 3);
+                    if (hh < heads) { // D is 64, 128 or 256: every lane has a head
+                        const int64_t at = row + ((int64_t)hh << a.lgp);
+                        *reinterpret_cast<uint32_t *>(cache + at * (D / 2) + 4 * j) = e8 == 255 ? 0u : c;
+                        if (j % 4 == 0)
+                            scales[at * (D / 32) + j / 4] = (uint8_t)e8;
                     }
-                    if (!eight)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            r1[2 * e] = q[2 * e] * cs[4 + e] - q[2 * e + 1] * sn[4 + e];
-                            r1[2 * e + 1] = q[2 * e + 1] * cs[4 + e] + q[2 * e] * sn[4 + e];
-                        }
-                } else if (eight && c0 >= half) {
-#pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        r0[e] = p[e] * cs[e] + q[e] * sn[e];
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        r0[e] = p[e] * cs[e] - q[e] * sn[e];
-                        if (!eight)
-                            r1[e] = q[e] * cs[e] + p[e] * sn[e];
-                    }
+                } else if (hl < hp && hh < heads) {
+                    uint16_t *d = w < 2 ? a.q_out + (sq.q0 + i) * a.qo_tok + (h0 + hh) * a.qo_head
+                                        : reinterpret_cast<uint16_t *>(cache) + (row + ((int64_t)hh << a.lgp)) * D;
+                    __builtin_nontemporal_store(x0[e], reinterpret_cast<u32x4 *>(d + c0));
+                    __builtin_nontemporal_store(x1[e], reinterpret_cast<u32x4 *>(d + c1));
                 }
-                y0 = to_bf16(r0);
-                if (!eight)
-                    y1 = to_bf16(r1);
             }
-            if (what == 0) {
-                uint16_t *d = a.q_out + (sq.q0 + i) * a.qo_tok + head * a.qo_head;
-                *reinterpret_cast<u32x4 *>(d + c0) = y0;
-                *reinterpret_cast<u32x4 *>(d + c1) = y1;
-                continue;
-            }
-            const int64_t row = attn_page_row(pg, a.Hkv, head, pos, a.lgp);
-            if constexpr (!F4) {
-                uint16_t *d = reinterpret_cast<uint16_t *>(what == 1 ? a.ck : a.cv) + row * D;
-                *reinterpret_cast<u32x4 *>(d + c0) = y0;
-                *reinterpret_cast<u32x4 *>(d + c1) = y1;
-            } else {
-                uint32_t am = 0;
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    am = max(am, max(y0[e] << 16 & 0x7fff0000u, y0[e] & 0x7fff0000u));
-                const uint32_t e8 = e8m0_of(quad_max(am));
-                const float sc = e8m0(e8);
-                uint32_t code = 0;
-                if (e8 != 255) {
-                    code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, lo_bf16(y0[0]), hi_bf16(y0[0]), sc, 0);
-                    code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, lo_bf16(y0[1]), hi_bf16(y0[1]), sc, 1);
-                    code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, lo_bf16(y0[2]), hi_bf16(y0[2]), sc, 2);
-                    code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, lo_bf16(y0[3]), hi_bf16(y0[3]), sc, 3);
-                }
-                *reinterpret_cast<uint32_t *>((what == 1 ? a.ck : a.cv) + row * (D / 2) + 4 * j) = code;
-                if (j % 4 == 0)
-                    (what == 1 ? a.cks : a.cvs)[row * (D / 32) + j / 4] = (uint8_t)e8;
-            }
+            h += U * hp;
+            if (h >= heads)
+                break;
+            load(h);
         }
+    }
 }
 
-// Read back: eight elements of a K or V row per thread and token. A token without a place in the cache
-// gives zeros.
+// Read back: a wave per token, eight elements of a head per lane, four heads of a lane in flight. A token
+// without a place in the cache gives zeros. HBM-bound by what it writes, which goes past the L2: 32768 tokens
+// of 8 heads from 4 bits 38.3 us through it, 28.4 past it.
 template <bool F4>
 __global__ __launch_bounds__(256) void attn_kv_read_kernel(const attn_kv_args a) {
-    const int per = a.tblk * a.ublk;
-    const int b = uniform(wg_id_x() / per), L = wg_id_x() % per;
-    const int ub = uniform(L % a.ublk), tb = uniform(L / a.ublk);
+    const int b = uniform(wg_id_x() / a.tblk), tb = wg_id_x() - b * a.tblk;
     const attn_seq sq = attn_seq_of(scalar_i32(a.q_start, b), scalar_i32(a.q_start, b + 1),
                                     scalar_i32(a.kv_len, b), a.T, a.cols, a.lgp);
-    const int unit = ub * 256 + wi_id_x(), D = a.D, n = D / 8;
-    const bool isv = unit >= a.Hkv * n;
-    const int x = unit - (isv ? a.Hkv * n : 0), head = x / n, j = x % n;
-    if (x >= a.Hkv * n)
-        return;
+    const int lane = wi_id_x() & 63, w = uniform(wi_id_x() >> 6), D = a.D;
+    const int uh = D / 8, hp = 64 / uh, hl = lane / uh, j = lane % uh;
     const int32_t *table = a.table + (int64_t)b * a.cols;
-    const uint8_t *pages = isv ? a.cv : a.ck, *scales = isv ? a.cvs : a.cks;
-    uint16_t *dst = (isv ? a.v_out + head * a.v_head : a.k_out + head * a.k_head) + 8 * j;
-    const int64_t tok_s = isv ? a.v_tok : a.k_tok;
-    for (int i0 = tb * a.tpw; i0 < sq.n; i0 += a.tblk * a.tpw)
-        for (int i = i0; i < min(i0 + a.tpw, sq.n); ++i) {
-            const int pos = sq.len - sq.n + i;
-            const int pg = pos >= 0 && pos < sq.kend ? scalar_i32(table, pos >> a.lgp) : -1;
-            u32x4 y = zero4();
-            if (attn_page_ok(pg, a.pages)) {
-                const int64_t row = attn_page_row(pg, a.Hkv, head, pos, a.lgp);
-                if constexpr (F4)
-                    y = fp4_to_bf16(*reinterpret_cast<const uint32_t *>(pages + row * (D / 2) + 4 * j),
-                                    e8m0(scales[row * (D / 32) + j / 4]));
-                else
-                    y = *reinterpret_cast<const u32x4 *>(pages + row * D * 2 + 16 * j);
+    constexpr int U = 4;
+    for (int i = tb * 4 + w; i < sq.n; i += a.tblk * 4) {
+        const int pos = sq.len - sq.n + i;
+        const int pg = pos >= 0 && pos < sq.kend ? scalar_i32(table, pos >> a.lgp) : -1;
+        const bool ok = attn_page_ok(pg, a.pages);
+        const int64_t row = attn_page_row(ok ? pg : 0, a.Hkv, 0, ok ? pos : 0, a.lgp);
+        const int64_t tok = sq.q0 + i;
+        auto rows = [&](const uint8_t *pages, const uint8_t *scales, uint16_t *dst, int64_t dhead)
+            __attribute__((always_inline)) {
+            const int64_t phead = (int64_t)(F4 ? D / 2 : 2 * D) << a.lgp;
+            const uint8_t *src = pages + row * (F4 ? D / 2 : 2 * D);
+            for (int h0 = 0; h0 < a.Hkv; h0 += U * hp) {
+                u32x4 x[U];
+                uint32_t sc[U];
+#pragma unroll
+                for (int e = 0; e < U; ++e) {
+                    if (h0 + e * hp >= a.Hkv)
+                        break;
+                    const int h = min(h0 + e * hp + hl, a.Hkv - 1);
+                    if constexpr (F4) {
+                        x[e][0] = *reinterpret_cast<const uint32_t *>(src + h * phead + 4 * j);
+                        sc[e] = scales[row * (D / 32) + h * (phead / 16) + j / 4];
+                    } else {
+                        x[e] = *reinterpret_cast<const u32x4 *>(src + h * phead + 16 * j);
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < U; ++e) {
+                    if (h0 + e * hp >= a.Hkv)
+                        break;
+                    const int h = h0 + e * hp + hl;
+                    u32x4 y = x[e];
+                    if constexpr (F4)
+                        y = fp4_to_bf16(x[e][0], e8m0(sc[e]));
+                    if (hl < hp && h < a.Hkv)
+                        __builtin_nontemporal_store(ok ? y : zero4(), reinterpret_cast<u32x4 *>(dst + h * dhead + 8 * j));
+                }
             }
-            *reinterpret_cast<u32x4 *>(dst + (sq.q0 + i) * tok_s) = y;
-        }
+        };
+        rows(a.ck, a.cks, a.k_out + tok * a.k_tok, a.k_head);
+        rows(a.cv, a.cvs, a.v_out + tok * a.v_tok, a.v_head);
+    }
 }
 
 // ---- launchers -------------------------------------------------------------------------------
@@ -1330,7 +1358,7 @@ extern "C" int attn_hip_launch_paged(const struct attn_paged_args *ap, const str
     if (t_plan)
         plan_note(grid, dim3(256), "attn_paged_merge_kernel rows=%d", 256 >> (cut->lglp + cut->lgsg));
     else
-        with_flag(cut->merge_loads == 2, [&](auto FEW) {
+        (void)with_flag(cut->merge_loads == 2, [&](auto FEW) {
             hipLaunchKernelGGL((attn_paged_merge_kernel<decltype(FEW)::value ? 2 : 8>), grid, dim3(256), 0, st,
                                a, cut->lglp, cut->lgsg, cut->merge_tiles);
             return hipSuccess;
@@ -1340,7 +1368,7 @@ extern "C" int attn_hip_launch_paged(const struct attn_paged_args *ap, const str
 
 extern "C" int attn_hip_launch_kv_append(const struct attn_kv_args *ap, int bits, int pairs, void *stream) {
     const attn_kv_args &a = *ap;
-    const long grid = (long)a.B * a.tblk * a.ublk;
+    const long grid = (long)a.B * a.tblk;
     if (grid <= 0 || grid > ATTN_PAGED_MAX_GRID)
         return (int)hipErrorInvalidValue;
     return (int)with_flag(bits == 4, [&](auto F) {
@@ -1354,7 +1382,7 @@ extern "C" int attn_hip_launch_kv_append(const struct attn_kv_args *ap, int bits
 
 extern "C" int attn_hip_launch_kv_read(const struct attn_kv_args *ap, int bits, void *stream) {
     const attn_kv_args &a = *ap;
-    const long grid = (long)a.B * a.tblk * a.ublk;
+    const long grid = (long)a.B * a.tblk;
     if (grid <= 0 || grid > ATTN_PAGED_MAX_GRID)
         return (int)hipErrorInvalidValue;
     return (int)with_flag(bits == 4, [&](auto F) {
