@@ -132,7 +132,7 @@ static void paged_run(const char *who, const struct attn_kv_cache *c, const stru
     if (max_kv > c->table_cols * c->page)
         max_kv = c->table_cols * c->page;
     const struct attn_paged_cut cut =
-        attn_paged_cut_of(c->B, c->Hkv, Hq / c->Hkv, T, max_q, max_kv, c->D);
+        attn_paged_cut_of(c->B, c->Hkv, Hq / c->Hkv, T, max_q, max_kv, c->D, c->bits, causal != 0);
     a.tps = cut.tps, a.nsplit = cut.nsplit, a.teams = cut.teams, a.deal = cut.deal, a.share = cut.share;
     /* the scratch of attn_flash: m, l and acc[D] of ATTN_SLOTS partials, each on 256 bytes */
     a.pm = (float *)scratch;

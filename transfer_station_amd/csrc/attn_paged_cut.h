@@ -50,10 +50,11 @@ struct attn_paged_cut {
     int rows16, tps, nsplit, teams, deal, share;
     int64_t grid;
     int lglp, lgsg, merge_tiles, merge_loads;
+    int halves; /* prefill: eight waves on key halves instead of four */
 };
 
 static inline struct attn_paged_cut attn_paged_cut_of(int B, int Hkv, int g, int T, int max_q, int max_kv,
-                                                      int D) {
+                                                      int D, int bits, int causal) {
     if (max_kv > 1 << 30) /* what a row of the table can hold */
         max_kv = 1 << 30;
     const int64_t rows = (int64_t)(max_q < T ? max_q : T) * g;
@@ -64,10 +65,14 @@ static inline struct attn_paged_cut attn_paged_cut_of(int B, int Hkv, int g, int
         tps = ATTN_PAGED_MAX_GRID / 16 / seqs > 1 ? ATTN_PAGED_MAX_GRID / 16 / seqs : 1;
     const int64_t cap = ATTN_SLOTS / ((int64_t)T * Hkv * g);
     const int64_t units = ((int64_t)max_kv + 127) / 128;
-    struct attn_paged_cut c = {rows16, (int)tps, 1, 0, 1, 1 << 30, 0, 0, 0, 0, 8};
+    struct attn_paged_cut c = {rows16, (int)tps, 1, 0, 1, 1 << 30, 0, 0, 0, 0, 8, 0};
     int64_t likely = 1; /* parts of a sequence */
     if (rows16 <= 2) {
-        int64_t teams = (ATTN_PAGED_DECODE_WG + tps - 1) / tps;
+        /* Two workgroups per CU, but one at head dims past 128 in bf16 (us, 512 -> 256 workgroups: 32 sequences
+         * of 4096 keys 177 -> 170, one of 32768 33.5 -> 31), and in 4 bits where they would have less than four
+         * units each (one of 32768 22.0 -> 20.4; 32 of 4096 stay at 57, 71 with 256). */
+        const int one = D > 128 && (bits == 16 || seqs * units < 2048);
+        int64_t teams = ((one ? ATTN_PAGED_DECODE_WG / 2 : ATTN_PAGED_DECODE_WG) + tps - 1) / tps;
         if (teams > seqs * units)
             teams = seqs * units;
         if (cap >= 2) {
@@ -78,7 +83,28 @@ static inline struct attn_paged_cut attn_paged_cut_of(int B, int Hkv, int g, int
         }
         c.grid = (c.teams ? c.teams : seqs) * tps;
     } else {
-        int64_t ns = (512 + seqs * tps - 1) / (seqs * tps);
+        /* Eight waves on key halves, one workgroup per CU (256 of them), where there is at most a round of
+         * them, or two of a causal prompt's tiles, whose lengths differ. Four waves, two workgroups per
+         * CU, otherwise. us at D = 128, 32 heads on 8 kv heads, four waves -> key halves: 512 tokens over
+         * 8192 keys 85 -> 79, 128 over 4096 30.6 -> 26.7, prompts of 1200 35.7 -> 30.2 and 2048 55.4 -> 52.2;
+         * kept at four: 1200 over 8192 (300 tiles) 204 and 224, 4096 over 4096 147 and 162. */
+        const int64_t w = seqs * tps;
+        c.halves = rows16 == 8 && D <= 128 &&
+                   (w <= 256 || (w <= 512 && causal && max_kv / 2 <= max_q));
+        int64_t ns = 1;
+        if (!c.halves) {
+            ns = (512 + w - 1) / w;
+        } else if (w <= 256) {
+            /* The parts that take the least time: rounds of a tile over its part's keys (us at 4.3 TFLOP/s per
+             * CU), and for each part its rows written and read again (6 TB/s). */
+            double best = 0;
+            for (int64_t n = 1; n <= 16 && (n == 1 || n * 256 <= max_kv); ++n) {
+                const double t = (double)((w * n + 255) / 256) / (double)n * 128 * max_kv * D * 4 / 4.3e6 +
+                                 (n > 1 ? 4 + (double)n * (double)seqs * (double)rows * D * 8 / 6e6 : 0);
+                if (n == 1 || t < best)
+                    best = t, ns = n;
+            }
+        }
         ns = ns > units ? units : ns;
         ns = ns > cap ? cap : ns;
         ns = ns > ATTN_PAGED_MAX_PARTS ? ATTN_PAGED_MAX_PARTS : ns;

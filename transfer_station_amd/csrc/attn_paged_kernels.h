@@ -50,17 +50,23 @@ __device__ __forceinline__ uint32_t bf16_pair(float a, float b) {
     return __builtin_bit_cast(uint32_t, r);
 }
 
-// A score in units of log2, from the raw dot product: capped, then lowered by the distance.
-// cap tanh(x / cap) = cap (1 - 2 / (2^(2 log2(e) x / cap) + 1)) is off by a few 2^-24 of the cap,
-// which is below what P's rounding to bf16 does.
-__device__ __forceinline__ float score2(float s, float c, float cap_in, float cap_out, float slope,
-                                        int dist) {
-    float t = s * c;
-    if (cap_out != 0.f) {
-        const float y = fast_exp2(s * cap_in);
-        t = cap_out - 2.f * cap_out * __builtin_amdgcn_rcpf(y + 1.f);
+// Scores in units of log2 from raw dot products: each(f) applies f(score, offset of its key behind the first)
+// to all of them, `first` is how far the row's position lies behind the first key. The tests are uniform, and
+// outside the loops over the scores.
+//   cap tanh(x / cap) = cap (1 - 2 / (2^(2 log2(e) x / cap) + 1)), off by a few 2^-24 of the cap, which is below
+//   what P's rounding to bf16 does; the distance is exact up to 2^24 tokens, and its absolute value free.
+template <typename E>
+__device__ __forceinline__ void modify_scores(const attn_paged_args &a, float slope, int first, E &&each) {
+    if (a.cap_out != 0.f)
+        each([&](float s, int) {
+            return fmaf(-2.f * a.cap_out, __builtin_amdgcn_rcpf(fast_exp2(s * a.cap_in) + 1.f), a.cap_out);
+        });
+    else
+        each([&](float s, int) { return s * a.c; });
+    if (a.slopes) {
+        const float d = (float)first;
+        each([&](float s, int off) { return fmaf(-slope, fabsf(d - (float)off), s); });
     }
-    return t - slope * (float)abs(dist);
 }
 
 __device__ __forceinline__ attn_seq seq_at(const attn_paged_args &a, int b) {
@@ -153,10 +159,13 @@ struct kv_block {
     int64_t row;
     int n;
 };
+// The id of the page that key kb's block is in, for kend >= 1. Its scalar load is issued a tile ahead: waited
+// for where its rows are asked for, every tile began with its latency.
+__device__ __forceinline__ int page_id(const attn_paged_args &a, const int32_t *table, int kb, int kend) {
+    return scalar_i32(table, min(kb, kend - 1) >> a.lgp);
+}
 template <int N = 16>
-__device__ __forceinline__ kv_block block_at(const attn_paged_args &a, const int32_t *table, int u,
-                                             int kb, int kend) {
-    const int pg = scalar_i32(table, min(kb, kend - 1) >> a.lgp);
+__device__ __forceinline__ kv_block block_in(const attn_paged_args &a, int pg, int u, int kb, int kend) {
     const bool ok = attn_page_ok(pg, a.pages);
     return kv_block{attn_page_row(ok ? pg : 0, a.Hkv, u, kb, a.lgp), ok ? max(0, min(N, kend - kb)) : 0};
 }
@@ -362,7 +371,7 @@ __global__ __launch_bounds__(256, 2) void attn_paged_decode_kernel(const attn_pa
                 }
             }
         };
-        auto compute = [&](int tb, int tn, const kv_block &b0, const kv_block &b1, const kv_block &n0,
+        auto compute = [&](int tb, const kv_block &b0, const kv_block &b1, const kv_block &n0,
                            const kv_block &n1, frags &f) __attribute__((always_inline)) {
             bf16x8 kf[2][KN], pk[NRB];
             f32x4 s[NRB][2];
@@ -389,19 +398,25 @@ __global__ __launch_bounds__(256, 2) void attn_paged_decode_kernel(const attn_pa
             __builtin_amdgcn_sched_barrier(0);
             if (kLate)
                 load_v(b0, b1, f);
-            else if (tn < kstop)
+            else
                 load_k(n0, n1, f);
 #pragma unroll
             for (int i = 0; i < NRB; ++i) {
                 // Register (t, j) of this lane holds key tb + 16t + 4grp + j for row r16.
+                if (MOD)
+                    modify_scores(a, slope[i], pos[i] - tb - 4 * grp, [&](auto f) __attribute__((always_inline)) {
+#pragma unroll
+                        for (int t = 0; t < 2; ++t)
+#pragma unroll
+                            for (int j = 0; j < 4; ++j)
+                                s[i][t][j] = f(s[i][t][j], 16 * t + j);
+                    });
                 float mx = kNegInf;
 #pragma unroll
                 for (int t = 0; t < 2; ++t)
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         const int key = tb + 16 * t + 4 * grp + j;
-                        if (MOD)
-                            s[i][t][j] = score2(s[i][t][j], a.c, a.cap_in, a.cap_out, slope[i], pos[i] - key);
                         if (key > lim[i] || (t ? b1.n : b0.n) == 0)
                             s[i][t][j] = kNegInf;
                         mx = fmaxf(mx, s[i][t][j]);
@@ -446,12 +461,27 @@ __global__ __launch_bounds__(256, 2) void attn_paged_decode_kernel(const attn_pa
         int tb = k0 + 32 * w;
         if (tb < kstop) {
             frags f[AHEAD];
-            kv_block b0[AHEAD + 1], b1[AHEAD + 1];
+            kv_block b0[AHEAD], b1[AHEAD];
+            int pg0[AHEAD], pg1[AHEAD], pn0, pn1;
 #pragma unroll
             for (int i = 0; i < AHEAD; ++i) {
-                b0[i] = block_at(a, table, u, tb + 128 * i, k1);
-                b1[i] = block_at(a, table, u, tb + 128 * i + 16, k1);
-                if (!kLate && tb + 128 * i < kstop) {
+                pg0[i] = page_id(a, table, tb + 128 * i, k1);
+                pg1[i] = page_id(a, table, tb + 128 * i + 16, k1);
+            }
+            pn0 = page_id(a, table, tb + 128 * AHEAD, k1);
+            pn1 = page_id(a, table, tb + 128 * AHEAD + 16, k1);
+            // Blocks of the tile at t; past the last tile they are empty and their loads read nothing. No branch
+            // goes around a load: a wait behind it would have to be for all of them.
+            auto blocks = [&](int t, int p0, int p1, kv_block &x, kv_block &y) __attribute__((always_inline)) {
+                x = block_in(a, p0, u, t, k1);
+                y = block_in(a, p1, u, t + 16, k1);
+                if (t >= kstop)
+                    x.n = y.n = 0;
+            };
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i) {
+                blocks(tb + 128 * i, pg0[i], pg1[i], b0[i], b1[i]);
+                if (!kLate) {
                     load_v(b0[i], b1[i], f[i]);
                     load_k(b0[i], b1[i], f[i]);
                 }
@@ -462,17 +492,18 @@ __global__ __launch_bounds__(256, 2) void attn_paged_decode_kernel(const attn_pa
                     const int t = tb + 128 * i, tn = t + 128 * AHEAD;
                     if (i > 0 && t >= kstop)
                         break;
-                    const kv_block n0 = block_at(a, table, u, tn, k1);
-                    const kv_block n1 = block_at(a, table, u, tn + 16, k1);
+                    kv_block n0, n1;
+                    blocks(tn, pn0, pn1, n0, n1);
+                    pn0 = page_id(a, table, tn + 128, k1);
+                    pn1 = page_id(a, table, tn + 144, k1);
                     if (kLate) {
                         load_k(b0[i], b1[i], f[i]);
                     } else {
                         put_v(f[i]);
                         __builtin_amdgcn_sched_barrier(0);
-                        if (tn < kstop)
-                            load_v(n0, n1, f[i]);
+                        load_v(n0, n1, f[i]);
                     }
-                    compute(t, tn, b0[i], b1[i], n0, n1, f[i]);
+                    compute(t, b0[i], b1[i], n0, n1, f[i]);
                     b0[i] = n0;
                     b1[i] = n1;
                 }
@@ -683,14 +714,19 @@ __global__ __launch_bounds__(256) void attn_paged_merge_kernel(const attn_paged_
 // The running maximum is raised only where a tile's is more than 2^8 above it, so that O is rarely rescaled;
 // p stays below 2^8.
 // ------------------------------------------------------------------------------------------
+// Bound on a lane's sum of p over a tile against a maximum that may lie below the tile's: p costs no precision
+// up to it, only exponent range.
+constexpr float kPagedSum = 65536.0f;
+
 constexpr int paged_tile_keys(int DP, bool F4) { return DP == 64 ? (F4 ? 64 : 128) : DP == 128 ? 64 : 32; }
 
-template <int DP, bool F4, bool MOD, int KH>
-__global__ __launch_bounds__(256, 2) void attn_paged_prefill_kernel(const attn_paged_args a) {
-    constexpr int KT = paged_tile_keys(DP, F4), KN = DP / 16, RWV = KT / 4; // rows a wave stages
-    constexpr int PW = KT * DP / 2048;                    // 1 KB blocks of a bf16 tile per wave
+template <int DP, bool F4, bool MOD, int KH, int NW>
+__global__ __launch_bounds__(64 * NW, 8 / NW) void attn_paged_prefill_kernel(const attn_paged_args a) {
+    constexpr int KT = paged_tile_keys(DP, F4) * NW / 4, KN = DP / 16, RWV = KT / NW; // rows a wave stages
+    constexpr int PW = KT * DP / 512 / NW;                // 1 KB blocks of a bf16 tile per wave
     constexpr int NBK = RWV <= 16 ? 1 : RWV / 16;         // blocks of 16 keys per wave
-    constexpr int NR = 4 / KH, BQ = 32 * NR, KW = KT / KH, NT = KW / 32; // rows, keys of a wave
+    constexpr int AUX = KH == 2 && NW == 4 ? kDmaNT : 0;  // a sequence's only row tile: its keys are read once
+    constexpr int NR = NW / KH, BQ = 32 * NR, KW = KT / KH, NT = KW / 32; // rows, keys of a wave
     constexpr int LB = RWV * DP / 2 / 64; // 4 bits: bytes of codes per lane (16, or 8 at DP = 64)
     static_assert(NT >= 1 && PW % NBK == 0 && (!F4 || (NBK == 1 && LB * 2 % 16 == 0)), "tile shape");
     // Each buffer is a variable of its own: the compiler tells LDS accesses apart by variable.
@@ -717,7 +753,6 @@ __global__ __launch_bounds__(256, 2) void attn_paged_prefill_kernel(const attn_p
     const int wr = KH > 1 ? w % NR : w, kh = KH > 1 ? w / NR : 0;
     const int g = a.Hq / a.Hkv, R = sq.n * g, D = a.D;
     const float c = MOD ? 1.f : a.c;
-    const float lift = 8.f / c; // how far a score may pass the running maximum
 
     // Offsets of this lane's operand reads (elements): K row kperm, chunk 2kk + hi; V rows 8hi + i16 / 4
     // (+ 4), columns 16 (g16 & 1) + 4 (i16 & 3); and the wave's keys of the tile.
@@ -748,24 +783,32 @@ __global__ __launch_bounds__(256, 2) void attn_paged_prefill_kernel(const attn_p
     };
     constexpr int RB = DP / 2, SB = DP / 32; // bytes of a row's codes and scales
     // The wave's rows of the tile from key kb: into LDS, or (4 bits) into registers.
-    auto load = [&](int kb, [[maybe_unused]] uint16_t *Kd, [[maybe_unused]] uint16_t *Vd,
-                    [[maybe_unused]] stage &f) __attribute__((always_inline)) {
+    int pid[NBK]; // the pages of the wave's blocks of the next tile to load
+    auto pages_of = [&](int kb) __attribute__((always_inline)) {
+#pragma unroll
+        for (int h = 0; h < NBK; ++h)
+            pid[h] = page_id(a, table, kb + RWV * w + 16 * h, k1);
+    };
+    auto load = [&](int kb, [[maybe_unused]] int kstop, [[maybe_unused]] uint16_t *Kd,
+                    [[maybe_unused]] uint16_t *Vd, [[maybe_unused]] stage &f) __attribute__((always_inline)) {
         if constexpr (!F4) {
             const uint32_t rb = (uint32_t)D * 2u;
 #pragma unroll
             for (int h = 0; h < NBK; ++h) {
-                const kv_block m = block_at<(RWV < 16 ? RWV : 16)>(a, table, u, kb + RWV * w + 16 * h, k1);
+                const kv_block m = block_in<(RWV < 16 ? RWV : 16)>(a, pid[h], u, kb + RWV * w + 16 * h, k1);
                 const auto kr = make_rsrc(a.k + m.row * rb, m.n * rb);
                 const auto vr = make_rsrc(a.v + m.row * rb, m.n * rb);
 #pragma unroll
                 for (int p = h * PW / NBK; p < (h + 1) * PW / NBK; ++p)
-                    dma16<0>(kr, Kd + (w * PW + p) * 512, kso[p]);
+                    dma16<0, AUX>(kr, Kd + (w * PW + p) * 512, kso[p]);
 #pragma unroll
                 for (int p = h * PW / NBK; p < (h + 1) * PW / NBK; ++p)
-                    dma16<0>(vr, Vd + (w * PW + p) * 512, vso[p]);
+                    dma16<0, AUX>(vr, Vd + (w * PW + p) * 512, vso[p]);
             }
         } else {
-            const kv_block m = block_at<(RWV < 16 ? RWV : 16)>(a, table, u, kb + RWV * w, k1);
+            kv_block m = block_in<(RWV < 16 ? RWV : 16)>(a, pid[0], u, kb + RWV * w, k1);
+            if (kb >= kstop) // nothing is read; no branch goes around the loads, whose waits would then be for all
+                m.n = 0;
             const auto kr = make_rsrc(a.k + m.row * RB, m.n * RB), vr = make_rsrc(a.v + m.row * RB, m.n * RB);
             const auto ksr = make_rsrc(a.ks + m.row * SB, m.n * SB);
             const auto vsr = make_rsrc(a.vs + m.row * SB, m.n * SB);
@@ -811,14 +854,12 @@ __global__ __launch_bounds__(256, 2) void attn_paged_prefill_kernel(const attn_p
                 fp4_to_bf16(y[j], vsc);
         }
     };
-    // Every 16 keys of the tile from kb have a page, and the part reaches past them.
-    auto whole = [&](int kb) __attribute__((always_inline)) {
-        bool ok = kb + KT <= k1;
-#pragma unroll
-        for (int j = 0; j < KT; j += 16)
-            ok &= attn_page_ok(scalar_i32(table, min(kb + j, k1 - 1) >> a.lgp), a.pages) != 0;
-        return ok;
-    };
+    // Whether any page of the part is none: looked for once, so that tiles need no look of their own.
+    bool lost = false;
+    if (k1 > k0)
+        for (int x = (k0 >> a.lgp) + lane; x <= (k1 - 1) >> a.lgp; x += 64)
+            lost |= !attn_page_ok(table[x], a.pages);
+    const bool holes = __builtin_amdgcn_ballot_w64(lost) != 0;
 
     for (int tile = t0; (int64_t)tile * BQ < R; tile += a.tps) {
         const int row0 = tile * BQ, row = row0 + 32 * wr + l32;
@@ -852,7 +893,7 @@ __global__ __launch_bounds__(256, 2) void attn_paged_prefill_kernel(const attn_p
                 o[db][i] = 0.f;
 
         // One tile from key kb, in the buffers Kb and Vb.
-        auto compute = [&](int kb, bool all, const uint16_t *Kb, const uint16_t *Vb)
+        auto compute = [&](int kb, const uint16_t *Kb, const uint16_t *Vb)
             __attribute__((always_inline)) {
             const int kw = kb + kh * KW; // the wave's first key
             if (kw > wmax)
@@ -885,18 +926,19 @@ __global__ __launch_bounds__(256, 2) void attn_paged_prefill_kernel(const attn_p
             }
             // Register i of sub-tile t: key kw + 32t + 16 (i / 8) + 8hi + i % 8.
             if (MOD)
+                modify_scores(a, slope, pos - kw - 8 * hi, [&](auto f) __attribute__((always_inline)) {
 #pragma unroll
-                for (int t = 0; t < NT; ++t)
+                    for (int t = 0; t < NT; ++t)
 #pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        s[t][i] = score2(s[t][i], a.c, a.cap_in, a.cap_out, slope,
-                                         pos - (kw + 32 * t + 16 * (i >> 3) + 8 * hi + (i & 7)));
-            if (!all || kw + KW - 1 > wmin) {
-                // A block without a page hides its keys: looked up again here, where it is rare.
+                        for (int i = 0; i < 16; ++i)
+                            s[t][i] = f(s[t][i], 32 * t + 16 * (i >> 3) + (i & 7));
+                });
+            if (holes || kw + KW - 1 > wmin) {
+                // A block without a page hides its keys.
                 uint32_t none = 0;
 #pragma unroll
-                for (int j = 0; j < KW / 16; ++j)
-                    none |= attn_page_ok(scalar_i32(table, min(kw + 16 * j, k1 - 1) >> a.lgp), a.pages) ? 0u : 1u << j;
+                for (int j = 0; holes && j < KW / 16; ++j)
+                    none |= attn_page_ok(page_id(a, table, kw + 16 * j, k1), a.pages) ? 0u : 1u << j;
 #pragma unroll
                 for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -905,15 +947,31 @@ __global__ __launch_bounds__(256, 2) void attn_paged_prefill_kernel(const attn_p
                             (none >> (2 * t + (i >> 3)) & 1))
                             s[t][i] = kNegInf;
             }
-            float mx = kNegInf;
+            bf16x8 pk[2 * NT];
+            // p against the running maximum m as it is; a lane whose sum of them passes kPagedSum (or whose row
+            // has no m yet) sends its wave to raise m to the tile's maximum and take p again.
+            float psum;
+            auto weigh = [&]() __attribute__((always_inline)) {
+                const float mc = m_run == kNegInf ? 0.f : m_run * c;
+                psum = 0.f;
 #pragma unroll
-            for (int t = 0; t < NT; ++t)
+                for (int t = 0; t < NT; ++t)
 #pragma unroll
-                for (int i = 0; i < 16; i += 2)
-                    mx = max3f(mx, s[t][i], s[t][i + 1]);
-            mx = max_xor32(mx);
-            if (__builtin_amdgcn_ballot_w64(mx > m_run + lift) != 0) {
-                const float mnew = fmaxf(m_run, mx);
+                    for (int i = 0; i < 16; ++i) {
+                        const float p = fast_exp2(fmaf(s[t][i], c, -mc));
+                        psum += p;
+                        pk[2 * t + (i >> 3)][i & 7] = (__bf16)p;
+                    }
+            };
+            weigh();
+            if (__builtin_amdgcn_ballot_w64(!(psum <= kPagedSum) || m_run == kNegInf) != 0) {
+                float mx = kNegInf;
+#pragma unroll
+                for (int t = 0; t < NT; ++t)
+#pragma unroll
+                    for (int i = 0; i < 16; i += 2)
+                        mx = max3f(mx, s[t][i], s[t][i + 1]);
+                const float mnew = fmaxf(m_run, max_xor32(mx));
                 const float alpha = fast_exp2((m_run - (mnew == kNegInf ? 0.f : mnew)) * c);
                 m_run = mnew;
                 l_run *= alpha;
@@ -922,17 +980,9 @@ __global__ __launch_bounds__(256, 2) void attn_paged_prefill_kernel(const attn_p
 #pragma unroll
                     for (int i = 0; i < 16; ++i)
                         o[db][i] *= alpha;
+                weigh();
             }
-            const float mc = m_run == kNegInf ? 0.f : m_run * c;
-            bf16x8 pk[2 * NT];
-#pragma unroll
-            for (int t = 0; t < NT; ++t)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const float p = fast_exp2(fmaf(s[t][i], c, -mc));
-                    l_run += p;
-                    pk[2 * t + (i >> 3)][i & 7] = (__bf16)p;
-                }
+            l_run += psum;
             const uint16_t *vp = Vb + vfo;
 #pragma unroll
             for (int cc = 0; cc < 2 * NT; ++cc)
@@ -946,35 +996,33 @@ __global__ __launch_bounds__(256, 2) void attn_paged_prefill_kernel(const attn_p
         auto wait_loads = [] { __builtin_amdgcn_s_waitcnt(waitcnt_vm(0)); };
 
         stage st[2];
-        bool all = true;
         if (k0 < kstop) {
-            load(k0, Ks0, Vs0, st[0]);
-            all = whole(k0);
+            pages_of(k0);
+            load(k0, kstop, Ks0, Vs0, st[0]);
+            pages_of(k0 + KT);
             if constexpr (F4) {
-                if (k0 + KT < kstop)
-                    load(k0 + KT, Ks1, Vs1, st[1]);
+                load(k0 + KT, kstop, Ks1, Vs1, st[1]);
+                pages_of(k0 + 2 * KT);
                 put(st[0], Ks0, Vs0);
-            } else {
-                wait_loads();
             }
         }
+        // Q has arrived as well: waited for at its first use, inside the loop, it would be waited for there on
+        // every tile, together with the loads of the next ones.
+        wait_loads();
         __syncthreads();
         // Tile i (0 or 1, in buffer i); f: the registers of the tile after it (4 bits).
         auto step = [&](int kb, const uint16_t *Kb, const uint16_t *Vb, uint16_t *Kn, uint16_t *Vn, stage &f,
                         stage &f2) __attribute__((always_inline)) {
-            const bool more = kb + KT < kstop, more2 = kb + 2 * KT < kstop;
+            const bool more = kb + KT < kstop;
             if constexpr (F4) {
-                if (more2)
-                    load(kb + 2 * KT, nullptr, nullptr, f2);
+                load(kb + 2 * KT, kstop, nullptr, nullptr, f2);
             } else if (more) {
-                load(kb + KT, Kn, Vn, f);
+                load(kb + KT, kstop, Kn, Vn, f);
             }
-            const bool now = all;
-            all = more && whole(kb + KT);
-            compute(kb, now, Kb, Vb);
+            pages_of(kb + (F4 ? 3 : 2) * KT);
+            compute(kb, Kb, Vb);
             if constexpr (F4) {
-                if (more)
-                    put(f, Kn, Vn);
+                put(f, Kn, Vn);
             } else {
                 wait_loads(); // this wave's part of the next tile has arrived
             }
@@ -990,8 +1038,8 @@ __global__ __launch_bounds__(256, 2) void attn_paged_prefill_kernel(const attn_p
         bool writes = valid;
         if constexpr (KH > 1) {
             // Join the halves of the tiles: the second half's waves leave (m, l) and O in LDS.
-            static_assert(KT >= 64, "a wave's O fits a buffer");
-            float *kho = reinterpret_cast<float *>(wr == 0 ? Ks0 : Vs0) + lane;
+            static_assert(KT * 4 >= 64 * NW, "O of the second half's waves fits two buffers");
+            float *kho = reinterpret_cast<float *>(wr & 1 ? Vs0 : Ks0) + (wr >> 1) * DP * 32 + lane;
             if (kh == 1) {
                 kh_ml[wr * 64 + lane] = m_run * c;
                 kh_ml[NR * 64 + wr * 64 + lane] = l_run;
@@ -1317,19 +1365,27 @@ hipError_t launch_paged_d(const attn_paged_args &a, const attn_paged_cut &cut, h
                 return with_flag(a.tps == 1, [&](auto NT) {
                     return decode(std::integral_constant<int, 2>{}, NT);
                 });
-        auto prefill = [&](auto KHF) {
-            constexpr int kK = decltype(KHF)::value;
+        auto prefill = [&](auto KHF, auto NWF) {
+            constexpr int kK = decltype(KHF)::value, kW = decltype(NWF)::value;
             if (t_plan)
-                plan_note(grid, block, "attn_paged_prefill_kernel<%d, %d, %s, %d> parts=%d share=%d", DP,
-                          F4 ? 4 : 16, tf(kM), kK, a.nsplit, a.share);
+                plan_note(grid, dim3(64 * kW), "attn_paged_prefill_kernel<%d, %d, %s, %d, %d> parts=%d share=%d",
+                          DP, F4 ? 4 : 16, tf(kM), kK, kW, a.nsplit, a.share);
             else
-                hipLaunchKernelGGL((attn_paged_prefill_kernel<DP, F4, kM, kK>), grid, block, 0, st, a);
+                hipLaunchKernelGGL((attn_paged_prefill_kernel<DP, F4, kM, kK, kW>), grid, dim3(64 * kW), 0, st,
+                                   a);
             return hipGetLastError();
         };
-        if constexpr (DP <= 128)
+        constexpr std::integral_constant<int, 1> one;
+        constexpr std::integral_constant<int, 2> two;
+        constexpr std::integral_constant<int, 4> four;
+        constexpr std::integral_constant<int, 8> eight;
+        if constexpr (DP <= 128) {
             if (cut.rows16 == 4)
-                return prefill(std::integral_constant<int, 2>{});
-        return prefill(std::integral_constant<int, 1>{});
+                return prefill(two, four);
+            if (cut.halves)
+                return prefill(two, eight);
+        }
+        return prefill(one, four);
     });
 }
 
