@@ -320,7 +320,7 @@ def test_split_parts_join():
         c = pu.Cache([(n, kv), (n, 100)], Hkv, 128, 64, bits, 3)
         c.fill(17)
         plan = ts.attn_paged_plan(c.device(), c.N, Hq, 1, None, n, kv)
-        assert plan[-1][0] == "attn_paged_merge_kernel", plan
+        assert plan[-1][0].startswith("attn_paged_merge_kernel<"), plan
         q = pu.normal((c.N, Hq, 128), 5, 3.0)
         ref, bound = pu.attend_ref(c, q, Hq, 1)
         check(pu.attend(c, q, Hq, 1), ref, bound, (bits, n, kv))

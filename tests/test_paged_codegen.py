@@ -1,0 +1,89 @@
+"""CPU checks of the paged kernels' generated gfx950 code (no GPU needed): what their speed rests on and no result
+shows. Decode keeps a tile's loads in flight while it works on the one before; prefill orders its LDS-DMA itself;
+neither spills where the registers were counted on."""
+import os
+import re
+import shutil
+import subprocess
+
+import pytest
+
+from transfer_station_amd import build as _build
+
+ROCM = os.environ.get("ROCM_PATH", "/opt/rocm")
+OBJDUMP = os.path.join(ROCM, "llvm", "bin", "llvm-objdump")
+READELF = os.path.join(ROCM, "llvm", "bin", "llvm-readelf")
+
+
+@pytest.fixture(scope="module")
+def code(tmp_path_factory):
+    """(instruction lists, spilled vector registers) by kernel name."""
+    tmp = str(tmp_path_factory.mktemp("paged"))
+    if not os.path.exists(_build.lib_path()):
+        pytest.skip("library not built")
+    if not os.access(READELF, os.X_OK) or not os.access(OBJDUMP, os.X_OK):
+        pytest.skip("llvm tools not found under %s" % ROCM)
+    copy = os.path.join(tmp, "lib.so")
+    shutil.copy(_build.lib_path(), copy)
+    subprocess.run([OBJDUMP, "--offloading", copy], cwd=tmp, check=True, stdout=subprocess.DEVNULL,
+                   stderr=subprocess.DEVNULL)
+    obj = os.path.join(tmp, [f for f in os.listdir(tmp) if f.endswith("gfx950")][0])
+    text = subprocess.run([OBJDUMP, "-d", "--mcpu=gfx950", obj], check=True, stdout=subprocess.PIPE,
+                          universal_newlines=True).stdout
+    notes = subprocess.run([READELF, "--notes", obj], check=True, stdout=subprocess.PIPE,
+                           universal_newlines=True).stdout
+    funcs, cur = {}, None
+    for line in text.split("\n"):
+        m = re.match(r"^[0-9a-f]+ <(\S+)>:", line)
+        if m:
+            cur = funcs.setdefault(m.group(1), []) if "paged" in m.group(1) else None
+        elif cur is not None and line.startswith("\t"):
+            ins = line.strip().split("//")[0].strip()
+            if ins:
+                cur.append(ins)
+    spills = {m.group(1): int(m.group(2)) for m in re.finditer(
+        r"\.symbol: +'?(\S*?paged\S*?)\.kd'?\n(?:.*\n)*? +\.vgpr_spill_count: +(\d+)", notes)}
+    return funcs, spills
+
+
+def test_no_spills(code):
+    spills = code[1]
+    decode = {n: c for n, c in spills.items() if "paged_decode" in n}
+    prefill = {n: c for n, c in spills.items() if re.search(r"paged_prefill_kernelILi(64|128)E", n)}
+    assert len(decode) >= 30 and len(prefill) >= 20, (len(decode), len(prefill))
+    bad = {n: c for n, c in {**decode, **prefill}.items() if c}
+    assert not bad, bad
+
+
+def test_decode_keeps_the_next_tiles_loads_in_flight(code):
+    """Of bf16 rows, up to D = 128 and for one block of 16 rows: no wait between the products of a tile is for all
+    loads. The next tile's V is asked for before this tile's scores and its K before the products with V, so four
+    loads or more stay out (with two blocks of rows the compiler puts V behind half the scores, which is as fast)."""
+    n = 0
+    for name, ins in code[0].items():
+        if not re.search(r"paged_decode_kernelILi(64|128)ELb0ELi1E", name):
+            continue
+        n += 1
+        mf = [i for i, x in enumerate(ins) if x.startswith("v_mfma")]
+        waits = [int(re.search(r"vmcnt\((\d+)\)", x).group(1)) for x in ins[mf[0] - 8:mf[-1]]
+                 if x.startswith("s_waitcnt") and "vmcnt" in x]
+        assert len(waits) >= 4 and min(waits) >= 4, (name, waits)
+    assert n == 8, n
+
+
+def test_prefill_waits_for_its_dma_at_the_end_of_a_tile(code):
+    """No wait on the DMA in flight stands before an LDS read of the tile at work."""
+    n = 0
+    for name, ins in code[0].items():
+        if not re.search(r"paged_prefill_kernelILi\d+ELb0E", name):
+            continue
+        n += 1
+        mf = [i for i, x in enumerate(ins) if x.startswith("v_mfma")]
+        bad = []
+        for i in range(mf[0], mf[-1]):
+            if ins[i].startswith("s_waitcnt") and "vmcnt" in ins[i]:
+                nxt = [y for y in ins[i + 1:i + 6] if not y.startswith(("s_waitcnt", "s_nop"))]
+                if nxt and nxt[0].startswith("ds_read"):
+                    bad.append(i)
+        assert not bad, (name, bad)
+    assert n >= 12

@@ -141,6 +141,44 @@ def test_refusals():
             assert msg in err, (code, err)
 
 
+PLANS = [
+    # bits, D, B, Hq, Hkv, max_q, max_kv, causal, modified scores, first kernel, its notes, grid, kernels
+    # one to 16 rows of a kv head: 512 workgroups, 256 in bf16 past D = 128, fewer where there are fewer units
+    (16, 128, 64, 32, 8, 1, 8192, 1, 0, "decode_kernel<128, 16, 1, false, true>", "teams=512 parts=32", 512, 2),
+    (16, 128, 1, 32, 8, 1, 777, 1, 0, "decode_kernel<128, 16, 1, false, true>", "teams=56 parts=8", 56, 2),
+    (16, 256, 32, 32, 8, 1, 4096, 1, 0, "decode_kernel<256, 16, 1, false, true>", "teams=256 parts=33", 256, 2),
+    (4, 256, 32, 32, 8, 1, 4096, 1, 1, "decode_kernel<256, 4, 1, true, true>", "teams=512 parts=33", 512, 2),
+    (4, 256, 1, 16, 4, 1, 32768, 1, 0, "decode_kernel<256, 4, 1, false, true>", "teams=256 parts=256", 256, 2),
+    # more rows in all than there are partial slots for two parts: a workgroup per sequence
+    (16, 64, 2100, 32, 8, 1, 500, 1, 0, "decode_kernel<64, 16, 1, false, true>", "teams=0 parts=1", 16800, 1),
+    # two row blocks; at D > 128 one, twice
+    (16, 128, 16, 32, 8, 8, 4000, 1, 0, "decode_kernel<128, 16, 2, false, true>", "teams=512 parts=16", 512, 2),
+    (4, 256, 16, 32, 8, 8, 4000, 1, 0, "decode_kernel<256, 4, 1, false, false>", "teams=256 parts=16", 512, 2),
+    # 33 to 64 rows: key halves of four waves
+    (16, 128, 16, 64, 8, 8, 4001, 1, 1, "prefill_kernel<128, 16, true, 2, 4>", "parts=4 share=1024", 512, 2),
+    (16, 256, 16, 64, 8, 8, 4001, 1, 0, "decode_kernel<256, 16, 1, false, false>", "teams=64 parts=8", 256, 2),
+    # more: up to a round of tiles, and two of a causal prompt, on key halves of eight waves
+    (16, 128, 1, 32, 8, 512, 8192, 1, 0, "prefill_kernel<128, 16, false, 2, 8>", "parts=2 share=4096", 256, 2),
+    (16, 128, 1, 32, 8, 1024, 8192, 1, 0, "prefill_kernel<128, 16, false, 2, 8>", "parts=1 share=1073741824", 256, 1),
+    (16, 128, 1, 32, 8, 2048, 2048, 1, 0, "prefill_kernel<128, 16, false, 2, 8>", "parts=1 share=1073741824", 512, 1),
+    (16, 128, 1, 32, 8, 2048, 2048, 0, 0, "prefill_kernel<128, 16, false, 1, 4>", "parts=1 share=1073741824", 512, 1),
+    (16, 128, 1, 32, 8, 1200, 8192, 1, 0, "prefill_kernel<128, 16, false, 1, 4>", "parts=1 share=1073741824", 304, 1),
+    (4, 64, 6, 24, 6, 2000, 3000, 1, 0, "prefill_kernel<64, 4, false, 1, 4>", "parts=1 share=1073741824", 2304, 1),
+    (16, 256, 1, 32, 8, 512, 4096, 1, 0, "prefill_kernel<256, 16, false, 1, 4>", "parts=4 share=1024", 512, 2),
+]
+
+
+@pytest.mark.parametrize("case", PLANS, ids=[str(i) for i in range(len(PLANS))])
+def test_kernel_choice(case):
+    """The cut at both sides of its rules: it goes by the call's numbers alone."""
+    bits, D, B, Hq, Hkv, mq, mk, causal, mod, name, notes, grid, n = case
+    c = ts.KvCache(4096, 4096, 4096, 4096, 4096, B, 65536 // 64, 1000, 64, Hkv, D, bits, 4096, 4096)
+    p = ts.attn_paged_plan(c, B * mq, Hq, causal, ts.Scores(0.0, 30.0 if mod else 0.0), mq, mk)
+    print(p)
+    assert p[0][0] == "attn_paged_" + name and p[0][1] == notes and int(p[0][2]) == grid
+    assert len(p) == n and (n == 1 or p[1][0].startswith("attn_paged_merge_kernel<"))
+
+
 def test_reference_quantiser():
     """The tests' own quantiser against the definition, element by element."""
     x = pu.normal((4, 64), 3, 5.0)

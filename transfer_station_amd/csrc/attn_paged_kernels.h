@@ -153,8 +153,8 @@ __device__ __forceinline__ int seq_of_unit(const attn_paged_args &a, const line 
     }
 }
 
-// 16 keys of the cache from key kb (a multiple of 16; or N from a multiple of N): their rows' place, and how many of them there are
-// (0 where the page id is none, or past the sequence's end).
+// N = 16 keys of the cache from key kb (a multiple of N): their rows' place, and how many of them there are (0
+// where the page id is none, or past the sequence's end).
 struct kv_block {
     int64_t row;
     int n;
@@ -228,356 +228,356 @@ __global__ __launch_bounds__(256, 2) void attn_paged_decode_kernel(const attn_pa
     uint16_t *vt = &Vw[w * VTILE];
 
     while (left > 0 && u < a.Hkv) {
-    const attn_seq sq = seq_at(a, b);
-    const int units = attn_units(sq.n, sq.kend), R = sq.n * g;
-    const int take = a.teams ? min(left, units - off) : 1;
-    attn_cover cover = {0, 1};
-    if (a.teams) {
-        cover = attn_cover_of(pos0 - off, max(units, 1), ln.quota);
-        cover = attn_cover{uniform(cover.first), uniform(cover.live)};
-    }
-    const int live = cover.live, sp = team - cover.first;
-    const int k0 = min(off * 128, sq.kend), k1 = a.teams ? min((off + take) * 128, sq.kend) : sq.kend;
-    const int32_t *table = a.table + (int64_t)b * a.cols;
-    for (int tile = t0; take > 0 && (int64_t)tile * 16 * NRB < R; tile += a.tps) {
-        const int row0 = tile * 16 * NRB;
-        bf16x8 qb[NRB][KN];
-        int lim[NRB], pos[NRB];
-        float m_run[NRB], l_run[NRB], slope[NRB];
-        f32x4 o[NRB][DP / 16];
-#pragma unroll
-        for (int i = 0; i < NRB; ++i) {
-            const int row = row0 + 16 * i + r16;
-            const bool valid = row < R;
-            const int tok = valid ? row / g : 0, h = u * g + (valid ? row % g : 0);
-            const uint16_t *q = a.q + (sq.q0 + tok) * a.q_tok + h * a.q_head;
-#pragma unroll
-            for (int kk = 0; kk < KN; ++kk) {
-                const int col = F4 ? grp * (DP / 4) + kk * 8 : kk * 32 + grp * 8;
-                u32x4 x = zero4();
-                if (valid && col < D)
-                    x = *reinterpret_cast<const u32x4 *>(q + col);
-                qb[i][kk] = as_bf16x8(x);
-            }
-            pos[i] = sq.len - sq.n + tok;
-            lim[i] = a.causal ? min(pos[i], k1 - 1) : k1 - 1;
-            slope[i] = MOD && a.slopes ? a.slopes[h] * 1.44269504088896341f : 0.f;
-            m_run[i] = kNegInf;
-            l_run[i] = 0.f;
-#pragma unroll
-            for (int db = 0; db < DP / 16; ++db)
-                o[i][db] = f32x4{0.f, 0.f, 0.f, 0.f};
+        const attn_seq sq = seq_at(a, b);
+        const int units = attn_units(sq.n, sq.kend), R = sq.n * g;
+        const int take = a.teams ? min(left, units - off) : 1;
+        attn_cover cover = {0, 1};
+        if (a.teams) {
+            cover = attn_cover_of(pos0 - off, max(units, 1), ln.quota);
+            cover = attn_cover{uniform(cover.first), uniform(cover.live)};
         }
-        // Keys from the tile's last row's position on are hidden from it.
-        const int kstop = a.causal ? min(k1, sq.len - sq.n + (min(row0 + 16 * NRB, R) - 1) / g + 1) : k1;
-
-        struct frags {
-            u32x4 k[F4 ? 1 : 2 * KN], v[F4 ? 1 : NV];
-            uint32_t kw[F4 ? 2 * KN : 1], ksc[F4 ? 2 : 1];
-            uint32_t vw[F4 ? NV4 * PB / 4 : 1], vsc[F4 ? NV4 : 1];
-        };
-        // The loads of the next tile are issued as soon as this one's have been used: V's once it is in LDS,
-        // K's once the scores are there. K and V of a tile, Q and O do not fit 256 registers at DP = 256 in
-        // bf16: there a tile's K is loaded at its start, and V once the scores have freed K's registers.
-        constexpr bool kLate = DP == 256 && !F4;
-        auto load_k = [&](const kv_block &b0, const kv_block &b1, frags &f) __attribute__((always_inline)) {
-#pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                const kv_block &bl = t ? b1 : b0;
-                if constexpr (!F4) {
-                    const uint32_t rb = (uint32_t)D * 2u; // bytes of a row
-                    const auto kr = make_rsrc(a.k + bl.row * rb, bl.n * rb);
-#pragma unroll
-                    for (int kk = 0; kk < KN; ++kk) {
-                        const int col = kk * 32 + grp * 8;
-                        f.k[t * KN + kk] = buf16<NTL>(kr, col < D ? r16 * rb + col * 2 : 0x80000000u);
-                    }
-                } else {
-                    constexpr int RB = DP / 2, SB = DP / 32; // bytes of a row's codes and scales
-                    const auto kr = make_rsrc(a.k + bl.row * RB, bl.n * RB);
-                    const auto sr = make_rsrc(a.ks + bl.row * SB, bl.n * SB);
-                    if constexpr (DP == 64) {
-                        const u32x2 x = __builtin_amdgcn_raw_buffer_load_b64(
-                            kr, r16 * RB + grp * (RB / 4), 0, NTL ? kDmaNT : 0);
-                        f.kw[t * KN] = x[0];
-                        f.kw[t * KN + 1] = x[1];
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < KN / 4; ++j) {
-                            const u32x4 x = buf16<NTL>(kr, r16 * RB + grp * (RB / 4) + 16 * j);
-#pragma unroll
-                            for (int i = 0; i < 4; ++i)
-                                f.kw[t * KN + 4 * j + i] = x[i];
-                        }
-                    }
-                    if constexpr (NSC == 2)
-                        f.ksc[t] = __builtin_amdgcn_raw_buffer_load_b16(sr, r16 * SB + grp * 2, 0, 0);
-                    else
-                        f.ksc[t] = __builtin_amdgcn_raw_buffer_load_b8(sr, r16 * SB + grp * SB / 4, 0, 0);
-                }
-            }
-        };
-        auto load_v = [&](const kv_block &b0, const kv_block &b1, frags &f) __attribute__((always_inline)) {
-            if constexpr (!F4) {
-                const uint32_t rb = (uint32_t)D * 2u;
-                const auto vr0 = make_rsrc(a.v + b0.row * rb, b0.n * rb);
-                const auto vr1 = make_rsrc(a.v + b1.row * rb, b1.n * rb);
-                const uint32_t v0 = (lane % (DP / 8)) * 8 < D
-                                        ? (lane / (DP / 8)) * rb + (lane % (DP / 8)) * 16
-                                        : 0x80000000u;
-#pragma unroll
-                for (int r = 0; r < NV; ++r)
-                    f.v[r] = buf16<NTL>(r < NV / 2 ? vr0 : vr1, v0 + (r % (NV / 2)) * (512 / DP) * rb);
-            } else {
-                constexpr int RB = DP / 2, SB = DP / 32;
-#pragma unroll
-                for (int r = 0; r < NV4; ++r) {
-                    const kv_block &bl = r < NV4 / 2 ? b0 : b1;
-                    const auto vr = make_rsrc(a.v + bl.row * RB, bl.n * RB);
-                    const auto sr = make_rsrc(a.vs + bl.row * SB, bl.n * SB);
-                    const int row = lane / LPR + r % (NV4 / 2) * RPL, piece = lane % LPR;
-                    if constexpr (DP == 64) {
-                        const u32x2 x = __builtin_amdgcn_raw_buffer_load_b64(
-                            vr, row * RB + piece * PB, 0, NTL ? kDmaNT : 0);
-                        f.vw[2 * r] = x[0];
-                        f.vw[2 * r + 1] = x[1];
-                    } else {
-                        const u32x4 x = buf16<NTL>(vr, row * RB + piece * PB);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            f.vw[4 * r + i] = x[i];
-                    }
-                    f.vsc[r] = __builtin_amdgcn_raw_buffer_load_b8(sr, row * SB + piece * SB / LPR, 0, 0);
-                }
-            }
-        };
-        auto put_v = [&](const frags &f) __attribute__((always_inline)) {
-            lds_wave_fence(); // the previous tile's transposed reads are complete
-            if constexpr (!F4) {
-#pragma unroll
-                for (int r = 0; r < NV; ++r) {
-                    const int at = lane + 64 * r;
-                    *reinterpret_cast<u32x4 *>(&vt[at / (DP / 8) * VSTR + at % (DP / 8) * 8]) = f.v[r];
-                }
-            } else {
-#pragma unroll
-                for (int r = 0; r < NV4; ++r) {
-                    const int row = lane / LPR + r * RPL, piece = lane % LPR;
-                    const float sc = e8m0(f.vsc[r]);
-#pragma unroll
-                    for (int j = 0; j < PB / 4; ++j)
-                        *reinterpret_cast<u32x4 *>(&vt[row * VSTR + piece * 2 * PB + 8 * j]) =
-                            fp4_to_bf16(f.vw[r * (PB / 4) + j], sc);
-                }
-            }
-        };
-        auto compute = [&](int tb, const kv_block &b0, const kv_block &b1, const kv_block &n0,
-                           const kv_block &n1, frags &f) __attribute__((always_inline)) {
-            bf16x8 kf[2][KN], pk[NRB];
-            f32x4 s[NRB][2];
-#pragma unroll
-            for (int t = 0; t < 2; ++t)
-#pragma unroll
+        const int live = cover.live, sp = team - cover.first;
+        const int k0 = min(off * 128, sq.kend), k1 = a.teams ? min((off + take) * 128, sq.kend) : sq.kend;
+        const int32_t *table = a.table + (int64_t)b * a.cols;
+        for (int tile = t0; take > 0 && (int64_t)tile * 16 * NRB < R; tile += a.tps) {
+            const int row0 = tile * 16 * NRB;
+            bf16x8 qb[NRB][KN];
+            int lim[NRB], pos[NRB];
+            float m_run[NRB], l_run[NRB], slope[NRB];
+            f32x4 o[NRB][DP / 16];
+    #pragma unroll
+            for (int i = 0; i < NRB; ++i) {
+                const int row = row0 + 16 * i + r16;
+                const bool valid = row < R;
+                const int tok = valid ? row / g : 0, h = u * g + (valid ? row % g : 0);
+                const uint16_t *q = a.q + (sq.q0 + tok) * a.q_tok + h * a.q_head;
+    #pragma unroll
                 for (int kk = 0; kk < KN; ++kk) {
-                    if constexpr (F4)
-                        kf[t][kk] = as_bf16x8(fp4_to_bf16(
-                            f.kw[t * KN + kk],
-                            e8m0(NSC == 2 ? (f.ksc[t] >> (kk / 4 * 8)) & 0xff : f.ksc[t])));
-                    else
-                        kf[t][kk] = as_bf16x8(f.k[t * KN + kk]);
+                    const int col = F4 ? grp * (DP / 4) + kk * 8 : kk * 32 + grp * 8;
+                    u32x4 x = zero4();
+                    if (valid && col < D)
+                        x = *reinterpret_cast<const u32x4 *>(q + col);
+                    qb[i][kk] = as_bf16x8(x);
                 }
-#pragma unroll
-            for (int i = 0; i < NRB; ++i)
-#pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    s[i][t] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                    for (int kk = 0; kk < KN; ++kk)
-                        s[i][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[t][kk], qb[i][kk], s[i][t], 0, 0, 0);
-                }
-            __builtin_amdgcn_sched_barrier(0);
-            if (kLate)
-                load_v(b0, b1, f);
-            else
-                load_k(n0, n1, f);
-#pragma unroll
-            for (int i = 0; i < NRB; ++i) {
-                // Register (t, j) of this lane holds key tb + 16t + 4grp + j for row r16.
-                if (MOD)
-                    modify_scores(a, slope[i], pos[i] - tb - 4 * grp, [&](auto f) __attribute__((always_inline)) {
-#pragma unroll
-                        for (int t = 0; t < 2; ++t)
-#pragma unroll
-                            for (int j = 0; j < 4; ++j)
-                                s[i][t][j] = f(s[i][t][j], 16 * t + j);
-                    });
-                float mx = kNegInf;
-#pragma unroll
-                for (int t = 0; t < 2; ++t)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const int key = tb + 16 * t + 4 * grp + j;
-                        if (key > lim[i] || (t ? b1.n : b0.n) == 0)
-                            s[i][t][j] = kNegInf;
-                        mx = fmaxf(mx, s[i][t][j]);
-                    }
-                mx = max_xor32(max_xor16(mx));
-                if (__builtin_amdgcn_ballot_w64(mx > m_run[i] + lift) != 0) {
-                    const float mnew = fmaxf(m_run[i], mx);
-                    const float alpha = fast_exp2((m_run[i] - (mnew == kNegInf ? 0.f : mnew)) * c);
-                    m_run[i] = mnew;
-                    l_run[i] *= alpha;
-#pragma unroll
-                    for (int db = 0; db < DP / 16; ++db)
-                        o[i][db] *= alpha;
-                }
-                const float mc = m_run[i] == kNegInf ? 0.f : m_run[i] * c;
-                float psum = 0.f;
-#pragma unroll
-                for (int t = 0; t < 2; ++t)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const float p = fast_exp2(fmaf(s[i][t][j], c, -mc));
-                        psum += p;
-                        pk[i][4 * t + j] = (__bf16)p;
-                    }
-                l_run[i] += psum;
+                pos[i] = sq.len - sq.n + tok;
+                lim[i] = a.causal ? min(pos[i], k1 - 1) : k1 - 1;
+                slope[i] = MOD && a.slopes ? a.slopes[h] * 1.44269504088896341f : 0.f;
+                m_run[i] = kNegInf;
+                l_run[i] = 0.f;
+    #pragma unroll
+                for (int db = 0; db < DP / 16; ++db)
+                    o[i][db] = f32x4{0.f, 0.f, 0.f, 0.f};
             }
-            if (kLate)
-                put_v(f);
-            lds_wave_fence(); // this tile's V is in LDS before the transposed reads
-            const uint16_t *vb = &vt[(4 * grp + (r16 >> 2)) * VSTR + 4 * (r16 & 3)];
-#pragma unroll
-            for (int db = 0; db < DP / 16; ++db) {
-                const bf16x8 x = join_tr(lds_read_tr(vb + db * 16), lds_read_tr(vb + db * 16 + 16 * VSTR));
-#pragma unroll
-                for (int i = 0; i < NRB; ++i)
-                    o[i][db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, pk[i], o[i][db], 0, 0, 0);
-            }
-        };
-        // Tiles in flight per wave: one and a half ahead of the one at work, or, with 4-bit rows, which are
-        // short, two and a half.
-        constexpr int AHEAD = F4 ? 2 : 1;
-        int tb = k0 + 32 * w;
-        if (tb < kstop) {
-            frags f[AHEAD];
-            kv_block b0[AHEAD], b1[AHEAD];
-            int pg0[AHEAD], pg1[AHEAD], pn0, pn1;
-#pragma unroll
-            for (int i = 0; i < AHEAD; ++i) {
-                pg0[i] = page_id(a, table, tb + 128 * i, k1);
-                pg1[i] = page_id(a, table, tb + 128 * i + 16, k1);
-            }
-            pn0 = page_id(a, table, tb + 128 * AHEAD, k1);
-            pn1 = page_id(a, table, tb + 128 * AHEAD + 16, k1);
-            // Blocks of the tile at t; past the last tile they are empty and their loads read nothing. No branch
-            // goes around a load: a wait behind it would have to be for all of them.
-            auto blocks = [&](int t, int p0, int p1, kv_block &x, kv_block &y) __attribute__((always_inline)) {
-                x = block_in(a, p0, u, t, k1);
-                y = block_in(a, p1, u, t + 16, k1);
-                if (t >= kstop)
-                    x.n = y.n = 0;
-            };
-#pragma unroll
-            for (int i = 0; i < AHEAD; ++i) {
-                blocks(tb + 128 * i, pg0[i], pg1[i], b0[i], b1[i]);
-                if (!kLate) {
-                    load_v(b0[i], b1[i], f[i]);
-                    load_k(b0[i], b1[i], f[i]);
-                }
-            }
-            for (; tb < kstop; tb += 128 * AHEAD)
-#pragma unroll
-                for (int i = 0; i < AHEAD; ++i) {
-                    const int t = tb + 128 * i, tn = t + 128 * AHEAD;
-                    if (i > 0 && t >= kstop)
-                        break;
-                    kv_block n0, n1;
-                    blocks(tn, pn0, pn1, n0, n1);
-                    pn0 = page_id(a, table, tn + 128, k1);
-                    pn1 = page_id(a, table, tn + 144, k1);
-                    if (kLate) {
-                        load_k(b0[i], b1[i], f[i]);
-                    } else {
-                        put_v(f[i]);
-                        __builtin_amdgcn_sched_barrier(0);
-                        load_v(n0, n1, f[i]);
-                    }
-                    compute(t, b0[i], b1[i], n0, n1, f[i]);
-                    b0[i] = n0;
-                    b1[i] = n1;
-                }
-        }
-#pragma unroll
-        for (int i = 0; i < NRB; ++i)
-            l_run[i] = sum_xor32(sum_xor16(l_run[i]));
+            // Keys from the tile's last row's position on are hidden from it.
+            const int kstop = a.causal ? min(k1, sq.len - sq.n + (min(row0 + 16 * NRB, R) - 1) / g + 1) : k1;
 
-        // Merge the waves: O^T register (db, j) of this lane holds d = 16db + 4grp + j of row r16.
-        float *om = reinterpret_cast<float *>(Vw); // [4][16][DP + 4]
-        if (grp == 0)
-#pragma unroll
-            for (int i = 0; i < NRB; ++i) {
-                red_m[i][w][r16] = m_run[i] * c; // in log2 units; -inf stays
-                red_l[i][w][r16] = l_run[i];
-            }
-#pragma unroll
-        for (int i = 0; i < NRB; ++i) {
-            __syncthreads();
-#pragma unroll
-            for (int db = 0; db < DP / 16; ++db)
-                *reinterpret_cast<f32x4 *>(&om[(w * 16 + r16) * (DP + 4) + db * 16 + 4 * grp]) = o[i][db];
-            __syncthreads();
-            const int rowb = row0 + 16 * i, nrow = min(16, R - rowb);
-            for (int idx = tid; idx < nrow * (DP / 4); idx += 256) {
-                const int r = idx / (DP / 4), d = 4 * (idx % (DP / 4));
-                if (d >= D)
-                    continue;
-                float mx = kNegInf;
-#pragma unroll
-                for (int ww = 0; ww < 4; ++ww)
-                    mx = fmaxf(mx, red_m[i][ww][r]);
-                const float muse = mx == kNegInf ? 0.f : mx;
-                f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-                float lsum = 0.f;
-#pragma unroll
-                for (int ww = 0; ww < 4; ++ww) {
-                    const float wgt = fast_exp2(red_m[i][ww][r] - muse);
-                    const f32x4 x = *reinterpret_cast<const f32x4 *>(&om[(ww * 16 + r) * (DP + 4) + d]);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        acc[j] += wgt * x[j];
-                    lsum += wgt * red_l[i][ww][r];
-                }
-                const int64_t tok = sq.q0 + (rowb + r) / g;
-                const int h = u * g + (rowb + r) % g;
-                const int64_t slot = (tok * a.Hq + h) * a.nsplit;
-                if (live == 1) {
-                    const float inv = lsum > 0.f ? 1.0f / lsum : 0.f;
-                    *reinterpret_cast<u32x2 *>(a.o + tok * a.o_tok + h * a.o_head + d) =
-                        u32x2{bf16_pair(acc[0] * inv, acc[1] * inv), bf16_pair(acc[2] * inv, acc[3] * inv)};
-                    if (d == 0 && a.nsplit > 1)
-                        a.pm[slot] = -kNegInf; // the row is written
-                } else {
-                    if (d == 0) {
-                        a.pm[slot + sp] = mx;
-                        a.pl[slot + sp] = lsum;
+            struct frags {
+                u32x4 k[F4 ? 1 : 2 * KN], v[F4 ? 1 : NV];
+                uint32_t kw[F4 ? 2 * KN : 1], ksc[F4 ? 2 : 1];
+                uint32_t vw[F4 ? NV4 * PB / 4 : 1], vsc[F4 ? NV4 : 1];
+            };
+            // The loads of the next tile are issued as soon as this one's have been used: V's once it is in LDS,
+            // K's once the scores are there. K and V of a tile, Q and O do not fit 256 registers at DP = 256 in
+            // bf16: there a tile's K is loaded at its start, and V once the scores have freed K's registers.
+            constexpr bool kLate = DP == 256 && !F4;
+            auto load_k = [&](const kv_block &b0, const kv_block &b1, frags &f) __attribute__((always_inline)) {
+    #pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    const kv_block &bl = t ? b1 : b0;
+                    if constexpr (!F4) {
+                        const uint32_t rb = (uint32_t)D * 2u; // bytes of a row
+                        const auto kr = make_rsrc(a.k + bl.row * rb, bl.n * rb);
+    #pragma unroll
+                        for (int kk = 0; kk < KN; ++kk) {
+                            const int col = kk * 32 + grp * 8;
+                            f.k[t * KN + kk] = buf16<NTL>(kr, col < D ? r16 * rb + col * 2 : 0x80000000u);
+                        }
+                    } else {
+                        constexpr int RB = DP / 2, SB = DP / 32; // bytes of a row's codes and scales
+                        const auto kr = make_rsrc(a.k + bl.row * RB, bl.n * RB);
+                        const auto sr = make_rsrc(a.ks + bl.row * SB, bl.n * SB);
+                        if constexpr (DP == 64) {
+                            const u32x2 x = __builtin_amdgcn_raw_buffer_load_b64(
+                                kr, r16 * RB + grp * (RB / 4), 0, NTL ? kDmaNT : 0);
+                            f.kw[t * KN] = x[0];
+                            f.kw[t * KN + 1] = x[1];
+                        } else {
+    #pragma unroll
+                            for (int j = 0; j < KN / 4; ++j) {
+                                const u32x4 x = buf16<NTL>(kr, r16 * RB + grp * (RB / 4) + 16 * j);
+    #pragma unroll
+                                for (int i = 0; i < 4; ++i)
+                                    f.kw[t * KN + 4 * j + i] = x[i];
+                            }
+                        }
+                        if constexpr (NSC == 2)
+                            f.ksc[t] = __builtin_amdgcn_raw_buffer_load_b16(sr, r16 * SB + grp * 2, 0, 0);
+                        else
+                            f.ksc[t] = __builtin_amdgcn_raw_buffer_load_b8(sr, r16 * SB + grp * SB / 4, 0, 0);
                     }
-                    *reinterpret_cast<f32x4 *>(a.pacc + (slot + sp) * D + d) = acc;
-                    if (sp == live - 1) // no parts behind the last
-                        for (int s = live + d / 4; s < a.nsplit; s += D / 4)
-                            a.pm[slot + s] = kNegInf;
+                }
+            };
+            auto load_v = [&](const kv_block &b0, const kv_block &b1, frags &f) __attribute__((always_inline)) {
+                if constexpr (!F4) {
+                    const uint32_t rb = (uint32_t)D * 2u;
+                    const auto vr0 = make_rsrc(a.v + b0.row * rb, b0.n * rb);
+                    const auto vr1 = make_rsrc(a.v + b1.row * rb, b1.n * rb);
+                    const uint32_t v0 = (lane % (DP / 8)) * 8 < D
+                                            ? (lane / (DP / 8)) * rb + (lane % (DP / 8)) * 16
+                                            : 0x80000000u;
+    #pragma unroll
+                    for (int r = 0; r < NV; ++r)
+                        f.v[r] = buf16<NTL>(r < NV / 2 ? vr0 : vr1, v0 + (r % (NV / 2)) * (512 / DP) * rb);
+                } else {
+                    constexpr int RB = DP / 2, SB = DP / 32;
+    #pragma unroll
+                    for (int r = 0; r < NV4; ++r) {
+                        const kv_block &bl = r < NV4 / 2 ? b0 : b1;
+                        const auto vr = make_rsrc(a.v + bl.row * RB, bl.n * RB);
+                        const auto sr = make_rsrc(a.vs + bl.row * SB, bl.n * SB);
+                        const int row = lane / LPR + r % (NV4 / 2) * RPL, piece = lane % LPR;
+                        if constexpr (DP == 64) {
+                            const u32x2 x = __builtin_amdgcn_raw_buffer_load_b64(
+                                vr, row * RB + piece * PB, 0, NTL ? kDmaNT : 0);
+                            f.vw[2 * r] = x[0];
+                            f.vw[2 * r + 1] = x[1];
+                        } else {
+                            const u32x4 x = buf16<NTL>(vr, row * RB + piece * PB);
+    #pragma unroll
+                            for (int i = 0; i < 4; ++i)
+                                f.vw[4 * r + i] = x[i];
+                        }
+                        f.vsc[r] = __builtin_amdgcn_raw_buffer_load_b8(sr, row * SB + piece * SB / LPR, 0, 0);
+                    }
+                }
+            };
+            auto put_v = [&](const frags &f) __attribute__((always_inline)) {
+                lds_wave_fence(); // the previous tile's transposed reads are complete
+                if constexpr (!F4) {
+    #pragma unroll
+                    for (int r = 0; r < NV; ++r) {
+                        const int at = lane + 64 * r;
+                        *reinterpret_cast<u32x4 *>(&vt[at / (DP / 8) * VSTR + at % (DP / 8) * 8]) = f.v[r];
+                    }
+                } else {
+    #pragma unroll
+                    for (int r = 0; r < NV4; ++r) {
+                        const int row = lane / LPR + r * RPL, piece = lane % LPR;
+                        const float sc = e8m0(f.vsc[r]);
+    #pragma unroll
+                        for (int j = 0; j < PB / 4; ++j)
+                            *reinterpret_cast<u32x4 *>(&vt[row * VSTR + piece * 2 * PB + 8 * j]) =
+                                fp4_to_bf16(f.vw[r * (PB / 4) + j], sc);
+                    }
+                }
+            };
+            auto compute = [&](int tb, const kv_block &b0, const kv_block &b1, const kv_block &n0,
+                               const kv_block &n1, frags &f) __attribute__((always_inline)) {
+                bf16x8 kf[2][KN], pk[NRB];
+                f32x4 s[NRB][2];
+    #pragma unroll
+                for (int t = 0; t < 2; ++t)
+    #pragma unroll
+                    for (int kk = 0; kk < KN; ++kk) {
+                        if constexpr (F4)
+                            kf[t][kk] = as_bf16x8(fp4_to_bf16(
+                                f.kw[t * KN + kk],
+                                e8m0(NSC == 2 ? (f.ksc[t] >> (kk / 4 * 8)) & 0xff : f.ksc[t])));
+                        else
+                            kf[t][kk] = as_bf16x8(f.k[t * KN + kk]);
+                    }
+    #pragma unroll
+                for (int i = 0; i < NRB; ++i)
+    #pragma unroll
+                    for (int t = 0; t < 2; ++t) {
+                        s[i][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    #pragma unroll
+                        for (int kk = 0; kk < KN; ++kk)
+                            s[i][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[t][kk], qb[i][kk], s[i][t], 0, 0, 0);
+                    }
+                __builtin_amdgcn_sched_barrier(0);
+                if (kLate)
+                    load_v(b0, b1, f);
+                else
+                    load_k(n0, n1, f);
+    #pragma unroll
+                for (int i = 0; i < NRB; ++i) {
+                    // Register (t, j) of this lane holds key tb + 16t + 4grp + j for row r16.
+                    if (MOD)
+                        modify_scores(a, slope[i], pos[i] - tb - 4 * grp, [&](auto f) __attribute__((always_inline)) {
+    #pragma unroll
+                            for (int t = 0; t < 2; ++t)
+    #pragma unroll
+                                for (int j = 0; j < 4; ++j)
+                                    s[i][t][j] = f(s[i][t][j], 16 * t + j);
+                        });
+                    float mx = kNegInf;
+    #pragma unroll
+                    for (int t = 0; t < 2; ++t)
+    #pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const int key = tb + 16 * t + 4 * grp + j;
+                            if (key > lim[i] || (t ? b1.n : b0.n) == 0)
+                                s[i][t][j] = kNegInf;
+                            mx = fmaxf(mx, s[i][t][j]);
+                        }
+                    mx = max_xor32(max_xor16(mx));
+                    if (__builtin_amdgcn_ballot_w64(mx > m_run[i] + lift) != 0) {
+                        const float mnew = fmaxf(m_run[i], mx);
+                        const float alpha = fast_exp2((m_run[i] - (mnew == kNegInf ? 0.f : mnew)) * c);
+                        m_run[i] = mnew;
+                        l_run[i] *= alpha;
+    #pragma unroll
+                        for (int db = 0; db < DP / 16; ++db)
+                            o[i][db] *= alpha;
+                    }
+                    const float mc = m_run[i] == kNegInf ? 0.f : m_run[i] * c;
+                    float psum = 0.f;
+    #pragma unroll
+                    for (int t = 0; t < 2; ++t)
+    #pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const float p = fast_exp2(fmaf(s[i][t][j], c, -mc));
+                            psum += p;
+                            pk[i][4 * t + j] = (__bf16)p;
+                        }
+                    l_run[i] += psum;
+                }
+                if (kLate)
+                    put_v(f);
+                lds_wave_fence(); // this tile's V is in LDS before the transposed reads
+                const uint16_t *vb = &vt[(4 * grp + (r16 >> 2)) * VSTR + 4 * (r16 & 3)];
+    #pragma unroll
+                for (int db = 0; db < DP / 16; ++db) {
+                    const bf16x8 x = join_tr(lds_read_tr(vb + db * 16), lds_read_tr(vb + db * 16 + 16 * VSTR));
+    #pragma unroll
+                    for (int i = 0; i < NRB; ++i)
+                        o[i][db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, pk[i], o[i][db], 0, 0, 0);
+                }
+            };
+            // Tiles in flight per wave: one and a half ahead of the one at work, or, with 4-bit rows, which are
+            // short, two and a half.
+            constexpr int AHEAD = F4 ? 2 : 1;
+            int tb = k0 + 32 * w;
+            if (tb < kstop) {
+                frags f[AHEAD];
+                kv_block b0[AHEAD], b1[AHEAD];
+                int pg0[AHEAD], pg1[AHEAD], pn0, pn1;
+    #pragma unroll
+                for (int i = 0; i < AHEAD; ++i) {
+                    pg0[i] = page_id(a, table, tb + 128 * i, k1);
+                    pg1[i] = page_id(a, table, tb + 128 * i + 16, k1);
+                }
+                pn0 = page_id(a, table, tb + 128 * AHEAD, k1);
+                pn1 = page_id(a, table, tb + 128 * AHEAD + 16, k1);
+                // Blocks of the tile at t; past the last tile they are empty and their loads read nothing. No branch
+                // goes around a load: a wait behind it would have to be for all of them.
+                auto blocks = [&](int t, int p0, int p1, kv_block &x, kv_block &y) __attribute__((always_inline)) {
+                    x = block_in(a, p0, u, t, k1);
+                    y = block_in(a, p1, u, t + 16, k1);
+                    if (t >= kstop)
+                        x.n = y.n = 0;
+                };
+    #pragma unroll
+                for (int i = 0; i < AHEAD; ++i) {
+                    blocks(tb + 128 * i, pg0[i], pg1[i], b0[i], b1[i]);
+                    if (!kLate) {
+                        load_v(b0[i], b1[i], f[i]);
+                        load_k(b0[i], b1[i], f[i]);
+                    }
+                }
+                for (; tb < kstop; tb += 128 * AHEAD)
+    #pragma unroll
+                    for (int i = 0; i < AHEAD; ++i) {
+                        const int t = tb + 128 * i, tn = t + 128 * AHEAD;
+                        if (i > 0 && t >= kstop)
+                            break;
+                        kv_block n0, n1;
+                        blocks(tn, pn0, pn1, n0, n1);
+                        pn0 = page_id(a, table, tn + 128, k1);
+                        pn1 = page_id(a, table, tn + 144, k1);
+                        if (kLate) {
+                            load_k(b0[i], b1[i], f[i]);
+                        } else {
+                            put_v(f[i]);
+                            __builtin_amdgcn_sched_barrier(0);
+                            load_v(n0, n1, f[i]);
+                        }
+                        compute(t, b0[i], b1[i], n0, n1, f[i]);
+                        b0[i] = n0;
+                        b1[i] = n1;
+                    }
+            }
+    #pragma unroll
+            for (int i = 0; i < NRB; ++i)
+                l_run[i] = sum_xor32(sum_xor16(l_run[i]));
+
+            // Merge the waves: O^T register (db, j) of this lane holds d = 16db + 4grp + j of row r16.
+            float *om = reinterpret_cast<float *>(Vw); // [4][16][DP + 4]
+            if (grp == 0)
+    #pragma unroll
+                for (int i = 0; i < NRB; ++i) {
+                    red_m[i][w][r16] = m_run[i] * c; // in log2 units; -inf stays
+                    red_l[i][w][r16] = l_run[i];
+                }
+    #pragma unroll
+            for (int i = 0; i < NRB; ++i) {
+                __syncthreads();
+    #pragma unroll
+                for (int db = 0; db < DP / 16; ++db)
+                    *reinterpret_cast<f32x4 *>(&om[(w * 16 + r16) * (DP + 4) + db * 16 + 4 * grp]) = o[i][db];
+                __syncthreads();
+                const int rowb = row0 + 16 * i, nrow = min(16, R - rowb);
+                for (int idx = tid; idx < nrow * (DP / 4); idx += 256) {
+                    const int r = idx / (DP / 4), d = 4 * (idx % (DP / 4));
+                    if (d >= D)
+                        continue;
+                    float mx = kNegInf;
+    #pragma unroll
+                    for (int ww = 0; ww < 4; ++ww)
+                        mx = fmaxf(mx, red_m[i][ww][r]);
+                    const float muse = mx == kNegInf ? 0.f : mx;
+                    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+                    float lsum = 0.f;
+    #pragma unroll
+                    for (int ww = 0; ww < 4; ++ww) {
+                        const float wgt = fast_exp2(red_m[i][ww][r] - muse);
+                        const f32x4 x = *reinterpret_cast<const f32x4 *>(&om[(ww * 16 + r) * (DP + 4) + d]);
+    #pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            acc[j] += wgt * x[j];
+                        lsum += wgt * red_l[i][ww][r];
+                    }
+                    const int64_t tok = sq.q0 + (rowb + r) / g;
+                    const int h = u * g + (rowb + r) % g;
+                    const int64_t slot = (tok * a.Hq + h) * a.nsplit;
+                    if (live == 1) {
+                        const float inv = lsum > 0.f ? 1.0f / lsum : 0.f;
+                        *reinterpret_cast<u32x2 *>(a.o + tok * a.o_tok + h * a.o_head + d) =
+                            u32x2{bf16_pair(acc[0] * inv, acc[1] * inv), bf16_pair(acc[2] * inv, acc[3] * inv)};
+                        if (d == 0 && a.nsplit > 1)
+                            a.pm[slot] = -kNegInf; // the row is written
+                    } else {
+                        if (d == 0) {
+                            a.pm[slot + sp] = mx;
+                            a.pl[slot + sp] = lsum;
+                        }
+                        *reinterpret_cast<f32x4 *>(a.pacc + (slot + sp) * D + d) = acc;
+                        if (sp == live - 1) // no parts behind the last
+                            for (int s = live + d / 4; s < a.nsplit; s += D / 4)
+                                a.pm[slot + s] = kNegInf;
+                    }
                 }
             }
+            __syncthreads(); // the merge area is V tiles again
         }
-        __syncthreads(); // the merge area is V tiles again
-    }
-    left -= take;
-    pos0 += take;
-    off = 0;
-    if (++b == a.B) {
-        b = 0;
-        ++u;
-    }
+        left -= take;
+        pos0 += take;
+        off = 0;
+        if (++b == a.B) {
+            b = 0;
+            ++u;
+        }
     }
 }
 
@@ -1214,8 +1214,7 @@ __global__ __launch_bounds__(256) void attn_kv_append_kernel(const attn_kv_args 
                     cs[e + f] = y0[f], sn[e + f] = y1[f];
             }
         }
-        if (w < 2 ? !placed && a.rot != 0
-                  : !placed || pos >= sq.kend || !attn_page_ok(pg, a.pages))
+        if (!placed || (w > 1 && (pos >= sq.kend || !attn_page_ok(pg, a.pages))))
             continue;
         const int64_t row = attn_page_row(pg, a.Hkv, 0, max(pos, 0), a.lgp);
         for (int h = 0;;) {
@@ -1349,11 +1348,12 @@ hipError_t launch_paged_d(const attn_paged_args &a, const attn_paged_cut &cut, h
         auto decode = [&](auto NB, auto NT) {
             constexpr int kN = decltype(NB)::value;
             constexpr bool kT = decltype(NT)::value;
-            if (t_plan)
+            if (t_plan) {
                 plan_note(grid, block, "attn_paged_decode_kernel<%d, %d, %d, %s, %s> teams=%d parts=%d", DP,
                           F4 ? 4 : 16, kN, tf(kM), tf(kT), a.teams, a.nsplit);
-            else
-                hipLaunchKernelGGL((attn_paged_decode_kernel<DP, F4, kN, kM, kT>), grid, block, 0, st, a);
+                return hipSuccess;
+            }
+            hipLaunchKernelGGL((attn_paged_decode_kernel<DP, F4, kN, kM, kT>), grid, block, 0, st, a);
             return hipGetLastError();
         };
         if (cut.rows16 == 1)
@@ -1367,12 +1367,12 @@ hipError_t launch_paged_d(const attn_paged_args &a, const attn_paged_cut &cut, h
                 });
         auto prefill = [&](auto KHF, auto NWF) {
             constexpr int kK = decltype(KHF)::value, kW = decltype(NWF)::value;
-            if (t_plan)
+            if (t_plan) {
                 plan_note(grid, dim3(64 * kW), "attn_paged_prefill_kernel<%d, %d, %s, %d, %d> parts=%d share=%d",
                           DP, F4 ? 4 : 16, tf(kM), kK, kW, a.nsplit, a.share);
-            else
-                hipLaunchKernelGGL((attn_paged_prefill_kernel<DP, F4, kM, kK, kW>), grid, dim3(64 * kW), 0, st,
-                                   a);
+                return hipSuccess;
+            }
+            hipLaunchKernelGGL((attn_paged_prefill_kernel<DP, F4, kM, kK, kW>), grid, dim3(64 * kW), 0, st, a);
             return hipGetLastError();
         };
         constexpr std::integral_constant<int, 1> one;
@@ -1410,16 +1410,18 @@ extern "C" int attn_hip_launch_paged(const struct attn_paged_args *ap, const str
                          : launch_paged_d<256, false>(a, *cut, st);
     if (e != hipSuccess || a.nsplit == 1)
         return (int)e;
-    const dim3 grid((unsigned)((long)a.B * a.Hkv * cut->merge_tiles));
-    if (t_plan)
-        plan_note(grid, dim3(256), "attn_paged_merge_kernel rows=%d", 256 >> (cut->lglp + cut->lgsg));
-    else
-        (void)with_flag(cut->merge_loads == 2, [&](auto FEW) {
-            hipLaunchKernelGGL((attn_paged_merge_kernel<decltype(FEW)::value ? 2 : 8>), grid, dim3(256), 0, st,
-                               a, cut->lglp, cut->lgsg, cut->merge_tiles);
+    const dim3 mgrid((unsigned)((long)a.B * a.Hkv * cut->merge_tiles));
+    return (int)with_flag(cut->merge_loads == 2, [&](auto FEW) {
+        constexpr int kL = decltype(FEW)::value ? 2 : 8;
+        if (t_plan) {
+            plan_note(mgrid, dim3(256), "attn_paged_merge_kernel<%d> rows=%d", kL,
+                      256 >> (cut->lglp + cut->lgsg));
             return hipSuccess;
-        });
-    return (int)hipGetLastError();
+        }
+        hipLaunchKernelGGL(attn_paged_merge_kernel<kL>, mgrid, dim3(256), 0, st, a, cut->lglp, cut->lgsg,
+                           cut->merge_tiles);
+        return hipGetLastError();
+    });
 }
 
 extern "C" int attn_hip_launch_kv_append(const struct attn_kv_args *ap, int bits, int pairs, void *stream) {
