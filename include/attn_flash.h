@@ -157,9 +157,10 @@ struct attn_scores {
  * (q_out may be q; q and q_out may both be NULL). The first `rot` elements of a head turn (0: none), in
  * pairs (i, i + rot/2), or with `pairs` (2i, 2i + 1): (x1, x2) -> (x1 c - x2 s, x2 c + x1 s) in fp32,
  * rounded once to bf16, with c and s from row p of rope [rope_rows][rot], cosines in its first half, for
- * position p. In 4 bits the rounded rows are quantised: a group's scale is the smallest power of two
- * in [2^-126, 2^125] under which its largest element is at most 7, elements round to nearest, ties to even; a group with a
- * NaN or an infinity reads as NaN. Tokens whose position is below 0 or has no row in rope are skipped. */
+ * position p. In 4 bits the rounded rows are quantised: a group's scale is the smallest power of two in
+ * [2^-126, 2^125] under which its largest element is at most 7, elements round to nearest, ties to even; a
+ * group with a NaN or an infinity reads as NaN. Tokens whose position is below 0 or has no row in rope are
+ * skipped, q's rows too. */
 void attn_kv_append(const struct attn_kv_cache *c, const struct attn_rows *q, const struct attn_rows *q_out,
                     const struct attn_rows *k, const struct attn_rows *v, int T, int Hq, const float *rope,
                     int rope_rows, int rot, int pairs, int max_q);
@@ -172,7 +173,7 @@ void attn_kv_read(const struct attn_kv_cache *c, const struct attn_rows *k, cons
 /* Attention of a call's rows over their sequences' caches, o in bf16: row i of sequence b sees keys
  * j < kv_len[b], and with causal j <= its position; kv = h / (Hq/Hkv). A row that sees none is written as
  * zeros. P is rounded to bf16 before P.V, as in attn_flash, and as there a NaN or an infinity in V reaches
- * the rows of its key tile that do not see it. o must not overlap q. scores may be NULL (1/sqrt(D)). scratch
+ * the rows of its key tile that do not see it. o must not be q or overlap it. scores may be NULL (1/sqrt(D)). scratch
  * is an attn_flash scratch of this D (attn_flash_scratch_bytes); calls that may overlap need one each. */
 void attn_paged(const struct attn_kv_cache *c, const struct attn_rows *q, const struct attn_rows *o, int T,
                 int Hq, int causal, const struct attn_scores *scores, int max_q, int max_kv, void *scratch);

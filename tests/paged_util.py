@@ -199,9 +199,9 @@ def attend_ref(cache, q, Hq, causal, scale=0.0, softcap=0.0, slopes=None, hidden
 
 
 def attend(cache, q, Hq, causal, scale=0.0, softcap=0.0, slopes=None, max_q=None, max_kv=None, pad=3,
-           stride=0, desc=None):
+           stride=0, desc=None, poison=0xFF):
     """O [N][Hq][D] as float32, from q in a wider buffer between guards; rows behind the last sequence and
-    between rows have to stay as they were."""
+    between rows have to stay as they were (bytes `poison`)."""
     N, D = cache.N, cache.D
     T = N + pad
     tok = Hq * D + stride
@@ -212,7 +212,7 @@ def attend(cache, q, Hq, causal, scale=0.0, softcap=0.0, slopes=None, max_q=None
     with ts.DeviceBuffer.from_array(qh) as dq, ts.DeviceBuffer(T * tok * 2) as do, \
             ts.DeviceBuffer(ts.attn_flash_scratch_bytes(D, 128)) as ds, \
             ts.DeviceBuffer.from_array(np.asarray(slopes if slopes is not None else [0], np.float32)) as dl:
-        do.fill_bytes(0xFF)
+        do.fill_bytes(poison)
         ds.fill_bytes(0xFF)
         if slopes is not None:
             sc.slopes = dl.ptr
@@ -221,7 +221,7 @@ def attend(cache, q, Hq, causal, scale=0.0, softcap=0.0, slopes=None, max_q=None
                       max_kv or max([k for _, k in cache.seqs] + [1]), ds)
         ts.synchronize()
         raw = do.download(np.uint16).reshape(T, tok)
-    assert np.all(raw[N:] == 0xFFFF) and np.all(raw[:, Hq * D:] == 0xFFFF)
+    assert np.all(raw[N:] == poison * 0x101) and np.all(raw[:, Hq * D:] == poison * 0x101)
     return f32(raw[:N, :Hq * D]).reshape(N, Hq, D)
 
 

@@ -281,13 +281,13 @@ static void walk(void) {
                 start[b + 1] = bad_int(start[b + 1]), kv[b] = bad_int(kv[b]);
         struct attn_kv_cache c = {(void *)4096, (void *)4096, NULL, NULL, table, kv,  start, B,
                                   cols,         pages,        page, Hkv,  D,     ATTN_KV_BF16};
-        const struct attn_rows r = {(void *)4096, 8, 8};
+        const struct attn_rows r = {(void *)4096, 8, 8}, o = {(void *)8192, 8, 8};
         const size_t len = 8u * ATTN_SLOTS + 4u * ATTN_SLOTS * (size_t)D;
         if (it % 50 == 0) { /* the partials of the largest slot */
             scratch_len = len;
             scratch_base = aligned_alloc(256, (len + 255) / 256 * 256);
         }
-        attn_paged(&c, &r, &r, T, g * Hkv, (int)(rnd() % 2), NULL, pick_int(1, 400), pick_int(1, 5000),
+        attn_paged(&c, &r, &o, T, g * Hkv, (int)(rnd() % 2), NULL, pick_int(1, 400), pick_int(1, 5000),
                    scratch_base ? (void *)scratch_base : (void *)4096);
         free(scratch_base);
         scratch_base = NULL;

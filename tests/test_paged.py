@@ -340,6 +340,31 @@ def test_scores_far_apart(bits, n):
     check(pu.attend(c, q, 2, 1), ref, bound, (bits, n))
 
 
+@pytest.mark.parametrize("bits,n,kv", [(16, 1, 100), (16, 1, 5000), (4, 1, 5000), (16, 8, 4000), (4, 20, 3000),
+                                       (16, 100, 2000), (4, 100, 700), (16, 40, 64)])
+def test_nan_and_infinities_stay_in_their_rows(bits, n, kv):
+    """A NaN or an infinity in a row of q, or a NaN in a key, makes NaN of the rows that meet it, whole or in
+    parts, and of no other."""
+    Hq, Hkv, D = 4, 2, 128
+    c = pu.Cache([(n, kv), (n, kv // 2)], Hkv, D, 32, bits, 3)
+    c.fill(23)
+    pg, at = c.places(0, kv - (n + 1) // 2, kv)  # the key of a row in the middle of the new ones
+    x, nan = (c.ks, 255) if bits == 4 else (c.k, 0xFF)
+    x[pg[0], 1, at[0]] = nan
+    q = pu.normal((c.N, Hq, D), 5)
+    ref, bound = pu.attend_ref(c, q, Hq, 1)
+    lost = np.isnan(ref).any(-1)
+    assert lost.sum() == 2 * ((n + 1) // 2)
+    q[0, 0, 5] = 0x7FC0  # NaN
+    q[c.N - 1, 0, 7] = 0x7F80  # inf
+    lost[0, 0] = lost[c.N - 1, 0] = True
+    o = pu.attend(c, q, Hq, 1, poison=0x3F)
+    print(np.isnan(o).all(-1).sum(), lost.sum())
+    assert np.array_equal(np.isnan(o).any(-1), lost) and np.array_equal(np.isnan(o).all(-1), lost)
+    check(np.where(lost[..., None], 0, o), np.where(lost[..., None], 0, ref),
+          np.where(lost[..., None], 0, bound), (bits, n, kv))
+
+
 def test_cache_past_4_gib():
     """Pages whose byte offsets pass 32 bits."""
     D, Hkv, page = 128, 8, 256

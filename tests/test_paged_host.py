@@ -105,6 +105,7 @@ REFUSED = [
     (attend(sc="ts.Scores(0.0, 0.0, 4097)"), "slopes must be"),
     (attend(s="None"), "scratch must be"),
     (attend(s=4128), "scratch must be"),
+    (attend(), "o must not be q"),
     (append("none"), "attn_kv_append: the cache must be non-NULL"),
     (append(Hq=5), "Hq % Hkv"),
     (append(q="None"), "q_out without q"),

@@ -149,6 +149,8 @@ void attn_paged(const struct attn_kv_cache *c, const struct attn_rows *q, const 
     paged_check_rows(who, "o", o);
     if (misaligned(scratch, ATTN_SCRATCH_ALIGN))
         paged_fail(who, "scratch must be non-NULL and ATTN_SCRATCH_ALIGN-aligned");
+    if (o->data == q->data)
+        paged_fail(who, "o must not be q");
     paged_run(who, c, q, o, T, Hq, causal, sc, max_q, max_kv, scratch);
 }
 

@@ -178,6 +178,15 @@ template <bool NT> __device__ __forceinline__ u32x4 buf16(__amdgpu_buffer_rsrc_t
     return __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, NT ? kDmaNT : 0);
 }
 
+// A part's maximum as the merge is told it. There +inf says that the row is written and -inf that the part has
+// nothing: an infinite score, and a part of NaN alone, go by finite ones, and their sums carry the NaN.
+__device__ __forceinline__ float part_max(float m, float l) {
+    uint32_t bits = __builtin_bit_cast(uint32_t, l);
+    asm("" : "+v"(bits)); // as a comparison of floats, which the compiler makes of it, it would leave out NaN
+    const bool lost = m == kNegInf && bits << 1 != 0;
+    return lost ? 0.f : fminf(m, 3.402823466e38f);
+}
+
 // ------------------------------------------------------------------------------------------
 // Few query rows per kv head. One workgroup per (sequence b, kv head u, part sp of its keys, tile of
 // 16 NRB rows); a sequence's rows are its tokens' heads of the group, token by token. The four waves take
@@ -559,7 +568,7 @@ __global__ __launch_bounds__(256, 2) void attn_paged_decode_kernel(const attn_pa
                             a.pm[slot] = -kNegInf; // the row is written
                     } else {
                         if (d == 0) {
-                            a.pm[slot + sp] = mx;
+                            a.pm[slot + sp] = part_max(mx, lsum);
                             a.pl[slot + sp] = lsum;
                         }
                         *reinterpret_cast<f32x4 *>(a.pacc + (slot + sp) * D + d) = acc;
@@ -1085,7 +1094,7 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void attn_paged_prefill_kernel(con
                     }
             } else {
                 if (hi == 0) {
-                    a.pm[slot + sp] = m_run * c;
+                    a.pm[slot + sp] = part_max(m_run * c, l_run);
                     a.pl[slot + sp] = l_run;
                     if (sp == live - 1) // no parts behind the last
                         for (int s = live; s < a.nsplit; ++s)
