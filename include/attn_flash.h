@@ -173,8 +173,10 @@ void attn_kv_read(const struct attn_kv_cache *c, const struct attn_rows *k, cons
 /* Attention of a call's rows over their sequences' caches, o in bf16: row i of sequence b sees keys
  * j < kv_len[b], and with causal j <= its position; kv = h / (Hq/Hkv). A row that sees none is written as
  * zeros. P is rounded to bf16 before P.V, as in attn_flash, and as there a NaN or an infinity in V reaches
- * the rows of its key tile that do not see it. o must not be q or overlap it. scores may be NULL (1/sqrt(D)). scratch
- * is an attn_flash scratch of this D (attn_flash_scratch_bytes); calls that may overlap need one each. */
+ * the rows of its key tile that do not see it. Scores past 2^30, whose rounding to fp32 is coarser than
+ * exp can take, give rows without a meaning. o must not be q or overlap it. scores may be NULL (1/sqrt(D)).
+ * scratch is an attn_flash scratch of this D (attn_flash_scratch_bytes); calls that may overlap need one
+ * each. */
 void attn_paged(const struct attn_kv_cache *c, const struct attn_rows *q, const struct attn_rows *o, int T,
                 int Hq, int causal, const struct attn_scores *scores, int max_q, int max_kv, void *scratch);
 

@@ -360,6 +360,8 @@ __global__ __launch_bounds__(256, 2) void attn_paged_decode_kernel(const attn_pa
                     }
                 }
             };
+            // 4 bits: of the eight lanes that write together, which hold pieces of one row or two, several would
+            // have their chunk j on the same banks; so it lies at j ^ swap of its piece.
             auto put_v = [&](const frags &f) __attribute__((always_inline)) {
                 lds_wave_fence(); // the previous tile's transposed reads are complete
                 if constexpr (!F4) {
@@ -372,10 +374,11 @@ __global__ __launch_bounds__(256, 2) void attn_paged_decode_kernel(const attn_pa
     #pragma unroll
                     for (int r = 0; r < NV4; ++r) {
                         const int row = lane / LPR + r * RPL, piece = lane % LPR;
+                        const int swap = DP == 64 ? row & 1 : piece >> 1;
                         const float sc = e8m0(f.vsc[r]);
-    #pragma unroll
+#pragma unroll
                         for (int j = 0; j < PB / 4; ++j)
-                            *reinterpret_cast<u32x4 *>(&vt[row * VSTR + piece * 2 * PB + 8 * j]) =
+                            *reinterpret_cast<u32x4 *>(&vt[row * VSTR + piece * 2 * PB + 8 * (j ^ swap)]) =
                                 fp4_to_bf16(f.vw[r * (PB / 4) + j], sc);
                     }
                 }
@@ -455,10 +458,13 @@ __global__ __launch_bounds__(256, 2) void attn_paged_decode_kernel(const attn_pa
                 if (kLate)
                     put_v(f);
                 lds_wave_fence(); // this tile's V is in LDS before the transposed reads
-                const uint16_t *vb = &vt[(4 * grp + (r16 >> 2)) * VSTR + 4 * (r16 & 3)];
-    #pragma unroll
+                const uint16_t *vrow = &vt[(4 * grp + (r16 >> 2)) * VSTR];
+                const int quad = F4 && DP == 64 ? (r16 & 3) ^ (r16 >> 1 & 2) : r16 & 3; // put_v's swap
+                const uint16_t *const vb[2] = {vrow + 4 * quad, vrow + 4 * (quad ^ 2)};
+#pragma unroll
                 for (int db = 0; db < DP / 16; ++db) {
-                    const bf16x8 x = join_tr(lds_read_tr(vb + db * 16), lds_read_tr(vb + db * 16 + 16 * VSTR));
+                    const uint16_t *y = F4 && DP > 64 ? vb[db >> 2 & 1] + (db ^ db >> 3) * 16 : vb[0] + db * 16;
+                    const bf16x8 x = join_tr(lds_read_tr(y), lds_read_tr(y + 16 * VSTR));
     #pragma unroll
                     for (int i = 0; i < NRB; ++i)
                         o[i][db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, pk[i], o[i][db], 0, 0, 0);
@@ -718,8 +724,9 @@ __global__ __launch_bounds__(256) void attn_paged_merge_kernel(const attn_paged_
 // with the LDS layouts of attn_prefill_fast_kernel. KH = 1: a wave takes 32 rows and all keys of a tile;
 // KH = 2: waves w and w + 2 take the same 32 rows and a half of each tile, joined through LDS at the end.
 //   * bf16: LDS-DMA, a wave KT / 4 keys of each tile, block by block of 16 (or 8) with a descriptor each.
-//   * 4 bits: a lane loads 32 codes of a row and their scale a tile and a half ahead, and puts them into LDS
-//     as bf16 at the end of the tile before.
+//   * 4 bits: a lane loads 32 codes of a row and their scale at the start of the tile before, and puts them into
+//     LDS as bf16 at its end (two tiles ahead is no faster, and at DP = 256 its registers spill: 2 x 2048 causal,
+//     32 heads 220 us, 166 with one).
 // The running maximum is raised only where a tile's is more than 2^8 above it, so that O is rarely rescaled;
 // p stays below 2^8.
 // ------------------------------------------------------------------------------------------
@@ -766,7 +773,8 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void attn_paged_prefill_kernel(con
     // Offsets of this lane's operand reads (elements): K row kperm, chunk 2kk + hi; V rows 8hi + i16 / 4
     // (+ 4), columns 16 (g16 & 1) + 4 (i16 & 3); and the wave's keys of the tile.
     const int kperm = (l32 & ~12) | ((l32 & 4) << 1) | ((l32 & 8) >> 1);
-    const int kfo = (kperm >> 3) * 8 * DP + (kperm & 7) * 16 + ((hi ^ ((kperm >> 3) & 1)) * 8) + kh * KW * DP;
+    const int kfo = (kperm >> 3) * 8 * DP + (kperm & 7) * 16 +
+                    (((hi ^ kperm >> 3 ^ (F4 ? kperm >> 2 : 0)) & 1) * 8) + kh * KW * DP;
     const int vfo = hi * 8 * DP + (i16 >> 2) * 32 + (2 * (g16 & 1) + ((i16 & 3) >> 1)) * 8 + (i16 & 1) * 4 +
                     kh * KW * DP;
 
@@ -836,8 +844,10 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void attn_paged_prefill_kernel(con
             f.vs = __builtin_amdgcn_raw_buffer_load_b8(vsr, soff, 0, 0);
         }
     };
-    // 4 bits: the lane's chunks of eight elements into the tile's layouts. K: the rows of a 16-lane pass hit
-    // other banks. V: rows four apart would not, so each starts at another of its chunks.
+    // 4 bits: the lane's chunks of eight elements into the tile's layouts, eight lanes (rows) at a time over 128
+    // bytes of banks. K: rows four apart swap the chunks of a pair. V: rows two apart start at another of
+    // their chunks; four apart at DP = 64, where they have only two of them, and at DP = 256, where the second
+    // exchange spills (2 x 2048 causal, 32 heads: 172 us with it, 166 without).
     auto put = [&](const stage &f, uint16_t *Kd, uint16_t *Vd) __attribute__((always_inline)) {
         constexpr int NC = LB / 4;
         const int r = RWV * w + srow, c0 = sgrp * NC;
@@ -846,9 +856,9 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void attn_paged_prefill_kernel(con
         for (int j = 0; j < NC; ++j) {
             const int cc = c0 + j;
             *reinterpret_cast<u32x4 *>(&Kd[(r >> 3) * 8 * DP + (cc >> 1) * 128 + (r & 7) * 16 +
-                                           ((cc & 1) ^ ((r >> 3) & 1)) * 8]) = fp4_to_bf16(f.k[j], ksc);
+                                           ((cc ^ r >> 3 ^ r >> 2) & 1) * 8]) = fp4_to_bf16(f.k[j], ksc);
         }
-        const int rot = (srow >> 2) & (NC - 1);
+        const int rot = (DP == 128 ? srow >> 1 : srow >> 2) & (NC - 1);
         uint32_t x[NC], y[NC];
 #pragma unroll
         for (int j = 0; j < NC; ++j)
@@ -1004,43 +1014,36 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void attn_paged_prefill_kernel(con
         };
         auto wait_loads = [] { __builtin_amdgcn_s_waitcnt(waitcnt_vm(0)); };
 
-        stage st[2];
+        stage st;
         if (k0 < kstop) {
             pages_of(k0);
-            load(k0, kstop, Ks0, Vs0, st[0]);
+            load(k0, kstop, Ks0, Vs0, st);
             pages_of(k0 + KT);
-            if constexpr (F4) {
-                load(k0 + KT, kstop, Ks1, Vs1, st[1]);
-                pages_of(k0 + 2 * KT);
-                put(st[0], Ks0, Vs0);
-            }
+            if constexpr (F4)
+                put(st, Ks0, Vs0);
         }
         // Q has arrived as well: waited for at its first use, inside the loop, it would be waited for there on
         // every tile, together with the loads of the next ones.
         wait_loads();
         __syncthreads();
-        // Tile i (0 or 1, in buffer i); f: the registers of the tile after it (4 bits).
-        auto step = [&](int kb, const uint16_t *Kb, const uint16_t *Vb, uint16_t *Kn, uint16_t *Vn, stage &f,
-                        stage &f2) __attribute__((always_inline)) {
-            const bool more = kb + KT < kstop;
-            if constexpr (F4) {
-                load(kb + 2 * KT, kstop, nullptr, nullptr, f2);
-            } else if (more) {
-                load(kb + KT, kstop, Kn, Vn, f);
-            }
-            pages_of(kb + (F4 ? 3 : 2) * KT);
+        // A tile in buffer Kb, Vb; the next one's rows are on their way meanwhile.
+        auto step = [&](int kb, const uint16_t *Kb, const uint16_t *Vb, uint16_t *Kn, uint16_t *Vn)
+            __attribute__((always_inline)) {
+            if (F4 || kb + KT < kstop) // 4 bits: without a branch, see load
+                load(kb + KT, kstop, Kn, Vn, st);
+            pages_of(kb + 2 * KT);
             compute(kb, Kb, Vb);
             if constexpr (F4) {
-                put(f, Kn, Vn);
+                put(st, Kn, Vn);
             } else {
                 wait_loads(); // this wave's part of the next tile has arrived
             }
             __syncthreads();
         };
         for (int kb = k0; kb < kstop; kb += 2 * KT) {
-            step(kb, Ks0, Vs0, Ks1, Vs1, st[1], st[0]);
+            step(kb, Ks0, Vs0, Ks1, Vs1);
             if (kb + KT < kstop)
-                step(kb + KT, Ks1, Vs1, Ks0, Vs0, st[0], st[1]);
+                step(kb + KT, Ks1, Vs1, Ks0, Vs0);
         }
         l_run = sum_xor32(l_run);
 
