@@ -214,8 +214,23 @@ ATTEND = [
     (16, 256, 16, 8, 2, [(8, 70)], 1, 0, 0, None, None),
     (4, 128, 16, 8, 1, [(8, 257), (2, 31)], 1, 20.0, 0, None, None),
     (4, 256, 16, 4, 1, [(9, 90)], 1, 0, 0, None, None),
+    (16, 256, 64, 4, 1, [(1, 260), (3, 40)], 1, 12.0, 0, None, None),
+    (4, 128, 64, 8, 2, [(4, 700), (1, 20)], 1, 0, 1, None, None),
+    (4, 256, 64, 8, 2, [(1, 410), (1, 7)], 1, 0, 0, None, None),
+    (16, 256, 32, 8, 2, [(7, 150), (1, 3)], 1, 0, 1, None, None),
+    (4, 256, 32, 8, 2, [(8, 90), (5, 5)], 0, 7.0, 0, None, None),
+    # two row blocks
+    (16, 128, 32, 8, 2, [(7, 400), (3, 2), (5, 129)], 1, 0, 0, None, None),
+    (16, 112, 16, 4, 1, [(5, 77), (8, 300)], 1, 11.0, 1, None, None),
+    (16, 64, 64, 6, 2, [(10, 200), (1, 31)], 0, 0, 0, None, None),
+    (16, 48, 16, 2, 1, [(12, 12), (16, 90)], 1, 0, 1, None, None),
+    (4, 128, 128, 8, 2, [(8, 600), (2, 1)], 1, 0, 0, None, None),
+    (4, 128, 16, 8, 2, [(6, 99)], 1, 40.0, 0, None, None),
+    (4, 64, 32, 4, 1, [(5, 260), (7, 64)], 1, 0, 0, None, None),
+    (4, 64, 16, 10, 2, [(6, 65)], 1, 0, 1, None, None),
     # 33 to 64 rows of a kv head: key halves
     (16, 128, 32, 16, 2, [(8, 900), (5, 70), (4, 2)], 1, 0, 1, None, None),
+    (16, 128, 16, 8, 1, [(8, 300), (0, 9), (5, 40)], 1, 0, 0, None, None),
     (16, 64, 16, 8, 1, [(8, 300), (0, 9), (6, 6)], 0, 0, 0, None, None),
     (16, 48, 64, 10, 1, [(5, 333), (4, 40)], 1, 9.0, 0, None, None),
     (4, 128, 64, 16, 2, [(7, 500), (8, 33)], 1, 0, 0, None, None),
@@ -235,6 +250,15 @@ ATTEND = [
     (4, 128, 16, 8, 2, [(65, 130), (100, 100)], 1, 0, 0, None, None),
     (4, 64, 64, 6, 2, [(150, 400)], 1, 50.0, 1, None, None),
     (4, 256, 32, 4, 1, [(40, 77)], 0, 0, 0, None, None),
+    (16, 256, 16, 2, 2, [(66, 200), (90, 90)], 1, 0, 0, None, None),
+    (4, 256, 64, 2, 1, [(50, 120)], 1, 6.0, 0, None, None),
+    (4, 64, 16, 4, 1, [(50, 60)], 1, 0, 0, None, None),
+    (4, 128, 16, 4, 1, [(50, 260)], 0, 0, 1, None, None),
+    (16, 128, 32, 4, 1, [(50, 260)], 1, 6.0, 0, None, None),
+    (4, 64, 32, 16, 1, [(4, 100)], 1, 0, 0, None, None),
+    # more row tiles than CUs
+    *[(bits, D, 16, 8, 8, [(70 + i % 60, 3 * i + 20) for i in range(40)], 0, cap, 0, None, None)
+      for bits, D in ((16, 128), (16, 64), (4, 128), (4, 64)) for cap in (0, 25.0)],
     # bounds that sequences pass: rows and keys behind them are served too
     (16, 128, 16, 8, 2, [(9, 300), (50, 60)], 1, 0, 0, 1, 16),
     (16, 128, 64, 8, 8, [(300, 700)], 1, 0, 0, 70, 200),

@@ -8,6 +8,8 @@ import subprocess
 
 import pytest
 
+import transfer_station_amd as ts
+from test_paged import ATTEND
 from transfer_station_amd import build as _build
 
 ROCM = os.environ.get("ROCM_PATH", "/opt/rocm")
@@ -50,7 +52,7 @@ def test_no_spills(code):
     spills = code[1]
     decode = {n: c for n, c in spills.items() if "paged_decode" in n}
     prefill = {n: c for n, c in spills.items() if re.search(r"paged_prefill_kernelILi(64|128)E", n)}
-    assert len(decode) >= 30 and len(prefill) >= 20, (len(decode), len(prefill))
+    assert len(decode) >= 24 and len(prefill) >= 20, (len(decode), len(prefill))
     bad = {n: c for n, c in {**decode, **prefill}.items() if c}
     assert not bad, bad
 
@@ -68,7 +70,7 @@ def test_decode_keeps_the_next_tiles_loads_in_flight(code):
         waits = [int(re.search(r"vmcnt\((\d+)\)", x).group(1)) for x in ins[mf[0] - 8:mf[-1]]
                  if x.startswith("s_waitcnt") and "vmcnt" in x]
         assert len(waits) >= 4 and min(waits) >= 4, (name, waits)
-    assert n == 8, n
+    assert n == 4, n
 
 
 def test_prefill_waits_for_its_dma_at_the_end_of_a_tile(code):
@@ -87,3 +89,24 @@ def test_prefill_waits_for_its_dma_at_the_end_of_a_tile(code):
                     bad.append(i)
         assert not bad, (name, bad)
     assert n >= 12
+
+
+def test_every_attention_kernel_is_reached(code):
+    """The plans of the calls that the GPU tests make name every instance that the library holds."""
+    seen = set()
+    for bits, D, page, Hq, Hkv, seqs, causal, cap, slopes, mq, mk in ATTEND:
+        cols = max([-(-k // page) for _, k in seqs] + [1]) + 1
+        c = ts.KvCache(4096, 4096, 4096, 4096, 4096, len(seqs), cols, 1000, page, Hkv, D, bits, 4096, 4096)
+        plan = ts.attn_paged_plan(c, sum(n for n, _ in seqs) + 3, Hq, causal,
+                                  ts.Scores(0.0, cap, 4096 if slopes else None),
+                                  mq or max([n for n, _ in seqs] + [1]), mk or max([k for _, k in seqs] + [1]))
+        seen.update(k[0] for k in plan if "merge" not in k[0])
+    held = set()
+    for name in code[0]:
+        m = re.search(r"(attn_paged_\w+?_kernel)I(Li\d+E)(Lb\dE)((?:L[ib]\d+E)+)E", name)
+        if m:
+            args = [m.group(2)[2:-1], "4" if m.group(3) == "Lb1E" else "16"]
+            args += [x[1:] if x[0] == "i" else ("false", "true")[int(x[1:])]
+                     for x in re.findall(r"L([ib]\d+)E", m.group(4))]
+            held.add("%s<%s>" % (m.group(1), ", ".join(args)))
+    assert len(held) >= 40 and held == seen, (sorted(held - seen), sorted(seen - held))

@@ -26,7 +26,8 @@
 //   attn_merge{2,w,}_kernel                log-sum-exp merge of split partials (2 splits / up to
 //                                          64 / any, one workgroup per row)
 //   attn_pack_v16_kernel<TK,VEC>           V [Hkv][Sk][D] -> V^T [Hkv][D][Sk]
-// VT selects a pre-transposed V ([Hkv][D][Sk], pack_v_full's layout).
+// VT selects a pre-transposed V ([Hkv][D][Sk], pack_v_full's layout). The paged cache's kernels are in
+// attn_paged_kernels.h, at the end.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 #include <stdlib.h>

@@ -188,13 +188,19 @@ __device__ __forceinline__ float part_max(float m, float l) {
 }
 
 // ------------------------------------------------------------------------------------------
-// Few query rows per kv head. One workgroup per (sequence b, kv head u, part sp of its keys, tile of
-// 16 NRB rows); a sequence's rows are its tokens' heads of the group, token by token. The four waves take
-// interleaved tiles of 32 keys (two blocks of 16), each with a softmax of its own:
+// Few query rows per kv head. A workgroup takes its quota of the decode line (attn_quota) -- keys of one
+// sequence and kv head after the other -- for one tile of 16 NRB rows (or, without teams, a whole sequence); a
+// sequence's rows are its tokens' heads of the group, token by token. The four waves take interleaved tiles of 32
+// keys (two blocks of 16), each with a softmax of its own:
 //   S^T[key][row] = K . Q^T   (v_mfma_f32_16x16x32_bf16, K from memory straight into the operand)
 //   O^T[d][row]  += V^T . P^T (V through a wave-private LDS tile and the transposed read)
-// and merge in LDS at the end. Tiles past the grid's (a sequence with more rows than max_q says) follow
-// in the same workgroup, keys past the grid's in the last part.
+// and merge in LDS at the end of each sequence. Tiles past the grid's (a sequence with more rows than max_q says)
+// follow in the same workgroup.
+//
+// Bound by HBM: 64 sequences of 4096 keys, 8 kv heads, D = 128: bf16 163 us (6.6 TB/s), 4 bits 52.6 (5.4 TB/s, where
+// the unpacking takes 11 instructions per MFMA); of 250 to 8192 keys 162 us for 1.02 GB. Equal quotas are why: with
+// a workgroup per part of a sequence the same ragged batch took 198. One sequence of 32768, D = 256, 4 bits, is
+// 14.4 us of latency: start, four units, the join.
 // ------------------------------------------------------------------------------------------
 template <int DP, bool F4, int NRB, bool MOD, bool NTL>
 __global__ __launch_bounds__(256, 2) void attn_paged_decode_kernel(const attn_paged_args a) {
@@ -601,7 +607,8 @@ __global__ __launch_bounds__(256, 2) void attn_paged_decode_kernel(const attn_pa
 // parts, NL loads of each thread on their way before the weights are known. The attention kernel says what
 // a row has: +inf as the first m where it wrote the row itself, -inf behind the last part (whose acc is
 // whatever it was: it gets no weight and is not multiplied). What bounds it is latency: the maxima, sums
-// and columns of a row are all asked for at once, right behind the sequence's start.
+// and columns of a row are all asked for at once, right behind the sequence's start. 2.8 us where nothing or
+// little was cut, 4.4 for 16 rows of 65 parts at D = 256, 6.4 for 16384 rows of two parts.
 constexpr int kPagedMaxSplit = ATTN_PAGED_MAX_PARTS;
 template <int NL>
 __global__ __launch_bounds__(256) void attn_paged_merge_kernel(const attn_paged_args a, int lglp, int lgsg,
@@ -727,8 +734,13 @@ __global__ __launch_bounds__(256) void attn_paged_merge_kernel(const attn_paged_
 //   * 4 bits: a lane loads 32 codes of a row and their scale at the start of the tile before, and puts them into
 //     LDS as bf16 at its end (two tiles ahead is no faster, and at DP = 256 its registers spill: 2 x 2048 causal,
 //     32 heads 220 us, 166 with one).
-// The running maximum is raised only where a tile's is more than 2^8 above it, so that O is rarely rescaled;
-// p stays below 2^8.
+// The running maximum is raised only where a lane's sum of p over a tile passes kPagedSum, so that O is rarely
+// rescaled and most tiles look for no maximum.
+//
+// Bound by its instruction mix: per tile MFMA, exp and LDS reads on two waves per SIMD (5.2 VALU and MFMA
+// instructions per MFMA at D = 128, 6.5 with the unpacking). 32 heads on 8 kv heads, 2 x 4096 without a mask: D =
+// 128 525 us (1047 TFLOP/s) in bf16 and 530 in 4 bits, D = 64 324; 2 x 2048 causal at D = 256 147 and 164; 512
+// tokens over 8192 keys 74 and the merge. LDS-DMA instead of registers in bf16: 614 -> 526 at D = 128.
 // ------------------------------------------------------------------------------------------
 // Bound on a lane's sum of p over a tile against a maximum that may lie below the tile's: p costs no precision
 // up to it, only exponent range.
@@ -1124,7 +1136,8 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void attn_paged_prefill_kernel(con
 // products and sums rounded apart, the result once to bf16), the wave's lanes lie across several heads, and
 // four of a lane's heads are in flight, so that the cosines and sines are read once per wave. K and V of the
 // 4-bit cache go eight elements to a lane, four lanes to a group. HBM-bound: each element is read and
-// written once, past the L2, whose copies the attention on other XCDs could not use.
+// written once, past the L2, whose copies the attention on other XCDs could not use. 12700 tokens of 32 + 2 x 8
+// heads, D = 128, bf16: 56 us, 5.6 TB/s read and written, the rate of a copy (a wave per token 62.7); one token 2.5 us.
 // ------------------------------------------------------------------------------------------
 __device__ __forceinline__ float lo_bf16(uint32_t x) { return __builtin_bit_cast(float, x << 16); }
 __device__ __forceinline__ float hi_bf16(uint32_t x) {
@@ -1341,7 +1354,8 @@ __global__ __launch_bounds__(256) void attn_kv_read_kernel(const attn_kv_args a)
                     if constexpr (F4)
                         y = fp4_to_bf16(x[e][0], e8m0(sc[e]));
                     if (hl < hp && h < a.Hkv)
-                        __builtin_nontemporal_store(ok ? y : zero4(), reinterpret_cast<u32x4 *>(dst + h * dhead + 8 * j));
+                        __builtin_nontemporal_store(ok ? y : zero4(),
+                                                    reinterpret_cast<u32x4 *>(dst + h * dhead + 8 * j));
                 }
             }
         };
@@ -1368,15 +1382,18 @@ hipError_t launch_paged_d(const attn_paged_args &a, const attn_paged_cut &cut, h
             hipLaunchKernelGGL((attn_paged_decode_kernel<DP, F4, kN, kM, kT>), grid, block, 0, st, a);
             return hipGetLastError();
         };
-        if (cut.rows16 == 1)
-            return with_flag(a.tps == 1, [&](auto NT) {
-                return decode(std::integral_constant<int, 1>{}, NT);
-            });
-        if constexpr (DP <= 128)
+        constexpr std::integral_constant<int, 1> one;
+        constexpr std::integral_constant<int, 2> two;
+        // Non-temporal where a row tile is the only one of its sequence, which at D <= 128 it always is.
+        if constexpr (DP > 128) {
+            if (cut.rows16 == 1)
+                return with_flag(a.tps == 1, [&](auto NT) { return decode(one, NT); });
+        } else {
+            if (cut.rows16 == 1)
+                return decode(one, std::true_type{});
             if (cut.rows16 == 2)
-                return with_flag(a.tps == 1, [&](auto NT) {
-                    return decode(std::integral_constant<int, 2>{}, NT);
-                });
+                return decode(two, std::true_type{});
+        }
         auto prefill = [&](auto KHF, auto NWF) {
             constexpr int kK = decltype(KHF)::value, kW = decltype(NWF)::value;
             if (t_plan) {
@@ -1387,8 +1404,6 @@ hipError_t launch_paged_d(const attn_paged_args &a, const attn_paged_cut &cut, h
             hipLaunchKernelGGL((attn_paged_prefill_kernel<DP, F4, kM, kK, kW>), grid, dim3(64 * kW), 0, st, a);
             return hipGetLastError();
         };
-        constexpr std::integral_constant<int, 1> one;
-        constexpr std::integral_constant<int, 2> two;
         constexpr std::integral_constant<int, 4> four;
         constexpr std::integral_constant<int, 8> eight;
         if constexpr (DP <= 128) {
