@@ -154,10 +154,10 @@ struct attn_scores {
 };
 
 /* Writes a call's K and V rows into the cache, K with its position's rotation, and the rotated Q to q_out
- * (q_out may be q; q and q_out may both be NULL). The first `rot` elements of a head turn (0: none), in
- * pairs (i, i + rot/2), or with `pairs` (2i, 2i + 1): (x1, x2) -> (x1 c - x2 s, x2 c + x1 s) in fp32,
- * rounded once to bf16, with c and s from row p of rope [rope_rows][rot], cosines in its first half, for
- * position p. In 4 bits the rounded rows are quantised: a group's scale is the smallest power of two in
+ * (q_out may be q, with its strides; q and q_out may both be NULL). The first `rot` elements of a head turn
+ * (0: none), in pairs (i, i + rot/2), or with `pairs` (2i, 2i + 1): (x1, x2) -> (x1 c - x2 s, x2 c + x1 s)
+ * in fp32, rounded once to bf16, with c and s from row p of rope [rope_rows][rot], cosines in its first half,
+ * for position p. In 4 bits the rounded rows are quantised: a group's scale is the smallest power of two in
  * [2^-126, 2^125] under which its largest element is at most 7, elements round to nearest, ties to even; a
  * group with a NaN or an infinity reads as NaN. Tokens whose position is below 0 or has no row in rope are
  * skipped, q's rows too. */

@@ -110,6 +110,8 @@ REFUSED = [
     (append(Hq=5), "Hq % Hkv"),
     (append(q="None"), "q_out without q"),
     (append(qo="None"), "q_out needs"),
+    (append(qo="ts.Rows(r.data, r.token + 8, r.head)"), "needs q's strides"),
+    (append(qo="ts.Rows(r.data, r.token, r.head + 8)"), "needs q's strides"),
     (append(k="none"), "k needs"),
     (append(v="ts.Rows(4096, 4, 8)"), "v needs"),
     (append(rot=136), "rot must be"),

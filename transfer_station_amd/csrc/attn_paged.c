@@ -190,6 +190,8 @@ void attn_kv_append(const struct attn_kv_cache *c, const struct attn_rows *q, co
         paged_check_heads(who, c, T, Hq);
         paged_check_rows(who, "q", q);
         paged_check_rows(who, "q_out", q_out);
+        if (q_out->data == q->data && (q_out->token != q->token || q_out->head != q->head))
+            paged_fail(who, "q_out at q's address needs q's strides");
     } else if (q_out) {
         paged_fail(who, "q_out without q");
     }
