@@ -259,6 +259,9 @@ ATTEND = [
     # more row tiles than CUs
     *[(bits, D, 16, 8, 8, [(70 + i % 60, 3 * i + 20) for i in range(40)], 0, cap, 0, None, None)
       for bits, D in ((16, 128), (16, 64), (4, 128), (4, 64)) for cap in (0, 25.0)],
+    # four parts of a row, and many
+    (4, 64, 32, 16, 2, [(8, 100 + 10 * i) for i in range(31)] + [(5, 512)], 1, 0, 0, None, None),
+    (16, 128, 64, 8, 2, [(1, 5000), (1, 2500)], 1, 0, 0, None, None),
     # bounds that sequences pass: rows and keys behind them are served too
     (16, 128, 16, 8, 2, [(9, 300), (50, 60)], 1, 0, 0, 1, 16),
     (16, 128, 64, 8, 8, [(300, 700)], 1, 0, 0, 70, 200),

@@ -100,8 +100,9 @@ def test_every_attention_kernel_is_reached(code):
         plan = ts.attn_paged_plan(c, sum(n for n, _ in seqs) + 3, Hq, causal,
                                   ts.Scores(0.0, cap, 4096 if slopes else None),
                                   mq or max([n for n, _ in seqs] + [1]), mk or max([k for _, k in seqs] + [1]))
-        seen.update(k[0] for k in plan if "merge" not in k[0])
-    held = set()
+        seen.update(k[0] for k in plan)
+    held = {"attn_paged_merge_kernel<%s>" % x for n in code[0]
+            for x in re.findall(r"attn_paged_merge_kernelILi(\d+)E", n)}
     for name in code[0]:
         m = re.search(r"(attn_paged_\w+?_kernel)I(Li\d+E)(Lb\dE)((?:L[ib]\d+E)+)E", name)
         if m:
@@ -109,4 +110,4 @@ def test_every_attention_kernel_is_reached(code):
             args += [x[1:] if x[0] == "i" else ("false", "true")[int(x[1:])]
                      for x in re.findall(r"L([ib]\d+)E", m.group(4))]
             held.add("%s<%s>" % (m.group(1), ", ".join(args)))
-    assert len(held) >= 40 and held == seen, (sorted(held - seen), sorted(seen - held))
+    assert len(held) >= 50 and held == seen, (sorted(held - seen), sorted(seen - held))

@@ -1438,8 +1438,8 @@ extern "C" int attn_hip_launch_paged(const struct attn_paged_args *ap, const str
     if (e != hipSuccess || a.nsplit == 1)
         return (int)e;
     const dim3 mgrid((unsigned)((long)a.B * a.Hkv * cut->merge_tiles));
-    return (int)with_flag(cut->merge_loads == 2, [&](auto FEW) {
-        constexpr int kL = decltype(FEW)::value ? 2 : 8;
+    auto merge = [&](auto L) {
+        constexpr int kL = decltype(L)::value;
         if (t_plan) {
             plan_note(mgrid, dim3(256), "attn_paged_merge_kernel<%d> rows=%d", kL,
                       256 >> (cut->lglp + cut->lgsg));
@@ -1448,7 +1448,10 @@ extern "C" int attn_hip_launch_paged(const struct attn_paged_args *ap, const str
         hipLaunchKernelGGL(attn_paged_merge_kernel<kL>, mgrid, dim3(256), 0, st, a, cut->lglp, cut->lgsg,
                            cut->merge_tiles);
         return hipGetLastError();
-    });
+    };
+    return (int)(cut->merge_loads == 2   ? merge(std::integral_constant<int, 2>{})
+                 : cut->merge_loads == 4 ? merge(std::integral_constant<int, 4>{})
+                                         : merge(std::integral_constant<int, 8>{}));
 }
 
 extern "C" int attn_hip_launch_kv_append(const struct attn_kv_args *ap, int bits, int pairs, void *stream) {
