@@ -15,7 +15,7 @@
 #include <stdlib.h>
 #include <string.h>
 
-static int failures, split_calls;
+static int failures, split_calls, full_calls;
 #define CHECK(cond, ...)                                                                           \
     do {                                                                                           \
         if (!(cond)) {                                                                             \
@@ -118,6 +118,7 @@ int attn_hip_launch_paged(const struct attn_paged_args *a, const struct attn_pag
     /* What the sequences did not reach is in bounds too: T is the call's, not theirs. */
     const int64_t last = (int64_t)a->T * a->Hq * a->nsplit - 1;
     CHECK(last < ATTN_SLOTS, "%lld slots", (long long)last + 1);
+    full_calls += last == ATTN_SLOTS - 1;
     a->pl[last] = 1.f;
     a->pacc[last * a->D + a->D - 1] = 1.f;
     free(seen);
@@ -130,27 +131,44 @@ static int pick(int lo, int hi) {
     return lo + (int)((rng_state >> 8) % (uint32_t)(hi - lo + 1));
 }
 
+static void call(int B, int T, int Hkv, int g, int D, int cols, const int32_t *start, const int32_t *kv, int bk,
+                 int causal, int max_q, int max_kv) {
+    int32_t *table = calloc((size_t)B * cols, sizeof *table);
+    const struct attn_kv_cache c = {(void *)4096, (void *)4096, NULL, NULL, table, kv, start, B, cols,
+                                    3,            32,           Hkv,  D,    ATTN_KV_BF16};
+    const struct attn_rows r = {(void *)4096, 8, 8}, o = {(void *)8192, 8, 8};
+    const size_t len = attn_flash_scratch_bytes(D, bk);
+    CHECK(len % 256 == 0, "scratch of %zu bytes", len);
+    char *scratch = aligned_alloc(ATTN_SCRATCH_ALIGN, len);
+    attn_paged(&c, &r, &o, T, g * Hkv, causal, NULL, max_q, max_kv, scratch);
+    free(scratch), free(table);
+}
+
 int main(void) {
-    for (int it = 0; it < 400; ++it) {
+    for (int it = 0; it < 300; ++it) {
         const int B = pick(1, 40), Hkv = pick(1, 4), g = pick(1, 8), D = 16 * pick(1, 16);
         const int q = it % 4 == 0 ? 1 : it % 4 == 1 ? pick(1, 12) : pick(1, 300), cols = pick(1, 200);
-        int32_t *kv = malloc(sizeof *kv * (size_t)B), *start = malloc(sizeof *start * (size_t)(B + 1));
-        int32_t *table = calloc((size_t)B * cols, sizeof *table);
+        int32_t kv[40], start[41];
         start[0] = 0;
         for (int b = 0; b < B; ++b) {
             start[b + 1] = start[b] + (pick(0, 4) ? pick(1, q) : 0);
             kv[b] = pick(0, cols * 32 + 40);
         }
-        const int T = start[B] + pick(1, 9), bk = 16 << pick(0, 8);
-        const struct attn_kv_cache c = {(void *)4096, (void *)4096, NULL, NULL, table, kv, start, B, cols,
-                                        3,            32,           Hkv,  D,    ATTN_KV_BF16};
-        const struct attn_rows r = {(void *)4096, 8, 8}, o = {(void *)8192, 8, 8};
-        const size_t len = attn_flash_scratch_bytes(D, bk);
-        CHECK(len % 256 == 0, "scratch of %zu bytes", len);
-        char *scratch = aligned_alloc(ATTN_SCRATCH_ALIGN, len);
-        attn_paged(&c, &r, &o, T, g * Hkv, pick(0, 1), NULL, pick(1, 2 * q), pick(1, cols * 40), scratch);
-        free(scratch), free(kv), free(start), free(table);
+        call(B, start[B] + pick(1, 9), Hkv, g, D, cols, start, kv, 16 << pick(0, 8), pick(0, 1), pick(1, 2 * q),
+             pick(1, cols * 40));
     }
+    /* Rows times parts that fill the scratch to its last slot: single tokens, drafts and chunks. */
+    for (int lg = 0; lg <= 15; ++lg)
+        for (int which = 0; which < 9; ++which) {
+            const int Hkv = which % 3 == 2 ? 8 : 1, g = which % 3 == 0 ? 1 : 4, D = which < 3 ? 64 : which < 6 ? 128 : 256;
+            if (1 << lg < Hkv * g)
+                continue;
+            const int T = (1 << lg) / (Hkv * g), n = T < 70 ? T : 70;
+            const int32_t kv[2] = {60000, 3000}, start[3] = {0, T - n, T};
+            for (int mq = 1; mq <= 64; mq *= 8)
+                call(2, T, Hkv, g, D, 2048, start, kv, 128, 1, mq, 65536);
+        }
+    CHECK(full_calls > 20, "%d calls fill the scratch", full_calls);
     CHECK(split_calls > 150, "%d calls with parts", split_calls);
     if (failures)
         return 1;
