@@ -7,6 +7,14 @@ import pytest
 import paged_util as pu
 import transfer_station_amd as ts
 from test_paged import check
+from transfer_station_amd import _lib
+
+
+def memcpy_from(ptr, shape):
+    out = np.empty(shape, np.uint16)
+    _lib.check(_lib.lib().attn_dev_memcpy_dtoh(out.ctypes.data, ptr, out.nbytes), "hipMemcpy")
+    return out
+
 
 # One of each kernel: bits, D, page, Hq, Hkv, (new, length) by sequence.
 KERNELS = [
@@ -319,3 +327,212 @@ def test_single_tokens_beside_a_chunk(bits, D):
     q = pu.normal((c.N, Hq, D), 5)
     ref, bound = pu.attend_ref(c, q, Hq, 1)
     check(pu.attend(c, q, Hq, 1), ref, bound, (bits, D))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [16, 4])
+def test_one_step_in_two_calls(bits):
+    """A step's single tokens and its chunk in a call each, on parts of the same arrays: the tokens' rows lie first, so
+    that their call's T ends with them, and the chunk's call takes the last sequence's entries."""
+    D, Hq, Hkv, page = 128, 8, 2, 32
+    seqs = [(1, 900), (1, 64), (1, 1), (1, 1500), (100, 700)]
+    c = pu.Cache(seqs, Hkv, D, page, bits, 3)
+    c.fill(11)
+    whole = pu.Cache(seqs, Hkv, D, page, bits, 3)
+    whole.fill(11)
+    x = pu.normal((c.N, Hq + 2 * Hkv, D), 5)
+    rope = pu.rope_table(1500, D)
+    W, k = (Hq + 2 * Hkv) * D, len(seqs) - 1
+    q_ref = np.empty((c.N, Hq, D), np.uint16)
+    for b, (n, kv) in enumerate(seqs):
+        r, pos = slice(c.start[b], c.start[b + 1]), np.arange(kv - n, kv)
+        q_ref[r] = pu.rotate(x[r, :Hq], pos, rope, D, 0)
+        whole.put(b, kv - n, pu.rotate(x[r, Hq:Hq + Hkv], pos, rope, D, 0), x[r, Hq + Hkv:])
+    with ts.DeviceBuffer.from_array(x) as dx, ts.DeviceBuffer(c.N * Hq * D * 2) as do, \
+            ts.DeviceBuffer(ts.attn_flash_scratch_bytes(D, 128)) as ds, ts.DeviceBuffer.from_array(rope) as dr:
+        do.fill_bytes(0xFF)
+        first = c.device()
+        d = c.bufs
+        ks, vs = (d["ks"], d["vs"]) if bits == 4 else (None, None)
+        first.B = k
+        last = ts.KvCache(d["k"], d["v"], d["table"].ptr + 4 * k * c.cols, d["kv_len"].ptr + 4 * k,
+                          d["start"].ptr + 4 * k, 1, c.cols, c.pages, page, Hkv, D, bits, ks, vs)
+        q, kk, v = (ts.Rows(dx.ptr + 2 * D * h, W, D) for h in (0, Hq, Hq + Hkv))
+        o = ts.Rows(do, Hq * D, D)
+        for desc, T, mq, mkv in ((first, k, 1, 1500), (last, c.N, 100, 700)):
+            ts.attn_kv_append(desc, q, q, kk, v, T, Hq, dr, len(rope), D, 0, mq)
+            ts.attn_paged(desc, q, o, T, Hq, 1, None, mq, mkv, ds)
+        ts.synchronize()
+        got_q = dx.download(np.uint16).reshape(x.shape)[:, :Hq]
+        O = pu.f32(do.download(np.uint16)).reshape(c.N, Hq, D)
+    c.download()
+    assert np.array_equal(got_q, q_ref)
+    for y in ("k", "v", "ks", "vs"):
+        assert np.array_equal(getattr(c, y), getattr(whole, y)), y
+    ref, bound = pu.attend_ref(c, q_ref, Hq, 1)
+    check(O, ref, bound, bits)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("n", [1, 8, 40])
+def test_shared_pages(bits, n):
+    """Sequences that share the pages of a prefix, one of them a page twice."""
+    D, Hq, Hkv, page = 64, 8, 2, 16
+    c = pu.Cache([(n, 300), (n, 210), (n, 500)], Hkv, D, page, bits, 3)
+    c.fill(11)
+    c.table[1, :12] = c.table[0, :12]
+    c.table[2, 20] = c.table[2, 3]
+    q = pu.normal((c.N, Hq, D), 5)
+    ref, bound = pu.attend_ref(c, q, Hq, 1)
+    check(pu.attend(c, q, Hq, 1), ref, bound, (bits, n))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [16, 4])
+def test_graph_of_a_chunk_replayed_with_other_lengths(bits):
+    """A captured step of up to 64 tokens a sequence (append, attend in prefill tiles, read back), replayed with other
+    tokens, starts, lengths and pages, none among them, each time against the same step run eagerly."""
+    D, Hq, Hkv, page, cols, T = 128, 8, 2, 16, 60, 140
+    hip = pu.Hip()
+    c = pu.Cache([(1, cols * page)] * 3, Hkv, D, page, bits, 3, spare=0, cols=cols)
+    c.fill(5)
+    desc = c.device()
+    clean = {y: getattr(c, y).copy() for y in ("k", "v", "ks", "vs")}
+    rope, W = pu.rope_table(cols * page, D), (Hq + 2 * Hkv) * D
+    with ts.DeviceBuffer(T * W * 2) as dx, ts.DeviceBuffer(T * Hq * D * 2) as dq, \
+            ts.DeviceBuffer(T * Hq * D * 2) as do, ts.DeviceBuffer(2 * T * Hkv * D * 2) as dk, \
+            ts.DeviceBuffer.from_array(rope) as dr, ts.DeviceBuffer(ts.attn_flash_scratch_bytes(D, 128)) as ds:
+        q, qo, o = ts.Rows(dx, W, D), ts.Rows(dq, Hq * D, D), ts.Rows(do, Hq * D, D)
+        k, v = (ts.Rows(dx.ptr + 2 * D * h, W, D) for h in (Hq, Hq + Hkv))
+        bk, bv = ts.Rows(dk, 2 * Hkv * D, D), ts.Rows(dk.ptr + 2 * Hkv * D, 2 * Hkv * D, D)
+        plan = ts.attn_paged_plan(desc, T, Hq, 1, None, 64, cols * page)
+        assert "prefill" in plan[0][0] and len(plan) == 2, plan
+
+        def step():
+            ts.attn_kv_append(desc, q, qo, k, v, T, Hq, dr, len(rope), D, 0, 64)
+            ts.attn_paged(desc, qo, o, T, Hq, 1, None, 64, cols * page, ds)
+            ts.attn_kv_read(desc, bk, bv, T, 64)
+
+        st = hip.stream()
+        ex = hip.capture(st, step)
+        for it, seqs in enumerate([[(64, 64), (1, 400), (30, 960)], [(0, 17), (64, 700), (64, 65)],
+                                   [(1, 1), (1, 2), (1, 959)], [(0, 0), (0, 0), (0, 0)], [(10, 200), (0, 9), (64, 64)]]):
+            c.seqs, c.kv_len = seqs, np.array([x for _, x in seqs], np.int32)
+            c.start = np.concatenate([[0], np.cumsum([x for x, _ in seqs])]).astype(np.int32)
+            c.N = int(c.start[-1])
+            c.table = np.random.default_rng(it).permutation(c.pages)[:3 * cols].astype(np.int32).reshape(3, cols)
+            got = []
+            for run in (lambda: hip("hipGraphLaunch", ex, st), step):
+                for y in clean:
+                    setattr(c, y, clean[y].copy())
+                c.device()
+                dx.upload(pu.normal((T, Hq + 2 * Hkv, D), 40 + it))
+                for d in (dq, do, dk):
+                    d.fill_bytes(0xFF)
+                ts.synchronize()
+                run()
+                ts.synchronize()
+                c.download()
+                got.append([d.download(np.uint16) for d in (do, dq, dk)] + [getattr(c, y).copy() for y in clean])
+            for a, b in zip(*got):
+                assert np.array_equal(a, b), it
+            O = got[0][0].reshape(T, Hq, D)
+            assert np.all(O[c.N:] == 0xFFFF)
+            if c.N:
+                ref, bound = pu.attend_ref(c, got[0][1].reshape(T, Hq, D)[:c.N], Hq, 1)
+                check(pu.f32(O[:c.N]), ref, bound, it)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("Hq", [4, 128])
+def test_rows_past_4_gib(bits, Hq):
+    """Token tensors whose rows lie 2 GiB apart, by tokens and then by heads."""
+    D, Hkv, page, n, kv = 64, 4, 32, 3, 600
+    far = (1 << 30) + 8
+    H = Hq + 2 * Hkv
+    c = pu.Cache([(n, kv)], Hkv, D, page, bits, 3)
+    c.fill(11)
+    rope = pu.rope_table(kv, D)
+    x = pu.normal((n, H, D), 5)
+    with ts.DeviceBuffer(3 * 2 * far + (1 << 20)) as big, ts.DeviceBuffer.from_array(rope) as dr, \
+            ts.DeviceBuffer(ts.attn_flash_scratch_bytes(D, 128)) as ds, \
+            ts.DeviceBuffer(n * Hq * D * 2) as near:
+        for i in range(n):
+            pu.memcpy_to(big.ptr + 2 * i * far, x[i])
+
+        def rows(h):
+            return ts.Rows(big.ptr + 2 * D * h, far, D)
+
+        desc = c.device()
+        ts.attn_kv_append(desc, rows(0), rows(0), rows(Hq), rows(Hq + Hkv), n, Hq, dr, kv, D, 0, n)
+        ts.attn_paged(desc, rows(0), rows(H), n, Hq, 1, None, n, kv, ds)
+        ts.attn_kv_read(desc, rows(2 * H), rows(2 * H + Hkv), n, n)
+        ts.attn_paged(desc, rows(0), ts.Rows(near, Hq * D, D), n, Hq, 1, None, n, kv, ds)
+        ts.synchronize()
+        got = np.stack([memcpy_from(big.ptr + 2 * i * far, (4 * H, D)) for i in range(n)])
+        same = near.download(np.uint16).reshape(n, Hq, D)
+        c.download()
+        pos = np.arange(kv - n, kv)
+        q = pu.rotate(x[:, :Hq], pos, rope, D, 0)
+        assert np.array_equal(got[:, :Hq], q)
+        ref, bound = pu.attend_ref(c, q, Hq, 1)
+        check(pu.f32(got[:, H:H + Hq]), ref, bound, (bits, Hq))
+        assert np.array_equal(got[:, H:H + Hq], same)
+        K, V = c.get(0, kv - n, kv)
+        assert np.array_equal(pu.f32(got[:, 2 * H:2 * H + Hkv]), K)
+        assert np.array_equal(pu.f32(got[:, 2 * H + Hkv:2 * H + 2 * Hkv]), V)
+        # heads apart: three of them, one kv head
+        if bits == 16 and Hq == 4:
+            d = pu.Cache([(n, kv)], 1, D, page, bits, 3)
+            d.fill(12)
+            y = pu.normal((n, 3, D), 6)
+            for h in range(3):
+                pu.memcpy_to(big.ptr + 2 * h * far, np.ascontiguousarray(y[:, h]))
+            ts.attn_paged(d.device(), ts.Rows(big, D, far), ts.Rows(big.ptr + 4096, D, far), n, 3, 1, None, n, kv, ds)
+            ts.synchronize()
+            O = np.stack([memcpy_from(big.ptr + 4096 + 2 * h * far, (n, D)) for h in range(3)], 1)
+            ref, bound = pu.attend_ref(d, y, 3, 1)
+            check(pu.f32(O), ref, bound, "heads")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits,D,n", [(16, 16, 1), (4, 64, 1), (16, 16, 9), (16, 16, 20), (4, 64, 30)])
+def test_the_longest_sequence(bits, D, n):
+    """2^30 keys in a table row whose entries name a few pages over and over, and one page once, at the very end, which
+    holds the keys that the rows look for: one that all of them see, and the last of all, which the last row sees.
+    These outweigh each other key by e^39, and there are e^20.8 of those, so that what they add is lost in the
+    roundings: 2^-8 each of P and O, and 2^-8 for the scores', of a magnitude of 40 and D + 16 times 2^-24 each."""
+    page, cols, Hkv, Hq = 256, 1 << 22, 1, 4
+    c = pu.Cache([(n, 8 * page)], Hkv, D, page, bits, 3, spare=0, cols=8)
+    K, V = pu.normal((8 * page, Hkv, D), 1, 0.01), pu.normal((8 * page, Hkv, D), 2)
+    K[-1], K[-n - 1] = 0x3F80, 0x3F80  # ones: the last key of all, and one that every row sees
+    c.put(0, 0, K, V)
+    held = c.get(0, 0, 8 * page)
+    table = np.empty((1, cols), np.int32)
+    table[0] = c.table[0, np.arange(cols) % 7]
+    table[0, -1] = c.table[0, 7]
+    q = np.full((n, Hq, D), pu.bf16(np.float32(40.0 / D ** 0.5)), np.uint16)  # a score of 40 with a key of ones
+    base = c.device()
+    with ts.DeviceBuffer.from_array(table) as dt, ts.DeviceBuffer.from_array(np.array([1 << 30], np.int32)) as dl, \
+            ts.DeviceBuffer.from_array(q) as dq, ts.DeviceBuffer(q.nbytes) as do, \
+            ts.DeviceBuffer(ts.attn_flash_scratch_bytes(D, 128)) as ds:
+        do.fill_bytes(0xFF)
+        desc = ts.KvCache(c.bufs["k"], c.bufs["v"], dt, dl, base.q_start, 1, cols, 8, page, Hkv, D, bits,
+                          c.bufs["ks"] if bits == 4 else None, c.bufs["vs"] if bits == 4 else None)
+        ts.attn_paged(desc, ts.Rows(dq, Hq * D, D), ts.Rows(do, Hq * D, D), n, Hq, 1, None, n, 1 << 30, ds)
+        ts.synchronize()
+        O = pu.f32(do.download(np.uint16)).reshape(n, Hq, D)
+    times = np.array([(cols - 1) // 7 + (p < (cols - 1) % 7) for p in range(7)] + [1], np.float64)
+    count = np.repeat(times, page)
+    x = pu.f32(q[0, 0]).astype(np.float64)
+    s = D ** -0.5 * (held[0][:, 0] @ x)
+    for i in range(n):
+        w = count * np.exp(s - 40.0)
+        w[8 * page - (n - 1 - i):] = 0  # keys behind the row's position
+        w /= w.sum()
+        ref, A = w @ held[1][:, 0], w @ np.abs(held[1][:, 0])
+        assert w[-n - 1] > 0.4, w[-n - 1]
+        bound = 2.0 ** -8 * np.abs(ref) + A * 2.0 ** -8 * 1.01 + 2.0 ** -8 * A
+        assert np.all(np.abs(O[i] - ref) <= bound), (i, float(np.abs(O[i] - ref).max()))
