@@ -536,3 +536,26 @@ def test_the_longest_sequence(bits, D, n):
         assert w[-n - 1] > 0.4, w[-n - 1]
         bound = 2.0 ** -8 * np.abs(ref) + A * 2.0 ** -8 * 1.01 + 2.0 ** -8 * A
         assert np.all(np.abs(O[i] - ref) <= bound), (i, float(np.abs(O[i] - ref).max()))
+
+
+@pytest.mark.gpu
+def test_every_code_under_every_scale():
+    """A cache that another program wrote: 16 codes in both halves of a byte under all 256 scale bytes read as
+    code times 2^(e - 127) to the last bit, below bf16's normal numbers too, as infinities past its range and as NaN
+    under 255."""
+    D, page = 64, 256
+    c = pu.Cache([(page, page)], 1, D, page, 4, 1, spare=0)
+    low = np.arange(32) % 16
+    c.k[0, 0] = np.tile((low | (low[::-1] << 4)).astype(np.uint8), (page, 1))
+    c.v[0, 0] = np.tile((low[::-1] | (low << 4)).astype(np.uint8), (page, 1))
+    c.ks[0, 0] = np.stack([np.arange(256), np.arange(256)[::-1]], 1)
+    c.vs[0, 0] = c.ks[0, 0, ::-1]
+    with ts.DeviceBuffer(page * D * 2) as dk, ts.DeviceBuffer(page * D * 2) as dv:
+        ts.attn_kv_read(c.device(), ts.Rows(dk, D, D), ts.Rows(dv, D, D), page, page)
+        ts.synchronize()
+        got = [pu.f32(d.download(np.uint16)).astype(np.float64).reshape(page, D) for d in (dk, dv)]
+    for x, want in zip(got, c.get(0, 0, page)):
+        want = want[:, 0]
+        want = np.where(np.abs(want) >= 2.0 ** 128, np.copysign(np.inf, want), want)
+        assert np.isinf(want).any() and np.isnan(want).any() and (np.abs(want) < 2.0 ** -127).any()
+        assert np.array_equal(x, want, equal_nan=True)
