@@ -111,20 +111,31 @@ int attn_flash_plan(int Hq, int Hkv, int Sq, int Sk, int D, int causal, int bk, 
  *   bits 16: bf16 [pages][Hkv][page][D], D % 16 == 0, 16 <= D <= 256
  *   bits 4:  E2M1 codes [pages][Hkv][page][D/2] bytes, the even element in the low half, and one E8M0 scale
  *            byte e per 32 elements, [pages][Hkv][page][D/32]: an element is its code's value (0, 0.5, 1,
- *            1.5, 2, 3, 4, 6, the high bit negates) times 2^(e-127). D is 64, 128 or 256.
+ *            1.5, 2, 3, 4, 6, the high bit negates) times 2^(e-127) as a bf16 number, infinite past its range
+ *            (which takes an e of 253 or 254), or NaN where e is 255. D is 64, 128 or 256.
  * Sequence b holds kv_len[b] tokens, token p in page table[b * table_cols + p / page]. The tokens of a call
  * are rows of token tensors: sequence b's n_b = q_start[b+1] - q_start[b] of them are rows q_start[b] on,
  * and the last n_b of its kv_len[b] tokens (row i is position kv_len[b] - n_b + i). Rows of no sequence are
- * left as they are; kv_len counts a call's own tokens.
+ * left as they are; kv_len counts a call's own tokens. Limits: B * Hkv <= 2^20, T * Hq <= 2^30, and table rows
+ * for at most 2^38 tokens over all sequences and kv heads.
  *
  * table, kv_len and q_start lie in device memory and may hold anything: an entry of the table outside
  * [0, pages) names no page (its keys are hidden from attention, its tokens are not appended, read back as
- * zeros); a length is cut to what a row of the table holds, a start to [0, T] (starts fall nowhere).
+ * zeros); of a length past what a row of the table holds only so many keys are seen, and a start is cut to
+ * [0, T]. Starts are meant to rise: a sequence that ends before its start has no rows, and a row that two
+ * sequences claim may hold neither's answer.
  * Pages may be shared between sequences that read them; a page that a call appends to belongs to one
  * sequence, and no call of another stream reads it meanwhile.
  *
- * max_q and max_kv are the caller's bounds of n_b and kv_len[b]. They choose kernels and cut the work; a
- * sequence that passes them is served all the same, only slower. */
+ * max_q and max_kv are the caller's bounds of n_b and kv_len[b], and T of the rows. They choose kernels and cut
+ * the work; a sequence that passes max_q or max_kv is served all the same, only slower. Two costs of loose bounds:
+ *   - Every sequence is cut as if it had max_q rows. Single tokens beside a prompt go through the prompt's tiles in
+ *     attn_paged, and attn_kv_append launches B * max_q workgroups, attn_kv_read a quarter. Such a step is faster as
+ *     two calls on parts of the same arrays, the single tokens' rows first: theirs with T ending at their last row, the
+ *     prompts' with table + b * table_cols, kv_len + b and q_start + b.
+ *   - The scratch holds 65536 partial rows, so a sequence's keys are split into 65536 / (T * Hq) parts at most, and
+ *     not at all with T * Hq above 32768: T far above the rows in use leaves one long sequence to few workgroups.
+ */
 #define ATTN_KV_BF16 16
 #define ATTN_KV_FP4 4
 #define ATTN_KV_PAGE_MIN 16 /* a page is a power of two of tokens */
@@ -154,9 +165,10 @@ struct attn_scores {
 };
 
 /* Writes a call's K and V rows into the cache, K with its position's rotation, and the rotated Q to q_out
- * (q_out may be q, with its strides; q and q_out may both be NULL). The first `rot` elements of a head turn
- * (0: none), in pairs (i, i + rot/2), or with `pairs` (2i, 2i + 1): (x1, x2) -> (x1 c - x2 s, x2 c + x1 s)
- * in fp32, rounded once to bf16, with c and s from row p of rope [rope_rows][rot], cosines in its first half,
+ * (q_out may be q, with its strides, and else overlaps none of the rows; q and q_out may both be NULL). The
+ * first `rot` elements of a head turn (a multiple of 16; 0: none), in pairs (i, i + rot/2), or with `pairs`
+ * (2i, 2i + 1): (x1, x2) -> (x1 c - x2 s, x2 c + x1 s) in fp32, rounded once to bf16, with c and s from row p of
+ * rope [rope_rows][rot], cosines in its first half,
  * for position p. In 4 bits the rounded rows are quantised: a group's scale is the smallest power of two in
  * [2^-126, 2^125] under which its largest element is at most 7, elements round to nearest, ties to even; a
  * group with a NaN or an infinity reads as NaN. Tokens whose position is below 0 or has no row in rope are
@@ -173,8 +185,9 @@ void attn_kv_read(const struct attn_kv_cache *c, const struct attn_rows *k, cons
 /* Attention of a call's rows over their sequences' caches, o in bf16: row i of sequence b sees keys
  * j < kv_len[b], and with causal j <= its position; kv = h / (Hq/Hkv). A row that sees none is written as
  * zeros. P is rounded to bf16 before P.V, as in attn_flash, and as there a NaN or an infinity in V reaches
- * the rows of its key tile that do not see it. Scores past 2^30, whose rounding to fp32 is coarser than
- * exp can take, give rows without a meaning. o must not be q or overlap it. scores may be NULL (1/sqrt(D)).
+ * the rows of its key tile that do not see it. P.V is summed before the division by the row's sum: elements of
+ * V past 2^86 may overflow on the way. Scores past 2^30, whose rounding to fp32 is coarser than exp can take, give
+ * rows without a meaning. o must not be q or overlap it. scores may be NULL (1/sqrt(D)).
  * scratch is an attn_flash scratch of this D (attn_flash_scratch_bytes); calls that may overlap need one
  * each. */
 void attn_paged(const struct attn_kv_cache *c, const struct attn_rows *q, const struct attn_rows *o, int T,

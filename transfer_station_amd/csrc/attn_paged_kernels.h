@@ -216,8 +216,12 @@ __device__ __forceinline__ float part_max(float m, float l) {
 //
 // Bound by HBM: 64 sequences of 4096 keys, 8 kv heads, D = 128: bf16 163 us (6.6 TB/s), 4 bits 52.6 (5.4 TB/s, where
 // the unpacking takes 11 instructions per MFMA); of 250 to 8192 keys 162 us for 1.02 GB. Equal quotas are why: with
-// a workgroup per part of a sequence the same ragged batch took 198. One sequence of 32768, D = 256, 4 bits, is
-// 14.4 us of latency: start, four units, the join.
+// a workgroup per part of a sequence the same ragged batch took 198. They hold as long as the partial slots, one per
+// row of T and part, allow as many parts: 512 sequences of 64 heads have two each, so that no quota is below the
+// longest sequence, and with one of 32768 keys among 1000s they take 1004 us, 344 without it. One sequence of
+// 32768, D = 256, 4 bits, is 14.4 us of latency: start, four units, the join.
+// Past D = 128 a row tile is 16 rows and reads all keys for itself: 16 x 8 tokens over 2000 to 4000 keys, 32 heads on 8,
+// at D = 256 bf16 114 us, 4 bits 47; at D = 128, where it is 32 rows, 46 and 28.
 // ------------------------------------------------------------------------------------------
 template <int DP, bool F4, int NRB, bool MOD, bool NTL>
 __global__ __launch_bounds__(256, 2) void attn_paged_decode_kernel(const attn_paged_args a) {
@@ -624,8 +628,8 @@ __global__ __launch_bounds__(256, 2) void attn_paged_decode_kernel(const attn_pa
 // parts, NL loads of each thread on their way before the weights are known. The attention kernel says what
 // a row has: +inf as the first m where it wrote the row itself, -inf behind the last part (whose acc is
 // whatever it was: it gets no weight and is not multiplied). What bounds it is latency: the maxima, sums
-// and columns of a row are all asked for at once, right behind the sequence's start. 2.8 us where nothing or
-// little was cut, 4.4 for 16 rows of 65 parts at D = 256, 6.4 for 16384 rows of two parts.
+// and columns of a row are all asked for at once, right behind the sequence's start. 2.8-4.7 us where nothing
+// or little was cut, 4.3-5.1 for 16 rows of 65 parts at D = 256, 6.4-6.8 for 16384 rows of two parts.
 constexpr int kPagedMaxSplit = ATTN_PAGED_MAX_PARTS;
 template <int NL>
 __global__ __launch_bounds__(256) void attn_paged_merge_kernel(const attn_paged_args a, int lglp, int lgsg,
@@ -754,10 +758,14 @@ __global__ __launch_bounds__(256) void attn_paged_merge_kernel(const attn_paged_
 // The running maximum is raised only where a lane's sum of p over a tile passes kPagedSum, so that O is rarely
 // rescaled and most tiles look for no maximum.
 //
-// Bound by its instruction mix: per tile MFMA, exp and LDS reads on two waves per SIMD (5.2 VALU and MFMA
-// instructions per MFMA at D = 128, 6.5 with the unpacking). 32 heads on 8 kv heads, 2 x 4096 without a mask: D =
-// 128 525 us (1047 TFLOP/s) in bf16 and 530 in 4 bits, D = 64 324; 2 x 2048 causal at D = 256 147 and 164; 512
-// tokens over 8192 keys 74 and the merge. LDS-DMA instead of registers in bf16: 614 -> 526 at D = 128.
+// No unit is full; two waves per SIMD (three in 4 bits at D = 64) do not cover each other's waits. At D = 128 the matrix
+// unit is at work in half of the SIMDs' cycles and the VALU issues in 39% (5.2 VALU and MFMA instructions per MFMA, 6.5
+// with the unpacking), at D = 64 in 39 and 56%; a wave waits 28 to 33% of its time for data, barriers and LDS,
+// and as long for its turn to issue. 32 heads on 8 kv heads, 2 x 4096 without a mask: D = 128 535 us (1028 TFLOP/s) in
+// bf16 and 536 in 4 bits, 656 with a cap of 30, 621 with the distance; D = 64 316 and 301. 2 x 2048 causal: D = 32, 64,
+// 80, 96, 128, 192 and 256 51, 57, 76, 78, 85, 138 and 151 (head dims between 64, 128 and 256 run at the next one's
+// cost), 164 in 4 bits at 256. 512 tokens over 8192 keys 75 and the merge. LDS-DMA instead of registers in bf16: 614
+// -> 526 at D = 128.
 // ------------------------------------------------------------------------------------------
 // Bound on a lane's sum of p over a tile against a maximum that may lie below the tile's: p costs no precision
 // up to it, only exponent range.
@@ -1151,10 +1159,12 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void attn_paged_prefill_kernel(con
 // Append. A workgroup takes one token at a time, its four waves two halves of q's heads, k and v. A lane holds
 // the two eights of a head that rotate with each other ((x1, x2) -> (x1 c - x2 s, x2 c + x1 s), in fp32,
 // products and sums rounded apart, the result once to bf16), the wave's lanes lie across several heads, and
-// four of a lane's heads are in flight, so that the cosines and sines are read once per wave. K and V of the
+// two of a lane's heads are in flight, so that the cosines and sines are read once per wave. K and V of the
 // 4-bit cache go eight elements to a lane, four lanes to a group. HBM-bound: each element is read and
 // written once, past the L2, whose copies the attention on other XCDs could not use. 12700 tokens of 32 + 2 x 8
-// heads, D = 128, bf16: 56 us, 5.6 TB/s read and written, the rate of a copy (a wave per token 62.7); one token 2.5 us.
+// heads, D = 128, bf16: 56 us, 5.6 TB/s read and written, the rate of a copy (a wave per token 62.7); one token 2.4 us.
+// The grid is max_q workgroups per sequence, which end at once where a sequence has fewer tokens: 512 single tokens take
+// 4.3 us, with a prompt of 512 tokens among them 134.
 // ------------------------------------------------------------------------------------------
 __device__ __forceinline__ float lo_bf16(uint32_t x) { return __builtin_bit_cast(float, x << 16); }
 __device__ __forceinline__ float hi_bf16(uint32_t x) {
@@ -1327,7 +1337,7 @@ __global__ __launch_bounds__(256) void attn_kv_append_kernel(const attn_kv_args 
 
 // Read back: a wave per token, eight elements of a head per lane, four heads of a lane in flight. A token
 // without a place in the cache gives zeros. HBM-bound by what it writes, which goes past the L2: 32768 tokens
-// of 8 heads from 4 bits 38.3 us through it, 28.4 past it.
+// of 8 heads from 4 bits 38.3 us through it, 28.4 past it; from bf16 48 (5.6 TB/s read and written).
 template <bool F4>
 __global__ __launch_bounds__(256) void attn_kv_read_kernel(const attn_kv_args a) {
     const int b = uniform(wg_id_x() / a.tblk), tb = wg_id_x() - b * a.tblk;
