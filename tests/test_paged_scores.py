@@ -94,6 +94,64 @@ def test_scores_on_both_sides_of_a_large_cap(bits, n, cap, sigma):
     check(pu.attend(c, q, 2, 1, 0.0, cap), ref, bound, (bits, n, cap))
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("cap", [30.0, 1e4])
+@pytest.mark.parametrize("bits,n,kv", [(16, 1, 100), (4, 1, 3000), (16, 8, 900), (4, 20, 700), (16, 100, 600), (4, 40, 96)])
+def test_nan_and_infinities_under_a_cap(bits, n, kv, cap):
+    """An infinity in a row of q gives scores of the cap and its negative; a NaN there, or in a key, makes NaN of the
+    rows that meet it and of no other."""
+    Hq, Hkv, D = 4, 2, 128
+    c = pu.Cache([(n, kv), (n, kv // 2)], Hkv, D, 32, bits, 3)
+    c.fill(23)
+    for b, m in ((0, kv), (1, kv // 2)):  # the column that meets the infinity: half the keys on either side
+        K, V = ([pu.bf16(x.astype(np.float32)) for x in c.get(b, 0, m)])
+        K[:, :, 64:96] = pu.bf16(np.where(np.arange(m) % 2, 1.0, -1.0)[:, None, None] * np.ones((m, Hkv, 32), np.float32))
+        c.put(b, 0, K, V)
+    pg, at = c.places(0, kv - (n + 1) // 2, kv)
+    x, nan = (c.ks, 255) if bits == 4 else (c.k, 0xFF)
+    x[pg[0], 1, at[0]] = nan
+    q = pu.normal((c.N, Hq, D), 5)
+    q[c.N - 1, 0, 70], q[c.N - 1, 1, 70] = 0x7F80, 0xFF80  # inf and -inf, which meet kv head 0
+    q[0, 0, 5] = 0x7FC0  # NaN
+    with np.errstate(invalid="ignore"):
+        ref, bound = scores_ref(c, q, Hq, D ** -0.5, cap)
+    lost = np.isnan(ref).any(-1)
+    assert lost[0, 0] and lost.sum() == 1 + 2 * ((n + 1) // 2) and not lost[c.N - 1].any()
+    # the infinities' rows: every other key they see, alike, whatever the product's roundings
+    m = kv // 2
+    V = c.get(1, 0, m)[1][:, 0]
+    for h, keys in ((0, V[1::2]), (1, V[0::2])):
+        bound[c.N - 1, h] = (2.0 ** -8 * np.abs(keys.mean(0)) + np.abs(keys).mean(0) * (2.0 ** -8 * 1.01 + m * 2.0 ** -24 +
+                                                                                   2 * 2.0 ** -20 * min(cap, 256)))
+        ref[c.N - 1, h] = keys.mean(0)
+    O = pu.attend(c, q, Hq, 1, 0.0, cap, poison=0x3F)
+    assert np.array_equal(np.isnan(O).any(-1), lost) and np.array_equal(np.isnan(O).all(-1), lost)
+    check(np.where(lost[..., None], 0, O), np.where(lost[..., None], 0, ref), np.where(lost[..., None], 0, bound),
+          (bits, n, kv, cap))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits,n", [(16, 1), (4, 1), (16, 8), (16, 40), (4, 90)])
+@pytest.mark.parametrize("top", [16, 24, 29])
+def test_scores_up_to_two_to_the_thirtieth(bits, n, top):
+    """One key of a score of 2^top and others of three quarters of it and less: each row is that key's V to the
+    rounding of P and O, wherever the key lies and however the roundings of such scores fall."""
+    D, page, kv = 64, 32, 1500
+    K, V = np.zeros((kv, 1, D), np.float32), pu.normal((kv, 1, D), 2)
+    K[:, 0, 0] = np.array([0.5, 1, -1, 2, -3, 4, 1.5])[np.arange(kv) % 7]
+    K[0, 0, 1] = 6.0  # the scales of all groups alike in 4 bits
+    for at in (0, 31, 128, 700, kv - n - 1):
+        k = K.copy()
+        k[at, 0, 0] = 6.0
+        c = pu.Cache([(n, kv)], 1, D, page, bits, 3)
+        c.put(0, 0, pu.bf16(k), V)
+        q = np.zeros((n, 2, D), np.uint16)
+        q[:, :, 0] = pu.bf16(np.float32(2.0 ** top / 6.0 * D ** 0.5))
+        O = pu.attend(c, q, 2, 1)
+        v = c.get(0, at, at + 1)[1][0, 0]
+        check(O, np.broadcast_to(v, O.shape), np.broadcast_to(2 * 2.0 ** -8 * 1.01 * np.abs(v), O.shape), (bits, n, top, at))
+
+
 def test_the_bound_tells_a_cap_apart_that_loses_small_scores():
     """The bound of these tests against cap (1 - 2 / (2^x + 1)) taken in float32 throughout: it holds for a cap of 40,
     and not for 1e6."""
