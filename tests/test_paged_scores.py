@@ -152,6 +152,64 @@ def test_scores_up_to_two_to_the_thirtieth(bits, n, top):
         check(O, np.broadcast_to(v, O.shape), np.broadcast_to(2 * 2.0 ** -8 * 1.01 * np.abs(v), O.shape), (bits, n, top, at))
 
 
+def large_scores(bits, D, Hq, kv, levels, rows_q0, page=256, n=1):
+    """(cache, q, reference, bound): scores of about 2^20 that fp32 holds exactly. Column 0 gives every key the same
+    large score, a power of two times 1 to 2 by the row's q; column 32 adds twice the key's level (in 0, 0.5 .. 6, which
+    4 bits hold). D is 64 or 256, so that 1/sqrt(D) is a power of two and all products and sums are exact; what is left
+    are the roundings of P and O and of exp2: 2^-21 once per weight and once per rescale, and 2^-22 of the distance to
+    the row's largest score, for log2(e)'s."""
+    r = int(D ** 0.5)
+    K, V = np.zeros((kv, 1, D), np.float32), pu.normal((kv, 1, D), 2)
+    K[:, 0, 0], K[:, 0, 32] = 4.0, levels
+    c = pu.Cache([(n, kv)], 1, D, page, bits, 3)
+    c.put(0, 0, pu.bf16(K), V)
+    q = np.zeros((n, Hq, D), np.float32)
+    q[:, :, 0], q[:, :, 32] = 2.0 ** 20 / 4 * r * rows_q0, 2.0 * r
+    q = pu.bf16(q)
+    v = c.get(0, 0, kv)[1][:, 0]
+    t = 2.0 * levels.astype(np.float64)
+    w = np.exp(t - t.max())
+    w /= w.sum()
+    ref, A = w @ v, w @ np.abs(v)
+    delta = 2 * (2.0 ** -22 * (t.max() - t.min()) + 2.0 ** -21 * (4 + 2))
+    bound = 2.0 ** -8 * np.abs(ref) + A * (2.0 ** -8 * 1.01 + delta + 2.0 ** -12)
+    return c, q, np.broadcast_to(ref, q.shape), np.broadcast_to(bound, q.shape)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits,D,Hq,kv", [(16, 64, 8, 1600), (4, 64, 8, 1600), (16, 256, 8, 1600), (4, 256, 8, 1600),
+                                          (16, 64, 24, 1600), (16, 64, 64, 160000), (16, 64, 128, 160000),
+                                          (4, 64, 128, 160000), (16, 256, 128, 160000)])
+def test_keys_before_a_rise_keep_their_weight(bits, D, Hq, kv):
+    """A maximum that rises late, at scores of 2^20: the keys before, as many as outweigh the step, count as much as the
+    key that raises it, to the rounding of P. No parts (T is large), so that one workgroup sees all keys in turn."""
+    levels = np.zeros(kv)
+    j = np.arange(kv)
+    if kv == 1600:  # decode: a step of e^6 against 416 keys, all of the one wave whose maximum rises
+        levels[(j % 128 < 32) & (j < 1536)] = 3.0
+        levels[1536:1568] = 0.0
+        levels[1541] = 6.0
+    else:  # prefill: a step of e^12
+        levels[kv - 70] = 6.0
+    c, q, ref, bound = large_scores(bits, D, Hq, kv, levels, 1 + np.arange(Hq) % 64 / 64)
+    O = pu.attend(c, q, Hq, 0, pad=40000 // Hq)
+    check(O, ref, bound, (bits, D, Hq))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits,D,Hq", [(16, 64, 8), (4, 64, 8), (4, 256, 8), (16, 64, 24), (16, 64, 64), (4, 64, 64),
+                                       (16, 64, 128), (4, 64, 128), (16, 256, 128)])
+def test_parts_and_halves_keep_their_weight(bits, D, Hq):
+    """Parts, key halves and waves whose maxima differ a little, at scores of 2^20, joined by what they are."""
+    kv = 6000
+    levels = np.array([0, 0.5, 1, 1.5, 2])[np.random.default_rng(3).integers(0, 5, kv)]
+    step = np.repeat(np.random.default_rng(4).integers(0, 3, kv // 16), 16) * 0.5
+    levels = np.where(levels + step > 2, 2.0, levels + step)
+    levels[np.arange(kv) % 1024 < 300] = 0.0
+    c, q, ref, bound = large_scores(bits, D, Hq, kv, levels, 1 + np.arange(Hq) % 64 / 64)
+    check(pu.attend(c, q, Hq, 0), ref, bound, (bits, D, Hq))
+
+
 def test_the_bound_tells_a_cap_apart_that_loses_small_scores():
     """The bound of these tests against cap (1 - 2 / (2^x + 1)) taken in float32 throughout: it holds for a cap of 40,
     and not for 1e6."""

@@ -195,6 +195,15 @@ template <bool NT> __device__ __forceinline__ u32x4 buf16(__amdgpu_buffer_rsrc_t
     return __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, NT ? kDmaNT : 0);
 }
 
+// What a sum of p changes by when the maximum that p is taken against rises from m0 to m1: p is 2^(s c - m c) with m c
+// rounded, so the factor is between the rounded products. Taken from m0 - m1 it was off by their roundings, at
+// scores of 2^20 by up to 9%.
+__device__ __forceinline__ float rescale(float m0, float m1, float c) {
+#pragma clang fp contract(off)
+    const float a = m0 * c, b = m1 == kNegInf ? 0.f : m1 * c;
+    return fast_exp2(a - b);
+}
+
 // A part's maximum as the merge is told it. There +inf says that the row is written and -inf that the part has
 // nothing: an infinite score, and a part of NaN alone, go by finite ones, and their sums carry the NaN.
 __device__ __forceinline__ float part_max(float m, float l) {
@@ -463,7 +472,7 @@ __global__ __launch_bounds__(256, 2) void attn_paged_decode_kernel(const attn_pa
                     mx = max_xor32(max_xor16(mx));
                     if (__builtin_amdgcn_ballot_w64(mx > m_run[i] + lift) != 0) {
                         const float mnew = fmaxf(m_run[i], mx);
-                        const float alpha = fast_exp2((m_run[i] - (mnew == kNegInf ? 0.f : mnew)) * c);
+                        const float alpha = rescale(m_run[i], mnew, c);
                         m_run[i] = mnew;
                         l_run[i] *= alpha;
     #pragma unroll
@@ -1028,7 +1037,7 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void attn_paged_prefill_kernel(con
                     for (int i = 0; i < 16; i += 2)
                         mx = max3f(mx, s[t][i], s[t][i + 1]);
                 const float mnew = fmaxf(m_run, max_xor32(mx));
-                const float alpha = fast_exp2((m_run - (mnew == kNegInf ? 0.f : mnew)) * c);
+                const float alpha = rescale(m_run, mnew, c);
                 m_run = mnew;
                 l_run *= alpha;
 #pragma unroll
@@ -1085,12 +1094,13 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void attn_paged_prefill_kernel(con
         l_run = sum_xor32(l_run);
 
         bool writes = valid;
+        float m_log = m_run * c; // in log2 units; -inf stays
         if constexpr (KH > 1) {
             // Join the halves of the tiles: the second half's waves leave (m, l) and O in LDS.
             static_assert(KT * 4 >= 64 * NW, "O of the second half's waves fits two buffers");
             float *kho = reinterpret_cast<float *>(wr & 1 ? Vs0 : Ks0) + (wr >> 1) * DP * 32 + lane;
             if (kh == 1) {
-                kh_ml[wr * 64 + lane] = m_run * c;
+                kh_ml[wr * 64 + lane] = m_log;
                 kh_ml[NR * 64 + wr * 64 + lane] = l_run;
 #pragma unroll
                 for (int db = 0; db < DP / 32; ++db)
@@ -1101,10 +1111,10 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void attn_paged_prefill_kernel(con
             __syncthreads();
             if (kh == 0) {
                 const float m1 = kh_ml[wr * 64 + lane], l1 = kh_ml[NR * 64 + wr * 64 + lane];
-                const float mm = fmaxf(m_run * c, m1), mu = mm == kNegInf ? 0.f : mm;
-                const float w0 = fast_exp2(m_run * c - mu), w1 = fast_exp2(m1 - mu);
+                const float mm = fmaxf(m_log, m1);
+                const float w0 = rescale(m_log, mm, 1.f), w1 = rescale(m1, mm, 1.f);
                 l_run = w0 * l_run + w1 * l1;
-                m_run = mm / c;
+                m_log = mm;
 #pragma unroll
                 for (int db = 0; db < DP / 32; ++db)
 #pragma unroll
@@ -1134,7 +1144,7 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void attn_paged_prefill_kernel(con
                     }
             } else {
                 if (hi == 0) {
-                    a.pm[slot + sp] = part_max(m_run * c, l_run);
+                    a.pm[slot + sp] = part_max(m_log, l_run);
                     a.pl[slot + sp] = l_run;
                     if (sp == live - 1) // no parts behind the last
                         for (int s = live; s < a.nsplit; ++s)
