@@ -2,7 +2,8 @@
 back, and attention over the cache, in bf16 or in 4 bits. No counterpart in the reference.
 
 Device memory is given as DeviceBuffer or raw addresses, as everywhere in this package; KvCache, Rows and
-Scores are made once and kept for as long as their tensors live."""
+Scores are made once and kept for as long as their tensors live. T, max_q and max_kv are bounds, which choose kernels and
+cut the work; the header says what loose ones cost."""
 import ctypes
 
 from ._lib import lib
