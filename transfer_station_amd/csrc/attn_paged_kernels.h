@@ -58,7 +58,7 @@ __device__ __forceinline__ uint32_t bf16_pair(float a, float b) {
 //   does. Past it a |y| below a quarter takes cap y (1 - y^2 / 3 + 2 y^4 / 15 - ..), up to y^8 with the last term
 //   spread over the others by a Chebyshev polynomial (2^-26 in all): off by a few 2^-24 of the score, so that a
 //   cap far above the scores leaves them as they are. In w = 0.3287 y^2 the last coefficient is -1/2, an immediate.
-//   Seven instructions more, behind a uniform branch: 512 tokens over 8192 keys 102 us with a cap of 30, 130 with one of
+//   Nine instructions more, behind a uniform branch: 512 tokens over 8192 keys 102 us with a cap of 30, 130 with one of
 //   1000 (64 sequences of 4096 in bf16 164 with either, in 4 bits 57 and 63).
 //   The distance is exact up to 2^24 tokens, and its absolute value free.
 constexpr float kCapNear = 256.0f * 1.44269504088896341f; // log2(e) times a cap of 256
