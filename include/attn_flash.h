@@ -197,6 +197,58 @@ void attn_paged(const struct attn_kv_cache *c, const struct attn_rows *q, const 
 int attn_paged_plan(const struct attn_kv_cache *c, int T, int Hq, int causal,
                     const struct attn_scores *scores, int max_q, int max_kv, char *buf, size_t len);
 
+/* ---- Cross attention -----------------------------------------------------------------------------
+ * No counterpart in the reference. The attention of an encoder-decoder model, for training and serving: each
+ * sequence's rows (a prompt, a target text, a single token, the beams of one input) attend to all of its encoder's
+ * states, whose number is another. Batches are ragged: packed one sequence behind the other, or padded. Work is
+ * stream-ordered on the calling thread's stream, nothing is allocated and no device memory is read on the host, so
+ * that every call may be captured into a graph and replayed with other lengths.
+ */
+/* Rows of each sequence in a token tensor of T rows: from start[b] on, len[b] of them, or, with len NULL, up to
+ * start[b + 1]. start ([B], or [B + 1] with len NULL) and len ([B]) lie in device memory and may hold anything: a start
+ * is cut to [0, T], and a sequence to the rows behind it. max is the caller's bound of a sequence's rows. It chooses
+ * kernels and cuts the work; a sequence that passes it is served all the same, only slower. */
+struct attn_spans {
+    const int32_t *start, *len;
+    int32_t T, max;
+};
+
+/* D % 16 == 0, 16 <= D <= 256; scale 0: 1/sqrt(D). Limits: B * Hkv <= 2^20, q.T * Hq and k.T * Hkv <= 2^30. The token
+ * strides of all tensors of a call are in [D, ATTN_TOKEN_MAX] elements. */
+#define ATTN_TOKEN_MAX (1 << 22)
+struct attn_cross_call {
+    struct attn_spans q, k;
+    int32_t B, Hq, Hkv, D;
+    float scale;
+};
+
+/* O[t][h] = sum_j P_j V[j][kv], P = softmax_j(scale * Q[t][h].K[j][kv]) over the states j of row t's sequence,
+ * kv = h / (Hq/Hkv), in bf16; lse[t * Hq + h] = log sum_j exp(scale * Q.K), natural, in fp32 (lse may be NULL). A row
+ * whose sequence has no states gets zeros and -inf; rows of no sequence are left as they are. Sequences may share
+ * states (their spans may overlap), not rows. P is rounded to bf16 before P.V, as in attn_flash; states that no
+ * sequence names are not read, whatever they hold. o must not overlap q, k or v.
+ * scratch: attn_cross_scratch_bytes(c) bytes, ATTN_SCRATCH_ALIGN-aligned; calls that may overlap need one each. */
+size_t attn_cross_scratch_bytes(const struct attn_cross_call *c);
+void attn_cross(const struct attn_cross_call *c, const struct attn_rows *q, const struct attn_rows *k,
+                const struct attn_rows *v, const struct attn_rows *o, float *lse, void *scratch);
+
+/* The gradients of q, k and v, in bf16, from that of o (d_o) and what the forward call left in o and lse. dK and dV are
+ * summed over the heads of a group. P and dS are rounded to bf16 before their products. States of a sequence without
+ * rows get zeros; rows and states of no sequence are left as they are. Here sequences may share neither rows nor
+ * states: what two of them claim may hold neither's gradient. dq, dk and dv must overlap none of the other tensors.
+ * Sums have a fixed order: the same call gives the same bits.
+ * scratch: attn_cross_grad_scratch_bytes(c) bytes: 4 q.T Hq, and, where few sequences leave the GPU unfilled, up to 128
+ * MB of partial gradients. */
+size_t attn_cross_grad_scratch_bytes(const struct attn_cross_call *c);
+void attn_cross_grad(const struct attn_cross_call *c, const struct attn_rows *q, const struct attn_rows *k,
+                     const struct attn_rows *v, const struct attn_rows *o, const float *lse,
+                     const struct attn_rows *d_o, const struct attn_rows *dq, const struct attn_rows *dk,
+                     const struct attn_rows *dv, void *scratch);
+
+/* The kernels that attn_cross (or, with grad, attn_cross_grad) would launch, as attn_flash_plan gives them; nothing is
+ * launched or read. */
+int attn_cross_plan(const struct attn_cross_call *c, int grad, char *buf, size_t len);
+
 /* Stream selection for the calling thread (no counterpart in the reference, which has
  * no device). `stream` is a hipStream_t; NULL selects the null stream. */
 void attn_flash_set_stream(void *stream);

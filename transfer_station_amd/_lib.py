@@ -26,6 +26,11 @@ _SIGNATURES = {
                    [_c.c_void_p]),
     "attn_paged_plan": (_c.c_int, [_c.c_void_p] + [_c.c_int] * 3 + [_c.c_void_p] + [_c.c_int] * 2 +
                         [_c.c_char_p, _c.c_size_t]),
+    "attn_cross_scratch_bytes": (_c.c_size_t, [_c.c_void_p]),
+    "attn_cross": (None, [_c.c_void_p] * 7),
+    "attn_cross_grad_scratch_bytes": (_c.c_size_t, [_c.c_void_p]),
+    "attn_cross_grad": (None, [_c.c_void_p] * 11),
+    "attn_cross_plan": (_c.c_int, [_c.c_void_p, _c.c_int, _c.c_char_p, _c.c_size_t]),
     "attn_flash_set_stream": (None, [_c.c_void_p]),
     "attn_flash_get_stream": (_c.c_void_p, []),
     # include/attn_devutil.h

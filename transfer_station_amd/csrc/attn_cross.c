@@ -1,0 +1,257 @@
+/* attn_cross.c -- C host layer of cross attention: attn_cross, attn_cross_grad and their workspaces.
+ *
+ * Checks the arguments (a bad one aborts with a message, as in attn_flash), cuts the work and launches it on the
+ * calling thread's stream. Starts and lengths lie in device memory and are not read here: the kernels hold every use
+ * of them inside its tensor (attn_cross_rule.h).
+ */
+#define __HIP_PLATFORM_AMD__ 1
+#include "attn_flash.h"
+
+#include "attn_cross_rule.h"
+#include "attn_decode_rule.h"
+
+#include <hip/hip_runtime_api.h>
+#include <math.h>
+#include <stdio.h>
+#include <stdlib.h>
+#include <string.h>
+
+int attn_hip_launch_cross(const struct attn_cross_args *a, const struct attn_cross_cut *cut, int max_q, void *stream);
+int attn_hip_launch_cross_grad(const struct attn_cross_args *a, const struct attn_cross_cut *cut, int kv, int most,
+                               void *stream);
+void attn_hip_plan_begin(char *buf, size_t len);
+long attn_hip_plan_end(void);
+
+static void cross_fail(const char *who, const char *what) {
+    fprintf(stderr, "%s: %s\n", who, what);
+    abort();
+}
+
+static void cross_hip_check(int err, const char *who) {
+    if (err != 0) {
+        fprintf(stderr, "%s: HIP error %d (%s)\n", who, err, hipGetErrorString((hipError_t)err));
+        abort();
+    }
+}
+
+static int misaligned(const void *p, size_t to) { return !p || (uintptr_t)p % to != 0; }
+
+static int bound_of(const struct attn_spans *s) { return s->max < s->T ? s->max : s->T; }
+
+static void cross_check_spans(const char *who, const char *what, const struct attn_spans *s) {
+    if (misaligned(s->start, 4) || (s->len && misaligned(s->len, 4)) || s->T < 1 || s->T > 1 << 30 || s->max < 1) {
+        fprintf(stderr, "%s: %s needs device pointers to int32, T in [1, 2^30] and max >= 1\n", who, what);
+        abort();
+    }
+}
+
+static void cross_check_call(const char *who, const struct attn_cross_call *c) {
+    if (!c)
+        cross_fail(who, "the call must be non-NULL");
+    if (c->D < 16 || c->D > ATTN_D_MAX || c->D % 16 != 0)
+        cross_fail(who, "need D % 16 == 0 and D in [16, 256]");
+    if (c->B < 1 || c->Hkv < 1 || c->Hq < 1 || c->Hq % c->Hkv != 0)
+        cross_fail(who, "need B >= 1, Hkv >= 1, Hq >= 1 and Hq % Hkv == 0");
+    if ((int64_t)c->B * c->Hkv > 1 << 20)
+        cross_fail(who, "need B * Hkv <= 2^20");
+    cross_check_spans(who, "q", &c->q);
+    cross_check_spans(who, "k", &c->k);
+    if ((int64_t)c->q.T * c->Hq > 1 << 30 || (int64_t)c->k.T * c->Hkv > 1 << 30)
+        cross_fail(who, "need q.T * Hq <= 2^30 and k.T * Hkv <= 2^30");
+    if (!(c->scale == 0.f || (c->scale >= 1e-6f && c->scale <= 1e6f)))
+        cross_fail(who, "scale must be 0 (1/sqrt(D)) or in [1e-6, 1e6]");
+    if ((int64_t)c->B * c->Hkv * ((int64_t)bound_of(&c->q) * (c->Hq / c->Hkv) / 16 + 8) > 1 << 30 ||
+        (int64_t)c->B * c->Hkv * ((int64_t)bound_of(&c->k) / ATTN_CROSS_KEYS + 8) > 1 << 30)
+        cross_fail(who, "B, the heads and max ask for too many tiles");
+}
+
+static void cross_check_rows(const char *who, const char *what, const struct attn_rows *r, int D) {
+    if (!r || misaligned(r->data, 16) || r->head < 0 || r->token % 8 != 0 || r->head % 8 != 0 || r->token < D ||
+        r->token > ATTN_TOKEN_MAX) {
+        fprintf(stderr,
+                "%s: %s needs a 16-byte aligned device pointer, strides that are multiples of 8 and a token stride in "
+                "[D, 2^22]\n",
+                who, what);
+        abort();
+    }
+}
+
+static int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+/* Pieces per group so that the number of pieces is a multiple of 8 (attn_place_of). */
+static int deal_of(int64_t groups, int tps) {
+    int d = 8;
+    while (d > 1 && (groups * (d / 2)) % 8 == 0)
+        d /= 2;
+    return d < tps ? d : tps;
+}
+
+/* Parts so that `base` workgroups become `target`, each of `least` units or more of `total`. */
+static struct attn_cross_cut cross_cut(int64_t groups, int tps, int64_t total, int64_t least, int64_t target,
+                                       int64_t most, int step) {
+    struct attn_cross_cut cut;
+    memset(&cut, 0, sizeof cut);
+    const int64_t base = groups * tps;
+    int64_t n = ceil_div(target, base), by_len = total / least;
+    n = n < by_len ? n : by_len;
+    n = n < most ? n : most;
+    n = n < ATTN_CROSS_MAX_PARTS ? n : ATTN_CROSS_MAX_PARTS;
+    n = n < 2 ? 1 : n;
+    cut.share = (int)(ceil_div(ceil_div(total, n), step) * step);
+    cut.nsplit = (int)n;
+    cut.tps = tps;
+    cut.deal = deal_of(groups * n, tps);
+    cut.grid = (long)attn_place_grid(groups * n, tps, cut.deal);
+    return cut;
+}
+
+static struct attn_cross_cut forward_cut(const struct attn_cross_call *c) {
+    const int64_t R = (int64_t)bound_of(&c->q) * (c->Hq / c->Hkv), groups = (int64_t)c->B * c->Hkv;
+    const int64_t slots = ATTN_SLOTS / ((int64_t)c->q.T * c->Hq);
+    const int rows16 = R <= 16 ? 1 : R <= 32 ? (c->D <= 128 ? 2 : 1) : 0;
+    const int rows = rows16 ? 16 * rows16 : ATTN_CROSS_ROWS;
+    struct attn_cross_cut cut =
+        cross_cut(groups, (int)ceil_div(R, rows), bound_of(&c->k), rows16 ? 128 : 256, rows16 ? 2048 : 512, slots,
+                  ATTN_CROSS_KEY_STEP);
+    cut.rows16 = rows16;
+    return cut;
+}
+
+static struct attn_cross_cut dq_cut(const struct attn_cross_call *c) {
+    const int64_t R = (int64_t)bound_of(&c->q) * (c->Hq / c->Hkv), groups = (int64_t)c->B * c->Hkv;
+    return cross_cut(groups, (int)ceil_div(R, ATTN_CROSS_ROWS), bound_of(&c->k), 256, c->D <= 128 ? 512 : 256,
+                     ATTN_CROSS_GRAD_FLOATS / ((int64_t)c->q.T * c->Hq * c->D), ATTN_CROSS_KEY_STEP);
+}
+
+static struct attn_cross_cut dkv_cut(const struct attn_cross_call *c) {
+    const int64_t steps = ceil_div(bound_of(&c->q), attn_cross_step_rows(c->D)) * (c->Hq / c->Hkv);
+    return cross_cut((int64_t)c->B * c->Hkv, (int)ceil_div(bound_of(&c->k), ATTN_CROSS_KEYS), steps, 2,
+                     c->D <= 128 ? 512 : 256, ATTN_CROSS_GRAD_FLOATS / ((int64_t)c->k.T * c->Hkv * c->D * 2), 1);
+}
+
+size_t attn_cross_scratch_bytes(const struct attn_cross_call *c) {
+    cross_check_call("attn_cross_scratch_bytes", c);
+    return attn_flash_scratch_bytes(c->D, ATTN_BK_DEFAULT);
+}
+
+static size_t delta_bytes(const struct attn_cross_call *c) {
+    return ((size_t)c->q.T * c->Hq * sizeof(float) + 255) / 256 * 256;
+}
+
+size_t attn_cross_grad_scratch_bytes(const struct attn_cross_call *c) {
+    cross_check_call("attn_cross_grad_scratch_bytes", c);
+    const struct attn_cross_cut dq = dq_cut(c), dkv = dkv_cut(c);
+    const size_t q = dq.nsplit > 1 ? (size_t)dq.nsplit * c->q.T * c->Hq * c->D : 0;
+    const size_t kv = dkv.nsplit > 1 ? (size_t)dkv.nsplit * c->k.T * c->Hkv * c->D * 2 : 0;
+    return delta_bytes(c) + (q > kv ? q : kv) * sizeof(float);
+}
+
+static struct attn_cross_args cross_args(const struct attn_cross_call *c) {
+    struct attn_cross_args a;
+    memset(&a, 0, sizeof a);
+    a.scale = c->scale != 0.f ? c->scale : (float)(1.0 / sqrt((double)c->D));
+    a.c = (float)((c->scale != 0.f ? (double)c->scale : 1.0 / sqrt((double)c->D)) * 1.4426950408889634);
+    a.q_start = c->q.start, a.k_start = c->k.start;
+    a.q_is_len = c->q.len != NULL, a.k_is_len = c->k.len != NULL;
+    a.q_second = c->q.len ? c->q.len : c->q.start + 1;
+    a.k_second = c->k.len ? c->k.len : c->k.start + 1;
+    a.B = c->B, a.Tq = c->q.T, a.Tk = c->k.T, a.Hq = c->Hq, a.Hkv = c->Hkv, a.D = c->D;
+    return a;
+}
+
+static void set_cut(struct attn_cross_args *a, const struct attn_cross_cut *cut) {
+    a->tps = cut->tps, a->nsplit = cut->nsplit, a->share = cut->share, a->deal = cut->deal;
+}
+
+static void cross_run(const char *who, const struct attn_cross_call *c, const struct attn_rows *q,
+                      const struct attn_rows *k, const struct attn_rows *v, const struct attn_rows *o, float *lse,
+                      void *scratch) {
+    struct attn_cross_args a = cross_args(c);
+    const struct attn_cross_cut cut = forward_cut(c);
+    set_cut(&a, &cut);
+    a.q = (const uint16_t *)q->data, a.q_tok = q->token, a.q_head = q->head;
+    a.k = (const uint16_t *)k->data, a.k_tok = k->token, a.k_head = k->head;
+    a.v = (const uint16_t *)v->data, a.v_tok = v->token, a.v_head = v->head;
+    a.o = (uint16_t *)o->data, a.o_tok = o->token, a.o_head = o->head;
+    a.lse = lse;
+    /* the scratch of attn_flash: m, l and acc[D] of ATTN_SLOTS partials, each on 256 bytes */
+    a.pm = (float *)scratch;
+    a.pl = a.pm + ATTN_SLOTS;
+    a.pacc = a.pl + ATTN_SLOTS;
+    cross_hip_check(attn_hip_launch_cross(&a, &cut, bound_of(&c->q), attn_flash_get_stream()), who);
+}
+
+void attn_cross(const struct attn_cross_call *c, const struct attn_rows *q, const struct attn_rows *k,
+                const struct attn_rows *v, const struct attn_rows *o, float *lse, void *scratch) {
+    static const char *who = "attn_cross";
+    cross_check_call(who, c);
+    cross_check_rows(who, "q", q, c->D);
+    cross_check_rows(who, "k", k, c->D);
+    cross_check_rows(who, "v", v, c->D);
+    cross_check_rows(who, "o", o, c->D);
+    if (o->data == q->data || o->data == k->data || o->data == v->data)
+        cross_fail(who, "o must not be q, k or v");
+    if (lse && misaligned(lse, 4))
+        cross_fail(who, "lse must be NULL or a device pointer to floats");
+    if (misaligned(scratch, ATTN_SCRATCH_ALIGN))
+        cross_fail(who, "scratch must be non-NULL and ATTN_SCRATCH_ALIGN-aligned");
+    cross_run(who, c, q, k, v, o, lse, scratch);
+}
+
+static void grad_run(const char *who, const struct attn_cross_call *c, const struct attn_rows *const *in,
+                     const float *lse, const struct attn_rows *const *out, void *scratch) {
+    struct attn_cross_args a = cross_args(c);
+    a.q = (const uint16_t *)in[0]->data, a.q_tok = in[0]->token, a.q_head = in[0]->head;
+    a.k = (const uint16_t *)in[1]->data, a.k_tok = in[1]->token, a.k_head = in[1]->head;
+    a.v = (const uint16_t *)in[2]->data, a.v_tok = in[2]->token, a.v_head = in[2]->head;
+    a.o = (uint16_t *)in[3]->data, a.o_tok = in[3]->token, a.o_head = in[3]->head; /* read */
+    a.go = (const uint16_t *)in[4]->data, a.go_tok = in[4]->token, a.go_head = in[4]->head;
+    a.dq = (uint16_t *)out[0]->data, a.dq_tok = out[0]->token, a.dq_head = out[0]->head;
+    a.dk = (uint16_t *)out[1]->data, a.dk_tok = out[1]->token, a.dk_head = out[1]->head;
+    a.dv = (uint16_t *)out[2]->data, a.dv_tok = out[2]->token, a.dv_head = out[2]->head;
+    a.lse = (float *)(uintptr_t)lse; /* read */
+    a.delta = (float *)scratch;
+    a.pacc = (float *)((char *)scratch + delta_bytes(c));
+    const struct attn_cross_cut dq = dq_cut(c), dkv = dkv_cut(c);
+    set_cut(&a, &dq);
+    cross_hip_check(attn_hip_launch_cross_grad(&a, &dq, 0, bound_of(&c->q), attn_flash_get_stream()), who);
+    set_cut(&a, &dkv);
+    cross_hip_check(attn_hip_launch_cross_grad(&a, &dkv, 1, bound_of(&c->k), attn_flash_get_stream()), who);
+}
+
+void attn_cross_grad(const struct attn_cross_call *c, const struct attn_rows *q, const struct attn_rows *k,
+                     const struct attn_rows *v, const struct attn_rows *o, const float *lse,
+                     const struct attn_rows *d_o, const struct attn_rows *dq, const struct attn_rows *dk,
+                     const struct attn_rows *dv, void *scratch) {
+    static const char *who = "attn_cross_grad";
+    static const char *const names[] = {"q", "k", "v", "o", "d_o", "dq", "dk", "dv"};
+    const struct attn_rows *const all[] = {q, k, v, o, d_o, dq, dk, dv};
+    cross_check_call(who, c);
+    for (int i = 0; i < 8; ++i)
+        cross_check_rows(who, names[i], all[i], c->D);
+    for (int i = 5; i < 8; ++i)
+        for (int j = 0; j < i; ++j)
+            if (all[i]->data == all[j]->data)
+                cross_fail(who, "dq, dk and dv must be none of the other tensors");
+    if (misaligned(lse, 4))
+        cross_fail(who, "lse must be a device pointer to floats");
+    if (misaligned(scratch, ATTN_SCRATCH_ALIGN))
+        cross_fail(who, "scratch must be non-NULL and ATTN_SCRATCH_ALIGN-aligned");
+    grad_run(who, c, all, lse, all + 5, scratch);
+}
+
+int attn_cross_plan(const struct attn_cross_call *c, int grad, char *buf, size_t len) {
+    static const char *who = "attn_cross_plan";
+    const struct attn_rows r = {(void *)(uintptr_t)256, 256, 256};
+    const struct attn_rows *const all[] = {&r, &r, &r, &r, &r, &r, &r, &r};
+    cross_check_call(who, c);
+    if (!buf || len == 0)
+        cross_fail(who, "buf must be non-NULL and len above 0");
+    attn_hip_plan_begin(buf, len);
+    if (grad)
+        grad_run(who, c, all, (const float *)r.data, all, r.data);
+    else
+        cross_run(who, c, &r, &r, &r, &r, NULL, r.data);
+    const long n = attn_hip_plan_end();
+    return n < 0 || n > 0x7fffffffL ? -1 : (int)n;
+}

@@ -1,0 +1,1010 @@
+// attn_cross_kernels.h -- gfx950 kernels of cross attention over ragged batches: forward with the log-sum-exp of
+// each row (attn_cross) and the gradients (attn_cross_grad). Part of attn_kernels.hip.
+//
+//   S = scale Q.K, lse = log sum exp S, P = exp(S - lse), O = P.V
+//   delta = sum_d dO O, dS = P (dO.V - delta), dQ = scale dS.K, dK = scale dS^T.Q, dV = P^T.dO
+//
+// in fp32 but for the operands of the MFMAs: Q, K, V and dO as they are, P and dS rounded to bf16 (half a unit of
+// 2^-8, as much as the outputs' own rounding); outputs are rounded once. Nothing is accumulated by atomics: each
+// output has one workgroup, or parts that are added in order, so that a call gives the same bits every time.
+//
+// Tiles lie in LDS in one layout that serves both ways of reading them without bank conflicts: rows in groups of
+// four, a group's rows in blocks of 64 bytes, and in a block the four 16-byte chunks in an order that the group picks
+// (chunk ^ group mod 4).
+//   * As a row operand (16 bytes of a row per lane, 32 rows): sixteen neighbouring rows lie on different banks.
+//   * Transposed (ds_read_b64_tr_b16: 8 bytes per lane of four rows): a group's four rows are 256 bytes apart from none.
+#ifndef ATTN_CROSS_KERNELS_H
+#define ATTN_CROSS_KERNELS_H
+
+#include "attn_cross_rule.h"
+#include "attn_device.h"
+#include "attn_launch.h"
+
+namespace {
+
+__device__ __forceinline__ attn_range rows_of(const int32_t *start, const int32_t *second, int is_len, int b, int T) {
+    const attn_range r = attn_range_of(scalar_i32(start, b), scalar_i32(second, b), is_len, T);
+    return attn_range{uniform(r.at), uniform(r.n)};
+}
+__device__ __forceinline__ attn_range q_rows(const attn_cross_args &a, int b) {
+    return rows_of(a.q_start, a.q_second, a.q_is_len, b, a.Tq);
+}
+__device__ __forceinline__ attn_range k_rows(const attn_cross_args &a, int b) {
+    return rows_of(a.k_start, a.k_second, a.k_is_len, b, a.Tk);
+}
+
+__device__ __forceinline__ attn_cut part_of(int total, int share, int nsplit, int step) {
+    const attn_cut c = attn_cut_of(total, share, nsplit, step);
+    return attn_cut{uniform(c.live), uniform(c.per)};
+}
+
+constexpr float kLog2e = 1.44269504088896341f, kLn2 = 0.693147180559945309f;
+
+// The log-sum-exp of a row from its maximum in units of log2 and its sum: -inf where there is nothing.
+__device__ __forceinline__ float lse_of(float m, float l) { return (m + __builtin_amdgcn_logf(l)) * kLn2; }
+
+__device__ __forceinline__ f32x16 mfma32(bf16x8 x, bf16x8 y, f32x16 z) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, y, z, 0, 0, 0);
+}
+
+// ROWS rows of a token tensor into LDS by four waves' LDS-DMA: what each lane reads for its 16 bytes of each KB that
+// its wave writes. Columns past D, and rows past the last, lie outside the buffer and arrive as zeros.
+template <int DP, int ROWS> struct cross_stage {
+    static constexpr int PW = ROWS * DP / 2048;
+    static_assert(PW >= 1, "a wave writes whole KBs");
+    uint32_t off[PW];
+    __device__ __forceinline__ void init(int w, int lane, int64_t tok, int D) {
+#pragma unroll
+        for (int p = 0; p < PW; ++p) {
+            const int x = (w * PW + p) * 1024 + 16 * lane;
+            const int rg = x / (8 * DP), y = x % (8 * DP);
+            const int r = rg * 4 + (y % 256) / 64, c = y / 256 * 4 + ((y % 64 / 16) ^ (rg & 3));
+            off[p] = c * 8 < D ? (uint32_t)r * (uint32_t)(tok * 2) + c * 16 : 0x80000000u;
+        }
+    }
+    // rows: how many there are from `first` on, at least one.
+    __device__ __forceinline__ void load(const uint16_t *first, int rows, int64_t tok, int D, uint16_t *lds,
+                                         int w) const {
+        const auto r = make_rsrc(first, (uint32_t)(min(rows, ROWS) - 1) * (uint32_t)(tok * 2) + D * 2);
+#pragma unroll
+        for (int p = 0; p < PW; ++p)
+            dma16<0>(r, lds + (w * PW + p) * 512, off[p]);
+    }
+};
+
+// A lane's places in such tiles, in elements.
+template <int DP> struct cross_lane {
+    int nat0, nat1, tr0, tr1;
+    __device__ __forceinline__ explicit cross_lane(int lane) {
+        const int l32 = lane & 31, hi = lane >> 5, g1 = lane >> 4 & 1, i16 = lane & 15, x = l32 >> 2 & 3;
+        const int row = (l32 >> 2) * 4 * DP + (l32 & 3) * 32;
+        nat0 = row + (hi ^ x) * 8;
+        nat1 = row + (hi ^ x ^ 2) * 8;
+        const int c = 2 * g1 + (i16 >> 1 & 1);
+        const int tr = hi * 4 * DP + (i16 >> 2) * 32 + (i16 & 1) * 4;
+        tr0 = tr + (c ^ hi) * 8;
+        tr1 = tr + 8 * DP + (c ^ hi ^ 2) * 8;
+    }
+    // Row operand: lane l32 has row 32 t + l32, columns 16 kk + 8 hi .. + 7.
+    __device__ __forceinline__ bf16x8 nat(const uint16_t *tile, int t, int kk) const {
+        return as_bf16x8(
+            *reinterpret_cast<const u32x4 *>(tile + (kk & 1 ? nat1 : nat0) + t * 32 * DP + (kk >> 1) * 128));
+    }
+    // Transposed: lane l32 has column 32 db + l32 of rows 16 c + 4 hi .. + 3 and 16 c + 8 + 4 hi .. + 3, the rows whose
+    // scores registers 8 (c % 2) .. + 7 of a row operand's product hold.
+    __device__ __forceinline__ bf16x8 tr(const uint16_t *tile, int c, int db) const {
+        const uint16_t *x = tile + c * 16 * DP + db * 128;
+        return join_tr(lds_read_tr(x + tr0), lds_read_tr(x + tr1));
+    }
+};
+
+__device__ __forceinline__ void zero16(f32x16 &x) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+        x[i] = 0.f;
+}
+
+// A lane's row of an output tile O^T (register 4 j + i of block db: column 32 db + 8 j + 4 hi + i), times f, to bf16 or
+// as it is to fp32.
+template <int DP>
+__device__ __forceinline__ void put_row(const f32x16 *o, float f, uint16_t *dst, int hi, int D) {
+#pragma unroll
+    for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int d = db * 32 + 8 * j + 4 * hi;
+            if (d < D)
+                *reinterpret_cast<u32x2 *>(dst + d) = u32x2{bf16_pair(o[db][4 * j] * f, o[db][4 * j + 1] * f),
+                                                            bf16_pair(o[db][4 * j + 2] * f, o[db][4 * j + 3] * f)};
+        }
+}
+template <int DP> __device__ __forceinline__ void put_part(const f32x16 *o, float *dst, int hi, int D) {
+#pragma unroll
+    for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int d = db * 32 + 8 * j + 4 * hi;
+            if (d < D)
+                *reinterpret_cast<f32x4 *>(dst + d) =
+                    f32x4{o[db][4 * j], o[db][4 * j + 1], o[db][4 * j + 2], o[db][4 * j + 3]};
+        }
+}
+
+// Keys of a tile, by the tile's width: two tiles of K and V in two buffers are 64 KB.
+constexpr int cross_tile_keys(int DP) { return DP == 64 ? 128 : DP == 128 ? 64 : 32; }
+// A lane's sum of p over a tile up to which the running maximum may lie below the tile's.
+constexpr float kCrossSum = 65536.0f;
+
+// ------------------------------------------------------------------------------------------
+// Forward, many rows per kv head. One workgroup of four waves per (sequence, kv head, part of its states, tile of 128
+// rows): a sequence's rows are its tokens' heads of the group, token by token, 32 to a wave. Tiles of K and V go to LDS
+// by LDS-DMA, the next one's beside the products of this one:
+//   S^T[key][row] = K . Q^T, O^T[d][row] += V^T . P^T   (v_mfma_f32_32x32x16_bf16)
+// The running maximum is raised only where a lane's sum of p over a tile passes kCrossSum.
+// ------------------------------------------------------------------------------------------
+template <int DP> __global__ __launch_bounds__(256, 2) void attn_cross_kernel(const attn_cross_args a) {
+    constexpr int KT = cross_tile_keys(DP), KN = DP / 16, NT = KT / 32;
+    // Each buffer is a variable of its own: the compiler tells LDS accesses apart by variable.
+    __shared__ __attribute__((aligned(1024))) uint16_t Ks0[KT * DP], Ks1[KT * DP];
+    __shared__ __attribute__((aligned(1024))) uint16_t Vs0[KT * DP], Vs1[KT * DP];
+
+    const attn_place at = attn_place_of(wg_id_x(), a.B * a.Hkv * a.nsplit, a.tps, a.deal);
+    if (at.group < 0)
+        return;
+    const int sp = uniform(at.group / (a.B * a.Hkv)), bu = at.group - sp * (a.B * a.Hkv);
+    const int u = uniform(bu % a.Hkv), b = uniform(bu / a.Hkv);
+    const int tid = wi_id_x(), w = uniform(tid >> 6), lane = tid & 63, l32 = lane & 31, hi = lane >> 5;
+    const attn_range qr = q_rows(a, b), kr = k_rows(a, b);
+    const attn_cut cut = part_of(kr.n, a.share, a.nsplit, ATTN_CROSS_KEY_STEP);
+    if (sp >= cut.live)
+        return;
+    const int k0 = min(sp * cut.per, kr.n), k1 = min(k0 + cut.per, kr.n);
+    const int g = a.Hq / a.Hkv, R = qr.n * g, D = a.D;
+    const uint16_t *kp = a.k + kr.at * a.k_tok + u * a.k_head, *vp = a.v + kr.at * a.v_tok + u * a.v_head;
+    const cross_lane<DP> ln(lane);
+    cross_stage<DP, KT> ks, vs;
+    ks.init(w, lane, a.k_tok, D);
+    vs.init(w, lane, a.v_tok, D);
+    auto load = [&](int kb, uint16_t *Kd, uint16_t *Vd) __attribute__((always_inline)) {
+        ks.load(kp + kb * a.k_tok, k1 - kb, a.k_tok, D, Kd, w);
+        vs.load(vp + kb * a.v_tok, k1 - kb, a.v_tok, D, Vd, w);
+    };
+    auto wait_loads = [] { __builtin_amdgcn_s_waitcnt(waitcnt_vm(0)); };
+
+    for (int tile = uniform(at.tile); (int64_t)tile * ATTN_CROSS_ROWS < R; tile += a.tps) {
+        const int row = tile * ATTN_CROSS_ROWS + 32 * w + l32;
+        const bool valid = row < R;
+        const int tok = valid ? row / g : 0, h = u * g + (valid ? row % g : 0);
+        const uint16_t *q = a.q + (qr.at + tok) * a.q_tok + h * a.q_head;
+        const bool idle = tile * ATTN_CROSS_ROWS + 32 * w >= R; // the wave has no rows
+        bf16x8 qb[KN];
+#pragma unroll
+        for (int kk = 0; kk < KN; ++kk) {
+            const int col = kk * 16 + hi * 8;
+            u32x4 x = zero4();
+            if (valid && col < D)
+                x = *reinterpret_cast<const u32x4 *>(q + col);
+            qb[kk] = as_bf16x8(x);
+        }
+        float m_run = kNegInf, l_run = 0.f;
+        f32x16 o[DP / 32];
+#pragma unroll
+        for (int db = 0; db < DP / 32; ++db)
+            zero16(o[db]);
+
+        auto compute = [&](int kb, const uint16_t *Kb, const uint16_t *Vb) __attribute__((always_inline)) {
+            if (idle)
+                return;
+            f32x16 s[NT];
+            bf16x8 ka[2][KN];
+#pragma unroll
+            for (int kk = 0; kk < KN; ++kk)
+                ka[0][kk] = ln.nat(Kb, 0, kk);
+            __builtin_amdgcn_sched_group_barrier(0x100, KN, 0);
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                zero16(s[t]);
+#pragma unroll
+                for (int kk = 0; kk < KN; ++kk) {
+                    s[t] = mfma32(ka[t & 1][kk], qb[kk], s[t]);
+                    if (t + 1 < NT)
+                        ka[(t + 1) & 1][kk] = ln.nat(Kb, t + 1, kk);
+                }
+#pragma unroll
+                for (int kk = 0; kk < KN; ++kk) {
+                    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                    if (t + 1 < NT)
+                        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+                }
+            }
+            // Register i of sub-tile t: key kb + 32 t + 8 (i / 4) + 4 hi + i % 4.
+            if (kb + KT > k1)
+#pragma unroll
+                for (int t = 0; t < NT; ++t)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        if (kb + 32 * t + 8 * (i >> 2) + 4 * hi + (i & 3) >= k1)
+                            s[t][i] = kNegInf;
+            bf16x8 pk[2 * NT];
+            float psum;
+            auto weigh = [&]() __attribute__((always_inline)) {
+                const float mc = m_run == kNegInf ? 0.f : m_run * a.c;
+                psum = 0.f;
+#pragma unroll
+                for (int t = 0; t < NT; ++t)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const float p = fast_exp2(fmaf(s[t][i], a.c, -mc));
+                        psum += p;
+                        pk[2 * t + (i >> 3)][i & 7] = (__bf16)p;
+                    }
+            };
+            weigh();
+            if (__builtin_amdgcn_ballot_w64(!(psum <= kCrossSum) || m_run == kNegInf) != 0) {
+                float mx = kNegInf;
+#pragma unroll
+                for (int t = 0; t < NT; ++t)
+#pragma unroll
+                    for (int i = 0; i < 16; i += 2)
+                        mx = max3f(mx, s[t][i], s[t][i + 1]);
+                const float mnew = fmaxf(m_run, max_xor32(mx));
+                const float alpha = rescale(m_run, mnew, a.c);
+                m_run = mnew;
+                l_run *= alpha;
+#pragma unroll
+                for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        o[db][i] *= alpha;
+                weigh();
+            }
+            l_run += psum;
+#pragma unroll
+            for (int cc = 0; cc < 2 * NT; ++cc)
+#pragma unroll
+                for (int db = 0; db < DP / 32; ++db)
+                    o[db] = mfma32(ln.tr(Vb, cc, db), pk[cc], o[db]);
+        };
+        if (k0 < k1)
+            load(k0, Ks0, Vs0);
+        wait_loads(); // for Q too
+        __syncthreads();
+        auto step = [&](int kb, const uint16_t *Kb, const uint16_t *Vb, uint16_t *Kn, uint16_t *Vn)
+            __attribute__((always_inline)) {
+            if (kb + KT < k1)
+                load(kb + KT, Kn, Vn);
+            compute(kb, Kb, Vb);
+            wait_loads(); // this wave's part of the next tile has arrived
+            __syncthreads();
+        };
+        for (int kb = k0; kb < k1; kb += 2 * KT) {
+            step(kb, Ks0, Vs0, Ks1, Vs1);
+            if (kb + KT < k1)
+                step(kb + KT, Ks1, Vs1, Ks0, Vs0);
+        }
+        l_run = sum_xor32(l_run);
+        if (valid) {
+            const float m_log = m_run * a.c;
+            const int64_t slot = (int64_t)(qr.at + tok) * a.Hq + h;
+            if (cut.live == 1) {
+                put_row<DP>(o, l_run > 0.f ? 1.0f / l_run : 0.f, a.o + (qr.at + tok) * a.o_tok + h * a.o_head, hi, D);
+                if (a.lse && hi == 0)
+                    a.lse[slot] = lse_of(m_log, l_run);
+            } else {
+                if (hi == 0) {
+                    a.pm[slot * a.nsplit + sp] = m_log;
+                    a.pl[slot * a.nsplit + sp] = l_run;
+                }
+                put_part<DP>(o, a.pacc + (slot * a.nsplit + sp) * D, hi, D);
+            }
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------
+// Forward, few rows per kv head (single tokens, beams): a workgroup of four waves takes 16 NRB rows over a part of the
+// states, the waves interleaved tiles of 32 states, each with a softmax of its own:
+//   S^T[key][row] = K . Q^T   (v_mfma_f32_16x16x32_bf16, K from memory straight into the operand)
+//   O^T[d][row]  += V^T . P^T (V through a wave-private LDS tile and the transposed read)
+// and joins them in LDS. Bound by HBM. NTL: K and V are read once, past the L2.
+// ------------------------------------------------------------------------------------------
+template <int DP, int NRB, bool NTL>
+__global__ __launch_bounds__(256, 2) void attn_cross_rows_kernel(const attn_cross_args a) {
+    constexpr int VSTR = DP + 16; // elements of a V row in LDS: the eight rows of a pass on other banks
+    constexpr int KN = DP / 32, NV = DP / 16, VTILE = 32 * VSTR;
+    // K and V of a tile, Q and O do not fit 256 registers at DP = 256: there K is loaded at the tile's start, and V
+    // once the scores have freed K's registers.
+    constexpr bool kLate = DP == 256;
+    __shared__ __attribute__((aligned(16))) uint16_t Vw[4 * VTILE];
+    __shared__ float red_m[NRB][4][16], red_l[NRB][4][16];
+    static_assert(4 * 16 * (DP + 4) * 4 <= 4 * VTILE * 2, "the area for joining must fit in the V tiles");
+
+    const int tid = wi_id_x(), w = uniform(tid >> 6), lane = tid & 63;
+    const int r16 = lane & 15, grp = lane >> 4;
+    const attn_place at = attn_place_of(wg_id_x(), a.B * a.Hkv * a.nsplit, a.tps, a.deal);
+    if (at.group < 0)
+        return;
+    const int bu = uniform(at.group / a.nsplit), sp = at.group - bu * a.nsplit;
+    const int b = uniform(bu / a.Hkv), u = bu - b * a.Hkv;
+    const attn_range qr = q_rows(a, b), kr = k_rows(a, b);
+    const attn_cut cut = part_of(kr.n, a.share, a.nsplit, ATTN_CROSS_KEY_STEP);
+    if (sp >= cut.live)
+        return;
+    const int k0 = min(sp * cut.per, kr.n), k1 = min(k0 + cut.per, kr.n);
+    const int g = a.Hq / a.Hkv, R = qr.n * g, D = a.D;
+    const float c = a.c, lift = 8.f / c; // how far a score may pass the running maximum
+    const uint16_t *kp = a.k + kr.at * a.k_tok + u * a.k_head, *vp = a.v + kr.at * a.v_tok + u * a.v_head;
+    const uint32_t kb2 = (uint32_t)(a.k_tok * 2), vb2 = (uint32_t)(a.v_tok * 2); // bytes from row to row
+    uint16_t *vt = &Vw[w * VTILE];
+    const uint32_t koff = grp * 8 < D ? r16 * kb2 + grp * 16 : 0x80000000u;
+    const uint32_t voff = (lane % (DP / 8)) * 8 < D ? (lane / (DP / 8)) * vb2 + (lane % (DP / 8)) * 16 : 0x80000000u;
+
+    for (int tile = uniform(at.tile); (int64_t)tile * 16 * NRB < R; tile += a.tps) {
+        const int row0 = tile * 16 * NRB;
+        bf16x8 qb[NRB][KN];
+        float m_run[NRB], l_run[NRB];
+        f32x4 o[NRB][DP / 16];
+#pragma unroll
+        for (int i = 0; i < NRB; ++i) {
+            const int row = row0 + 16 * i + r16;
+            const bool valid = row < R;
+            const int tok = valid ? row / g : 0, h = u * g + (valid ? row % g : 0);
+            const uint16_t *q = a.q + (qr.at + tok) * a.q_tok + h * a.q_head;
+#pragma unroll
+            for (int kk = 0; kk < KN; ++kk) {
+                const int col = kk * 32 + grp * 8;
+                u32x4 x = zero4();
+                if (valid && col < D)
+                    x = *reinterpret_cast<const u32x4 *>(q + col);
+                qb[i][kk] = as_bf16x8(x);
+            }
+            m_run[i] = kNegInf;
+            l_run[i] = 0.f;
+#pragma unroll
+            for (int db = 0; db < DP / 16; ++db)
+                o[i][db] = f32x4{0.f, 0.f, 0.f, 0.f};
+        }
+        struct frags {
+            u32x4 k[2 * KN], v[NV];
+        };
+        // Rows past the part's end, or tiles behind it, lie outside the buffer: nothing is read, zeros arrive.
+        auto bytes = [&](int tb, uint32_t step) __attribute__((always_inline)) {
+            const int n = min(k1 - tb, 32);
+            return n > 0 ? (uint32_t)(n - 1) * step + D * 2 : 0u;
+        };
+        auto load_k = [&](int tb, frags &f) __attribute__((always_inline)) {
+            const auto r = make_rsrc(kp + (int64_t)min(tb, k1) * a.k_tok, bytes(tb, kb2));
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int kk = 0; kk < KN; ++kk)
+                    f.k[t * KN + kk] =
+                        buf16<NTL>(r, kk * 32 + grp * 8 < D ? koff + 16 * t * kb2 + kk * 64 : 0x80000000u);
+        };
+        auto load_v = [&](int tb, frags &f) __attribute__((always_inline)) {
+            const auto r = make_rsrc(vp + (int64_t)min(tb, k1) * a.v_tok, bytes(tb, vb2));
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+                f.v[i] = buf16<NTL>(r, voff + i * (512 / DP) * vb2);
+        };
+        auto put_v = [&](const frags &f) __attribute__((always_inline)) {
+            lds_wave_fence(); // the previous tile's transposed reads are complete
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const int x = lane + 64 * i;
+                *reinterpret_cast<u32x4 *>(&vt[x / (DP / 8) * VSTR + x % (DP / 8) * 8]) = f.v[i];
+            }
+        };
+        auto compute = [&](int tb, frags &f) __attribute__((always_inline)) {
+            bf16x8 pk[NRB];
+            f32x4 s[NRB][2];
+#pragma unroll
+            for (int i = 0; i < NRB; ++i)
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    s[i][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int kk = 0; kk < KN; ++kk)
+                        s[i][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(f.k[t * KN + kk]), qb[i][kk],
+                                                                          s[i][t], 0, 0, 0);
+                }
+            __builtin_amdgcn_sched_barrier(0);
+            if (kLate)
+                load_v(tb, f);
+            else
+                load_k(tb + 128, f);
+#pragma unroll
+            for (int i = 0; i < NRB; ++i) {
+                // Register (t, j) of this lane holds key tb + 16t + 4grp + j for row r16.
+                float mx = kNegInf;
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        if (tb + 16 * t + 4 * grp + j >= k1)
+                            s[i][t][j] = kNegInf;
+                        mx = fmaxf(mx, s[i][t][j]);
+                    }
+                mx = max_xor32(max_xor16(mx));
+                if (__builtin_amdgcn_ballot_w64(mx > m_run[i] + lift) != 0) {
+                    const float mnew = fmaxf(m_run[i], mx);
+                    const float alpha = rescale(m_run[i], mnew, c);
+                    m_run[i] = mnew;
+                    l_run[i] *= alpha;
+#pragma unroll
+                    for (int db = 0; db < DP / 16; ++db)
+                        o[i][db] *= alpha;
+                }
+                const float mc = m_run[i] == kNegInf ? 0.f : m_run[i] * c;
+                float psum = 0.f;
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const float p = fast_exp2(fmaf(s[i][t][j], c, -mc));
+                        psum += p;
+                        pk[i][4 * t + j] = (__bf16)p;
+                    }
+                l_run[i] += psum;
+            }
+            if (kLate)
+                put_v(f);
+            lds_wave_fence(); // this tile's V is in LDS before the transposed reads
+            const uint16_t *vrow = &vt[(4 * grp + (r16 >> 2)) * VSTR + 4 * (r16 & 3)];
+#pragma unroll
+            for (int db = 0; db < DP / 16; ++db) {
+                const bf16x8 x = join_tr(lds_read_tr(vrow + db * 16), lds_read_tr(vrow + db * 16 + 16 * VSTR));
+#pragma unroll
+                for (int i = 0; i < NRB; ++i)
+                    o[i][db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, pk[i], o[i][db], 0, 0, 0);
+            }
+        };
+        int tb = k0 + 32 * w;
+        if (tb < k1) {
+            frags f;
+            if (!kLate) {
+                load_v(tb, f);
+                load_k(tb, f);
+            }
+            for (; tb < k1; tb += 128) {
+                if (kLate) {
+                    load_k(tb, f);
+                } else {
+                    put_v(f);
+                    __builtin_amdgcn_sched_barrier(0);
+                    load_v(tb + 128, f);
+                }
+                compute(tb, f);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < NRB; ++i)
+            l_run[i] = sum_xor32(sum_xor16(l_run[i]));
+
+        // Join the waves: O^T register (db, j) of this lane holds d = 16db + 4grp + j of row r16.
+        float *om = reinterpret_cast<float *>(Vw); // [4][16][DP + 4]
+        if (grp == 0)
+#pragma unroll
+            for (int i = 0; i < NRB; ++i) {
+                red_m[i][w][r16] = m_run[i] * c; // in log2 units; -inf stays
+                red_l[i][w][r16] = l_run[i];
+            }
+#pragma unroll
+        for (int i = 0; i < NRB; ++i) {
+            __syncthreads();
+#pragma unroll
+            for (int db = 0; db < DP / 16; ++db)
+                *reinterpret_cast<f32x4 *>(&om[(w * 16 + r16) * (DP + 4) + db * 16 + 4 * grp]) = o[i][db];
+            __syncthreads();
+            const int rowb = row0 + 16 * i, nrow = min(16, R - rowb);
+            for (int idx = tid; idx < nrow * (DP / 4); idx += 256) {
+                const int r = idx / (DP / 4), d = 4 * (idx % (DP / 4));
+                if (d >= D)
+                    continue;
+                float mx = kNegInf;
+#pragma unroll
+                for (int ww = 0; ww < 4; ++ww)
+                    mx = fmaxf(mx, red_m[i][ww][r]);
+                const float muse = mx == kNegInf ? 0.f : mx;
+                f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+                float lsum = 0.f;
+#pragma unroll
+                for (int ww = 0; ww < 4; ++ww) {
+                    const float wgt = fast_exp2(red_m[i][ww][r] - muse);
+                    const f32x4 x = *reinterpret_cast<const f32x4 *>(&om[(ww * 16 + r) * (DP + 4) + d]);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        acc[j] += wgt * x[j];
+                    lsum += wgt * red_l[i][ww][r];
+                }
+                const int64_t tok = qr.at + (rowb + r) / g;
+                const int h = u * g + (rowb + r) % g;
+                const int64_t slot = tok * a.Hq + h;
+                if (cut.live == 1) {
+                    const float inv = lsum > 0.f ? 1.0f / lsum : 0.f;
+                    *reinterpret_cast<u32x2 *>(a.o + tok * a.o_tok + h * a.o_head + d) =
+                        u32x2{bf16_pair(acc[0] * inv, acc[1] * inv), bf16_pair(acc[2] * inv, acc[3] * inv)};
+                    if (a.lse && d == 0)
+                        a.lse[slot] = lse_of(mx, lsum);
+                } else {
+                    if (d == 0) {
+                        a.pm[slot * a.nsplit + sp] = mx;
+                        a.pl[slot * a.nsplit + sp] = lsum;
+                    }
+                    *reinterpret_cast<f32x4 *>(a.pacc + (slot * a.nsplit + sp) * D + d) = acc;
+                }
+            }
+        }
+        __syncthreads(); // the area for joining is V tiles again
+    }
+}
+
+// Joins the parts of each row: w_s = 2^(m_s - max m), O = sum w_s acc_s / sum w_s l_s, lse = log2-sum of both. A
+// workgroup takes 256 / LP rows of one sequence at a time, LP = 2^lglp lanes of four columns each.
+__global__ __launch_bounds__(256) void attn_cross_merge_kernel(const attn_cross_args a, int lglp, int tpm) {
+    const int b = uniform(wg_id_x() / tpm), t0 = wg_id_x() - b * tpm, tid = wi_id_x();
+    const attn_range qr = q_rows(a, b), kr = k_rows(a, b);
+    const attn_cut cut = part_of(kr.n, a.share, a.nsplit, ATTN_CROSS_KEY_STEP);
+    if (cut.live == 1)
+        return; // written already
+    const int64_t R = (int64_t)qr.n * a.Hq;
+    const int rpw = 256 >> lglp, d = 4 * (tid & ((1 << lglp) - 1));
+    for (int64_t row = (int64_t)t0 * rpw + (tid >> lglp); row < R; row += (int64_t)tpm * rpw) {
+        const int64_t slot = (int64_t)qr.at * a.Hq + row;
+        const float *pm = a.pm + slot * a.nsplit, *pl = a.pl + slot * a.nsplit;
+        const float *p = a.pacc + slot * a.nsplit * a.D + min(d, a.D - 4);
+        float mx = kNegInf;
+        for (int s = 0; s < cut.live; ++s)
+            mx = fmaxf(mx, pm[s]);
+        const float muse = mx == kNegInf ? 0.f : mx;
+        f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+        float sum = 0.f;
+#pragma unroll 4
+        for (int s = 0; s < cut.live; ++s) {
+            const float wgt = fast_exp2(pm[s] - muse);
+            const f32x4 x = *reinterpret_cast<const f32x4 *>(p + (int64_t)s * a.D);
+            sum += wgt * pl[s];
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                acc[j] += wgt * x[j];
+        }
+        if (d >= a.D)
+            continue;
+        const float inv = sum > 0.f ? 1.0f / sum : 0.f;
+        const int64_t tok = qr.at + row / a.Hq;
+        *reinterpret_cast<u32x2 *>(a.o + tok * a.o_tok + row % a.Hq * a.o_head + d) =
+            u32x2{bf16_pair(acc[0] * inv, acc[1] * inv), bf16_pair(acc[2] * inv, acc[3] * inv)};
+        if (a.lse && d == 0)
+            a.lse[slot] = lse_of(mx, sum);
+    }
+}
+
+// ------------------------------------------------------------------------------------------
+// dQ. Laid out as the forward kernel: 32 rows of a wave keep Q and dO in registers, tiles of K and V pass through LDS:
+//   S^T[key][row] = K . Q^T, dP^T[key][row] = V . dO^T, dQ^T[d][row] += K^T . dS^T
+// K's tile is read both ways. delta = sum dO O is taken on the way in and left for the kernel of dK and dV.
+// ------------------------------------------------------------------------------------------
+template <int DP>
+__global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_cross_dq_kernel(const attn_cross_args a) {
+    constexpr int KT = cross_tile_keys(DP), KN = DP / 16, NT = KT / 32;
+    __shared__ __attribute__((aligned(1024))) uint16_t Ks0[KT * DP], Ks1[KT * DP];
+    __shared__ __attribute__((aligned(1024))) uint16_t Vs0[KT * DP], Vs1[KT * DP];
+
+    const attn_place at = attn_place_of(wg_id_x(), a.B * a.Hkv * a.nsplit, a.tps, a.deal);
+    if (at.group < 0)
+        return;
+    const int sp = uniform(at.group / (a.B * a.Hkv)), bu = at.group - sp * (a.B * a.Hkv);
+    const int u = uniform(bu % a.Hkv), b = uniform(bu / a.Hkv);
+    const int tid = wi_id_x(), w = uniform(tid >> 6), lane = tid & 63, l32 = lane & 31, hi = lane >> 5;
+    const attn_range qr = q_rows(a, b), kr = k_rows(a, b);
+    const attn_cut cut = part_of(kr.n, a.share, a.nsplit, ATTN_CROSS_KEY_STEP);
+    if (sp >= cut.live)
+        return;
+    const int k0 = min(sp * cut.per, kr.n), k1 = min(k0 + cut.per, kr.n);
+    const int g = a.Hq / a.Hkv, R = qr.n * g, D = a.D;
+    const uint16_t *kp = a.k + kr.at * a.k_tok + u * a.k_head, *vp = a.v + kr.at * a.v_tok + u * a.v_head;
+    const cross_lane<DP> ln(lane);
+    cross_stage<DP, KT> ks, vs;
+    ks.init(w, lane, a.k_tok, D);
+    vs.init(w, lane, a.v_tok, D);
+    auto load = [&](int kb, uint16_t *Kd, uint16_t *Vd) __attribute__((always_inline)) {
+        ks.load(kp + kb * a.k_tok, k1 - kb, a.k_tok, D, Kd, w);
+        vs.load(vp + kb * a.v_tok, k1 - kb, a.v_tok, D, Vd, w);
+    };
+    auto wait_loads = [] { __builtin_amdgcn_s_waitcnt(waitcnt_vm(0)); };
+
+    for (int tile = uniform(at.tile); (int64_t)tile * ATTN_CROSS_ROWS < R; tile += a.tps) {
+        const int row = tile * ATTN_CROSS_ROWS + 32 * w + l32;
+        const bool valid = row < R, idle = tile * ATTN_CROSS_ROWS + 32 * w >= R;
+        const int tok = valid ? row / g : 0, h = u * g + (valid ? row % g : 0);
+        const int64_t slot = (int64_t)(qr.at + tok) * a.Hq + h;
+        bf16x8 qb[KN], gb[KN];
+        float delta = 0.f;
+        {
+            const uint16_t *q = a.q + (qr.at + tok) * a.q_tok + h * a.q_head;
+            const uint16_t *go = a.go + (qr.at + tok) * a.go_tok + h * a.go_head;
+            const uint16_t *o = a.o + (qr.at + tok) * a.o_tok + h * a.o_head;
+#pragma unroll
+            for (int kk = 0; kk < KN; ++kk) {
+                const int col = kk * 16 + hi * 8;
+                u32x4 x = zero4(), y = zero4(), z = zero4();
+                if (valid && col < D) {
+                    x = *reinterpret_cast<const u32x4 *>(q + col);
+                    y = *reinterpret_cast<const u32x4 *>(go + col);
+                    z = *reinterpret_cast<const u32x4 *>(o + col);
+                }
+                qb[kk] = as_bf16x8(x);
+                gb[kk] = as_bf16x8(y);
+                const bf16x8 ob = as_bf16x8(z);
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    delta = fmaf((float)gb[kk][i], (float)ob[i], delta);
+            }
+        }
+        delta = sum_xor32(delta);
+        const float lse2 = valid ? a.lse[slot] * kLog2e : 0.f;
+        if (valid && sp == 0 && hi == 0)
+            a.delta[slot] = delta;
+        f32x16 o[DP / 32];
+#pragma unroll
+        for (int db = 0; db < DP / 32; ++db)
+            zero16(o[db]);
+
+        auto compute = [&](int kb, const uint16_t *Kb, const uint16_t *Vb) __attribute__((always_inline)) {
+            if (idle)
+                return;
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                f32x16 s, dp;
+                zero16(s);
+                zero16(dp);
+#pragma unroll
+                for (int kk = 0; kk < KN; ++kk)
+                    s = mfma32(ln.nat(Kb, t, kk), qb[kk], s);
+#pragma unroll
+                for (int kk = 0; kk < KN; ++kk)
+                    dp = mfma32(ln.nat(Vb, t, kk), gb[kk], dp);
+                bf16x8 pk[2];
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    dp[i] = fast_exp2(fmaf(s[i], a.c, -lse2)) * (dp[i] - delta);
+                // Past the last key K and V are zeros, but exp(0 - lse) may be infinite.
+                if (kb + 32 * t + 32 > k1)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        if (kb + 32 * t + 8 * (i >> 2) + 4 * hi + (i & 3) >= k1)
+                            dp[i] = 0.f;
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    pk[i >> 3][i & 7] = (__bf16)dp[i];
+#pragma unroll
+                for (int cc = 0; cc < 2; ++cc)
+#pragma unroll
+                    for (int db = 0; db < DP / 32; ++db)
+                        o[db] = mfma32(ln.tr(Kb, 2 * t + cc, db), pk[cc], o[db]);
+            }
+        };
+        if (k0 < k1)
+            load(k0, Ks0, Vs0);
+        wait_loads();
+        __syncthreads();
+        auto step = [&](int kb, const uint16_t *Kb, const uint16_t *Vb, uint16_t *Kn, uint16_t *Vn)
+            __attribute__((always_inline)) {
+            if (kb + KT < k1)
+                load(kb + KT, Kn, Vn);
+            compute(kb, Kb, Vb);
+            wait_loads();
+            __syncthreads();
+        };
+        for (int kb = k0; kb < k1; kb += 2 * KT) {
+            step(kb, Ks0, Vs0, Ks1, Vs1);
+            if (kb + KT < k1)
+                step(kb + KT, Ks1, Vs1, Ks0, Vs0);
+        }
+        if (valid) {
+            if (cut.live == 1)
+                put_row<DP>(o, a.scale, a.dq + (qr.at + tok) * a.dq_tok + h * a.dq_head, hi, D);
+            else
+                put_part<DP>(o, a.pacc + (slot * a.nsplit + sp) * D, hi, D);
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------
+// dK and dV. One workgroup of four waves per (sequence, kv head, part of its rows, tile of 128 states): 32 states of a
+// wave keep K and V in registers, the rows of the group's heads, one head after the other, pass through LDS, Q and dO:
+//   S[row][key] = Q . K^T, dP[row][key] = dO . V^T, dV^T[d][key] += dO^T . P, dK^T[d][key] += Q^T . dS
+// Both tiles are read both ways.
+// ------------------------------------------------------------------------------------------
+template <int DP>
+__global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_cross_dkv_kernel(const attn_cross_args a) {
+    constexpr int QT = DP <= 128 ? 64 : 32, KN = DP / 16, NT = QT / 32;
+    __shared__ __attribute__((aligned(1024))) uint16_t Qs0[QT * DP], Qs1[QT * DP];
+    __shared__ __attribute__((aligned(1024))) uint16_t Gs0[QT * DP], Gs1[QT * DP];
+    __shared__ __attribute__((aligned(16))) float st0[2 * QT], st1[2 * QT]; // lse in log2 units, delta
+
+    const attn_place at = attn_place_of(wg_id_x(), a.B * a.Hkv * a.nsplit, a.tps, a.deal);
+    if (at.group < 0)
+        return;
+    const int sp = uniform(at.group / (a.B * a.Hkv)), bu = at.group - sp * (a.B * a.Hkv);
+    const int u = uniform(bu % a.Hkv), b = uniform(bu / a.Hkv);
+    const int tid = wi_id_x(), w = uniform(tid >> 6), lane = tid & 63, l32 = lane & 31, hi = lane >> 5;
+    const attn_range qr = q_rows(a, b), kr = k_rows(a, b);
+    const int g = a.Hq / a.Hkv, D = a.D;
+    const int per_head = uniform((qr.n + QT - 1) / QT), steps = per_head * g; // of QT rows of one head
+    const attn_cut cut = part_of(steps, a.share, a.nsplit, 1);
+    if (sp >= cut.live)
+        return;
+    const int t0 = min(sp * cut.per, steps), t1 = min(t0 + cut.per, steps);
+    const cross_lane<DP> ln(lane);
+    cross_stage<DP, QT> qs, gs;
+    qs.init(w, lane, a.q_tok, D);
+    gs.init(w, lane, a.go_tok, D);
+    auto wait_loads = [] { __builtin_amdgcn_s_waitcnt(waitcnt_vm(0)); };
+
+    for (int tile = uniform(at.tile); (int64_t)tile * ATTN_CROSS_KEYS < kr.n; tile += a.tps) {
+        const int key = tile * ATTN_CROSS_KEYS + 32 * w + l32;
+        const bool valid = key < kr.n, idle = tile * ATTN_CROSS_KEYS + 32 * w >= kr.n;
+        const int64_t tok = kr.at + (valid ? key : 0);
+        bf16x8 kf[KN], vf[KN];
+        {
+            const uint16_t *k = a.k + tok * a.k_tok + u * a.k_head, *v = a.v + tok * a.v_tok + u * a.v_head;
+#pragma unroll
+            for (int kk = 0; kk < KN; ++kk) {
+                const int col = kk * 16 + hi * 8;
+                u32x4 x = zero4(), y = zero4();
+                if (valid && col < D) {
+                    x = *reinterpret_cast<const u32x4 *>(k + col);
+                    y = *reinterpret_cast<const u32x4 *>(v + col);
+                }
+                kf[kk] = as_bf16x8(x);
+                vf[kk] = as_bf16x8(y);
+            }
+        }
+        f32x16 dk[DP / 32], dv[DP / 32];
+#pragma unroll
+        for (int db = 0; db < DP / 32; ++db) {
+            zero16(dk[db]);
+            zero16(dv[db]);
+        }
+        int lh = uniform(t0 / max(per_head, 1)), lt = t0 - lh * per_head; // the step to load: head and step of it
+        float st; // lse or delta of this thread's row of that step
+        auto load = [&](uint16_t *Qd, uint16_t *Gd) __attribute__((always_inline)) {
+            const int h = u * g + lh, r0 = lt * QT;
+            const int64_t first = qr.at + r0;
+            qs.load(a.q + first * a.q_tok + h * a.q_head, qr.n - r0, a.q_tok, D, Qd, w);
+            gs.load(a.go + first * a.go_tok + h * a.go_head, qr.n - r0, a.go_tok, D, Gd, w);
+            // Past the last row P is 0: 2^(0 - inf).
+            const int r = tid & (QT - 1);
+            st = tid < QT ? __builtin_inff() : 0.f;
+            if (tid < 2 * QT && r0 + r < qr.n)
+                st = tid < QT ? a.lse[(first + r) * a.Hq + h] * kLog2e : a.delta[(first + r) * a.Hq + h];
+            if (++lt == per_head) {
+                lt = 0;
+                ++lh;
+            }
+        };
+        auto compute = [&](const uint16_t *Qb, const uint16_t *Gb, const float *sb) __attribute__((always_inline)) {
+            if (idle)
+                return;
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                f32x16 s, dp;
+                zero16(s);
+                zero16(dp);
+#pragma unroll
+                for (int kk = 0; kk < KN; ++kk)
+                    s = mfma32(ln.nat(Qb, t, kk), kf[kk], s);
+#pragma unroll
+                for (int kk = 0; kk < KN; ++kk)
+                    dp = mfma32(ln.nat(Gb, t, kk), vf[kk], dp);
+                bf16x8 pk[2], dk8[2];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const f32x4 l = *reinterpret_cast<const f32x4 *>(sb + 32 * t + 8 * j + 4 * hi);
+                    const f32x4 e = *reinterpret_cast<const f32x4 *>(sb + QT + 32 * t + 8 * j + 4 * hi);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float p = fast_exp2(fmaf(s[4 * j + i], a.c, -l[i]));
+                        pk[j >> 1][4 * (j & 1) + i] = (__bf16)p;
+                        dk8[j >> 1][4 * (j & 1) + i] = (__bf16)(p * (dp[4 * j + i] - e[i]));
+                    }
+                }
+#pragma unroll
+                for (int cc = 0; cc < 2; ++cc)
+#pragma unroll
+                    for (int db = 0; db < DP / 32; ++db) {
+                        dv[db] = mfma32(ln.tr(Gb, 2 * t + cc, db), pk[cc], dv[db]);
+                        dk[db] = mfma32(ln.tr(Qb, 2 * t + cc, db), dk8[cc], dk[db]);
+                    }
+            }
+        };
+        if (t0 < t1) {
+            load(Qs0, Gs0);
+            if (tid < 2 * QT)
+                st0[tid] = st;
+        }
+        wait_loads();
+        __syncthreads();
+        auto step = [&](int i, const uint16_t *Qb, const uint16_t *Gb, const float *sb, uint16_t *Qn, uint16_t *Gn,
+                        float *sn) __attribute__((always_inline)) {
+            if (i + 1 < t1)
+                load(Qn, Gn);
+            compute(Qb, Gb, sb);
+            wait_loads();
+            if (i + 1 < t1 && tid < 2 * QT)
+                sn[tid] = st;
+            __syncthreads();
+        };
+        for (int i = t0; i < t1; i += 2) {
+            step(i, Qs0, Gs0, st0, Qs1, Gs1, st1);
+            if (i + 1 < t1)
+                step(i + 1, Qs1, Gs1, st1, Qs0, Gs0, st0);
+        }
+        if (valid) {
+            if (cut.live == 1) {
+                put_row<DP>(dk, a.scale, a.dk + tok * a.dk_tok + u * a.dk_head, hi, D);
+                put_row<DP>(dv, 1.f, a.dv + tok * a.dv_tok + u * a.dv_head, hi, D);
+            } else {
+                float *dst = a.pacc + ((tok * a.Hkv + u) * a.nsplit + sp) * 2 * D;
+                put_part<DP>(dk, dst, hi, D);
+                put_part<DP>(dv, dst + D, hi, D);
+            }
+        }
+    }
+}
+
+// Adds the parts of dQ's rows (KV = false), or of dK's and dV's, in order. 256 / LP rows of one sequence at a time.
+template <bool KV>
+__global__ __launch_bounds__(256) void attn_cross_sum_kernel(const attn_cross_args a, int lglp, int tpm, int step_rows) {
+    const int b = uniform(wg_id_x() / tpm), t0 = wg_id_x() - b * tpm, tid = wi_id_x();
+    const attn_range qr = q_rows(a, b), kr = k_rows(a, b);
+    const int g = a.Hq / a.Hkv, H = KV ? a.Hkv : a.Hq, W = KV ? 2 * a.D : a.D; // floats of a row's part
+    const attn_cut cut = KV ? part_of((qr.n + step_rows - 1) / step_rows * g, a.share, a.nsplit, 1)
+                            : part_of(kr.n, a.share, a.nsplit, ATTN_CROSS_KEY_STEP);
+    if (cut.live == 1)
+        return; // written already
+    const int first = KV ? kr.at : qr.at;
+    const int64_t R = (int64_t)(KV ? kr.n : qr.n) * H;
+    const int rpw = 256 >> lglp, d = 4 * (tid & ((1 << lglp) - 1));
+    for (int64_t row = (int64_t)t0 * rpw + (tid >> lglp); row < R; row += (int64_t)tpm * rpw) {
+        if (d >= W)
+            continue;
+        const float *p = a.pacc + ((int64_t)first * H + row) * a.nsplit * W + d;
+        f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+        for (int s = 0; s < cut.live; ++s) {
+            const f32x4 x = *reinterpret_cast<const f32x4 *>(p + (int64_t)s * W);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                acc[j] += x[j];
+        }
+        const int64_t tok = first + row / H;
+        const int h = row % H;
+        const bool v = KV && d >= a.D;
+        const float f = v ? 1.f : a.scale;
+        uint16_t *dst = !KV ? a.dq + tok * a.dq_tok + h * a.dq_head + d
+                        : v ? a.dv + tok * a.dv_tok + h * a.dv_head + d - a.D
+                            : a.dk + tok * a.dk_tok + h * a.dk_head + d;
+        *reinterpret_cast<u32x2 *>(dst) = u32x2{bf16_pair(acc[0] * f, acc[1] * f), bf16_pair(acc[2] * f, acc[3] * f)};
+    }
+}
+
+// ---- launchers -------------------------------------------------------------------------------
+// Calls f(std::integral_constant<int, DP>{}) with the tile width for head dim D.
+template <typename F> hipError_t with_width(int D, F &&f) {
+    return D <= 64    ? f(std::integral_constant<int, 64>{})
+           : D <= 128 ? f(std::integral_constant<int, 128>{})
+                      : f(std::integral_constant<int, 256>{});
+}
+
+// log2 of the lanes that rows of n floats take, four each: at most the workgroup.
+int lg_lanes(int n) {
+    int lg = 2;
+    while (4 << lg < n)
+        ++lg;
+    return lg;
+}
+
+bool cross_grid_ok(const attn_cross_args &a, const attn_cross_cut &cut) {
+    return cut.grid > 0 && cut.grid <= ATTN_CROSS_MAX_GRID && a.nsplit >= 1 && a.nsplit <= ATTN_CROSS_MAX_PARTS &&
+           a.tps >= 1 && a.deal >= 1;
+}
+
+// Workgroups per sequence that look over `rows` rows at rpw a time, not above 2^18 in all.
+int cross_sum_tiles(int B, int64_t rows, int rpw) {
+    const int64_t t = (rows + rpw - 1) / rpw, most = (1 << 18) / B;
+    return (int)(t < 1 || most < 1 ? 1 : t < most ? t : most);
+}
+
+} // namespace
+
+extern "C" int attn_hip_launch_cross(const struct attn_cross_args *ap, const struct attn_cross_cut *cut, int max_q,
+                                     void *stream) {
+    const attn_cross_args &a = *ap;
+    const hipStream_t st = (hipStream_t)stream;
+    if (!cross_grid_ok(a, *cut))
+        return (int)hipErrorInvalidValue;
+    const dim3 grid((unsigned)cut->grid), block(256);
+    const hipError_t e = with_width(a.D, [&](auto W) {
+        constexpr int DP = decltype(W)::value;
+        auto rows = [&](auto NB, auto NT) {
+            constexpr int kN = decltype(NB)::value;
+            constexpr bool kT = decltype(NT)::value;
+            if (t_plan) {
+                plan_note(grid, block, "attn_cross_rows_kernel<%d, %d, %s> parts=%d share=%d", DP, kN, tf(kT),
+                          a.nsplit, a.share);
+                return hipSuccess;
+            }
+            hipLaunchKernelGGL((attn_cross_rows_kernel<DP, kN, kT>), grid, block, 0, st, a);
+            return hipGetLastError();
+        };
+        constexpr std::integral_constant<int, 1> one;
+        // Past the L2 where a row tile is the only one of its sequence.
+        if constexpr (DP > 128) {
+            if (cut->rows16 == 1)
+                return with_flag(a.tps == 1, [&](auto NT) { return rows(one, NT); });
+        } else {
+            if (cut->rows16 == 1)
+                return rows(one, std::true_type{});
+            if (cut->rows16 == 2)
+                return rows(std::integral_constant<int, 2>{}, std::true_type{});
+        }
+        if (t_plan) {
+            plan_note(grid, block, "attn_cross_kernel<%d> parts=%d share=%d", DP, a.nsplit, a.share);
+            return hipSuccess;
+        }
+        hipLaunchKernelGGL((attn_cross_kernel<DP>), grid, block, 0, st, a);
+        return hipGetLastError();
+    });
+    if (e != hipSuccess || a.nsplit == 1)
+        return (int)e;
+    const int lglp = lg_lanes(a.D);
+    const int tpm = cross_sum_tiles(a.B, (int64_t)max_q * a.Hq, 256 >> lglp);
+    const dim3 mgrid((unsigned)(a.B * tpm));
+    if (t_plan) {
+        plan_note(mgrid, block, "attn_cross_merge_kernel");
+        return (int)hipSuccess;
+    }
+    hipLaunchKernelGGL(attn_cross_merge_kernel, mgrid, block, 0, st, a, lglp, tpm);
+    return (int)hipGetLastError();
+}
+
+// One of the two gradient kernels and, where it may leave parts, their sum. kv: dK and dV, after dQ.
+extern "C" int attn_hip_launch_cross_grad(const struct attn_cross_args *ap, const struct attn_cross_cut *cut, int kv,
+                                          int most, void *stream) {
+    const attn_cross_args &a = *ap;
+    const hipStream_t st = (hipStream_t)stream;
+    if (!cross_grid_ok(a, *cut))
+        return (int)hipErrorInvalidValue;
+    const dim3 grid((unsigned)cut->grid), block(256);
+    const hipError_t e = with_width(a.D, [&](auto W) {
+        constexpr int DP = decltype(W)::value;
+        if (t_plan) {
+            plan_note(grid, block, "attn_cross_%s_kernel<%d> parts=%d share=%d", kv ? "dkv" : "dq", DP, a.nsplit,
+                      a.share);
+            return hipSuccess;
+        }
+        if (kv)
+            hipLaunchKernelGGL((attn_cross_dkv_kernel<DP>), grid, block, 0, st, a);
+        else
+            hipLaunchKernelGGL((attn_cross_dq_kernel<DP>), grid, block, 0, st, a);
+        return hipGetLastError();
+    });
+    if (e != hipSuccess || a.nsplit == 1)
+        return (int)e;
+    const int lglp = lg_lanes(kv ? 2 * a.D : a.D);
+    const int tpm = cross_sum_tiles(a.B, (int64_t)most * (kv ? a.Hkv : a.Hq), 256 >> lglp);
+    const dim3 sgrid((unsigned)(a.B * tpm));
+    if (t_plan) {
+        plan_note(sgrid, block, "attn_cross_sum_kernel<%s>", tf(kv));
+        return (int)hipSuccess;
+    }
+    if (kv)
+        hipLaunchKernelGGL(attn_cross_sum_kernel<true>, sgrid, block, 0, st, a, lglp, tpm, attn_cross_step_rows(a.D));
+    else
+        hipLaunchKernelGGL(attn_cross_sum_kernel<false>, sgrid, block, 0, st, a, lglp, tpm, attn_cross_step_rows(a.D));
+    return (int)hipGetLastError();
+}
+
+#endif

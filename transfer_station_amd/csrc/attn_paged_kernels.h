@@ -23,16 +23,6 @@
 
 namespace {
 
-typedef __attribute__((ext_vector_type(2))) uint32_t u32x2;
-typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
-// Tables and lengths are read through the scalar cache: wave-uniform and not written by the kernel.
-typedef const __attribute__((address_space(4))) int32_t const_i32;
-__device__ __forceinline__ int scalar_i32(const int32_t *p, long i) {
-    return ((const_i32 *)(uintptr_t)p)[i];
-}
-
-__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
-
 // Eight 4-bit codes, times their scale, as eight bf16 values: exact, but for a scale so small or large
 // that bf16 has no such value.
 __device__ __forceinline__ u32x4 fp4_to_bf16(uint32_t w, float scale) {
@@ -44,11 +34,6 @@ __device__ __forceinline__ u32x4 fp4_to_bf16(uint32_t w, float scale) {
                  __builtin_bit_cast(uint32_t, c), __builtin_bit_cast(uint32_t, d)};
 }
 __device__ __forceinline__ float e8m0(uint32_t e) { return __builtin_bit_cast(float, e << 23); }
-
-__device__ __forceinline__ uint32_t bf16_pair(float a, float b) {
-    const bf16x2 r = {(__bf16)a, (__bf16)b};
-    return __builtin_bit_cast(uint32_t, r);
-}
 
 // Scores in units of log2 from raw dot products: each(f) applies f(score, offset of its key behind the first)
 // to all of them, `first` is how far the row's position lies behind the first key. The tests are uniform, and
@@ -190,19 +175,6 @@ __device__ __forceinline__ kv_block block_in(const attn_paged_args &a, int pg, i
 // b ? x : y of two values (of two array elements the operator itself would choose the address, and keep the
 // array in memory).
 __device__ __forceinline__ uint32_t pick(bool b, uint32_t x, uint32_t y) { return b ? x : y; }
-
-template <bool NT> __device__ __forceinline__ u32x4 buf16(__amdgpu_buffer_rsrc_t r, uint32_t off) {
-    return __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, NT ? kDmaNT : 0);
-}
-
-// What a sum of p changes by when the maximum that p is taken against rises from m0 to m1: p is 2^(s c - m c) with m c
-// rounded, so the factor is between the rounded products. Taken from m0 - m1 it was off by their roundings, at
-// scores of 2^20 by up to 9%.
-__device__ __forceinline__ float rescale(float m0, float m1, float c) {
-#pragma clang fp contract(off)
-    const float a = m0 * c, b = m1 == kNegInf ? 0.f : m1 * c;
-    return fast_exp2(a - b);
-}
 
 // A part's maximum as the merge is told it. There +inf says that the row is written and -inf that the part has
 // nothing: an infinite score, and a part of NaN alone, go by finite ones, and their sums carry the NaN.
