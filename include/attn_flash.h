@@ -249,6 +249,44 @@ void attn_cross_grad(const struct attn_cross_call *c, const struct attn_rows *q,
  * launched or read. */
 int attn_cross_plan(const struct attn_cross_call *c, int grad, char *buf, size_t len);
 
+/* ---- Beam search ---------------------------------------------------------------------------------
+ * No counterpart in the reference. One step of a beam search over the paged cache: choose the continuations that go
+ * on, and let the cache's sequences follow them. Stream-ordered, nothing allocated, capturable like the calls above.
+ */
+#define ATTN_BEAMS_MAX 256
+#define ATTN_BEAM_K_MAX 64
+#define ATTN_BEAM_V_MAX (1 << 20)
+#define ATTN_REORDER_MAX 32
+
+/* The beams of B batch entries: row b * beams + i of logits (bits 16: bf16, 32: fp32; `row` elements from row to row, at
+ * any alignment of an element) are beam i's over V tokens, scores[b * beams + i] is what it has reached. done (bytes, or
+ * NULL) marks beams that are complete. All device memory, but for the numbers. */
+struct attn_beams {
+    const void *logits;
+    int64_t row;
+    const float *scores;
+    const uint8_t *done;
+    int32_t bits, B, beams, V, K, done_token;
+};
+
+/* The K best continuations of each entry, best first: score = (x - log sum exp x) + scores, token and parent, the row
+ * (b * beams + i) that it continues; [B][K] each. Ties go to the lowest beam, then token. A done beam's only
+ * continuation is done_token, at its score; a logit of -inf is none, and a beam whose score is not finite, or that
+ * has a NaN or +inf among its logits, has none. Where an entry has fewer than K, the rest is score -inf, token -1 and
+ * the entry's first row. The sums of exponentials are taken in fp32, all else in fp64, and the score is rounded once.
+ * scratch: attn_beam_scratch_bytes(c) bytes, ATTN_SCRATCH_ALIGN-aligned; calls that may overlap need one each. */
+size_t attn_beam_scratch_bytes(const struct attn_beams *c);
+void attn_beam_select(const struct attn_beams *c, float *score, int32_t *token, int32_t *parent, void *scratch);
+
+/* The cache's sequences lie in groups of `beams` neighbours; sequence b continues parent[b] (device, [B], rows as
+ * attn_beam_select gives them: members of b's group; any other entry means b itself). All members of a group hold as many
+ * tokens as its first one's kv_len says. Their full pages are shared: with tables, the entries of the parent's row of
+ * the table for them replace b's, in place (the one call that writes the table). The tokens of the last, partly filled page
+ * are copied into b's own page of that column, with what the 16 bytes at their end hold besides; members must not share
+ * that page. A cache per layer that shares one table is reordered by a call per layer, `tables` set in one of them, in any
+ * order. An entry of the table outside the cache is not followed: its tokens are not copied. q_start is not used. */
+void attn_kv_reorder(const struct attn_kv_cache *c, const int32_t *parent, int beams, int tables);
+
 /* Stream selection for the calling thread (no counterpart in the reference, which has
  * no device). `stream` is a hipStream_t; NULL selects the null stream. */
 void attn_flash_set_stream(void *stream);

@@ -31,6 +31,9 @@ _SIGNATURES = {
     "attn_cross_grad_scratch_bytes": (_c.c_size_t, [_c.c_void_p]),
     "attn_cross_grad": (None, [_c.c_void_p] * 11),
     "attn_cross_plan": (_c.c_int, [_c.c_void_p, _c.c_int, _c.c_char_p, _c.c_size_t]),
+    "attn_beam_scratch_bytes": (_c.c_size_t, [_c.c_void_p]),
+    "attn_beam_select": (None, [_c.c_void_p] * 5),
+    "attn_kv_reorder": (None, [_c.c_void_p] * 2 + [_c.c_int] * 2),
     "attn_flash_set_stream": (None, [_c.c_void_p]),
     "attn_flash_get_stream": (_c.c_void_p, []),
     # include/attn_devutil.h

@@ -27,7 +27,8 @@
 //                                          64 / any, one workgroup per row)
 //   attn_pack_v16_kernel<TK,VEC>           V [Hkv][Sk][D] -> V^T [Hkv][D][Sk]
 // VT selects a pre-transposed V ([Hkv][D][Sk], pack_v_full's layout). The paged cache's kernels are in
-// attn_paged_kernels.h and cross attention's in attn_cross_kernels.h, both at the end.
+// attn_paged_kernels.h and cross attention's in attn_cross_kernels.h, beam
+// search's in attn_beam_kernels.h, all at the end.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 #include <stdlib.h>
@@ -3754,3 +3755,6 @@ extern "C" int attn_hip_static_scratch(void **ptr, size_t *bytes) {
 
 // ---- cross attention's kernels ----------------------------------------------------------------
 #include "attn_cross_kernels.h"
+
+// ---- beam search's kernels --------------------------------------------------------------------
+#include "attn_beam_kernels.h"
