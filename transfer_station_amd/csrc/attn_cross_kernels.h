@@ -47,6 +47,11 @@ __device__ __forceinline__ f32x16 mfma32(bf16x8 x, bf16x8 y, f32x16 z) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, y, z, 0, 0, 0);
 }
 
+// Bytes from a row's first element to the end of `rows` rows, 0 where there are none.
+__device__ __forceinline__ uint32_t row_bytes(int rows, int64_t tok, int D) {
+    return rows < 1 ? 0u : (uint32_t)(rows - 1) * (uint32_t)(tok * 2) + D * 2;
+}
+
 // ROWS rows of a token tensor into LDS by four waves' LDS-DMA: what each lane reads for its 16 bytes of each KB that
 // its wave writes. Columns past D, and rows past the last, lie outside the buffer and arrive as zeros.
 template <int DP, int ROWS> struct cross_stage {
@@ -65,7 +70,7 @@ template <int DP, int ROWS> struct cross_stage {
     // rows: how many there are from `first` on, at least one.
     __device__ __forceinline__ void load(const uint16_t *first, int rows, int64_t tok, int D, uint16_t *lds,
                                          int w) const {
-        const auto r = make_rsrc(first, (uint32_t)(min(rows, ROWS) - 1) * (uint32_t)(tok * 2) + D * 2);
+        const auto r = make_rsrc(first, row_bytes(min(rows, ROWS), tok, D));
 #pragma unroll
         for (int p = 0; p < PW; ++p)
             dma16<0>(r, lds + (w * PW + p) * 512, off[p]);
@@ -113,7 +118,7 @@ __device__ __forceinline__ void put_row(const f32x16 *o, float f, uint16_t *dst,
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const int d = db * 32 + 8 * j + 4 * hi;
-            if (d < D)
+            if (db * 32 + 16 * (j >> 1) < D) // D % 16 == 0: the same for all lanes
                 *reinterpret_cast<u32x2 *>(dst + d) = u32x2{bf16_pair(o[db][4 * j] * f, o[db][4 * j + 1] * f),
                                                             bf16_pair(o[db][4 * j + 2] * f, o[db][4 * j + 3] * f)};
         }
@@ -124,7 +129,7 @@ template <int DP> __device__ __forceinline__ void put_part(const f32x16 *o, floa
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const int d = db * 32 + 8 * j + 4 * hi;
-            if (d < D)
+            if (db * 32 + 16 * (j >> 1) < D)
                 *reinterpret_cast<f32x4 *>(dst + d) =
                     f32x4{o[db][4 * j], o[db][4 * j + 1], o[db][4 * j + 2], o[db][4 * j + 3]};
         }
@@ -175,17 +180,12 @@ template <int DP> __global__ __launch_bounds__(256, 2) void attn_cross_kernel(co
         const int row = tile * ATTN_CROSS_ROWS + 32 * w + l32;
         const bool valid = row < R;
         const int tok = valid ? row / g : 0, h = u * g + (valid ? row % g : 0);
-        const uint16_t *q = a.q + (qr.at + tok) * a.q_tok + h * a.q_head;
-        const bool idle = tile * ATTN_CROSS_ROWS + 32 * w >= R; // the wave has no rows
+        const uint16_t *q = a.q + (qr.at + tok) * a.q_tok + h * a.q_head; // without a row of its own: the first one's
+        const bool idle = tile * ATTN_CROSS_ROWS + 32 * w >= R;           // the wave has no rows
         bf16x8 qb[KN];
 #pragma unroll
-        for (int kk = 0; kk < KN; ++kk) {
-            const int col = kk * 16 + hi * 8;
-            u32x4 x = zero4();
-            if (valid && col < D)
-                x = *reinterpret_cast<const u32x4 *>(q + col);
-            qb[kk] = as_bf16x8(x);
-        }
+        for (int kk = 0; kk < KN; ++kk)
+            qb[kk] = as_bf16x8(kk * 16 < D ? *reinterpret_cast<const u32x4 *>(q + kk * 16 + hi * 8) : zero4());
         float m_run = kNegInf, l_run = 0.f;
         f32x16 o[DP / 32];
 #pragma unroll
@@ -628,7 +628,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_cross_dq_kernel(c
             for (int kk = 0; kk < KN; ++kk) {
                 const int col = kk * 16 + hi * 8;
                 u32x4 x = zero4(), y = zero4(), z = zero4();
-                if (valid && col < D) {
+                if (kk * 16 < D) {
                     x = *reinterpret_cast<const u32x4 *>(q + col);
                     y = *reinterpret_cast<const u32x4 *>(go + col);
                     z = *reinterpret_cast<const u32x4 *>(o + col);
@@ -642,7 +642,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_cross_dq_kernel(c
             }
         }
         delta = sum_xor32(delta);
-        const float lse2 = valid ? a.lse[slot] * kLog2e : 0.f;
+        const float lse2 = a.lse[slot] * kLog2e;
         if (valid && sp == 0 && hi == 0)
             a.delta[slot] = delta;
         f32x16 o[DP / 32];
@@ -718,7 +718,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_cross_dq_kernel(c
 // ------------------------------------------------------------------------------------------
 template <int DP>
 __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_cross_dkv_kernel(const attn_cross_args a) {
-    constexpr int QT = DP <= 128 ? 64 : 32, KN = DP / 16, NT = QT / 32;
+    constexpr int QT = DP <= 64 ? 64 : 32, KN = DP / 16, NT = QT / 32;
     __shared__ __attribute__((aligned(1024))) uint16_t Qs0[QT * DP], Qs1[QT * DP];
     __shared__ __attribute__((aligned(1024))) uint16_t Gs0[QT * DP], Gs1[QT * DP];
     __shared__ __attribute__((aligned(16))) float st0[2 * QT], st1[2 * QT]; // lse in log2 units, delta
@@ -746,19 +746,19 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_cross_dkv_kernel(
         const int key = tile * ATTN_CROSS_KEYS + 32 * w + l32;
         const bool valid = key < kr.n, idle = tile * ATTN_CROSS_KEYS + 32 * w >= kr.n;
         const int64_t tok = kr.at + (valid ? key : 0);
+        // The wave's rows of K and V, by lane: what lies past the last state or past D is outside the buffer, zeros.
         bf16x8 kf[KN], vf[KN];
         {
-            const uint16_t *k = a.k + tok * a.k_tok + u * a.k_head, *v = a.v + tok * a.v_tok + u * a.v_head;
+            const int64_t first = kr.at + tile * ATTN_CROSS_KEYS + 32 * w;
+            const int rows = min(32, kr.n - tile * ATTN_CROSS_KEYS - 32 * w);
+            const auto rk = make_rsrc(a.k + first * a.k_tok + u * a.k_head, row_bytes(rows, a.k_tok, D));
+            const auto rv = make_rsrc(a.v + first * a.v_tok + u * a.v_head, row_bytes(rows, a.v_tok, D));
+            const uint32_t ok = l32 * (uint32_t)(a.k_tok * 2) + hi * 16, ov = l32 * (uint32_t)(a.v_tok * 2) + hi * 16;
 #pragma unroll
             for (int kk = 0; kk < KN; ++kk) {
-                const int col = kk * 16 + hi * 8;
-                u32x4 x = zero4(), y = zero4();
-                if (valid && col < D) {
-                    x = *reinterpret_cast<const u32x4 *>(k + col);
-                    y = *reinterpret_cast<const u32x4 *>(v + col);
-                }
-                kf[kk] = as_bf16x8(x);
-                vf[kk] = as_bf16x8(y);
+                const bool in = kk * 16 < D; // D % 16 == 0
+                kf[kk] = as_bf16x8(buf16<false>(rk, in ? ok + kk * 32 : 0x80000000u));
+                vf[kk] = as_bf16x8(buf16<false>(rv, in ? ov + kk * 32 : 0x80000000u));
             }
         }
         f32x16 dk[DP / 32], dv[DP / 32];

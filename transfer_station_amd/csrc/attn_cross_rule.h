@@ -50,7 +50,7 @@ ATTN_HD struct attn_cut attn_cut_of(int total, int share, int nsplit, int step) 
 #define ATTN_CROSS_GRAD_FLOATS (1L << 25)
 
 /* Rows of a step of the kernel of dK and dV. */
-ATTN_HD int attn_cross_step_rows(int D) { return D <= 128 ? 64 : 32; }
+ATTN_HD int attn_cross_step_rows(int D) { return D <= 64 ? 64 : 32; }
 
 /* What one launch looks like: row (or state) tiles per group and its parts, and how the groups are dealt to the XCDs
  * (attn_place_of). */
