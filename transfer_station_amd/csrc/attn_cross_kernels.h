@@ -52,28 +52,32 @@ __device__ __forceinline__ uint32_t row_bytes(int rows, int64_t tok, int D) {
     return rows < 1 ? 0u : (uint32_t)(rows - 1) * (uint32_t)(tok * 2) + D * 2;
 }
 
-// ROWS rows of a token tensor into LDS by four waves' LDS-DMA: what each lane reads for its 16 bytes of each KB that
-// its wave writes. Columns past D, and rows past the last, lie outside the buffer and arrive as zeros.
+// ROWS rows of a token tensor into LDS by four waves' LDS-DMA. Wave w writes the KBs whose rows' groups are w mod 4 (at
+// DP = 64 2 w mod 8 and the next), so that a lane's chunk, and with it its offset, is the same in all of them but for the
+// rows' distance. Columns past D, and rows past the last, lie outside the buffer and arrive as zeros.
 template <int DP, int ROWS> struct cross_stage {
-    static constexpr int PW = ROWS * DP / 2048;
-    static_assert(PW >= 1, "a wave writes whole KBs");
-    uint32_t off[PW];
+    static constexpr int PW = ROWS * DP / 2048, HALVES = DP == 256 ? 2 : 1; // KBs of a wave; of a group of rows
+    static_assert(PW >= HALVES, "a wave writes whole groups");
+    uint32_t off[HALVES];
     __device__ __forceinline__ void init(int w, int lane, int64_t tok, int D) {
 #pragma unroll
-        for (int p = 0; p < PW; ++p) {
-            const int x = (w * PW + p) * 1024 + 16 * lane;
+        for (int p = 0; p < HALVES; ++p) {
+            const int x = (w * HALVES + p) * 1024 + 16 * lane;
             const int rg = x / (8 * DP), y = x % (8 * DP);
             const int r = rg * 4 + (y % 256) / 64, c = y / 256 * 4 + ((y % 64 / 16) ^ (rg & 3));
             off[p] = c * 8 < D ? (uint32_t)r * (uint32_t)(tok * 2) + c * 16 : 0x80000000u;
         }
     }
-    // rows: how many there are from `first` on, at least one.
+    // rows: how many there are from `first` on.
     __device__ __forceinline__ void load(const uint16_t *first, int rows, int64_t tok, int D, uint16_t *lds,
                                          int w) const {
         const auto r = make_rsrc(first, row_bytes(min(rows, ROWS), tok, D));
 #pragma unroll
-        for (int p = 0; p < PW; ++p)
-            dma16<0>(r, lds + (w * PW + p) * 512, off[p]);
+        for (int p = 0; p < PW; ++p) {
+            constexpr int H = HALVES;
+            const uint32_t far = (uint32_t)(p / H * (2048 * H / DP)) * (uint32_t)(tok * 2);
+            dma16<0>(r, lds + (w * H + p % H + p / H * 4 * H) * 512, opaque(off[p % H]) + far); // not held in registers
+        }
     }
 };
 
@@ -149,9 +153,10 @@ constexpr float kCrossSum = 65536.0f;
 // ------------------------------------------------------------------------------------------
 template <int DP> __global__ __launch_bounds__(256, 2) void attn_cross_kernel(const attn_cross_args a) {
     constexpr int KT = cross_tile_keys(DP), KN = DP / 16, NT = KT / 32;
-    // Each buffer is a variable of its own: the compiler tells LDS accesses apart by variable.
-    __shared__ __attribute__((aligned(1024))) uint16_t Ks0[KT * DP], Ks1[KT * DP];
-    __shared__ __attribute__((aligned(1024))) uint16_t Vs0[KT * DP], Vs1[KT * DP];
+    // K's tile and V's behind it. Each buffer is a variable of its own: the compiler tells LDS accesses apart by
+    // variable, and needs address registers for each.
+    constexpr int VO = KT * DP;
+    __shared__ __attribute__((aligned(1024))) uint16_t KV0[2 * VO], KV1[2 * VO];
 
     const attn_place at = attn_place_of(wg_id_x(), a.B * a.Hkv * a.nsplit, a.tps, a.deal);
     if (at.group < 0)
@@ -170,9 +175,9 @@ template <int DP> __global__ __launch_bounds__(256, 2) void attn_cross_kernel(co
     cross_stage<DP, KT> ks, vs;
     ks.init(w, lane, a.k_tok, D);
     vs.init(w, lane, a.v_tok, D);
-    auto load = [&](int kb, uint16_t *Kd, uint16_t *Vd) __attribute__((always_inline)) {
-        ks.load(kp + kb * a.k_tok, k1 - kb, a.k_tok, D, Kd, w);
-        vs.load(vp + kb * a.v_tok, k1 - kb, a.v_tok, D, Vd, w);
+    auto load = [&](int kb, uint16_t *to) __attribute__((always_inline)) {
+        ks.load(kp + kb * a.k_tok, k1 - kb, a.k_tok, D, to, w);
+        vs.load(vp + kb * a.v_tok, k1 - kb, a.v_tok, D, to + VO, w);
     };
     auto wait_loads = [] { __builtin_amdgcn_s_waitcnt(waitcnt_vm(0)); };
 
@@ -192,14 +197,14 @@ template <int DP> __global__ __launch_bounds__(256, 2) void attn_cross_kernel(co
         for (int db = 0; db < DP / 32; ++db)
             zero16(o[db]);
 
-        auto compute = [&](int kb, const uint16_t *Kb, const uint16_t *Vb) __attribute__((always_inline)) {
+        auto compute = [&](int kb, const uint16_t *kv) __attribute__((always_inline)) {
             if (idle)
                 return;
             f32x16 s[NT];
             bf16x8 ka[2][KN];
 #pragma unroll
             for (int kk = 0; kk < KN; ++kk)
-                ka[0][kk] = ln.nat(Kb, 0, kk);
+                ka[0][kk] = ln.nat(kv, 0, kk);
             __builtin_amdgcn_sched_group_barrier(0x100, KN, 0);
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
@@ -208,7 +213,7 @@ template <int DP> __global__ __launch_bounds__(256, 2) void attn_cross_kernel(co
                 for (int kk = 0; kk < KN; ++kk) {
                     s[t] = mfma32(ka[t & 1][kk], qb[kk], s[t]);
                     if (t + 1 < NT)
-                        ka[(t + 1) & 1][kk] = ln.nat(Kb, t + 1, kk);
+                        ka[(t + 1) & 1][kk] = ln.nat(kv, t + 1, kk);
                 }
 #pragma unroll
                 for (int kk = 0; kk < KN; ++kk) {
@@ -263,24 +268,23 @@ template <int DP> __global__ __launch_bounds__(256, 2) void attn_cross_kernel(co
             for (int cc = 0; cc < 2 * NT; ++cc)
 #pragma unroll
                 for (int db = 0; db < DP / 32; ++db)
-                    o[db] = mfma32(ln.tr(Vb, cc, db), pk[cc], o[db]);
+                    o[db] = mfma32(ln.tr(kv + VO, cc, db), pk[cc], o[db]);
         };
         if (k0 < k1)
-            load(k0, Ks0, Vs0);
+            load(k0, KV0);
         wait_loads(); // for Q too
         __syncthreads();
-        auto step = [&](int kb, const uint16_t *Kb, const uint16_t *Vb, uint16_t *Kn, uint16_t *Vn)
-            __attribute__((always_inline)) {
+        auto step = [&](int kb, const uint16_t *kv, uint16_t *next) __attribute__((always_inline)) {
             if (kb + KT < k1)
-                load(kb + KT, Kn, Vn);
-            compute(kb, Kb, Vb);
+                load(kb + KT, next);
+            compute(kb, kv);
             wait_loads(); // this wave's part of the next tile has arrived
             __syncthreads();
         };
         for (int kb = k0; kb < k1; kb += 2 * KT) {
-            step(kb, Ks0, Vs0, Ks1, Vs1);
+            step(kb, KV0, KV1);
             if (kb + KT < k1)
-                step(kb + KT, Ks1, Vs1, Ks0, Vs0);
+                step(kb + KT, KV1, KV0);
         }
         l_run = sum_xor32(l_run);
         if (valid) {
@@ -587,8 +591,8 @@ __global__ __launch_bounds__(256) void attn_cross_merge_kernel(const attn_cross_
 template <int DP>
 __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_cross_dq_kernel(const attn_cross_args a) {
     constexpr int KT = cross_tile_keys(DP), KN = DP / 16, NT = KT / 32;
-    __shared__ __attribute__((aligned(1024))) uint16_t Ks0[KT * DP], Ks1[KT * DP];
-    __shared__ __attribute__((aligned(1024))) uint16_t Vs0[KT * DP], Vs1[KT * DP];
+    constexpr int VO = KT * DP;
+    __shared__ __attribute__((aligned(1024))) uint16_t KV0[2 * VO], KV1[2 * VO];
 
     const attn_place at = attn_place_of(wg_id_x(), a.B * a.Hkv * a.nsplit, a.tps, a.deal);
     if (at.group < 0)
@@ -607,9 +611,9 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_cross_dq_kernel(c
     cross_stage<DP, KT> ks, vs;
     ks.init(w, lane, a.k_tok, D);
     vs.init(w, lane, a.v_tok, D);
-    auto load = [&](int kb, uint16_t *Kd, uint16_t *Vd) __attribute__((always_inline)) {
-        ks.load(kp + kb * a.k_tok, k1 - kb, a.k_tok, D, Kd, w);
-        vs.load(vp + kb * a.v_tok, k1 - kb, a.v_tok, D, Vd, w);
+    auto load = [&](int kb, uint16_t *to) __attribute__((always_inline)) {
+        ks.load(kp + kb * a.k_tok, k1 - kb, a.k_tok, D, to, w);
+        vs.load(vp + kb * a.v_tok, k1 - kb, a.v_tok, D, to + VO, w);
     };
     auto wait_loads = [] { __builtin_amdgcn_s_waitcnt(waitcnt_vm(0)); };
 
@@ -650,7 +654,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_cross_dq_kernel(c
         for (int db = 0; db < DP / 32; ++db)
             zero16(o[db]);
 
-        auto compute = [&](int kb, const uint16_t *Kb, const uint16_t *Vb) __attribute__((always_inline)) {
+        auto compute = [&](int kb, const uint16_t *kv) __attribute__((always_inline)) {
             if (idle)
                 return;
 #pragma unroll
@@ -660,10 +664,10 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_cross_dq_kernel(c
                 zero16(dp);
 #pragma unroll
                 for (int kk = 0; kk < KN; ++kk)
-                    s = mfma32(ln.nat(Kb, t, kk), qb[kk], s);
+                    s = mfma32(ln.nat(kv, t, kk), qb[kk], s);
 #pragma unroll
                 for (int kk = 0; kk < KN; ++kk)
-                    dp = mfma32(ln.nat(Vb, t, kk), gb[kk], dp);
+                    dp = mfma32(ln.nat(kv + VO, t, kk), gb[kk], dp);
                 bf16x8 pk[2];
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
@@ -681,25 +685,24 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_cross_dq_kernel(c
                 for (int cc = 0; cc < 2; ++cc)
 #pragma unroll
                     for (int db = 0; db < DP / 32; ++db)
-                        o[db] = mfma32(ln.tr(Kb, 2 * t + cc, db), pk[cc], o[db]);
+                        o[db] = mfma32(ln.tr(kv, 2 * t + cc, db), pk[cc], o[db]);
             }
         };
         if (k0 < k1)
-            load(k0, Ks0, Vs0);
+            load(k0, KV0);
         wait_loads();
         __syncthreads();
-        auto step = [&](int kb, const uint16_t *Kb, const uint16_t *Vb, uint16_t *Kn, uint16_t *Vn)
-            __attribute__((always_inline)) {
+        auto step = [&](int kb, const uint16_t *kv, uint16_t *next) __attribute__((always_inline)) {
             if (kb + KT < k1)
-                load(kb + KT, Kn, Vn);
-            compute(kb, Kb, Vb);
+                load(kb + KT, next);
+            compute(kb, kv);
             wait_loads();
             __syncthreads();
         };
         for (int kb = k0; kb < k1; kb += 2 * KT) {
-            step(kb, Ks0, Vs0, Ks1, Vs1);
+            step(kb, KV0, KV1);
             if (kb + KT < k1)
-                step(kb + KT, Ks1, Vs1, Ks0, Vs0);
+                step(kb + KT, KV1, KV0);
         }
         if (valid) {
             if (cut.live == 1)
@@ -716,12 +719,12 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_cross_dq_kernel(c
 //   S[row][key] = Q . K^T, dP[row][key] = dO . V^T, dV^T[d][key] += dO^T . P, dK^T[d][key] += Q^T . dS
 // Both tiles are read both ways.
 // ------------------------------------------------------------------------------------------
-template <int DP>
-__global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_cross_dkv_kernel(const attn_cross_args a) {
+template <int DP, bool DK, bool DV>
+__global__ __launch_bounds__(256, DP <= 128 || !DK ? 2 : 1) void attn_cross_dkv_kernel(const attn_cross_args a) {
     constexpr int QT = DP <= 64 ? 64 : 32, KN = DP / 16, NT = QT / 32;
-    __shared__ __attribute__((aligned(1024))) uint16_t Qs0[QT * DP], Qs1[QT * DP];
-    __shared__ __attribute__((aligned(1024))) uint16_t Gs0[QT * DP], Gs1[QT * DP];
-    __shared__ __attribute__((aligned(16))) float st0[2 * QT], st1[2 * QT]; // lse in log2 units, delta
+    constexpr int GO = QT * DP; // dO's tile behind Q's
+    __shared__ __attribute__((aligned(1024))) uint16_t QG0[2 * GO], QG1[2 * GO];
+    __shared__ __attribute__((aligned(16))) float st0[256], st1[256]; // lse in log2 units, from 64 on delta; the rest again
 
     const attn_place at = attn_place_of(wg_id_x(), a.B * a.Hkv * a.nsplit, a.tps, a.deal);
     if (at.group < 0)
@@ -743,9 +746,6 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_cross_dkv_kernel(
     auto wait_loads = [] { __builtin_amdgcn_s_waitcnt(waitcnt_vm(0)); };
 
     for (int tile = uniform(at.tile); (int64_t)tile * ATTN_CROSS_KEYS < kr.n; tile += a.tps) {
-        const int key = tile * ATTN_CROSS_KEYS + 32 * w + l32;
-        const bool valid = key < kr.n, idle = tile * ATTN_CROSS_KEYS + 32 * w >= kr.n;
-        const int64_t tok = kr.at + (valid ? key : 0);
         // The wave's rows of K and V, by lane: what lies past the last state or past D is outside the buffer, zeros.
         bf16x8 kf[KN], vf[KN];
         {
@@ -758,7 +758,8 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_cross_dkv_kernel(
             for (int kk = 0; kk < KN; ++kk) {
                 const bool in = kk * 16 < D; // D % 16 == 0
                 kf[kk] = as_bf16x8(buf16<false>(rk, in ? ok + kk * 32 : 0x80000000u));
-                vf[kk] = as_bf16x8(buf16<false>(rv, in ? ov + kk * 32 : 0x80000000u));
+                if (DK)
+                    vf[kk] = as_bf16x8(buf16<false>(rv, in ? ov + kk * 32 : 0x80000000u));
             }
         }
         f32x16 dk[DP / 32], dv[DP / 32];
@@ -767,26 +768,26 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_cross_dkv_kernel(
             zero16(dk[db]);
             zero16(dv[db]);
         }
-        int lh = uniform(t0 / max(per_head, 1)), lt = t0 - lh * per_head; // the step to load: head and step of it
-        float st; // lse or delta of this thread's row of that step
-        auto load = [&](uint16_t *Qd, uint16_t *Gd) __attribute__((always_inline)) {
-            const int h = u * g + lh, r0 = lt * QT;
+        // The step to load: head and step of it. Behind the part's last step come empty ones: nothing is read, and P
+        // is 0, as it is past a head's last row: 2^(0 - inf). No branch goes around a step, and the two of a turn are
+        // one block: at a branch the allocator copied accumulators to and fro, or to memory.
+        int ls = t0, lh = uniform(t0 / max(per_head, 1)), lt = t0 - lh * per_head;
+        float st; // of one row of that step: lse (even waves) or delta
+        auto load = [&](uint16_t *to) __attribute__((always_inline)) {
+            const int h = u * g + lh, r0 = lt * QT, rows = ls < t1 ? min(qr.n - r0, QT) : 0;
             const int64_t first = qr.at + r0;
-            qs.load(a.q + first * a.q_tok + h * a.q_head, qr.n - r0, a.q_tok, D, Qd, w);
-            gs.load(a.go + first * a.go_tok + h * a.go_head, qr.n - r0, a.go_tok, D, Gd, w);
-            // Past the last row P is 0: 2^(0 - inf).
-            const int r = tid & (QT - 1);
-            st = tid < QT ? __builtin_inff() : 0.f;
-            if (tid < 2 * QT && r0 + r < qr.n)
-                st = tid < QT ? a.lse[(first + r) * a.Hq + h] * kLog2e : a.delta[(first + r) * a.Hq + h];
-            if (++lt == per_head) {
+            qs.load(a.q + first * a.q_tok + h * a.q_head, rows, a.q_tok, D, to, w);
+            gs.load(a.go + first * a.go_tok + h * a.go_head, rows, a.go_tok, D, to + GO, w);
+            const int r = opaque(lane) & (QT - 1);
+            const float *src = (w & 1 ? a.delta : a.lse) + first * a.Hq + h;
+            const float x = src[max(min(r, rows - 1), 0) * a.Hq];
+            st = w & 1 ? x : r < rows ? x * kLog2e : __builtin_inff();
+            if (++ls < t1 && ++lt == per_head) { // the last step's place stays: the empty ones name it
                 lt = 0;
                 ++lh;
             }
         };
-        auto compute = [&](const uint16_t *Qb, const uint16_t *Gb, const float *sb) __attribute__((always_inline)) {
-            if (idle)
-                return;
+        auto compute = [&](const uint16_t *qg, const float *sb) __attribute__((always_inline)) {
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
                 f32x16 s, dp;
@@ -794,15 +795,26 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_cross_dkv_kernel(
                 zero16(dp);
 #pragma unroll
                 for (int kk = 0; kk < KN; ++kk)
-                    s = mfma32(ln.nat(Qb, t, kk), kf[kk], s);
+                    s = mfma32(ln.nat(qg, t, kk), kf[kk], s);
 #pragma unroll
-                for (int kk = 0; kk < KN; ++kk)
-                    dp = mfma32(ln.nat(Gb, t, kk), vf[kk], dp);
+                for (int kk = 0; DK && kk < KN; ++kk)
+                    dp = mfma32(ln.nat(qg + GO, t, kk), vf[kk], dp);
+                if constexpr (DP > 64) { // three operands on their way: more, and registers spill
+                    constexpr int N = DK ? 2 * KN : KN;
+                    __builtin_amdgcn_sched_group_barrier(0x100, 3, 0);
+#pragma unroll
+                    for (int x = 0; x < N - 3; ++x) {
+                        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+                    }
+                    __builtin_amdgcn_sched_group_barrier(0x008, 3, 0);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
                 bf16x8 pk[2], dk8[2];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const f32x4 l = *reinterpret_cast<const f32x4 *>(sb + 32 * t + 8 * j + 4 * hi);
-                    const f32x4 e = *reinterpret_cast<const f32x4 *>(sb + QT + 32 * t + 8 * j + 4 * hi);
+                    const f32x4 e = *reinterpret_cast<const f32x4 *>(sb + 64 + 32 * t + 8 * j + 4 * hi);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const float p = fast_exp2(fmaf(s[4 * j + i], a.c, -l[i]));
@@ -814,41 +826,46 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_cross_dkv_kernel(
                 for (int cc = 0; cc < 2; ++cc)
 #pragma unroll
                     for (int db = 0; db < DP / 32; ++db) {
-                        dv[db] = mfma32(ln.tr(Gb, 2 * t + cc, db), pk[cc], dv[db]);
-                        dk[db] = mfma32(ln.tr(Qb, 2 * t + cc, db), dk8[cc], dk[db]);
+                        if (DV)
+                            dv[db] = mfma32(ln.tr(qg + GO, 2 * t + cc, db), pk[cc], dv[db]);
+                        if (DK)
+                            dk[db] = mfma32(ln.tr(qg, 2 * t + cc, db), dk8[cc], dk[db]);
                     }
             }
         };
         if (t0 < t1) {
-            load(Qs0, Gs0);
-            if (tid < 2 * QT)
-                st0[tid] = st;
-        }
-        wait_loads();
-        __syncthreads();
-        auto step = [&](int i, const uint16_t *Qb, const uint16_t *Gb, const float *sb, uint16_t *Qn, uint16_t *Gn,
-                        float *sn) __attribute__((always_inline)) {
-            if (i + 1 < t1)
-                load(Qn, Gn);
-            compute(Qb, Gb, sb);
+            load(QG0);
+            st0[tid] = st;
             wait_loads();
-            if (i + 1 < t1 && tid < 2 * QT)
-                sn[tid] = st;
             __syncthreads();
-        };
-        for (int i = t0; i < t1; i += 2) {
-            step(i, Qs0, Gs0, st0, Qs1, Gs1, st1);
-            if (i + 1 < t1)
-                step(i + 1, Qs1, Gs1, st1, Qs0, Gs0, st0);
+            auto step = [&](const uint16_t *qg, const float *sb, uint16_t *next, float *sn)
+                __attribute__((always_inline)) {
+                load(next);
+                compute(qg, sb);
+                wait_loads();
+                sn[tid] = st;
+                __syncthreads();
+            };
+            for (int i = t0; i < t1; i += 2) {
+                step(QG0, st0, QG1, st1);
+                step(QG1, st1, QG0, st0);
+            }
         }
-        if (valid) {
+        // Taken from the lane anew, so that nothing of it is held through the loop.
+        const int ln2 = opaque(lane), hi2 = ln2 >> 5, key = tile * ATTN_CROSS_KEYS + 32 * w + (ln2 & 31);
+        const int64_t tok = kr.at + key;
+        if (key < kr.n) {
             if (cut.live == 1) {
-                put_row<DP>(dk, a.scale, a.dk + tok * a.dk_tok + u * a.dk_head, hi, D);
-                put_row<DP>(dv, 1.f, a.dv + tok * a.dv_tok + u * a.dv_head, hi, D);
+                if (DK)
+                    put_row<DP>(dk, a.scale, a.dk + tok * a.dk_tok + u * a.dk_head, hi2, D);
+                if (DV)
+                    put_row<DP>(dv, 1.f, a.dv + tok * a.dv_tok + u * a.dv_head, hi2, D);
             } else {
                 float *dst = a.pacc + ((tok * a.Hkv + u) * a.nsplit + sp) * 2 * D;
-                put_part<DP>(dk, dst, hi, D);
-                put_part<DP>(dv, dst + D, hi, D);
+                if (DK)
+                    put_part<DP>(dk, dst, hi2, D);
+                if (DV)
+                    put_part<DP>(dv, dst + D, hi2, D);
             }
         }
     }
@@ -981,14 +998,22 @@ extern "C" int attn_hip_launch_cross_grad(const struct attn_cross_args *ap, cons
     const hipError_t e = with_width(a.D, [&](auto W) {
         constexpr int DP = decltype(W)::value;
         if (t_plan) {
-            plan_note(grid, block, "attn_cross_%s_kernel<%d> parts=%d share=%d", kv ? "dkv" : "dq", DP, a.nsplit,
-                      a.share);
+            for (int i = 0; i < (kv && DP > 128 ? 2 : 1); ++i)
+                plan_note(grid, block, "attn_cross_%s_kernel<%d%s> parts=%d share=%d", kv ? "dkv" : "dq", DP,
+                          !kv ? "" : DP <= 128 ? ", true, true" : i ? ", false, true" : ", true, false", a.nsplit, a.share);
             return hipSuccess;
         }
-        if (kv)
-            hipLaunchKernelGGL((attn_cross_dkv_kernel<DP>), grid, block, 0, st, a);
-        else
+        if (!kv) {
             hipLaunchKernelGGL((attn_cross_dq_kernel<DP>), grid, block, 0, st, a);
+        } else if constexpr (DP <= 128) {
+            hipLaunchKernelGGL((attn_cross_dkv_kernel<DP, true, true>), grid, block, 0, st, a);
+        } else {
+            hipLaunchKernelGGL((attn_cross_dkv_kernel<DP, true, false>), grid, block, 0, st, a);
+            const hipError_t x = hipGetLastError();
+            if (x != hipSuccess)
+                return x;
+            hipLaunchKernelGGL((attn_cross_dkv_kernel<DP, false, true>), grid, block, 0, st, a);
+        }
         return hipGetLastError();
     });
     if (e != hipSuccess || a.nsplit == 1)
