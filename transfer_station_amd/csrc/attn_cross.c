@@ -61,8 +61,8 @@ static void cross_check_call(const char *who, const struct attn_cross_call *c) {
     if (!(c->scale == 0.f || (c->scale >= 1e-6f && c->scale <= 1e6f)))
         cross_fail(who, "scale must be 0 (1/sqrt(D)) or in [1e-6, 1e6]");
     if ((int64_t)c->B * c->Hkv * ((int64_t)bound_of(&c->q) * (c->Hq / c->Hkv) / 16 + 8) > 1 << 30 ||
-        (int64_t)c->B * c->Hkv * ((int64_t)bound_of(&c->k) / ATTN_CROSS_KEYS + 8) > 1 << 30)
-        cross_fail(who, "B, the heads and max ask for too many tiles");
+        (int64_t)c->B * c->Hkv * ((int64_t)c->k.T / ATTN_CROSS_KEYS + 8) > 1 << 30)
+        cross_fail(who, "B, the heads, q.max and k.T ask for too many tiles");
 }
 
 static void cross_check_rows(const char *who, const char *what, const struct attn_rows *r, int D) {
@@ -98,23 +98,49 @@ static struct attn_cross_cut cross_cut(int64_t groups, int tps, int64_t total, i
     n = n < ATTN_CROSS_MAX_PARTS ? n : ATTN_CROSS_MAX_PARTS;
     n = n < 2 ? 1 : n;
     cut.share = (int)(ceil_div(ceil_div(total, n), step) * step);
-    cut.nsplit = (int)n;
+    cut.nsplit = cut.parts = (int)n;
     cut.tps = tps;
     cut.deal = deal_of(groups * n, tps);
     cut.grid = (long)attn_place_grid(groups * n, tps, cut.deal);
     return cut;
 }
 
-static struct attn_cross_cut forward_cut(const struct attn_cross_call *c) {
-    const int64_t R = (int64_t)bound_of(&c->q) * (c->Hq / c->Hkv), groups = (int64_t)c->B * c->Hkv;
-    const int64_t slots = ATTN_SLOTS / ((int64_t)c->q.T * c->Hq);
-    const int rows16 = R <= 16 ? 1 : R <= 32 ? (c->D <= 128 ? 2 : 1) : 0;
-    const int rows = rows16 ? 16 * rows16 : ATTN_CROSS_ROWS;
-    struct attn_cross_cut cut =
-        cross_cut(groups, (int)ceil_div(R, rows), bound_of(&c->k), rows16 ? 128 : 256, rows16 ? 2048 : 512, slots,
-                  ATTN_CROSS_KEY_STEP);
-    cut.rows16 = rows16;
+/* Few rows of a kv head (up to 32: single tokens, beams) have a kernel of their own, and its workgroups equal shares of
+ * all sequences' states (attn_quota), whatever sequences they cut, where there is enough to share: a merge costs 4 us.
+ * Measured, whole sequences -> shares (of 256 workgroups; with 512 they were slower): 64 sequences of up to 8192 states,
+ * 8 kv heads, D = 128, 306 -> 268 us; 16 inputs' beams over up to 1500 states, 16 heads, D = 64, 22 -> 27.
+ * Four kv heads in a workgroup, a wave each, read 1 KB of neighbouring heads of a row at a time, not 256 bytes. Against four
+ * waves per head: the 64 sequences 268 -> 237, 32 of 4096 at D = 256 175 -> 167; one sequence of 32768 states, whose waves
+ * then have four times the parts, 31 -> 48, the beams 22 -> 25. */
+static struct attn_cross_cut rows_cut(const struct attn_cross_call *c, int64_t R, int64_t slots) {
+    struct attn_cross_cut cut;
+    memset(&cut, 0, sizeof cut);
+    const int64_t groups = (int64_t)c->B * c->Hkv, keys = bound_of(&c->k), bytes = groups * keys * c->D * 4;
+    cut.rows16 = R > 16 && c->D <= 128 ? 2 : 1;
+    cut.quads = c->Hkv % 4 == 0 && bytes >= ATTN_CROSS_TEAMS * (2L << 20);
+    cut.tps = (int)ceil_div(R, 16 * cut.rows16);
+    cut.nsplit = (int)(slots < ATTN_CROSS_MAX_PARTS ? slots : ATTN_CROSS_MAX_PARTS);
+    cut.deal = cut.share = 1;
+    const int64_t lines = groups / (cut.quads ? 4 : 1), units = ceil_div(keys, 128) * lines;
+    int64_t teams = ceil_div(ATTN_CROSS_TEAMS, cut.tps);
+    teams = teams < units ? teams : units;
+    if (cut.nsplit < 2 || teams < 2 || (lines * cut.tps >= ATTN_CROSS_TEAMS && bytes < ATTN_CROSS_TEAMS * (1L << 20))) {
+        cut.nsplit = 1;
+        teams = 0;
+    }
+    cut.teams = (int)teams;
+    cut.parts = (int)(teams ? ceil_div(teams, lines) + 1 : 1);
+    cut.grid = (long)((teams ? teams : lines) * cut.tps);
     return cut;
+}
+
+static struct attn_cross_cut forward_cut(const struct attn_cross_call *c) {
+    const int64_t R = (int64_t)bound_of(&c->q) * (c->Hq / c->Hkv);
+    const int64_t slots = ATTN_SLOTS / ((int64_t)c->q.T * c->Hq);
+    if (R <= 32)
+        return rows_cut(c, R, slots);
+    return cross_cut((int64_t)c->B * c->Hkv, (int)ceil_div(R, ATTN_CROSS_ROWS), bound_of(&c->k), 256, 512, slots,
+                     ATTN_CROSS_KEY_STEP);
 }
 
 static struct attn_cross_cut dq_cut(const struct attn_cross_call *c) {
@@ -124,7 +150,7 @@ static struct attn_cross_cut dq_cut(const struct attn_cross_call *c) {
 }
 
 static struct attn_cross_cut dkv_cut(const struct attn_cross_call *c) {
-    const int64_t steps = ceil_div(bound_of(&c->q), attn_cross_step_rows(c->D)) * (c->Hq / c->Hkv);
+    const int64_t steps = ceil_div(bound_of(&c->q), ATTN_CROSS_STEP) * (c->Hq / c->Hkv);
     return cross_cut((int64_t)c->B * c->Hkv, (int)ceil_div(bound_of(&c->k), ATTN_CROSS_KEYS), steps, 2,
                      c->D <= 128 ? 512 : 256, ATTN_CROSS_GRAD_FLOATS / ((int64_t)c->k.T * c->Hkv * c->D * 2), 1);
 }
@@ -155,12 +181,17 @@ static struct attn_cross_args cross_args(const struct attn_cross_call *c) {
     a.q_is_len = c->q.len != NULL, a.k_is_len = c->k.len != NULL;
     a.q_second = c->q.len ? c->q.len : c->q.start + 1;
     a.k_second = c->k.len ? c->k.len : c->k.start + 1;
-    a.B = c->B, a.Tq = c->q.T, a.Tk = c->k.T, a.Hq = c->Hq, a.Hkv = c->Hkv, a.D = c->D;
+    a.B = c->B, a.Tq = c->q.T, a.Tk = c->k.T, a.Hq = c->Hq, a.Hkv = c->Hkv, a.g = c->Hq / c->Hkv, a.D = c->D;
     return a;
 }
 
 static void set_cut(struct attn_cross_args *a, const struct attn_cross_cut *cut) {
     a->tps = cut->tps, a->nsplit = cut->nsplit, a->share = cut->share, a->deal = cut->deal;
+    a->tpp = (cut->tps + cut->deal - 1) / cut->deal;
+    a->by_tpp = attn_div_of(a->tpp), a->by_deal = attn_div_of(cut->deal);
+    a->by_nsplit = attn_div_of(cut->nsplit), a->by_heads = attn_div_of(a->Hkv), a->by_hq = attn_div_of(a->Hq), a->by_g = attn_div_of(a->g);
+    a->teams = cut->teams, a->wgs = (int)cut->grid, a->Hkv_wg = cut->quads ? a->Hkv / 4 : a->Hkv;
+    a->by_tps = attn_div_of(a->tps), a->by_B = attn_div_of(a->B), a->by_gwg = attn_div_of(a->Hq / a->Hkv_wg);
 }
 
 static void cross_run(const char *who, const struct attn_cross_call *c, const struct attn_rows *q,

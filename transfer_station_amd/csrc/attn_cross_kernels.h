@@ -19,6 +19,7 @@
 #include "attn_cross_rule.h"
 #include "attn_device.h"
 #include "attn_launch.h"
+#include "attn_line.h"
 
 namespace {
 
@@ -34,6 +35,8 @@ __device__ __forceinline__ attn_range k_rows(const attn_cross_args &a, int b) {
 }
 
 __device__ __forceinline__ attn_cut part_of(int total, int share, int nsplit, int step) {
+    if (nsplit == 1) // no divisions
+        return attn_cut{1, max(total, 1)};
     const attn_cut c = attn_cut_of(total, share, nsplit, step);
     return attn_cut{uniform(c.live), uniform(c.per)};
 }
@@ -140,7 +143,7 @@ template <int DP> __device__ __forceinline__ void put_part(const f32x16 *o, floa
 }
 
 // Keys of a tile, by the tile's width: two tiles of K and V in two buffers are 64 KB.
-constexpr int cross_tile_keys(int DP) { return DP == 64 ? 128 : DP == 128 ? 64 : 32; }
+constexpr int cross_tile_keys(int DP) { return DP <= 128 ? 64 : 32; }
 // A lane's sum of p over a tile up to which the running maximum may lie below the tile's.
 constexpr float kCrossSum = 65536.0f;
 
@@ -151,25 +154,24 @@ constexpr float kCrossSum = 65536.0f;
 //   S^T[key][row] = K . Q^T, O^T[d][row] += V^T . P^T   (v_mfma_f32_32x32x16_bf16)
 // The running maximum is raised only where a lane's sum of p over a tile passes kCrossSum.
 // ------------------------------------------------------------------------------------------
-template <int DP> __global__ __launch_bounds__(256, 2) void attn_cross_kernel(const attn_cross_args a) {
+template <int DP> __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void attn_cross_kernel(const attn_cross_args a) {
     constexpr int KT = cross_tile_keys(DP), KN = DP / 16, NT = KT / 32;
     // K's tile and V's behind it. Each buffer is a variable of its own: the compiler tells LDS accesses apart by
     // variable, and needs address registers for each.
     constexpr int VO = KT * DP;
     __shared__ __attribute__((aligned(1024))) uint16_t KV0[2 * VO], KV1[2 * VO];
 
-    const attn_place at = attn_place_of(wg_id_x(), a.B * a.Hkv * a.nsplit, a.tps, a.deal);
-    if (at.group < 0)
+    const attn_cross_place at = attn_cross_place_of(&a, wg_id_x());
+    if (at.b < 0)
         return;
-    const int sp = uniform(at.group / (a.B * a.Hkv)), bu = at.group - sp * (a.B * a.Hkv);
-    const int u = uniform(bu % a.Hkv), b = uniform(bu / a.Hkv);
+    const int b = at.b, u = at.u, sp = at.sp;
     const int tid = wi_id_x(), w = uniform(tid >> 6), lane = tid & 63, l32 = lane & 31, hi = lane >> 5;
     const attn_range qr = q_rows(a, b), kr = k_rows(a, b);
     const attn_cut cut = part_of(kr.n, a.share, a.nsplit, ATTN_CROSS_KEY_STEP);
     if (sp >= cut.live)
         return;
     const int k0 = min(sp * cut.per, kr.n), k1 = min(k0 + cut.per, kr.n);
-    const int g = a.Hq / a.Hkv, R = qr.n * g, D = a.D;
+    const int g = a.g, R = qr.n * g, D = a.D;
     const uint16_t *kp = a.k + kr.at * a.k_tok + u * a.k_head, *vp = a.v + kr.at * a.v_tok + u * a.v_head;
     const cross_lane<DP> ln(lane);
     cross_stage<DP, KT> ks, vs;
@@ -181,10 +183,10 @@ template <int DP> __global__ __launch_bounds__(256, 2) void attn_cross_kernel(co
     };
     auto wait_loads = [] { __builtin_amdgcn_s_waitcnt(waitcnt_vm(0)); };
 
-    for (int tile = uniform(at.tile); (int64_t)tile * ATTN_CROSS_ROWS < R; tile += a.tps) {
+    for (int tile = at.tile; (int64_t)tile * ATTN_CROSS_ROWS < R; tile += a.tps) {
         const int row = tile * ATTN_CROSS_ROWS + 32 * w + l32;
         const bool valid = row < R;
-        const int tok = valid ? row / g : 0, h = u * g + (valid ? row % g : 0);
+        const int tok = valid ? attn_div_by(row, a.by_g) : 0, h = u * g + (valid ? row - tok * g : 0);
         const uint16_t *q = a.q + (qr.at + tok) * a.q_tok + h * a.q_head; // without a row of its own: the first one's
         const bool idle = tile * ATTN_CROSS_ROWS + 32 * w >= R;           // the wave has no rows
         bf16x8 qb[KN];
@@ -306,280 +308,380 @@ template <int DP> __global__ __launch_bounds__(256, 2) void attn_cross_kernel(co
 }
 
 // ------------------------------------------------------------------------------------------
+// The decode line's units of a call (attn_line.h).
+struct cross_units {
+    static __device__ __forceinline__ int at(const attn_cross_args &a, int i) {
+        if (i >= a.B)
+            return 0;
+        const attn_range q = attn_range_of(a.q_start[i], a.q_second[i], a.q_is_len, a.Tq);
+        return attn_units(q.n, attn_range_of(a.k_start[i], a.k_second[i], a.k_is_len, a.Tk).n);
+    }
+    static __device__ __forceinline__ int one(const attn_cross_args &a) {
+        return attn_units(q_rows(a, 0).n, k_rows(a, 0).n);
+    }
+    static __device__ __forceinline__ int heads(const attn_cross_args &a) { return a.Hkv_wg; }
+};
+
 // Forward, few rows per kv head (single tokens, beams): a workgroup of four waves takes 16 NRB rows over a part of the
 // states, the waves interleaved tiles of 32 states, each with a softmax of its own:
 //   S^T[key][row] = K . Q^T   (v_mfma_f32_16x16x32_bf16, K from memory straight into the operand)
 //   O^T[d][row]  += V^T . P^T (V through a wave-private LDS tile and the transposed read)
 // and joins them in LDS. Bound by HBM. NTL: K and V are read once, past the L2.
 // ------------------------------------------------------------------------------------------
-template <int DP, int NRB, bool NTL>
+template <int DP, int NRB, bool NTL, int NW>
 __global__ __launch_bounds__(256, 2) void attn_cross_rows_kernel(const attn_cross_args a) {
     constexpr int VSTR = DP + 16; // elements of a V row in LDS: the eight rows of a pass on other banks
     constexpr int KN = DP / 32, NV = DP / 16, VTILE = 32 * VSTR;
-    // K and V of a tile, Q and O do not fit 256 registers at DP = 256: there K is loaded at the tile's start, and V
-    // once the scores have freed K's registers.
+    // K and V of a tile, Q and O do not fit 256 registers at DP = 256: there V is loaded once the scores have freed K's
+    // registers, and the next K once V is in LDS. (Left to itself the compiler asked for K one operand at a time.)
     constexpr bool kLate = DP == 256;
     __shared__ __attribute__((aligned(16))) uint16_t Vw[4 * VTILE];
     __shared__ float red_m[NRB][4][16], red_l[NRB][4][16];
-    static_assert(4 * 16 * (DP + 4) * 4 <= 4 * VTILE * 2, "the area for joining must fit in the V tiles");
+    static_assert(16 * (DP + 4) * 4 <= VTILE * 2, "the area for joining must fit in the V tiles");
 
     const int tid = wi_id_x(), w = uniform(tid >> 6), lane = tid & 63;
     const int r16 = lane & 15, grp = lane >> 4;
-    const attn_place at = attn_place_of(wg_id_x(), a.B * a.Hkv * a.nsplit, a.tps, a.deal);
-    if (at.group < 0)
-        return;
-    const int bu = uniform(at.group / a.nsplit), sp = at.group - bu * a.nsplit;
-    const int b = uniform(bu / a.Hkv), u = bu - b * a.Hkv;
-    const attn_range qr = q_rows(a, b), kr = k_rows(a, b);
-    const attn_cut cut = part_of(kr.n, a.share, a.nsplit, ATTN_CROSS_KEY_STEP);
-    if (sp >= cut.live)
-        return;
-    const int k0 = min(sp * cut.per, kr.n), k1 = min(k0 + cut.per, kr.n);
-    const int g = a.Hq / a.Hkv, R = qr.n * g, D = a.D;
+    const int team = w / NW, wk = w % NW; // of the workgroup's kv heads, and of that one's waves
+    const int g = a.g, D = a.D;
     const float c = a.c, lift = 8.f / c; // how far a score may pass the running maximum
-    const uint16_t *kp = a.k + kr.at * a.k_tok + u * a.k_head, *vp = a.v + kr.at * a.v_tok + u * a.v_head;
+    // This workgroup's row tile t0 and its place on the line: sequence b, group ug of kv heads, first unit `off` of the
+    // sequence, `left` units in all. Neighbouring workgroups share an XCD.
+    const int L = uniform(xcd_remap(wg_id_x(), a.wgs));
+    const int at = attn_div_by(L, a.by_tps), t0 = L - at * a.tps;
+    int ug, b, off = 0, left = 1, pos0 = 0;
+    line ln = {0, 1, 0, 0};
+    if (a.teams) {
+        ln = line_at<cross_units>(a, lane);
+        if ((int64_t)at * ln.quota >= (int64_t)ln.total * a.Hkv_wg)
+            return;
+        pos0 = at * ln.quota;
+        left = min(ln.quota, ln.total * a.Hkv_wg - pos0);
+        ug = uniform(pos0 / ln.total);
+        int before;
+        b = uniform(seq_of_unit<cross_units>(a, ln, lane, pos0 - ug * ln.total, before));
+        off = pos0 - ug * ln.total - before;
+    } else {
+        ug = attn_div_by(at, a.by_B);
+        b = at - ug * a.B;
+    }
     const uint32_t kb2 = (uint32_t)(a.k_tok * 2), vb2 = (uint32_t)(a.v_tok * 2); // bytes from row to row
     uint16_t *vt = &Vw[w * VTILE];
     const uint32_t koff = grp * 8 < D ? r16 * kb2 + grp * 16 : 0x80000000u;
     const uint32_t voff = (lane % (DP / 8)) * 8 < D ? (lane / (DP / 8)) * vb2 + (lane % (DP / 8)) * 16 : 0x80000000u;
 
-    for (int tile = uniform(at.tile); (int64_t)tile * 16 * NRB < R; tile += a.tps) {
-        const int row0 = tile * 16 * NRB;
-        bf16x8 qb[NRB][KN];
-        float m_run[NRB], l_run[NRB];
-        f32x4 o[NRB][DP / 16];
-#pragma unroll
-        for (int i = 0; i < NRB; ++i) {
-            const int row = row0 + 16 * i + r16;
-            const bool valid = row < R;
-            const int tok = valid ? row / g : 0, h = u * g + (valid ? row % g : 0);
-            const uint16_t *q = a.q + (qr.at + tok) * a.q_tok + h * a.q_head;
-#pragma unroll
-            for (int kk = 0; kk < KN; ++kk) {
-                const int col = kk * 32 + grp * 8;
-                u32x4 x = zero4();
-                if (valid && col < D)
-                    x = *reinterpret_cast<const u32x4 *>(q + col);
-                qb[i][kk] = as_bf16x8(x);
-            }
-            m_run[i] = kNegInf;
-            l_run[i] = 0.f;
-#pragma unroll
-            for (int db = 0; db < DP / 16; ++db)
-                o[i][db] = f32x4{0.f, 0.f, 0.f, 0.f};
+    while (left > 0 && ug < a.Hkv_wg) {
+        const attn_range qr = q_rows(a, b), kr = k_rows(a, b);
+        const int u = ug * (4 / NW) + team, R = qr.n * g, units = attn_units(qr.n, kr.n);
+        const int take = a.teams ? min(left, units - off) : 1;
+        attn_cover cover = {0, 1};
+        if (a.teams) {
+            cover = attn_cover_of(pos0 - off, max(units, 1), ln.quota);
+            cover = attn_cover{uniform(cover.first), uniform(cover.live)};
         }
-        struct frags {
-            u32x4 k[2 * KN], v[NV];
-        };
-        // Rows past the part's end, or tiles behind it, lie outside the buffer: nothing is read, zeros arrive.
-        auto bytes = [&](int tb, uint32_t step) __attribute__((always_inline)) {
-            const int n = min(k1 - tb, 32);
-            return n > 0 ? (uint32_t)(n - 1) * step + D * 2 : 0u;
-        };
-        auto load_k = [&](int tb, frags &f) __attribute__((always_inline)) {
-            const auto r = make_rsrc(kp + (int64_t)min(tb, k1) * a.k_tok, bytes(tb, kb2));
+        const int live = cover.live, sp = at - cover.first;
+        const int k0 = min(off * 128, kr.n), k1 = a.teams ? min((off + take) * 128, kr.n) : kr.n;
+        const uint16_t *kp = a.k + kr.at * a.k_tok + u * a.k_head, *vp = a.v + kr.at * a.v_tok + u * a.v_head;
+        for (int tile = t0; take > 0 && (int64_t)tile * 16 * NRB < R; tile += a.tps) {
+            const int row0 = tile * 16 * NRB;
+            bf16x8 qb[NRB][KN];
+            float m_run[NRB], l_run[NRB];
+            f32x4 o[NRB][DP / 16];
 #pragma unroll
-            for (int t = 0; t < 2; ++t)
+            for (int i = 0; i < NRB; ++i) {
+                const int row = row0 + 16 * i + r16;
+                const bool valid = row < R;
+                const int tok = valid ? attn_div_by(row, a.by_g) : 0, h = u * g + (valid ? row - tok * g : 0);
+                const uint16_t *q = a.q + (qr.at + tok) * a.q_tok + h * a.q_head;
 #pragma unroll
-                for (int kk = 0; kk < KN; ++kk)
-                    f.k[t * KN + kk] =
-                        buf16<NTL>(r, kk * 32 + grp * 8 < D ? koff + 16 * t * kb2 + kk * 64 : 0x80000000u);
-        };
-        auto load_v = [&](int tb, frags &f) __attribute__((always_inline)) {
-            const auto r = make_rsrc(vp + (int64_t)min(tb, k1) * a.v_tok, bytes(tb, vb2));
+                for (int kk = 0; kk < KN; ++kk) {
+                    const int col = kk * 32 + grp * 8;
+                    u32x4 x = zero4();
+                    if (valid && col < D)
+                        x = *reinterpret_cast<const u32x4 *>(q + col);
+                    qb[i][kk] = as_bf16x8(x);
+                }
+                m_run[i] = kNegInf;
+                l_run[i] = 0.f;
 #pragma unroll
-            for (int i = 0; i < NV; ++i)
-                f.v[i] = buf16<NTL>(r, voff + i * (512 / DP) * vb2);
-        };
-        auto put_v = [&](const frags &f) __attribute__((always_inline)) {
-            lds_wave_fence(); // the previous tile's transposed reads are complete
-#pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                const int x = lane + 64 * i;
-                *reinterpret_cast<u32x4 *>(&vt[x / (DP / 8) * VSTR + x % (DP / 8) * 8]) = f.v[i];
+                for (int db = 0; db < DP / 16; ++db)
+                    o[i][db] = f32x4{0.f, 0.f, 0.f, 0.f};
             }
-        };
-        auto compute = [&](int tb, frags &f) __attribute__((always_inline)) {
-            bf16x8 pk[NRB];
-            f32x4 s[NRB][2];
+            struct frags {
+                u32x4 k[2 * KN], v[NV];
+            };
+            // Rows past the part's end, or tiles behind it, lie outside the buffer: nothing is read, zeros arrive.
+            auto bytes = [&](int tb, uint32_t step) __attribute__((always_inline)) {
+                const int n = min(k1 - tb, 32);
+                return n > 0 ? (uint32_t)(n - 1) * step + D * 2 : 0u;
+            };
+            auto load_k = [&](int tb, frags &f) __attribute__((always_inline)) {
+                const auto r = make_rsrc(kp + (int64_t)min(tb, k1) * a.k_tok, bytes(tb, kb2));
 #pragma unroll
-            for (int i = 0; i < NRB; ++i)
-#pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    s[i][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+                for (int t = 0; t < 2; ++t)
 #pragma unroll
                     for (int kk = 0; kk < KN; ++kk)
-                        s[i][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(f.k[t * KN + kk]), qb[i][kk],
-                                                                          s[i][t], 0, 0, 0);
+                        f.k[t * KN + kk] =
+                            buf16<NTL>(r, kk * 32 + grp * 8 < D ? koff + 16 * t * kb2 + kk * 64 : 0x80000000u);
+            };
+            auto load_v = [&](int tb, frags &f) __attribute__((always_inline)) {
+                const auto r = make_rsrc(vp + (int64_t)min(tb, k1) * a.v_tok, bytes(tb, vb2));
+#pragma unroll
+                for (int i = 0; i < NV; ++i)
+                    f.v[i] = buf16<NTL>(r, voff + i * (512 / DP) * vb2);
+            };
+            auto put_v = [&](const frags &f) __attribute__((always_inline)) {
+                lds_wave_fence(); // the previous tile's transposed reads are complete
+#pragma unroll
+                for (int i = 0; i < NV; ++i) {
+                    const int x = lane + 64 * i;
+                    *reinterpret_cast<u32x4 *>(&vt[x / (DP / 8) * VSTR + x % (DP / 8) * 8]) = f.v[i];
                 }
-            __builtin_amdgcn_sched_barrier(0);
-            if (kLate)
-                load_v(tb, f);
-            else
-                load_k(tb + 128, f);
-#pragma unroll
-            for (int i = 0; i < NRB; ++i) {
-                // Register (t, j) of this lane holds key tb + 16t + 4grp + j for row r16.
-                float mx = kNegInf;
-#pragma unroll
-                for (int t = 0; t < 2; ++t)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        if (tb + 16 * t + 4 * grp + j >= k1)
-                            s[i][t][j] = kNegInf;
-                        mx = fmaxf(mx, s[i][t][j]);
-                    }
-                mx = max_xor32(max_xor16(mx));
-                if (__builtin_amdgcn_ballot_w64(mx > m_run[i] + lift) != 0) {
-                    const float mnew = fmaxf(m_run[i], mx);
-                    const float alpha = rescale(m_run[i], mnew, c);
-                    m_run[i] = mnew;
-                    l_run[i] *= alpha;
-#pragma unroll
-                    for (int db = 0; db < DP / 16; ++db)
-                        o[i][db] *= alpha;
-                }
-                const float mc = m_run[i] == kNegInf ? 0.f : m_run[i] * c;
-                float psum = 0.f;
-#pragma unroll
-                for (int t = 0; t < 2; ++t)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const float p = fast_exp2(fmaf(s[i][t][j], c, -mc));
-                        psum += p;
-                        pk[i][4 * t + j] = (__bf16)p;
-                    }
-                l_run[i] += psum;
-            }
-            if (kLate)
-                put_v(f);
-            lds_wave_fence(); // this tile's V is in LDS before the transposed reads
-            const uint16_t *vrow = &vt[(4 * grp + (r16 >> 2)) * VSTR + 4 * (r16 & 3)];
-#pragma unroll
-            for (int db = 0; db < DP / 16; ++db) {
-                const bf16x8 x = join_tr(lds_read_tr(vrow + db * 16), lds_read_tr(vrow + db * 16 + 16 * VSTR));
+            };
+            auto compute = [&](int tb, frags &f) __attribute__((always_inline)) {
+                bf16x8 pk[NRB];
+                f32x4 s[NRB][2];
 #pragma unroll
                 for (int i = 0; i < NRB; ++i)
-                    o[i][db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, pk[i], o[i][db], 0, 0, 0);
-            }
-        };
-        int tb = k0 + 32 * w;
-        if (tb < k1) {
-            frags f;
-            if (!kLate) {
-                load_v(tb, f);
-                load_k(tb, f);
-            }
-            for (; tb < k1; tb += 128) {
-                if (kLate) {
-                    load_k(tb, f);
-                } else {
-                    put_v(f);
-                    __builtin_amdgcn_sched_barrier(0);
-                    load_v(tb + 128, f);
-                }
-                compute(tb, f);
-            }
-        }
 #pragma unroll
-        for (int i = 0; i < NRB; ++i)
-            l_run[i] = sum_xor32(sum_xor16(l_run[i]));
+                    for (int t = 0; t < 2; ++t) {
+                        s[i][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                        for (int kk = 0; kk < KN; ++kk)
+                            s[i][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(f.k[t * KN + kk]), qb[i][kk],
+                                                                              s[i][t], 0, 0, 0);
+                    }
+                __builtin_amdgcn_sched_barrier(0);
+                if (kLate)
+                    load_v(tb, f);
+                else
+                    load_k(tb + 32 * NW, f);
+#pragma unroll
+                for (int i = 0; i < NRB; ++i) {
+                    // Register (t, j) of this lane holds key tb + 16t + 4grp + j for row r16.
+                    float mx = kNegInf;
+#pragma unroll
+                    for (int t = 0; t < 2; ++t)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            if (tb + 16 * t + 4 * grp + j >= k1)
+                                s[i][t][j] = kNegInf;
+                            mx = fmaxf(mx, s[i][t][j]);
+                        }
+                    mx = max_xor32(max_xor16(mx));
+                    if (__builtin_amdgcn_ballot_w64(mx > m_run[i] + lift) != 0) {
+                        const float mnew = fmaxf(m_run[i], mx);
+                        const float alpha = rescale(m_run[i], mnew, c);
+                        m_run[i] = mnew;
+                        l_run[i] *= alpha;
+#pragma unroll
+                        for (int db = 0; db < DP / 16; ++db)
+                            o[i][db] *= alpha;
+                    }
+                    const float mc = m_run[i] == kNegInf ? 0.f : m_run[i] * c;
+                    float psum = 0.f;
+#pragma unroll
+                    for (int t = 0; t < 2; ++t)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const float p = fast_exp2(fmaf(s[i][t][j], c, -mc));
+                            psum += p;
+                            pk[i][4 * t + j] = (__bf16)p;
+                        }
+                    l_run[i] += psum;
+                }
+                if (kLate) {
+                    put_v(f);
+                    load_k(tb + 32 * NW, f);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                lds_wave_fence(); // this tile's V is in LDS before the transposed reads
+                const uint16_t *vrow = &vt[(4 * grp + (r16 >> 2)) * VSTR + 4 * (r16 & 3)];
+#pragma unroll
+                for (int db = 0; db < DP / 16; ++db) {
+                    const bf16x8 x = join_tr(lds_read_tr(vrow + db * 16), lds_read_tr(vrow + db * 16 + 16 * VSTR));
+#pragma unroll
+                    for (int i = 0; i < NRB; ++i)
+                        o[i][db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, pk[i], o[i][db], 0, 0, 0);
+                }
+            };
+            int tb = k0 + 32 * wk;
+            if (tb < k1) {
+                frags f;
+                if (!kLate)
+                    load_v(tb, f);
+                load_k(tb, f);
+                for (; tb < k1; tb += 32 * NW) {
+                    if (!kLate) {
+                        put_v(f);
+                        __builtin_amdgcn_sched_barrier(0);
+                        load_v(tb + 32 * NW, f);
+                    }
+                    compute(tb, f);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < NRB; ++i)
+                l_run[i] = sum_xor32(sum_xor16(l_run[i]));
 
-        // Join the waves: O^T register (db, j) of this lane holds d = 16db + 4grp + j of row r16.
-        float *om = reinterpret_cast<float *>(Vw); // [4][16][DP + 4]
-        if (grp == 0)
+            // Join the waves: O^T register (db, j) of this lane holds d = 16db + 4grp + j of row r16.
+            float *om = reinterpret_cast<float *>(Vw); // [NW][16][DP + 4]
+            if (grp == 0)
+#pragma unroll
+                for (int i = 0; i < NRB; ++i) {
+                    red_m[i][w][r16] = m_run[i] * c; // in log2 units; -inf stays
+                    red_l[i][w][r16] = l_run[i];
+                }
 #pragma unroll
             for (int i = 0; i < NRB; ++i) {
-                red_m[i][w][r16] = m_run[i] * c; // in log2 units; -inf stays
-                red_l[i][w][r16] = l_run[i];
-            }
+                __syncthreads();
 #pragma unroll
-        for (int i = 0; i < NRB; ++i) {
-            __syncthreads();
+                for (int db = 0; db < DP / 16; ++db)
+                    *reinterpret_cast<f32x4 *>(&om[(w * 16 + r16) * (DP + 4) + db * 16 + 4 * grp]) = o[i][db];
+                __syncthreads();
+                const int rowb = row0 + 16 * i, nrow = min(16, R - rowb);
+                for (int idx = tid - 64 * NW * team; idx < nrow * (DP / 4); idx += 64 * NW) {
+                    const int r = idx / (DP / 4), d = 4 * (idx % (DP / 4));
+                    if (d >= D)
+                        continue;
+                    float mx = kNegInf;
 #pragma unroll
-            for (int db = 0; db < DP / 16; ++db)
-                *reinterpret_cast<f32x4 *>(&om[(w * 16 + r16) * (DP + 4) + db * 16 + 4 * grp]) = o[i][db];
-            __syncthreads();
-            const int rowb = row0 + 16 * i, nrow = min(16, R - rowb);
-            for (int idx = tid; idx < nrow * (DP / 4); idx += 256) {
-                const int r = idx / (DP / 4), d = 4 * (idx % (DP / 4));
-                if (d >= D)
-                    continue;
-                float mx = kNegInf;
+                    for (int ww = 0; ww < NW; ++ww)
+                        mx = fmaxf(mx, red_m[i][NW * team + ww][r]);
+                    const float muse = mx == kNegInf ? 0.f : mx;
+                    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+                    float lsum = 0.f;
 #pragma unroll
-                for (int ww = 0; ww < 4; ++ww)
-                    mx = fmaxf(mx, red_m[i][ww][r]);
-                const float muse = mx == kNegInf ? 0.f : mx;
-                f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-                float lsum = 0.f;
+                    for (int ww = 0; ww < NW; ++ww) {
+                        const float wgt = fast_exp2(red_m[i][NW * team + ww][r] - muse);
+                        const f32x4 x = *reinterpret_cast<const f32x4 *>(&om[((NW * team + ww) * 16 + r) * (DP + 4) + d]);
 #pragma unroll
-                for (int ww = 0; ww < 4; ++ww) {
-                    const float wgt = fast_exp2(red_m[i][ww][r] - muse);
-                    const f32x4 x = *reinterpret_cast<const f32x4 *>(&om[(ww * 16 + r) * (DP + 4) + d]);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        acc[j] += wgt * x[j];
-                    lsum += wgt * red_l[i][ww][r];
-                }
-                const int64_t tok = qr.at + (rowb + r) / g;
-                const int h = u * g + (rowb + r) % g;
-                const int64_t slot = tok * a.Hq + h;
-                if (cut.live == 1) {
-                    const float inv = lsum > 0.f ? 1.0f / lsum : 0.f;
-                    *reinterpret_cast<u32x2 *>(a.o + tok * a.o_tok + h * a.o_head + d) =
-                        u32x2{bf16_pair(acc[0] * inv, acc[1] * inv), bf16_pair(acc[2] * inv, acc[3] * inv)};
-                    if (a.lse && d == 0)
-                        a.lse[slot] = lse_of(mx, lsum);
-                } else {
-                    if (d == 0) {
-                        a.pm[slot * a.nsplit + sp] = mx;
-                        a.pl[slot * a.nsplit + sp] = lsum;
+                        for (int j = 0; j < 4; ++j)
+                            acc[j] += wgt * x[j];
+                        lsum += wgt * red_l[i][NW * team + ww][r];
                     }
-                    *reinterpret_cast<f32x4 *>(a.pacc + (slot * a.nsplit + sp) * D + d) = acc;
+                    const int i_tok = attn_div_by(rowb + r, a.by_g), h = u * g + rowb + r - i_tok * g;
+                    const int64_t tok = qr.at + i_tok;
+                    const int64_t slot = tok * a.Hq + h;
+                    if (live == 1) {
+                        const float inv = lsum > 0.f ? 1.0f / lsum : 0.f;
+                        *reinterpret_cast<u32x2 *>(a.o + tok * a.o_tok + h * a.o_head + d) =
+                            u32x2{bf16_pair(acc[0] * inv, acc[1] * inv), bf16_pair(acc[2] * inv, acc[3] * inv)};
+                        if (a.lse && d == 0)
+                            a.lse[slot] = lse_of(mx, lsum);
+                    } else {
+                        if (d == 0) {
+                            a.pm[slot * a.nsplit + sp] = mx;
+                            a.pl[slot * a.nsplit + sp] = lsum;
+                        }
+                        *reinterpret_cast<f32x4 *>(a.pacc + (slot * a.nsplit + sp) * D + d) = acc;
+                    }
                 }
             }
+            __syncthreads(); // the area for joining is V tiles again
         }
-        __syncthreads(); // the area for joining is V tiles again
+        left -= take;
+        pos0 += take;
+        off = 0;
+        if (++b == a.B) {
+            b = 0;
+            ++ug;
+        }
     }
 }
 
-// Joins the parts of each row: w_s = 2^(m_s - max m), O = sum w_s acc_s / sum w_s l_s, lse = log2-sum of both. A
-// workgroup takes 256 / LP rows of one sequence at a time, LP = 2^lglp lanes of four columns each.
+// Joins the parts of each row: w_s = 2^(m_s - max m), O = sum w_s acc_s / sum w_s l_s, lse the logarithm of the sum. A
+// workgroup takes 256 / (LP SG) rows of one sequence at a time: LP = 2^lglp lanes of four columns each, SG groups of
+// parts. What bounds it is latency: NP parts of a thread are asked for at once.
+template <int NP, int SG>
 __global__ __launch_bounds__(256) void attn_cross_merge_kernel(const attn_cross_args a, int lglp, int tpm) {
+    __shared__ __attribute__((aligned(16))) f32x4 accs[SG > 1 ? 256 : 1];
+    __shared__ float ms[SG > 1 ? 256 : 1], ls[SG > 1 ? 256 : 1];
     const int b = uniform(wg_id_x() / tpm), t0 = wg_id_x() - b * tpm, tid = wi_id_x();
     const attn_range qr = q_rows(a, b), kr = k_rows(a, b);
-    const attn_cut cut = part_of(kr.n, a.share, a.nsplit, ATTN_CROSS_KEY_STEP);
-    if (cut.live == 1)
-        return; // written already
-    const int64_t R = (int64_t)qr.n * a.Hq;
-    const int rpw = 256 >> lglp, d = 4 * (tid & ((1 << lglp) - 1));
-    for (int64_t row = (int64_t)t0 * rpw + (tid >> lglp); row < R; row += (int64_t)tpm * rpw) {
-        const int64_t slot = (int64_t)qr.at * a.Hq + row;
+    // The parts of a row: its sequence's, or those that the line's quotas make of it, which differ by the kv heads.
+    int parts = 1, units = 1, before = 0;
+    line ln = {0, 1, 0, 0};
+    if (a.teams) {
+        ln = line_at<cross_units>(a, tid & 63);
+        before = units_before<cross_units>(a, ln, tid & 63, b);
+        units = max(attn_units(qr.n, kr.n), 1);
+    } else {
+        parts = part_of(kr.n, a.share, a.nsplit, ATTN_CROSS_KEY_STEP).live;
+        if (parts == 1)
+            return; // written already
+    }
+    constexpr int kLgSG = SG == 1 ? 0 : 2;
+    static_assert(1 << kLgSG == SG, "");
+    const int R = qr.n * a.Hq, rpw = 256 >> (lglp + kLgSG), d = 4 * (tid & ((1 << lglp) - 1));
+    const int rl = tid >> (lglp + kLgSG), sg = tid >> lglp & (SG - 1);
+    for (int r0 = t0 * rpw; r0 < R; r0 += tpm * rpw) {
+        const int row = r0 + rl, i_tok = attn_div_by(min(row, R - 1), a.by_hq), h = min(row, R - 1) - i_tok * a.Hq;
+        const int64_t slot = (int64_t)qr.at * a.Hq + min(row, R - 1);
+        if (a.teams)
+            parts = attn_cover_of(attn_div_by(h, a.by_gwg) * ln.total + before, units, ln.quota).live;
         const float *pm = a.pm + slot * a.nsplit, *pl = a.pl + slot * a.nsplit;
         const float *p = a.pacc + slot * a.nsplit * a.D + min(d, a.D - 4);
-        float mx = kNegInf;
-        for (int s = 0; s < cut.live; ++s)
-            mx = fmaxf(mx, pm[s]);
-        const float muse = mx == kNegInf ? 0.f : mx;
+        float mx = kNegInf, sum = 0.f;
         f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-        float sum = 0.f;
-#pragma unroll 4
-        for (int s = 0; s < cut.live; ++s) {
-            const float wgt = fast_exp2(pm[s] - muse);
-            const f32x4 x = *reinterpret_cast<const f32x4 *>(p + (int64_t)s * a.D);
-            sum += wgt * pl[s];
+        for (int s0 = sg; s0 < parts; s0 += NP * SG) {
+            float m[NP], l[NP], top = mx;
+            f32x4 x[NP];
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                acc[j] += wgt * x[j];
+            for (int i = 0; i < NP; ++i) { // parts behind the last: the last again, without weight
+                const int s = min(s0 + SG * i, parts - 1);
+                m[i] = pm[s];
+                l[i] = pl[s];
+                x[i] = *reinterpret_cast<const f32x4 *>(p + (int64_t)s * a.D);
+            }
+#pragma unroll
+            for (int i = 0; i < NP; ++i)
+                top = fmaxf(top, m[i]); // the last one may be another group's: any maximum not below its own serves
+            const float use = top == kNegInf ? 0.f : top, old = fast_exp2(mx - use);
+            mx = top;
+            sum *= old;
+            acc *= old;
+#pragma unroll
+            for (int i = 0; i < NP; ++i) {
+                const bool in = s0 + SG * i < parts;
+                const float wgt = fast_exp2(m[i] - use);
+                sum += in ? wgt * l[i] : 0.f;
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    acc[j] += in ? wgt * x[i][j] : 0.f;
+            }
         }
-        if (d >= a.D)
-            continue;
-        const float inv = sum > 0.f ? 1.0f / sum : 0.f;
-        const int64_t tok = qr.at + row / a.Hq;
-        *reinterpret_cast<u32x2 *>(a.o + tok * a.o_tok + row % a.Hq * a.o_head + d) =
-            u32x2{bf16_pair(acc[0] * inv, acc[1] * inv), bf16_pair(acc[2] * inv, acc[3] * inv)};
-        if (a.lse && d == 0)
-            a.lse[slot] = lse_of(mx, sum);
+        if constexpr (SG > 1) {
+            __syncthreads(); // what the turn before left has been read
+            ms[tid] = mx;
+            ls[tid] = sum;
+            accs[tid] = acc;
+            __syncthreads();
+            if (sg == 0) {
+#pragma unroll
+                for (int k = 1; k < SG; ++k)
+                    mx = fmaxf(mx, ms[tid + (k << lglp)]);
+                const float all = mx == kNegInf ? 0.f : mx;
+                sum = 0.f;
+                acc = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int k = 0; k < SG; ++k) {
+                    const float wgt = fast_exp2(ms[tid + (k << lglp)] - all);
+                    const f32x4 y = accs[tid + (k << lglp)];
+                    sum += wgt * ls[tid + (k << lglp)];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        acc[j] += wgt * y[j];
+                }
+            }
+        }
+        if (sg == 0 && row < R && d < a.D && parts > 1) { // one part: written already
+            const float inv = sum > 0.f ? 1.0f / sum : 0.f;
+            const int64_t tok = qr.at + i_tok;
+            *reinterpret_cast<u32x2 *>(a.o + tok * a.o_tok + h * a.o_head + d) =
+                u32x2{bf16_pair(acc[0] * inv, acc[1] * inv), bf16_pair(acc[2] * inv, acc[3] * inv)};
+            if (a.lse && d == 0)
+                a.lse[slot] = lse_of(mx, sum);
+        }
     }
 }
 
@@ -589,23 +691,22 @@ __global__ __launch_bounds__(256) void attn_cross_merge_kernel(const attn_cross_
 // K's tile is read both ways. delta = sum dO O is taken on the way in and left for the kernel of dK and dV.
 // ------------------------------------------------------------------------------------------
 template <int DP>
-__global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_cross_dq_kernel(const attn_cross_args a) {
+__global__ __launch_bounds__(256, DP == 64 ? 3 : DP == 128 ? 2 : 1) void attn_cross_dq_kernel(const attn_cross_args a) {
     constexpr int KT = cross_tile_keys(DP), KN = DP / 16, NT = KT / 32;
     constexpr int VO = KT * DP;
     __shared__ __attribute__((aligned(1024))) uint16_t KV0[2 * VO], KV1[2 * VO];
 
-    const attn_place at = attn_place_of(wg_id_x(), a.B * a.Hkv * a.nsplit, a.tps, a.deal);
-    if (at.group < 0)
+    const attn_cross_place at = attn_cross_place_of(&a, wg_id_x());
+    if (at.b < 0)
         return;
-    const int sp = uniform(at.group / (a.B * a.Hkv)), bu = at.group - sp * (a.B * a.Hkv);
-    const int u = uniform(bu % a.Hkv), b = uniform(bu / a.Hkv);
+    const int b = at.b, u = at.u, sp = at.sp;
     const int tid = wi_id_x(), w = uniform(tid >> 6), lane = tid & 63, l32 = lane & 31, hi = lane >> 5;
     const attn_range qr = q_rows(a, b), kr = k_rows(a, b);
     const attn_cut cut = part_of(kr.n, a.share, a.nsplit, ATTN_CROSS_KEY_STEP);
     if (sp >= cut.live)
         return;
     const int k0 = min(sp * cut.per, kr.n), k1 = min(k0 + cut.per, kr.n);
-    const int g = a.Hq / a.Hkv, R = qr.n * g, D = a.D;
+    const int g = a.g, R = qr.n * g, D = a.D;
     const uint16_t *kp = a.k + kr.at * a.k_tok + u * a.k_head, *vp = a.v + kr.at * a.v_tok + u * a.v_head;
     const cross_lane<DP> ln(lane);
     cross_stage<DP, KT> ks, vs;
@@ -617,10 +718,10 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_cross_dq_kernel(c
     };
     auto wait_loads = [] { __builtin_amdgcn_s_waitcnt(waitcnt_vm(0)); };
 
-    for (int tile = uniform(at.tile); (int64_t)tile * ATTN_CROSS_ROWS < R; tile += a.tps) {
+    for (int tile = at.tile; (int64_t)tile * ATTN_CROSS_ROWS < R; tile += a.tps) {
         const int row = tile * ATTN_CROSS_ROWS + 32 * w + l32;
         const bool valid = row < R, idle = tile * ATTN_CROSS_ROWS + 32 * w >= R;
-        const int tok = valid ? row / g : 0, h = u * g + (valid ? row % g : 0);
+        const int tok = valid ? attn_div_by(row, a.by_g) : 0, h = u * g + (valid ? row - tok * g : 0);
         const int64_t slot = (int64_t)(qr.at + tok) * a.Hq + h;
         bf16x8 qb[KN], gb[KN];
         float delta = 0.f;
@@ -720,20 +821,19 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_cross_dq_kernel(c
 // Both tiles are read both ways.
 // ------------------------------------------------------------------------------------------
 template <int DP, bool DK, bool DV>
-__global__ __launch_bounds__(256, DP <= 128 || !DK ? 2 : 1) void attn_cross_dkv_kernel(const attn_cross_args a) {
-    constexpr int QT = DP <= 64 ? 64 : 32, KN = DP / 16, NT = QT / 32;
+__global__ __launch_bounds__(256, DP == 64 ? 3 : DP == 128 || !DK ? 2 : 1) void attn_cross_dkv_kernel(const attn_cross_args a) {
+    constexpr int QT = ATTN_CROSS_STEP, KN = DP / 16, NT = QT / 32;
     constexpr int GO = QT * DP; // dO's tile behind Q's
     __shared__ __attribute__((aligned(1024))) uint16_t QG0[2 * GO], QG1[2 * GO];
     __shared__ __attribute__((aligned(16))) float st0[256], st1[256]; // lse in log2 units, from 64 on delta; the rest again
 
-    const attn_place at = attn_place_of(wg_id_x(), a.B * a.Hkv * a.nsplit, a.tps, a.deal);
-    if (at.group < 0)
+    const attn_cross_place at = attn_cross_place_of(&a, wg_id_x());
+    if (at.b < 0)
         return;
-    const int sp = uniform(at.group / (a.B * a.Hkv)), bu = at.group - sp * (a.B * a.Hkv);
-    const int u = uniform(bu % a.Hkv), b = uniform(bu / a.Hkv);
+    const int b = at.b, u = at.u, sp = at.sp;
     const int tid = wi_id_x(), w = uniform(tid >> 6), lane = tid & 63, l32 = lane & 31, hi = lane >> 5;
     const attn_range qr = q_rows(a, b), kr = k_rows(a, b);
-    const int g = a.Hq / a.Hkv, D = a.D;
+    const int g = a.g, D = a.D;
     const int per_head = uniform((qr.n + QT - 1) / QT), steps = per_head * g; // of QT rows of one head
     const attn_cut cut = part_of(steps, a.share, a.nsplit, 1);
     if (sp >= cut.live)
@@ -745,7 +845,7 @@ __global__ __launch_bounds__(256, DP <= 128 || !DK ? 2 : 1) void attn_cross_dkv_
     gs.init(w, lane, a.go_tok, D);
     auto wait_loads = [] { __builtin_amdgcn_s_waitcnt(waitcnt_vm(0)); };
 
-    for (int tile = uniform(at.tile); (int64_t)tile * ATTN_CROSS_KEYS < kr.n; tile += a.tps) {
+    for (int tile = at.tile; (int64_t)tile * ATTN_CROSS_KEYS < kr.n; tile += a.tps) {
         // The wave's rows of K and V, by lane: what lies past the last state or past D is outside the buffer, zeros.
         bf16x8 kf[KN], vf[KN];
         {
@@ -873,18 +973,17 @@ __global__ __launch_bounds__(256, DP <= 128 || !DK ? 2 : 1) void attn_cross_dkv_
 
 // Adds the parts of dQ's rows (KV = false), or of dK's and dV's, in order. 256 / LP rows of one sequence at a time.
 template <bool KV>
-__global__ __launch_bounds__(256) void attn_cross_sum_kernel(const attn_cross_args a, int lglp, int tpm, int step_rows) {
+__global__ __launch_bounds__(256) void attn_cross_sum_kernel(const attn_cross_args a, int lglp, int tpm) {
     const int b = uniform(wg_id_x() / tpm), t0 = wg_id_x() - b * tpm, tid = wi_id_x();
     const attn_range qr = q_rows(a, b), kr = k_rows(a, b);
-    const int g = a.Hq / a.Hkv, H = KV ? a.Hkv : a.Hq, W = KV ? 2 * a.D : a.D; // floats of a row's part
-    const attn_cut cut = KV ? part_of((qr.n + step_rows - 1) / step_rows * g, a.share, a.nsplit, 1)
+    const int g = a.g, H = KV ? a.Hkv : a.Hq, W = KV ? 2 * a.D : a.D; // floats of a row's part
+    const attn_cut cut = KV ? part_of((qr.n + ATTN_CROSS_STEP - 1) / ATTN_CROSS_STEP * g, a.share, a.nsplit, 1)
                             : part_of(kr.n, a.share, a.nsplit, ATTN_CROSS_KEY_STEP);
     if (cut.live == 1)
         return; // written already
     const int first = KV ? kr.at : qr.at;
-    const int64_t R = (int64_t)(KV ? kr.n : qr.n) * H;
-    const int rpw = 256 >> lglp, d = 4 * (tid & ((1 << lglp) - 1));
-    for (int64_t row = (int64_t)t0 * rpw + (tid >> lglp); row < R; row += (int64_t)tpm * rpw) {
+    const int R = (KV ? kr.n : qr.n) * H, rpw = 256 >> lglp, d = 4 * (tid & ((1 << lglp) - 1));
+    for (int row = t0 * rpw + (tid >> lglp); row < R; row += tpm * rpw) {
         if (d >= W)
             continue;
         const float *p = a.pacc + ((int64_t)first * H + row) * a.nsplit * W + d;
@@ -896,8 +995,8 @@ __global__ __launch_bounds__(256) void attn_cross_sum_kernel(const attn_cross_ar
             for (int j = 0; j < 4; ++j)
                 acc[j] += x[j];
         }
-        const int64_t tok = first + row / H;
-        const int h = row % H;
+        const int i_tok = attn_div_by(row, KV ? a.by_heads : a.by_hq), h = row - i_tok * H;
+        const int64_t tok = first + i_tok;
         const bool v = KV && d >= a.D;
         const float f = v ? 1.f : a.scale;
         uint16_t *dst = !KV ? a.dq + tok * a.dq_tok + h * a.dq_head + d
@@ -945,27 +1044,31 @@ extern "C" int attn_hip_launch_cross(const struct attn_cross_args *ap, const str
     const dim3 grid((unsigned)cut->grid), block(256);
     const hipError_t e = with_width(a.D, [&](auto W) {
         constexpr int DP = decltype(W)::value;
-        auto rows = [&](auto NB, auto NT) {
-            constexpr int kN = decltype(NB)::value;
+        auto rows = [&](auto NB, auto NT, auto NWF) {
+            constexpr int kN = decltype(NB)::value, kW = decltype(NWF)::value;
             constexpr bool kT = decltype(NT)::value;
             if (t_plan) {
-                plan_note(grid, block, "attn_cross_rows_kernel<%d, %d, %s> parts=%d share=%d", DP, kN, tf(kT),
-                          a.nsplit, a.share);
+                plan_note(grid, block, "attn_cross_rows_kernel<%d, %d, %s, %d> parts=%d share=%d", DP, kN, tf(kT),
+                          kW, a.nsplit, a.share);
                 return hipSuccess;
             }
-            hipLaunchKernelGGL((attn_cross_rows_kernel<DP, kN, kT>), grid, block, 0, st, a);
+            hipLaunchKernelGGL((attn_cross_rows_kernel<DP, kN, kT, kW>), grid, block, 0, st, a);
             return hipGetLastError();
         };
         constexpr std::integral_constant<int, 1> one;
-        // Past the L2 where a row tile is the only one of its sequence.
+        constexpr std::integral_constant<int, 2> two;
+        constexpr std::integral_constant<int, 4> four;
+                        // Past the L2 where a row tile is the only one of its sequence, which up to D = 128 it always is.
         if constexpr (DP > 128) {
             if (cut->rows16 == 1)
-                return with_flag(a.tps == 1, [&](auto NT) { return rows(one, NT); });
+                return with_flag(a.tps == 1, [&](auto NT) {
+                    return cut->quads ? rows(one, NT, one) : rows(one, NT, four);
+                });
         } else {
             if (cut->rows16 == 1)
-                return rows(one, std::true_type{});
+                return cut->quads ? rows(one, std::true_type{}, one) : rows(one, std::true_type{}, four);
             if (cut->rows16 == 2)
-                return rows(std::integral_constant<int, 2>{}, std::true_type{});
+                return cut->quads ? rows(two, std::true_type{}, one) : rows(two, std::true_type{}, four);
         }
         if (t_plan) {
             plan_note(grid, block, "attn_cross_kernel<%d> parts=%d share=%d", DP, a.nsplit, a.share);
@@ -977,14 +1080,21 @@ extern "C" int attn_hip_launch_cross(const struct attn_cross_args *ap, const str
     if (e != hipSuccess || a.nsplit == 1)
         return (int)e;
     const int lglp = lg_lanes(a.D);
-    const int tpm = cross_sum_tiles(a.B, (int64_t)max_q * a.Hq, 256 >> lglp);
-    const dim3 mgrid((unsigned)(a.B * tpm));
-    if (t_plan) {
-        plan_note(mgrid, block, "attn_cross_merge_kernel");
-        return (int)hipSuccess;
-    }
-    hipLaunchKernelGGL(attn_cross_merge_kernel, mgrid, block, 0, st, a, lglp, tpm);
-    return (int)hipGetLastError();
+    auto merge = [&](auto N, auto G) {
+        constexpr int kN = decltype(N)::value, kG = decltype(G)::value;
+        const int tpm = cross_sum_tiles(a.B, (int64_t)max_q * a.Hq, (256 >> lglp) / kG);
+        const dim3 mgrid((unsigned)(a.B * tpm));
+        if (t_plan) {
+            plan_note(mgrid, block, "attn_cross_merge_kernel<%d, %d>", kN, kG);
+            return hipSuccess;
+        }
+        hipLaunchKernelGGL((attn_cross_merge_kernel<kN, kG>), mgrid, block, 0, st, a, lglp, tpm);
+        return hipGetLastError();
+    };
+    constexpr std::integral_constant<int, 1> one;
+    constexpr std::integral_constant<int, 4> four;
+    constexpr std::integral_constant<int, 16> sixteen;
+    return (int)(cut->parts <= 4 ? merge(four, one) : cut->parts <= 16 ? merge(sixteen, one) : merge(sixteen, four));
 }
 
 // One of the two gradient kernels and, where it may leave parts, their sum. kv: dK and dV, after dQ.
@@ -1026,9 +1136,9 @@ extern "C" int attn_hip_launch_cross_grad(const struct attn_cross_args *ap, cons
         return (int)hipSuccess;
     }
     if (kv)
-        hipLaunchKernelGGL(attn_cross_sum_kernel<true>, sgrid, block, 0, st, a, lglp, tpm, attn_cross_step_rows(a.D));
+        hipLaunchKernelGGL(attn_cross_sum_kernel<true>, sgrid, block, 0, st, a, lglp, tpm);
     else
-        hipLaunchKernelGGL(attn_cross_sum_kernel<false>, sgrid, block, 0, st, a, lglp, tpm, attn_cross_step_rows(a.D));
+        hipLaunchKernelGGL(attn_cross_sum_kernel<false>, sgrid, block, 0, st, a, lglp, tpm);
     return (int)hipGetLastError();
 }
 

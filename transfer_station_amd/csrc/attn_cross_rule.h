@@ -45,18 +45,36 @@ ATTN_HD struct attn_cut attn_cut_of(int total, int share, int nsplit, int step) 
 #define ATTN_CROSS_KEYS 128     /* states of a tile of the kernel of dK and dV: four waves of 32 */
 #define ATTN_CROSS_KEY_STEP 128 /* parts of the states are multiples of this */
 #define ATTN_CROSS_MAX_PARTS 64
+#define ATTN_CROSS_TEAMS 256 /* of the kernel for few rows: a workgroup per CU */
 #define ATTN_CROSS_MAX_GRID 0x7fffffffL
 /* Floats of partial gradients that a call of attn_cross_grad may take (128 MB). */
 #define ATTN_CROSS_GRAD_FLOATS (1L << 25)
 
-/* Rows of a step of the kernel of dK and dV. */
-ATTN_HD int attn_cross_step_rows(int D) { return D <= 64 ? 64 : 32; }
+#define ATTN_CROSS_STEP 32 /* rows of a step of the kernel of dK and dV */
+
+/* n / d for 0 <= n < 2^31 by a product: mul = ceil(2^(31 + l) / d), l = ceil(log2 d), which is below 2^32 and off by
+ * less than 2^l, so that the quotient is off by less than n 2^l / (d 2^(31 + l)) < 1 / d. The kernels' divisions by what a
+ * call fixes are of this kind: of the compiler's, five take a microsecond before the first load. */
+struct attn_div {
+    uint32_t mul, shift;
+};
+ATTN_HD struct attn_div attn_div_of(int d) {
+    struct attn_div x = {0, 31};
+    while ((int64_t)1 << (x.shift - 31) < d)
+        ++x.shift;
+    x.mul = (uint32_t)((((uint64_t)1 << x.shift) + (uint64_t)d - 1) / (uint64_t)d);
+    return x;
+}
+ATTN_HD int attn_div_by(int n, struct attn_div x) { return (int)(((uint64_t)(uint32_t)n * x.mul) >> x.shift); }
 
 /* What one launch looks like: row (or state) tiles per group and its parts, and how the groups are dealt to the XCDs
  * (attn_place_of). */
 struct attn_cross_cut {
     int tps, nsplit, share, deal;
     int rows16; /* blocks of 16 rows per workgroup of the kernel for few rows, 0: tiles of 128 */
+    int quads;  /* that kernel's form for four kv heads of a workgroup, a wave each */
+    int parts;  /* of a sequence of the call's bounds, about */
+    int teams;  /* that kernel: teams of the decode line, 0: whole sequences */
     long grid;
 };
 
@@ -68,10 +86,31 @@ struct attn_cross_args {
     int64_t dq_tok, dq_head, dk_tok, dk_head, dv_tok, dv_head;
     const int32_t *q_start, *q_second, *k_start, *k_second; /* second: lengths, or the next starts */
     int q_is_len, k_is_len;
-    int B, Tq, Tk, Hq, Hkv, D;
+    int B, Tq, Tk, Hq, Hkv, g, D; /* g = Hq / Hkv */
     float c, scale; /* scale log2(e), scale */
-    int tps, nsplit, share, deal;
+    int tps, nsplit, share, deal, tpp;
+    int teams, wgs, Hkv_wg; /* few rows: teams of the decode line, workgroups, groups of kv heads */
+    struct attn_div by_tpp, by_deal, by_nsplit, by_heads, by_hq, by_g; /* tpp, deal, nsplit, Hkv, Hq, g */
+    struct attn_div by_tps, by_B, by_gwg;                              /* tps, B, query heads of a group of kv heads */
     float *pm, *pl, *pacc; /* partial maxima, sums and rows; of gradients: rows in pacc */
 };
+
+/* Where a workgroup is: attn_place_of, and its group as a sequence, a kv head and a part of them (innermost). */
+struct attn_cross_place {
+    int b, u, sp, tile; /* b -1: none */
+};
+ATTN_HD struct attn_cross_place attn_cross_place_of(const struct attn_cross_args *a, int wg) {
+    const int i = wg >> 3, slot = attn_div_by(i, a->by_tpp);
+    const int piece = (wg & 7) + 8 * slot, group = attn_div_by(piece, a->by_deal);
+    const int bu = attn_div_by(group, a->by_nsplit);
+    struct attn_cross_place p;
+    p.tile = piece - group * a->deal + a->deal * (i - slot * a->tpp);
+    p.sp = group - bu * a->nsplit;
+    p.b = attn_div_by(bu, a->by_heads);
+    p.u = bu - p.b * a->Hkv;
+    if (p.b >= a->B || p.tile >= a->tps)
+        p.b = -1;
+    return p;
+}
 
 #endif

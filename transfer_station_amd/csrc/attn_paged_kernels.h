@@ -18,6 +18,7 @@
 
 #include "attn_device.h"
 #include "attn_launch.h"
+#include "attn_line.h"
 #include "attn_paged_cut.h"
 #include "attn_paged_rule.h"
 
@@ -76,84 +77,20 @@ __device__ __forceinline__ attn_seq seq_at(const attn_paged_args &a, int b) {
                        a.cols, a.lgp);
 }
 
-// Sum or maximum over the wave, in every lane.
-template <bool MAX> __device__ __forceinline__ int wave_all(int x) {
-    auto op = [](int p, int q) { return MAX ? max(p, q) : p + q; };
-    x = op(x, __builtin_amdgcn_update_dpp(x, x, 0x128, 0xf, 0xf, false)); // row_ror:8, 4, 2, 1
-    x = op(x, __builtin_amdgcn_update_dpp(x, x, 0x124, 0xf, 0xf, false));
-    x = op(x, __builtin_amdgcn_update_dpp(x, x, 0x122, 0xf, 0xf, false));
-    x = op(x, __builtin_amdgcn_update_dpp(x, x, 0x121, 0xf, 0xf, false));
-    const auto p = __builtin_amdgcn_permlane16_swap((unsigned)x, (unsigned)x, false, false);
-    x = op((int)p[0], (int)p[1]);
-    const auto r = __builtin_amdgcn_permlane32_swap((unsigned)x, (unsigned)x, false, false);
-    return op((int)r[0], (int)r[1]);
-}
-
-// x plus those of the lanes below (DPP row shifts, then the rows' last lanes broadcast to the rows behind).
-__device__ __forceinline__ int wave_scan(int x) {
-    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, true); // row_shr:1, 2, 4, 8
-    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, true);
-    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, true);
-    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, true);
-    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false); // row_bcast:15 into rows 1 and 3
-    return x + __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false); // row_bcast:31 into rows 2 and 3
-}
-
-// The decode line (attn_quota) as a wave sees it, 64 sequences at a time: a kv head's units and the quota.
-// One sequence needs no sum, and up to 64 are read once.
-struct line {
-    int total, quota;
-    int n, sum; // of sequence `lane`: units, and units up to and with it
-};
-__device__ __forceinline__ int units_at(const attn_paged_args &a, int i) {
-    if (i >= a.B)
-        return 0;
-    const attn_seq s = attn_seq_of(a.q_start[i], a.q_start[i + 1], a.kv_len[i], a.T, a.cols, a.lgp);
-    return attn_units(s.n, s.kend);
-}
-__device__ __forceinline__ line line_at(const attn_paged_args &a, int lane) {
-    line l;
-    int most;
-    if (a.B == 1) {
-        const attn_seq s = seq_at(a, 0);
-        l.n = l.sum = l.total = most = attn_units(s.n, s.kend);
-    } else {
-        l.n = units_at(a, lane);
-        l.sum = wave_scan(l.n);
-        l.total = __builtin_amdgcn_readlane(l.sum, 63);
-        int m = l.n;
-        for (int i0 = 64; i0 < a.B; i0 += 64) {
-            const int n = units_at(a, i0 + lane);
-            m = max(m, n);
-            l.total += __builtin_amdgcn_readlane(wave_scan(n), 63);
-        }
-        most = uniform(wave_all<true>(m));
-    }
-    l.quota = uniform(attn_quota(l.total, most, a.Hkv, a.teams, a.nsplit));
-    return l;
-}
-// The sequence that unit `at` of a kv head's line belongs to, and the units before that.
-__device__ __forceinline__ int seq_of_unit(const attn_paged_args &a, const line &l, int lane, int at,
-                                           int &before) {
-    before = 0;
-    if (a.B == 1)
-        return 0;
-    int n = l.n, sum = l.sum, base = 0;
-    for (int i0 = 0;;) {
-        const uint64_t past = __builtin_amdgcn_ballot_w64(base + sum > at);
-        if (past != 0) {
-            const int k = __builtin_ctzll(past);
-            before = base + __builtin_amdgcn_readlane(sum - n, k);
-            return i0 + k;
-        }
-        base += __builtin_amdgcn_readlane(sum, 63);
-        i0 += 64;
-        if (i0 >= a.B) // not reached for a unit of the line
+// The decode line's units of a call (attn_line.h).
+struct paged_units {
+    static __device__ __forceinline__ int at(const attn_paged_args &a, int i) {
+        if (i >= a.B)
             return 0;
-        n = units_at(a, i0 + lane);
-        sum = wave_scan(n);
+        const attn_seq s = attn_seq_of(a.q_start[i], a.q_start[i + 1], a.kv_len[i], a.T, a.cols, a.lgp);
+        return attn_units(s.n, s.kend);
     }
-}
+    static __device__ __forceinline__ int one(const attn_paged_args &a) {
+        const attn_seq s = seq_at(a, 0);
+        return attn_units(s.n, s.kend);
+    }
+    static __device__ __forceinline__ int heads(const attn_paged_args &a) { return a.Hkv; }
+};
 
 // N = 16 keys of the cache from key kb (a multiple of N): their rows' place, and how many of them there are (0
 // where the page id is none, or past the sequence's end).
@@ -229,14 +166,14 @@ __global__ __launch_bounds__(256, 2) void attn_paged_decode_kernel(const attn_pa
     int u, b, off = 0, left = 1, pos0 = 0;
     line ln = {0, 1, 0, 0};
     if (a.teams) {
-        ln = line_at(a, lane);
+        ln = line_at<paged_units>(a, lane);
         if ((int64_t)team * ln.quota >= (int64_t)ln.total * a.Hkv)
             return;
         pos0 = team * ln.quota;
         left = min(ln.quota, ln.total * a.Hkv - pos0);
         u = uniform(pos0 / ln.total);
         int before;
-        b = uniform(seq_of_unit(a, ln, lane, pos0 - u * ln.total, before));
+        b = uniform(seq_of_unit<paged_units>(a, ln, lane, pos0 - u * ln.total, before));
         off = pos0 - u * ln.total - before;
     } else {
         u = uniform(team / a.B);
