@@ -215,7 +215,7 @@ struct attn_spans {
 
 /* D % 16 == 0, 16 <= D <= 256; scale 0: 1/sqrt(D). Limits: B * Hkv <= 2^20, q.T * Hq and k.T * Hkv <= 2^30. The token
  * strides of all tensors of a call are in [D, ATTN_TOKEN_MAX] elements. */
-#define ATTN_TOKEN_MAX (1 << 22)
+#define ATTN_TOKEN_MAX 4194304 /* 2^22 */
 struct attn_cross_call {
     struct attn_spans q, k;
     int32_t B, Hq, Hkv, D;
@@ -255,7 +255,7 @@ int attn_cross_plan(const struct attn_cross_call *c, int grad, char *buf, size_t
  */
 #define ATTN_BEAMS_MAX 256
 #define ATTN_BEAM_K_MAX 64
-#define ATTN_BEAM_V_MAX (1 << 20)
+#define ATTN_BEAM_V_MAX 1048576 /* 2^20 */
 #define ATTN_REORDER_MAX 32
 
 /* The beams of B batch entries: row b * beams + i of logits (bits 16: bf16, 32: fp32; `row` elements from row to row, at

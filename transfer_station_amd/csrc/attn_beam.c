@@ -13,7 +13,7 @@
 #include <stdlib.h>
 #include <string.h>
 
-int attn_hip_launch_beam(const struct attn_beam_args *a, int bits, int chunk, void *stream);
+int attn_hip_launch_beam(const struct attn_beam_args *a, int bits, void *stream);
 int attn_hip_launch_reorder(const struct attn_reorder_args *a, void *stream);
 
 static void beam_fail(const char *who, const char *what) {
@@ -30,8 +30,8 @@ static void beam_hip_check(int err, const char *who) {
 
 static int misaligned(const void *p, size_t to) { return !p || (uintptr_t)p % to != 0; }
 
-/* Everything but the outputs; returns the chunk's length. */
-static int beam_check(const char *who, const struct attn_beams *c) {
+/* Everything but the outputs; how the rows are cut. */
+static struct attn_beam_cut beam_check(const char *who, const struct attn_beams *c) {
     if (!c)
         beam_fail(who, "the beams must be non-NULL");
     if (c->bits != 16 && c->bits != 32)
@@ -47,7 +47,7 @@ static int beam_check(const char *who, const struct attn_beams *c) {
         beam_fail(who, "scores must be a device pointer to B * beams floats");
     if (c->done && (c->done_token < 0 || c->done_token >= c->V))
         beam_fail(who, "done_token must be in [0, V)");
-    return attn_beam_chunk_of((int64_t)c->B * c->beams, c->V);
+    return attn_beam_cut_of((int64_t)c->B * c->beams, c->V, c->bits / 8);
 }
 
 static size_t keys_bytes(const struct attn_beams *c, int chunks) {
@@ -55,13 +55,13 @@ static size_t keys_bytes(const struct attn_beams *c, int chunks) {
 }
 
 size_t attn_beam_scratch_bytes(const struct attn_beams *c) {
-    const int chunk = beam_check("attn_beam_scratch_bytes", c), chunks = (c->V + chunk - 1) / chunk;
-    return keys_bytes(c, chunks) + (size_t)c->B * c->beams * chunks * 2 * sizeof(float);
+    const struct attn_beam_cut cut = beam_check("attn_beam_scratch_bytes", c);
+    return keys_bytes(c, cut.chunks) + (size_t)c->B * c->beams * cut.chunks * 2 * sizeof(float);
 }
 
 void attn_beam_select(const struct attn_beams *c, float *score, int32_t *token, int32_t *parent, void *scratch) {
     static const char *who = "attn_beam_select";
-    const int chunk = beam_check(who, c);
+    const struct attn_beam_cut cut = beam_check(who, c);
     if (misaligned(score, 4) || misaligned(token, 4) || misaligned(parent, 4))
         beam_fail(who, "score, token and parent must be device pointers to B * K values");
     if (score == c->scores)
@@ -71,11 +71,11 @@ void attn_beam_select(const struct attn_beams *c, float *score, int32_t *token, 
     struct attn_beam_args a;
     memset(&a, 0, sizeof a);
     a.logits = c->logits, a.row = c->row, a.scores = c->scores, a.done = c->done, a.done_token = c->done_token;
-    a.B = c->B, a.beams = c->beams, a.V = c->V, a.K = c->K, a.chunks = (c->V + chunk - 1) / chunk;
+    a.B = c->B, a.beams = c->beams, a.V = c->V, a.K = c->K, a.chunks = cut.chunks, a.steps = cut.steps;
     a.keys = (uint64_t *)scratch;
     a.ms = (float *)((char *)scratch + keys_bytes(c, a.chunks));
     a.score = score, a.token = token, a.parent = parent;
-    beam_hip_check(attn_hip_launch_beam(&a, c->bits, chunk, attn_flash_get_stream()), who);
+    beam_hip_check(attn_hip_launch_beam(&a, c->bits, attn_flash_get_stream()), who);
 }
 
 void attn_kv_reorder(const struct attn_kv_cache *c, const int32_t *parent, int beams, int tables) {

@@ -5,53 +5,71 @@
 #define ATTN_BEAM_KERNELS_H
 
 #include "attn_beam_rule.h"
+#include "attn_flash.h"
 #include "attn_device.h"
 #include "attn_launch.h"
 
 namespace {
 
-// Floats and doubles as unsigned numbers of the same order; 0 stands for none (a NaN with the sign bit).
+// Floats and doubles as unsigned numbers of the same order, -0 as 0; 0 stands for none (a NaN with the sign bit).
 __device__ __forceinline__ uint32_t ordered(float x) {
-    const uint32_t u = __builtin_bit_cast(uint32_t, x);
+    const uint32_t u = __builtin_bit_cast(uint32_t, x + 0.f);
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 __device__ __forceinline__ float unordered(uint32_t u) {
     return __builtin_bit_cast(float, u & 0x80000000u ? u & 0x7fffffffu : ~u);
 }
 __device__ __forceinline__ uint64_t ordered(double x) {
-    const uint64_t u = __builtin_bit_cast(uint64_t, x);
+    const uint64_t u = __builtin_bit_cast(uint64_t, x + 0.0);
     return u >> 63 ? ~u : u | 0x8000000000000000ull;
 }
 __device__ __forceinline__ double unordered(uint64_t u) {
     return __builtin_bit_cast(double, u >> 63 ? u & 0x7fffffffffffffffull : ~u);
 }
+constexpr float kLog2E = 1.44269504088896341f;
 constexpr uint32_t kOrderedNegInf = 0x007fffffu; // ordered(-inf): what is above it is a candidate
 // A test of the bits, which the compiler must not see as one of a float: those are compiled as if there were no NaN.
 __device__ __forceinline__ bool finite(float x) {
     return (opaque(__builtin_bit_cast(uint32_t, x)) & 0x7f800000u) != 0x7f800000u;
 }
 
-// A value that at least K of the wave's lanes reach (the lowest one where fewer are above `none`), and hardly more: the
-// interval between the smallest and the largest is halved until the count is between K and K + 7.
-template <typename U> __device__ __forceinline__ U wave_kth(U x, U none, int K) {
-    U lo = none, hi = ~(U)0; // count(>= lo) >= K or lo == none; count(>= hi) < K or unknown
-    if (__builtin_popcountll(__builtin_amdgcn_ballot_w64(x > none)) < K)
+// A value that at least K of the wave's lanes reach (`none` where fewer are above that), and hardly more: from a lane's own
+// value up or down in growing steps until the count passes K, then by halves until it is between K and K + 7.
+__device__ __forceinline__ uint32_t wave_kth(uint32_t x, uint32_t none, uint32_t step, int K) {
+    auto count = [&](uint32_t y) { return (int)__builtin_popcountll(__builtin_amdgcn_ballot_w64(x >= y)); };
+    if (count(none + 1) < K)
         return none;
-    while (lo + 1 < hi) {
-        const U mid = lo + (hi - lo) / 2;
-        const int n = __builtin_popcountll(__builtin_amdgcn_ballot_w64(x >= mid));
-        if (n >= K) {
-            lo = mid;
-            if (n < K + 8)
+    uint32_t lo = max((uint32_t)__builtin_amdgcn_readfirstlane((int)x), none + 1), hi = lo; // count(lo) >= K > count(hi)
+    if (count(lo) >= K) {
+        do {
+            lo = hi;
+            if (hi > ~step) {
+                hi = ~0u;
                 break;
-        } else {
+            }
+            hi += step;
+            step <<= 1;
+        } while (count(hi) >= K);
+    } else {
+        do {
+            hi = lo;
+            if (lo <= none + step) {
+                lo = none + 1;
+                break;
+            }
+            lo -= step;
+            step <<= 1;
+        } while (count(lo) < K);
+    }
+    while (count(lo) >= K + 8 && lo + 1 < hi) {
+        const uint32_t mid = lo + (hi - lo) / 2;
+        if (count(mid) >= K)
+            lo = mid;
+        else
             hi = mid;
-        }
     }
     return lo;
 }
-
-__device__ __forceinline__ uint32_t bits_lo(uint64_t x) { return (uint32_t)x; }
 
 // The threads' sum, in every thread. red: four ints; ends with a barrier, so that red may be used again.
 __device__ __forceinline__ int wg_sum(int x, int *red, int tid) {
@@ -67,127 +85,192 @@ __device__ __forceinline__ int wg_sum(int x, int *red, int tid) {
 }
 
 // ------------------------------------------------------------------------------------------
-// One chunk of a row: its maximum m and sum of e^(x - m), and its K largest logits, of equals those at the lowest index.
-// Each thread holds its elements in registers. The threads' own maxima give a threshold that at least K elements reach
-// (wave_kth, the largest of four waves); what reaches it goes to LDS, a few dozen elements, and each counts how many
-// are ahead of it. Where more reach it than LDS has room for (equal logits) the K-th element's value and index are
-// searched for bit by bit. HBM-bound: each logit is read once.
+// One chunk of a row: a reference r, its largest x log2(e) rounded, the sum of 2^(x log2(e) - r), and its K largest logits, of equals those at the lowest index.
+// The four waves take neighbouring pieces of it, a step of 4 KB at a time with the next on its way, each lane with a
+// maximum and sum of its own. A wave's threshold is a value that at least K of its lanes have reached (wave_kth), taken
+// anew as the number of steps doubles: some K logits pass it per doubling. They go to LDS; at the end those below the best
+// of the four thresholds fall away, and each of the rest counts how many are ahead of it. Where more pass than LDS has room
+// for (equal or ascending logits) the K-th element's value and index are searched for bit by bit, over the chunk in
+// memory. HBM-bound: each logit is read once.
 // ------------------------------------------------------------------------------------------
-constexpr int kBeamRoom = 512;
+constexpr int kBeamRoom = 256, kBeamBest = 512; // places for a wave's logits, and for those that are ranked
 
-template <typename T, int EPT> __global__ __launch_bounds__(256) void attn_beam_chunk_kernel(const attn_beam_args a) {
-    constexpr int VEC = 16 / sizeof(T), NVEC = EPT / VEC;
-    typedef T __attribute__((ext_vector_type(VEC), aligned(sizeof(T)))) vec;
-    __shared__ uint64_t room[kBeamRoom];
-    __shared__ float redf[4];
+template <typename T> __global__ __launch_bounds__(256, 4) void attn_beam_chunk_kernel(const attn_beam_args a) {
+    constexpr int VEC = 16 / sizeof(T), NV = 4, STEP = ATTN_BEAM_STEP(sizeof(T)); // logits of a wave's step
+    static_assert(STEP == 64 * VEC * NV, "");
+    __shared__ uint64_t room[4 * kBeamRoom], best[kBeamBest];
+    __shared__ float redm[4], reds[4];
     __shared__ uint32_t redu[4];
-    __shared__ int redi[4], taken;
-    const int row = wg_id_x() / a.chunks, chunk = wg_id_x() - row * a.chunks, tid = wi_id_x(), w = tid >> 6;
+    __shared__ int redi[4], redn[4], kept;
+    const int row = wg_id_x() / a.chunks, chunk = wg_id_x() - row * a.chunks, tid = wi_id_x(), lane = tid & 63;
+    const int w = uniform(tid >> 6);
     if ((a.done && a.done[row]) || !finite(a.scores[row]))
         return;
     const T *x = reinterpret_cast<const T *>(a.logits) + row * a.row;
-    const int first = chunk * 256 * EPT;
-    float e[EPT];
-    auto value = [](T t) {
+    const int first = chunk * 4 * a.steps * STEP, begin = first + w * a.steps * STEP;
+    const int end = min(begin + a.steps * STEP, a.V);
+    if (tid == 0)
+        kept = 0;
+    auto value = [](u32x4 v, int i) {
         if constexpr (sizeof(T) == 2)
-            return __builtin_bit_cast(float, (uint32_t)t << 16);
-        else
-            return t;
+            return __builtin_bit_cast(float, i & 1 ? v[i >> 1] & 0xffff0000u : v[i >> 1] << 16);
+        const uint32_t e = v[i]; // a value: of an element in place bit_cast takes the vector's first
+        return __builtin_bit_cast(float, e);
     };
-    // Element i of vector j has index first + (256 j + tid) VEC + i.
+    auto bits_of = [](T t) -> uint32_t {
+        if constexpr (sizeof(T) == 2)
+            return t;
+        else
+            return __builtin_bit_cast(uint32_t, t);
+    };
+    // Vector j of the step at `at` is 64 VEC j + VEC lane on; past the row's end there are logits of -inf.
+    auto load = [&](int at, u32x4 *v) __attribute__((always_inline)) {
+        if (at + STEP <= a.V) {
 #pragma unroll
-    for (int j = 0; j < NVEC; ++j) {
-        const int at = first + (256 * j + tid) * VEC;
-        if (at + VEC <= a.V) {
-            const vec v = __builtin_nontemporal_load(reinterpret_cast<const vec *>(x + at));
-#pragma unroll
-            for (int i = 0; i < VEC; ++i)
-                e[VEC * j + i] = value(v[i]);
+            for (int j = 0; j < NV; ++j)
+                v[j] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_a2 *>(x + at + (64 * j + lane) * VEC));
         } else {
 #pragma unroll
-            for (int i = 0; i < VEC; ++i)
-                e[VEC * j + i] = at + i < a.V ? value(x[at + i]) : kNegInf;
-        }
-    }
-    if (tid == 0)
-        taken = 0;
-    uint32_t top = 0; // a NaN's bits are above infinity's, or lowest of all; either makes the sum one
-    float mx = kNegInf;
+            for (int j = 0; j < NV; ++j) {
+                const int k = at + (64 * j + lane) * VEC;
+                if (k + VEC <= a.V) {
+                    v[j] = *reinterpret_cast<const u32x4_a2 *>(x + k);
+                    continue;
+                }
+                uint32_t e[VEC]; // element by element, past the end the last one's place
 #pragma unroll
-    for (int i = 0; i < EPT; ++i)
-        mx = fmaxf(mx, e[i]);
-    top = ordered(mx);
-    const uint32_t kth = wave_kth<uint32_t>(top, kOrderedNegInf, a.K);
-    float m = mx;
-    m = seg_all<true>(m, true);
-    if ((tid & 63) == 0) {
-        redf[w] = m;
-        redu[w] = kth;
-    }
-    __syncthreads();
-    m = fmaxf(fmaxf(redf[0], redf[1]), fmaxf(redf[2], redf[3]));
-    const uint32_t least = max(max(max(redu[0], redu[1]), max(redu[2], redu[3])), kOrderedNegInf + 1);
-    if (top >= least)
+                for (int i = 0; i < VEC; ++i)
+                    e[i] = bits_of(x[min(k + i, a.V - 1)]);
 #pragma unroll
-        for (int i = 0; i < EPT; ++i) {
-            const uint32_t u = ordered(e[i]);
-            if (u >= least) {
-                const int at = atomicAdd(&taken, 1);
-                if (at < kBeamRoom)
-                    room[at] = (uint64_t)u << 32 | ~(uint32_t)(first + (256 * (i / VEC) + tid) * VEC + i % VEC);
+                for (int i = 0; i < VEC; ++i)
+                    e[i] = k + i < a.V ? e[i] : sizeof(T) == 2 ? 0xff80u : 0xff800000u;
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    v[j][i] = sizeof(T) == 2 ? e[2 * i % VEC] | e[(2 * i + 1) % VEC] << 16 : e[i];
             }
         }
-    const float muse = m == kNegInf ? 0.f : m;
-    float sum = 0.f;
+    };
+    float m = kNegInf, ref = 0.f, sum = 0.f; // of this lane: sum of 2^(x log2(e) - ref), ref the rounded m log2(e)
+    uint32_t least = kOrderedNegInf + 1;
+    int taken = 0; // of this wave
+    u32x4 v[NV], next[NV];
+    if (begin < end)
+        load(begin, v);
+    for (int at = begin, n = 1; at < end; at += STEP, ++n) {
+        if (at + STEP < end)
+            load(at + STEP, next);
+        float top = kNegInf;
 #pragma unroll
-    for (int i = 0; i < EPT; ++i)
-        sum += fast_exp2((e[i] - muse) * 1.44269504088896341f);
-    sum = seg_all<false>(sum, true);
-    __syncthreads();
-    if ((tid & 63) == 0)
-        redf[w] = sum;
-    int n = taken;
+        for (int j = 0; j < NV; ++j)
+#pragma unroll
+            for (int i = 0; i < VEC; i += 2)
+                top = max3f(top, value(v[j], i), value(v[j], i + 1));
+        m = fmaxf(m, top);
+        const float to = m == kNegInf ? 0.f : m * kLog2E;
+        sum *= fast_exp2(ref - to);
+        ref = to;
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+#pragma unroll
+            for (int i = 0; i < VEC; ++i)
+                sum += fast_exp2(fmaf(value(v[j], i), kLog2E, -ref));
+        if ((n & (n - 1)) == 0)
+            least = max(least, wave_kth(ordered(m), kOrderedNegInf, 1u << 20, a.K));
+        const float pass = unordered(least);
+        if (__builtin_amdgcn_ballot_w64(top >= pass) != 0)
+#pragma unroll
+            for (int j = 0; j < NV; ++j)
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) {
+                    const float y = value(v[j], i);
+                    const uint64_t in = __builtin_amdgcn_ballot_w64(y >= pass);
+                    if (in == 0)
+                        continue;
+                    const int to = taken + __builtin_amdgcn_mbcnt_hi((uint32_t)(in >> 32),
+                                                                     __builtin_amdgcn_mbcnt_lo((uint32_t)in, 0));
+                    if (y >= pass && to < kBeamRoom)
+                        room[w * kBeamRoom + to] =
+                            (uint64_t)ordered(y) << 32 | ~(uint32_t)(at + (64 * j + lane) * VEC + i);
+                    taken += __builtin_popcountll(in);
+                }
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+            v[j] = next[j];
+    }
+    // A lane without a logit has a sum of 0, and no part in the reference.
+    const float wm = seg_all<true>(m == kNegInf ? kNegInf : ref, true), wuse = wm == kNegInf ? 0.f : wm;
+    sum = seg_all<false>(m == kNegInf ? 0.f : sum * fast_exp2(ref - wuse), true);
+    if (lane == 0) {
+        redm[w] = wm;
+        reds[w] = sum;
+        redu[w] = least;
+        redn[w] = taken;
+    }
     __syncthreads();
     const int64_t part = (int64_t)row * a.chunks + chunk;
     if (tid == 0) {
-        a.ms[2 * part] = m;
-        a.ms[2 * part + 1] = redf[0] + redf[1] + redf[2] + redf[3];
+        const float all = fmaxf(fmaxf(redm[0], redm[1]), fmaxf(redm[2], redm[3])), use = all == kNegInf ? 0.f : all;
+        float s = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            s += reds[i] * fast_exp2(redm[i] - use);
+        a.ms[2 * part] = all;
+        a.ms[2 * part + 1] = s;
     }
-    if (n > kBeamRoom) {
-        // The K-th largest value, then the index up to which elements of that value belong to the K.
+    least = max(max(redu[0], redu[1]), max(redu[2], redu[3]));
+    for (int i = lane; i < min(taken, kBeamRoom); i += 64) {
+        const uint64_t key = room[w * kBeamRoom + i];
+        if (key >> 32 >= least) {
+            const int to = atomicAdd(&kept, 1);
+            if (to < kBeamBest)
+                best[to] = key;
+        }
+    }
+    __syncthreads();
+    const int most = max(max(redn[0], redn[1]), max(redn[2], redn[3]));
+    if (most > kBeamRoom || kept > kBeamBest) {
+        const int last_at = min(first + 4 * a.steps * STEP, a.V);
+        auto each = [&](auto &&f) {
+            for (int i = first + tid; i < last_at; i += 256) {
+                float y;
+                if constexpr (sizeof(T) == 2)
+                    y = __builtin_bit_cast(float, (uint32_t)x[i] << 16);
+                else
+                    y = x[i];
+                f(ordered(y), (uint32_t)i);
+            }
+        };
         auto count = [&](auto &&f) {
             int c = 0;
-#pragma unroll
-            for (int i = 0; i < EPT; ++i)
-                c += f(ordered(e[i]), (uint32_t)(first + (256 * (i / VEC) + tid) * VEC + i % VEC)) ? 1 : 0;
+            each([&](uint32_t u, uint32_t i) { c += f(u, i) ? 1 : 0; });
             return wg_sum(c, redi, tid);
         };
-        uint32_t v = 0, last = 0;
+        // The K-th largest value, then the index up to which elements of that value belong to the K.
+        uint32_t k = 0, last = 0;
         for (uint32_t bit = 0x80000000u; bit; bit >>= 1)
-            if (count([&](uint32_t u, uint32_t) { return u >= (v | bit); }) >= a.K)
-                v |= bit;
-        const int need = a.K - count([&](uint32_t u, uint32_t) { return u > v; });
+            if (count([&](uint32_t u, uint32_t) { return u >= (k | bit); }) >= a.K)
+                k |= bit;
+        const int need = a.K - count([&](uint32_t u, uint32_t) { return u > k; });
         for (uint32_t bit = 0x80000000u; bit; bit >>= 1) // the largest index before which fewer than `need` lie
-            if (count([&](uint32_t u, uint32_t i) { return u == v && i < (last | bit); }) < need)
+            if (count([&](uint32_t u, uint32_t i) { return u == k && i < (last | bit); }) < need)
                 last |= bit;
         if (tid == 0)
-            taken = 0;
+            kept = 0;
         __syncthreads();
-#pragma unroll
-        for (int i = 0; i < EPT; ++i) {
-            const uint32_t u = ordered(e[i]), at = first + (256 * (i / VEC) + tid) * VEC + i % VEC;
-            if (u > v || (u == v && at <= last)) // K of them
-                room[atomicAdd(&taken, 1) & (kBeamRoom - 1)] = (uint64_t)u << 32 | ~at;
-        }
+        each([&](uint32_t u, uint32_t i) {
+            if (u > k || (u == k && i <= last)) // K of them
+                best[atomicAdd(&kept, 1) & (kBeamBest - 1)] = (uint64_t)u << 32 | ~i;
+        });
         __syncthreads();
-        n = min(taken, kBeamRoom);
     }
+    const int n = min(kept, kBeamBest);
     uint64_t *keys = a.keys + part * a.K;
     for (int i = tid; i < n; i += 256) {
-        const uint64_t mine = room[i];
+        const uint64_t mine = best[i];
         int rank = 0;
+#pragma unroll 8
         for (int j = 0; j < n; ++j)
-            rank += room[j] > mine ? 1 : 0;
+            rank += best[j] > mine ? 1 : 0;
         if (rank < a.K)
             keys[rank] = mine;
     }
@@ -197,91 +280,110 @@ template <typename T, int EPT> __global__ __launch_bounds__(256) void attn_beam_
 
 // ------------------------------------------------------------------------------------------
 // A batch entry's K best from its beams' chunks, by (x - lse) + score in fp64, of equals those of the lowest beam and
-// index. The chunks' lists are sorted: their heads give a threshold that at least K candidates reach, each list is
-// followed down to it, and what reaches it counts how many are ahead.
+// index: the threads' own maxima give a threshold that at least K candidates reach, and what reaches it counts how many are
+// ahead. Bound by latency: one round of loads, two sums over a beam's chunks, a search and a count.
 // ------------------------------------------------------------------------------------------
 constexpr int kBeamFinalRoom = 1024;
-constexpr int kBeamMax = 256;
 
 __global__ __launch_bounds__(256) void attn_beam_select_kernel(const attn_beam_args a) {
-    __shared__ double lse[kBeamMax], base[kBeamMax]; // lse of a done beam: 0, of one that offers nothing: infinite
-    __shared__ uint64_t rv[kBeamFinalRoom], redu[4];
-    __shared__ uint32_t ri[kBeamFinalRoom];
+    __shared__ double lse[ATTN_BEAMS_MAX], base[ATTN_BEAMS_MAX]; // of a done beam: 0; of one without a continuation: infinite
+    __shared__ uint8_t over[ATTN_BEAMS_MAX];
+    __shared__ uint64_t rv[kBeamFinalRoom];
+    __shared__ uint32_t ri[kBeamFinalRoom], redu[4];
     __shared__ int redi[4], taken;
-    const int b = wg_id_x(), tid = wi_id_x(), w = tid >> 6, lane = tid & 63;
+    const int b = wg_id_x(), tid = wi_id_x(), lane = tid & 63, w = uniform(tid >> 6);
     const int row0 = b * a.beams;
     if (tid == 0)
         taken = 0;
-    for (int i = w; i < a.beams; i += 4) {
+    // The first candidates are asked for at once; those of a beam without a continuation are anything.
+    constexpr int HOLD = 4;
+    const int per = a.chunks * a.K, all = a.beams * per; // candidates of a beam and of the entry
+    const uint64_t *keys = a.keys + (int64_t)row0 * per;
+    uint64_t held[HOLD];
+#pragma unroll
+    for (int r = 0; r < HOLD; ++r)
+        held[r] = keys[min(tid + 256 * r, all - 1)];
+    // Eight lanes to a beam, whose chunks they take in turn.
+    for (int i = tid >> 3; i < a.beams; i += 32) {
         const int row = row0 + i;
         const float s = a.scores[row];
         const bool done = a.done && a.done[row];
-        double l = __builtin_inf();
-        if (done && finite(s)) {
-            l = 0.0;
-        } else if (finite(s)) {
-            const float *ms = a.ms + (int64_t)row * a.chunks * 2;
-            float m = kNegInf;
-            for (int c = lane; c < a.chunks; c += 64)
-                m = fmaxf(m, ms[2 * c]);
-            m = seg_all<true>(m, true);
-            const float muse = m == kNegInf ? 0.f : m;
-            double sum = 0.0;
-            for (int c = lane; c < a.chunks; c += 64)
-                sum += (double)ms[2 * c + 1] * (double)fast_exp2((ms[2 * c] - muse) * 1.44269504088896341f);
+        const float *ms = a.ms + (int64_t)row * a.chunks * 2;
+        auto join = [](float &m, double &sum, float m1, double s1) {
+            const float both = fmaxf(m, m1), use = both == kNegInf ? 0.f : both;
+            sum = sum * (double)fast_exp2(m - use) + s1 * (double)fast_exp2(m1 - use);
+            m = both;
+        };
+        float m = kNegInf;
+        double sum = 0.0;
+#pragma unroll 4
+        for (int c = tid & 7; c < a.chunks; c += 8)
+            join(m, sum, ms[2 * c], ms[2 * c + 1]); // of a beam that is over: anything
 #pragma unroll
-            for (int j = 1; j < 64; j <<= 1)
-                sum += __shfl_xor(sum, j);
-            // A NaN, an infinity or no logit at all: the beam offers nothing.
-            if (finite(m) && finite((float)sum))
-                l = (double)m + log(sum);
+        for (int j = 1; j < 8; j <<= 1) {
+            const float m1 = __shfl_xor(m, j);
+            const double s1 = __shfl_xor(sum, j);
+            join(m, sum, m1, s1);
         }
-        if (lane == 0) {
+        double l = __builtin_inf();
+        if (done && finite(s))
+            l = 0.0;
+        else if (finite(s) && finite(m) && finite((float)sum)) // a NaN, an infinity or no logit at all: nothing
+            l = (double)m * 0.693147180559945309417 + log(sum);
+        if ((tid & 7) == 0) {
             lse[i] = l;
             base[i] = (double)s;
+            over[i] = done;
         }
     }
     __syncthreads();
-    const int lists = a.beams * a.chunks;
-    // Candidate r of list i: its score as an ordered number (0: none) and its place among the entry's candidates.
-    auto candidate = [&](int i, int r, uint32_t &place) -> uint64_t {
-        const int beam = i / a.chunks, row = row0 + beam;
+    __syncthreads();
+    // Candidate i's score as an ordered number (0: none) and its place among the entry's continuations.
+    auto candidate = [&](int i, uint64_t key, uint32_t &place) -> uint64_t {
+        const int beam = i / per;
         const double l = lse[beam];
         if (ordered(l) >= ordered(__builtin_inf()))
             return 0;
-        if (a.done && a.done[row]) {
+        if (over[beam]) {
             place = (uint32_t)beam * a.V + a.done_token;
-            return r == 0 && i == beam * a.chunks ? ordered(base[beam]) : 0;
+            return i == beam * per ? ordered(base[beam]) : 0;
         }
-        const uint64_t key = a.keys[((int64_t)row0 * a.chunks + i) * a.K + r];
         if (key == 0)
             return 0;
-        place = (uint32_t)beam * a.V + ~bits_lo(key);
+        place = (uint32_t)beam * a.V + ~(uint32_t)key;
         return ordered(((double)unordered((uint32_t)(key >> 32)) - l) + base[beam]);
     };
+    auto each = [&](auto &&f) __attribute__((always_inline)) {
+        uint32_t place = 0;
+#pragma unroll
+        for (int r = 0; r < HOLD; ++r)
+            if (tid + 256 * r < all) {
+                const uint64_t u = candidate(tid + 256 * r, held[r], place);
+                f(u, place);
+            }
+        for (int i = tid + 256 * HOLD; i < all; i += 256) {
+            const uint64_t u = candidate(i, keys[i], place);
+            f(u, place);
+        }
+    };
     uint64_t top = 0;
-    uint32_t place = 0;
-    for (int i = tid; i < lists; i += 256)
-        top = max(top, candidate(i, 0, place));
-    const uint64_t kth = wave_kth<uint64_t>(top, 0, a.K);
+    each([&](uint64_t u, uint32_t) { top = max(top, u); });
+    // A threshold of its upper halves, which K threads' upper halves reach.
+    const uint32_t kth = wave_kth((uint32_t)(top >> 32), 0, 1u << 16, a.K);
     if (lane == 0)
         redu[w] = kth;
     __syncthreads();
-    uint64_t least = max(max(max(redu[0], redu[1]), max(redu[2], redu[3])), (uint64_t)1);
+    const uint64_t least = max((uint64_t)max(max(redu[0], redu[1]), max(redu[2], redu[3])) << 32, (uint64_t)1);
     auto collect = [&](auto &&f) {
-        for (int i = tid; i < lists; i += 256)
-            for (int r = 0; r < a.K; ++r) {
-                const uint64_t u = candidate(i, r, place);
-                if (u < least)
-                    break;
-                if (f(u, place)) {
-                    const int at = atomicAdd(&taken, 1);
-                    if (at < kBeamFinalRoom) {
-                        rv[at] = u;
-                        ri[at] = place;
-                    }
+        each([&](uint64_t u, uint32_t place) {
+            if (u >= least && f(u, place)) {
+                const int at = atomicAdd(&taken, 1);
+                if (at < kBeamFinalRoom) {
+                    rv[at] = u;
+                    ri[at] = place;
                 }
             }
+        });
         __syncthreads();
     };
     collect([](uint64_t, uint32_t) { return true; });
@@ -290,13 +392,7 @@ __global__ __launch_bounds__(256) void attn_beam_select_kernel(const attn_beam_a
     if (n > kBeamFinalRoom) {
         auto count = [&](auto &&f) {
             int c = 0;
-            for (int i = tid; i < lists; i += 256)
-                for (int r = 0; r < a.K; ++r) {
-                    const uint64_t u = candidate(i, r, place);
-                    if (u < least)
-                        break;
-                    c += f(u, place) ? 1 : 0;
-                }
+            each([&](uint64_t u, uint32_t place) { c += u >= least && f(u, place) ? 1 : 0; });
             return wg_sum(c, redi, tid);
         };
         uint64_t v = 0;
@@ -324,6 +420,7 @@ __global__ __launch_bounds__(256) void attn_beam_select_kernel(const attn_beam_a
         const uint64_t u = rv[i];
         const uint32_t p = ri[i];
         int rank = 0;
+#pragma unroll 8
         for (int j = 0; j < n; ++j)
             rank += rv[j] > u || (rv[j] == u && ri[j] < p) ? 1 : 0;
         if (rank < a.K)
@@ -401,24 +498,18 @@ template <int NB> __global__ __launch_bounds__(256) void attn_kv_reorder_kernel(
 
 } // namespace
 
-extern "C" int attn_hip_launch_beam(const struct attn_beam_args *ap, int bits, int chunk, void *stream) {
+extern "C" int attn_hip_launch_beam(const struct attn_beam_args *ap, int bits, void *stream) {
     const attn_beam_args &a = *ap;
     const hipStream_t st = (hipStream_t)stream;
     const int64_t grid = (int64_t)a.B * a.beams * a.chunks;
-    if (grid <= 0 || grid > 0x7fffffff || a.beams > kBeamMax || a.K > 64 || (int64_t)a.chunks * chunk < a.V)
+    if (grid <= 0 || grid > 0x7fffffff || a.beams > ATTN_BEAMS_MAX || a.K > ATTN_BEAM_K_MAX ||
+        (int64_t)a.chunks * a.steps * 4 * ATTN_BEAM_STEP(bits / 8) < a.V)
         return (int)hipErrorInvalidValue;
     const dim3 g((unsigned)grid), block(256);
-    if (chunk == ATTN_BEAM_CHUNK) {
-        if (bits == 16)
-            hipLaunchKernelGGL((attn_beam_chunk_kernel<uint16_t, ATTN_BEAM_CHUNK / 256>), g, block, 0, st, a);
-        else
-            hipLaunchKernelGGL((attn_beam_chunk_kernel<float, ATTN_BEAM_CHUNK / 256>), g, block, 0, st, a);
-    } else {
-        if (bits == 16)
-            hipLaunchKernelGGL((attn_beam_chunk_kernel<uint16_t, ATTN_BEAM_CHUNK_SMALL / 256>), g, block, 0, st, a);
-        else
-            hipLaunchKernelGGL((attn_beam_chunk_kernel<float, ATTN_BEAM_CHUNK_SMALL / 256>), g, block, 0, st, a);
-    }
+    if (bits == 16)
+        hipLaunchKernelGGL(attn_beam_chunk_kernel<uint16_t>, g, block, 0, st, a);
+    else
+        hipLaunchKernelGGL(attn_beam_chunk_kernel<float>, g, block, 0, st, a);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess)
         return (int)e;
