@@ -234,7 +234,25 @@ template <int DP> __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void attn_
                             s[t][i] = kNegInf;
             bf16x8 pk[2 * NT];
             float psum;
-            auto weigh = [&]() __attribute__((always_inline)) {
+            // p against the running maximum; where there is none yet, or a lane's sum is too large, after it is raised.
+            for (bool up = __builtin_amdgcn_ballot_w64(m_run == kNegInf) != 0;; up = true) {
+                if (up) {
+                    float mx = kNegInf;
+#pragma unroll
+                    for (int t = 0; t < NT; ++t)
+#pragma unroll
+                        for (int i = 0; i < 16; i += 2)
+                            mx = max3f(mx, s[t][i], s[t][i + 1]);
+                    const float mnew = fmaxf(m_run, max_xor32(mx));
+                    const float alpha = rescale(m_run, mnew, a.c);
+                    m_run = mnew;
+                    l_run *= alpha;
+#pragma unroll
+                    for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i)
+                            o[db][i] *= alpha;
+                }
                 const float mc = m_run == kNegInf ? 0.f : m_run * a.c;
                 psum = 0.f;
 #pragma unroll
@@ -245,25 +263,8 @@ template <int DP> __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void attn_
                         psum += p;
                         pk[2 * t + (i >> 3)][i & 7] = (__bf16)p;
                     }
-            };
-            weigh();
-            if (__builtin_amdgcn_ballot_w64(!(psum <= kCrossSum) || m_run == kNegInf) != 0) {
-                float mx = kNegInf;
-#pragma unroll
-                for (int t = 0; t < NT; ++t)
-#pragma unroll
-                    for (int i = 0; i < 16; i += 2)
-                        mx = max3f(mx, s[t][i], s[t][i + 1]);
-                const float mnew = fmaxf(m_run, max_xor32(mx));
-                const float alpha = rescale(m_run, mnew, a.c);
-                m_run = mnew;
-                l_run *= alpha;
-#pragma unroll
-                for (int db = 0; db < DP / 32; ++db)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        o[db][i] *= alpha;
-                weigh();
+                if (up || __builtin_amdgcn_ballot_w64(!(psum <= kCrossSum)) == 0)
+                    break;
             }
             l_run += psum;
 #pragma unroll
@@ -691,7 +692,7 @@ __global__ __launch_bounds__(256) void attn_cross_merge_kernel(const attn_cross_
 // K's tile is read both ways. delta = sum dO O is taken on the way in and left for the kernel of dK and dV.
 // ------------------------------------------------------------------------------------------
 template <int DP>
-__global__ __launch_bounds__(256, DP == 64 ? 3 : DP == 128 ? 2 : 1) void attn_cross_dq_kernel(const attn_cross_args a) {
+__global__ __launch_bounds__(256, DP == 64 ? 4 : DP == 128 ? 2 : 1) void attn_cross_dq_kernel(const attn_cross_args a) {
     constexpr int KT = cross_tile_keys(DP), KN = DP / 16, NT = KT / 32;
     constexpr int VO = KT * DP;
     __shared__ __attribute__((aligned(1024))) uint16_t KV0[2 * VO], KV1[2 * VO];
@@ -760,6 +761,8 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : DP == 128 ? 2 : 1) void attn_cr
                 return;
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
+                if (t > 0 && kb + 32 * t >= k1)
+                    return;
                 f32x16 s, dp;
                 zero16(s);
                 zero16(dp);
