@@ -78,21 +78,13 @@ static void cross_check_rows(const char *who, const char *what, const struct att
 
 static int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-/* Pieces per group so that the number of pieces is a multiple of 8 (attn_place_of). */
-static int deal_of(int64_t groups, int tps) {
-    int d = 8;
-    while (d > 1 && (groups * (d / 2)) % 8 == 0)
-        d /= 2;
-    return d < tps ? d : tps;
-}
-
-/* Parts so that `base` workgroups become `target`, each of `least` units or more of `total`. */
+/* Parts so that `base` workgroups become up to `target`, which run at once, each of `least` units or more of `total`. */
 static struct attn_cross_cut cross_cut(int64_t groups, int tps, int64_t total, int64_t least, int64_t target,
                                        int64_t most, int step) {
     struct attn_cross_cut cut;
     memset(&cut, 0, sizeof cut);
     const int64_t base = groups * tps;
-    int64_t n = ceil_div(target, base), by_len = total / least;
+    int64_t n = target / base, by_len = total / least;
     n = n < by_len ? n : by_len;
     n = n < most ? n : most;
     n = n < ATTN_CROSS_MAX_PARTS ? n : ATTN_CROSS_MAX_PARTS;
@@ -100,8 +92,7 @@ static struct attn_cross_cut cross_cut(int64_t groups, int tps, int64_t total, i
     cut.share = (int)(ceil_div(ceil_div(total, n), step) * step);
     cut.nsplit = cut.parts = (int)n;
     cut.tps = tps;
-    cut.deal = deal_of(groups * n, tps);
-    cut.grid = (long)attn_place_grid(groups * n, tps, cut.deal);
+    cut.grid = (long)(base * n);
     return cut;
 }
 
@@ -120,7 +111,7 @@ static struct attn_cross_cut rows_cut(const struct attn_cross_call *c, int64_t R
     cut.quads = c->Hkv % 4 == 0 && bytes >= ATTN_CROSS_TEAMS * (2L << 20);
     cut.tps = (int)ceil_div(R, 16 * cut.rows16);
     cut.nsplit = (int)(slots < ATTN_CROSS_MAX_PARTS ? slots : ATTN_CROSS_MAX_PARTS);
-    cut.deal = cut.share = 1;
+    cut.share = 1;
     const int64_t lines = groups / (cut.quads ? 4 : 1), units = ceil_div(keys, 128) * lines;
     int64_t teams = ceil_div(ATTN_CROSS_TEAMS, cut.tps);
     teams = teams < units ? teams : units;
@@ -149,10 +140,19 @@ static struct attn_cross_cut dq_cut(const struct attn_cross_call *c) {
                      ATTN_CROSS_GRAD_FLOATS / ((int64_t)c->q.T * c->Hq * c->D), ATTN_CROSS_KEY_STEP);
 }
 
+/* Where tiles of states are no more than the CUs and each has rows enough, eight waves share one, as two teams that take its
+ * rows in turn: partial gradients cost 8 D bytes per state and part, written and read again. One team -> two: 4096 rows of
+ * 40 heads over 77 states, D = 64, 31.5 -> 28.4 us with their sum; 1500 of 16 heads on 4 over 300, D = 128, 42 -> 39; 37
+ * rows of 24 heads over 50 states, which keep one, 6.0 -> 8.0. */
 static struct attn_cross_cut dkv_cut(const struct attn_cross_call *c) {
+    const int64_t groups = (int64_t)c->B * c->Hkv, tps = ceil_div(bound_of(&c->k), ATTN_CROSS_KEYS);
     const int64_t steps = ceil_div(bound_of(&c->q), ATTN_CROSS_STEP) * (c->Hq / c->Hkv);
-    return cross_cut((int64_t)c->B * c->Hkv, (int)ceil_div(bound_of(&c->k), ATTN_CROSS_KEYS), steps, 2,
-                     c->D <= 128 ? 512 : 256, ATTN_CROSS_GRAD_FLOATS / ((int64_t)c->k.T * c->Hkv * c->D * 2), 1);
+    const int row_teams = c->D <= 128 && groups * tps <= 256 && groups * tps * steps >= 2048 ? 2 : 1;
+    struct attn_cross_cut cut =
+        cross_cut(groups, (int)tps, steps, 2 * row_teams, row_teams > 1 || c->D > 128 ? 256 : 512,
+                  ATTN_CROSS_GRAD_FLOATS / ((int64_t)c->k.T * c->Hkv * c->D * 2), row_teams);
+    cut.row_teams = row_teams;
+    return cut;
 }
 
 size_t attn_cross_scratch_bytes(const struct attn_cross_call *c) {
@@ -186,12 +186,10 @@ static struct attn_cross_args cross_args(const struct attn_cross_call *c) {
 }
 
 static void set_cut(struct attn_cross_args *a, const struct attn_cross_cut *cut) {
-    a->tps = cut->tps, a->nsplit = cut->nsplit, a->share = cut->share, a->deal = cut->deal;
-    a->tpp = (cut->tps + cut->deal - 1) / cut->deal;
-    a->by_tpp = attn_div_of(a->tpp), a->by_deal = attn_div_of(cut->deal);
-    a->by_nsplit = attn_div_of(cut->nsplit), a->by_heads = attn_div_of(a->Hkv), a->by_hq = attn_div_of(a->Hq), a->by_g = attn_div_of(a->g);
-    a->teams = cut->teams, a->wgs = (int)cut->grid, a->Hkv_wg = cut->quads ? a->Hkv / 4 : a->Hkv;
-    a->by_tps = attn_div_of(a->tps), a->by_B = attn_div_of(a->B), a->by_gwg = attn_div_of(a->Hq / a->Hkv_wg);
+    a->tps = cut->tps, a->nsplit = cut->nsplit, a->share = cut->share, a->wgs = (int)cut->grid;
+    a->teams = cut->teams, a->row_teams = cut->row_teams, a->Hkv_wg = cut->quads ? a->Hkv / 4 : a->Hkv;
+    a->by_tps = attn_div_of(a->tps), a->by_B = attn_div_of(a->B), a->by_heads = attn_div_of(a->Hkv);
+    a->by_hq = attn_div_of(a->Hq), a->by_g = attn_div_of(a->g), a->by_gwg = attn_div_of(a->Hq / a->Hkv_wg);
 }
 
 static void cross_run(const char *who, const struct attn_cross_call *c, const struct attn_rows *q,

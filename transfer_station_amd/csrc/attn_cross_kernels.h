@@ -162,8 +162,6 @@ template <int DP> __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void attn_
     __shared__ __attribute__((aligned(1024))) uint16_t KV0[2 * VO], KV1[2 * VO];
 
     const attn_cross_place at = attn_cross_place_of(&a, wg_id_x());
-    if (at.b < 0)
-        return;
     const int b = at.b, u = at.u, sp = at.sp;
     const int tid = wi_id_x(), w = uniform(tid >> 6), lane = tid & 63, l32 = lane & 31, hi = lane >> 5;
     const attn_range qr = q_rows(a, b), kr = k_rows(a, b);
@@ -347,7 +345,7 @@ __global__ __launch_bounds__(256, 2) void attn_cross_rows_kernel(const attn_cros
     const float c = a.c, lift = 8.f / c; // how far a score may pass the running maximum
     // This workgroup's row tile t0 and its place on the line: sequence b, group ug of kv heads, first unit `off` of the
     // sequence, `left` units in all. Neighbouring workgroups share an XCD.
-    const int L = uniform(xcd_remap(wg_id_x(), a.wgs));
+    const int L = attn_xcd_order(wg_id_x(), a.wgs);
     const int at = attn_div_by(L, a.by_tps), t0 = L - at * a.tps;
     int ug, b, off = 0, left = 1, pos0 = 0;
     line ln = {0, 1, 0, 0};
@@ -698,8 +696,6 @@ __global__ __launch_bounds__(256, DP == 64 ? 4 : DP == 128 ? 2 : 1) void attn_cr
     __shared__ __attribute__((aligned(1024))) uint16_t KV0[2 * VO], KV1[2 * VO];
 
     const attn_cross_place at = attn_cross_place_of(&a, wg_id_x());
-    if (at.b < 0)
-        return;
     const int b = at.b, u = at.u, sp = at.sp;
     const int tid = wi_id_x(), w = uniform(tid >> 6), lane = tid & 63, l32 = lane & 31, hi = lane >> 5;
     const attn_range qr = q_rows(a, b), kr = k_rows(a, b);
@@ -818,42 +814,44 @@ __global__ __launch_bounds__(256, DP == 64 ? 4 : DP == 128 ? 2 : 1) void attn_cr
 }
 
 // ------------------------------------------------------------------------------------------
-// dK and dV. One workgroup of four waves per (sequence, kv head, part of its rows, tile of 128 states): 32 states of a
-// wave keep K and V in registers, the rows of the group's heads, one head after the other, pass through LDS, Q and dO:
+// dK and dV. One workgroup per (sequence, kv head, part of its rows, tile of 128 states): 32 states of a wave keep K and V in
+// registers, the rows of the group's heads, one head after the other, pass through LDS, Q and dO:
 //   S[row][key] = Q . K^T, dP[row][key] = dO . V^T, dV^T[d][key] += dO^T . P, dK^T[d][key] += Q^T . dS
-// Both tiles are read both ways.
+// Both tiles are read both ways. Two teams of four waves (TEAMS = 2) have the same states and take steps of 32 rows in turn;
+// their sums are joined in LDS at the end.
 // ------------------------------------------------------------------------------------------
-template <int DP, bool DK, bool DV>
-__global__ __launch_bounds__(256, DP == 64 ? 3 : DP == 128 || !DK ? 2 : 1) void attn_cross_dkv_kernel(const attn_cross_args a) {
-    constexpr int QT = ATTN_CROSS_STEP, KN = DP / 16, NT = QT / 32;
+template <int DP, bool DK, bool DV, int TEAMS>
+__global__ __launch_bounds__(256 * TEAMS, TEAMS > 1 ? 1 : DP == 64 ? 3 : DP == 128 || !DK ? 2 : 1)
+void attn_cross_dkv_kernel(const attn_cross_args a) {
+    constexpr int QT = ATTN_CROSS_STEP, KN = DP / 16, KEYS = ATTN_CROSS_KEYS;
     constexpr int GO = QT * DP; // dO's tile behind Q's
-    __shared__ __attribute__((aligned(1024))) uint16_t QG0[2 * GO], QG1[2 * GO];
-    __shared__ __attribute__((aligned(16))) float st0[256], st1[256]; // lse in log2 units, from 64 on delta; the rest again
+    static_assert(QT == 32, "a step is one block of rows");
+    __shared__ __attribute__((aligned(1024))) uint16_t QG0[TEAMS * 2 * GO], QG1[TEAMS * 2 * GO];
+    __shared__ __attribute__((aligned(16))) float st0[TEAMS * 256], st1[TEAMS * 256]; // lse in log2 units, from 64 on delta
 
     const attn_cross_place at = attn_cross_place_of(&a, wg_id_x());
-    if (at.b < 0)
-        return;
     const int b = at.b, u = at.u, sp = at.sp;
     const int tid = wi_id_x(), w = uniform(tid >> 6), lane = tid & 63, l32 = lane & 31, hi = lane >> 5;
+    const int wk = w & 3, team = w >> 2;
     const attn_range qr = q_rows(a, b), kr = k_rows(a, b);
     const int g = a.g, D = a.D;
     const int per_head = uniform((qr.n + QT - 1) / QT), steps = per_head * g; // of QT rows of one head
-    const attn_cut cut = part_of(steps, a.share, a.nsplit, 1);
+    const attn_cut cut = part_of(steps, a.share, a.nsplit, TEAMS);
     if (sp >= cut.live)
         return;
     const int t0 = min(sp * cut.per, steps), t1 = min(t0 + cut.per, steps);
     const cross_lane<DP> ln(lane);
     cross_stage<DP, QT> qs, gs;
-    qs.init(w, lane, a.q_tok, D);
-    gs.init(w, lane, a.go_tok, D);
+    qs.init(wk, lane, a.q_tok, D);
+    gs.init(wk, lane, a.go_tok, D);
     auto wait_loads = [] { __builtin_amdgcn_s_waitcnt(waitcnt_vm(0)); };
 
-    for (int tile = at.tile; (int64_t)tile * ATTN_CROSS_KEYS < kr.n; tile += a.tps) {
+    for (int tile = at.tile; (int64_t)tile * KEYS < kr.n; tile += a.tps) {
         // The wave's rows of K and V, by lane: what lies past the last state or past D is outside the buffer, zeros.
         bf16x8 kf[KN], vf[KN];
         {
-            const int64_t first = kr.at + tile * ATTN_CROSS_KEYS + 32 * w;
-            const int rows = min(32, kr.n - tile * ATTN_CROSS_KEYS - 32 * w);
+            const int64_t first = kr.at + tile * KEYS + 32 * wk;
+            const int rows = min(32, kr.n - tile * KEYS - 32 * wk);
             const auto rk = make_rsrc(a.k + first * a.k_tok + u * a.k_head, row_bytes(rows, a.k_tok, D));
             const auto rv = make_rsrc(a.v + first * a.v_tok + u * a.v_head, row_bytes(rows, a.v_tok, D));
             const uint32_t ok = l32 * (uint32_t)(a.k_tok * 2) + hi * 16, ov = l32 * (uint32_t)(a.v_tok * 2) + hi * 16;
@@ -872,27 +870,38 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : DP == 128 || !DK ? 2 : 1) void 
             zero16(dv[db]);
         }
         // The step to load: head and step of it. Behind the part's last step come empty ones: nothing is read, and P
-        // is 0, as it is past a head's last row: 2^(0 - inf). No branch goes around a step, and the two of a turn are
-        // one block: at a branch the allocator copied accumulators to and fro, or to memory.
-        int ls = t0, lh = uniform(t0 / max(per_head, 1)), lt = t0 - lh * per_head;
+        // is 0, as it is past a head's last row: 2^(0 - inf). No branch goes around a step: there the
+        // allocator copied accumulators to and fro, or to memory.
+        const int from = max(min(t0 + team, t1 - 1), 0);
+        int ls = t0 + team, lh = uniform(from / max(per_head, 1)), lt = from - lh * per_head;
         float st; // of one row of that step: lse (even waves) or delta
         auto load = [&](uint16_t *to) __attribute__((always_inline)) {
             const int h = u * g + lh, r0 = lt * QT, rows = ls < t1 ? min(qr.n - r0, QT) : 0;
             const int64_t first = qr.at + r0;
-            qs.load(a.q + first * a.q_tok + h * a.q_head, rows, a.q_tok, D, to, w);
-            gs.load(a.go + first * a.go_tok + h * a.go_head, rows, a.go_tok, D, to + GO, w);
+            qs.load(a.q + first * a.q_tok + h * a.q_head, rows, a.q_tok, D, to + team * 2 * GO, wk);
+            gs.load(a.go + first * a.go_tok + h * a.go_head, rows, a.go_tok, D, to + team * 2 * GO + GO, wk);
             const int r = opaque(lane) & (QT - 1);
             const float *src = (w & 1 ? a.delta : a.lse) + first * a.Hq + h;
             const float x = src[max(min(r, rows - 1), 0) * a.Hq];
             st = w & 1 ? x : r < rows ? x * kLog2e : __builtin_inff();
-            if (++ls < t1 && ++lt == per_head) { // the last step's place stays: the empty ones name it
-                lt = 0;
-                ++lh;
+            ls += TEAMS;
+            // The last step's place stays: the empty ones name it. At D = 256 without a branch, with which registers spill
+            // (2 x 2048 rows of 16 heads on 8 over as many states: dV 346 us, without 209); below it is faster with one
+            // (32 heads on 8, 4096, D = 64: 672 and 736).
+            if constexpr (DP > 128) {
+                static_assert(TEAMS == 1, "one head further at most");
+                lt += ls < t1 ? 1 : 0;
+                const int over = lt == per_head ? 1 : 0;
+                lh += over;
+                lt -= over * per_head;
+            } else if (ls < t1) {
+                for (lt += TEAMS; lt >= per_head; lt -= per_head)
+                    ++lh;
             }
         };
         auto compute = [&](const uint16_t *qg, const float *sb) __attribute__((always_inline)) {
-#pragma unroll
-            for (int t = 0; t < NT; ++t) {
+            {
+                constexpr int t = 0; // of the steps' rows one block
                 f32x16 s, dp;
                 zero16(s);
                 zero16(dp);
@@ -941,23 +950,38 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : DP == 128 || !DK ? 2 : 1) void 
             st0[tid] = st;
             wait_loads();
             __syncthreads();
-            auto step = [&](const uint16_t *qg, const float *sb, uint16_t *next, float *sn)
-                __attribute__((always_inline)) {
+            auto step = [&](const uint16_t *qg, const float *sb, uint16_t *next, float *sn) __attribute__((always_inline)) {
                 load(next);
-                compute(qg, sb);
+                compute(qg + team * 2 * GO, sb + team * 256);
                 wait_loads();
                 sn[tid] = st;
                 __syncthreads();
             };
-            for (int i = t0; i < t1; i += 2) {
+            for (int i = t0; i < t1; i += 2 * TEAMS) {
                 step(QG0, st0, QG1, st1);
                 step(QG1, st1, QG0, st0);
             }
         }
+        if constexpr (TEAMS > 1) {
+            // The second team leaves its sums in the tiles' place: 4 waves x DP 128 bytes in two buffers of DP 256.
+            float *const place = reinterpret_cast<float *>(wk & 2 ? QG1 : QG0) + (wk & 1) * (DP * 32) + lane;
+            auto join = [&](f32x16 *x) __attribute__((always_inline)) {
+#pragma unroll
+                for (int i = 0; team == 1 && i < DP / 2; ++i)
+                    place[i * 64] = x[i / 16][i % 16];
+                __syncthreads();
+#pragma unroll
+                for (int i = 0; team == 0 && i < DP / 2; ++i)
+                    x[i / 16][i % 16] += place[i * 64];
+                __syncthreads();
+            };
+            join(dk);
+            join(dv);
+        }
         // Taken from the lane anew, so that nothing of it is held through the loop.
-        const int ln2 = opaque(lane), hi2 = ln2 >> 5, key = tile * ATTN_CROSS_KEYS + 32 * w + (ln2 & 31);
+        const int ln2 = opaque(lane), hi2 = ln2 >> 5, key = tile * KEYS + 32 * wk + (ln2 & 31);
         const int64_t tok = kr.at + key;
-        if (key < kr.n) {
+        if (team == 0 && key < kr.n) {
             if (cut.live == 1) {
                 if (DK)
                     put_row<DP>(dk, a.scale, a.dk + tok * a.dk_tok + u * a.dk_head, hi2, D);
@@ -980,7 +1004,7 @@ __global__ __launch_bounds__(256) void attn_cross_sum_kernel(const attn_cross_ar
     const int b = uniform(wg_id_x() / tpm), t0 = wg_id_x() - b * tpm, tid = wi_id_x();
     const attn_range qr = q_rows(a, b), kr = k_rows(a, b);
     const int g = a.g, H = KV ? a.Hkv : a.Hq, W = KV ? 2 * a.D : a.D; // floats of a row's part
-    const attn_cut cut = KV ? part_of((qr.n + ATTN_CROSS_STEP - 1) / ATTN_CROSS_STEP * g, a.share, a.nsplit, 1)
+    const attn_cut cut = KV ? part_of((qr.n + ATTN_CROSS_STEP - 1) / ATTN_CROSS_STEP * g, a.share, a.nsplit, a.row_teams)
                             : part_of(kr.n, a.share, a.nsplit, ATTN_CROSS_KEY_STEP);
     if (cut.live == 1)
         return; // written already
@@ -1027,7 +1051,7 @@ int lg_lanes(int n) {
 
 bool cross_grid_ok(const attn_cross_args &a, const attn_cross_cut &cut) {
     return cut.grid > 0 && cut.grid <= ATTN_CROSS_MAX_GRID && a.nsplit >= 1 && a.nsplit <= ATTN_CROSS_MAX_PARTS &&
-           a.tps >= 1 && a.deal >= 1;
+           a.tps >= 1;
 }
 
 // Workgroups per sequence that look over `rows` rows at rpw a time, not above 2^18 in all.
@@ -1110,24 +1134,35 @@ extern "C" int attn_hip_launch_cross_grad(const struct attn_cross_args *ap, cons
     const dim3 grid((unsigned)cut->grid), block(256);
     const hipError_t e = with_width(a.D, [&](auto W) {
         constexpr int DP = decltype(W)::value;
-        if (t_plan) {
-            for (int i = 0; i < (kv && DP > 128 ? 2 : 1); ++i)
-                plan_note(grid, block, "attn_cross_%s_kernel<%d%s> parts=%d share=%d", kv ? "dkv" : "dq", DP,
-                          !kv ? "" : DP <= 128 ? ", true, true" : i ? ", false, true" : ", true, false", a.nsplit, a.share);
-            return hipSuccess;
-        }
         if (!kv) {
+            if (t_plan) {
+                plan_note(grid, block, "attn_cross_dq_kernel<%d> parts=%d share=%d", DP, a.nsplit, a.share);
+                return hipSuccess;
+            }
             hipLaunchKernelGGL((attn_cross_dq_kernel<DP>), grid, block, 0, st, a);
-        } else if constexpr (DP <= 128) {
-            hipLaunchKernelGGL((attn_cross_dkv_kernel<DP, true, true>), grid, block, 0, st, a);
-        } else {
-            hipLaunchKernelGGL((attn_cross_dkv_kernel<DP, true, false>), grid, block, 0, st, a);
-            const hipError_t x = hipGetLastError();
-            if (x != hipSuccess)
-                return x;
-            hipLaunchKernelGGL((attn_cross_dkv_kernel<DP, false, true>), grid, block, 0, st, a);
+            return hipGetLastError();
         }
-        return hipGetLastError();
+        auto dkv = [&](auto K, auto V, auto T) {
+            constexpr bool kK = decltype(K)::value, kV = decltype(V)::value;
+            constexpr int kT = decltype(T)::value;
+            if (t_plan) {
+                plan_note(grid, dim3(256 * kT), "attn_cross_dkv_kernel<%d, %s, %s, %d> parts=%d share=%d", DP, tf(kK),
+                          tf(kV), kT, a.nsplit, a.share);
+                return hipSuccess;
+            }
+            hipLaunchKernelGGL((attn_cross_dkv_kernel<DP, kK, kV, kT>), grid, dim3(256 * kT), 0, st, a);
+            return hipGetLastError();
+        };
+        constexpr std::true_type yes;
+        constexpr std::false_type no;
+        constexpr std::integral_constant<int, 1> one;
+        constexpr std::integral_constant<int, 2> two;
+        if constexpr (DP > 128) {
+            const hipError_t x = dkv(yes, no, one);
+            return x != hipSuccess ? x : dkv(no, yes, one);
+        } else {
+            return cut->row_teams == 2 ? dkv(yes, yes, two) : dkv(yes, yes, one);
+        }
     });
     if (e != hipSuccess || a.nsplit == 1)
         return (int)e;

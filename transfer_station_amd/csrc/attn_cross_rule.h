@@ -67,14 +67,14 @@ ATTN_HD struct attn_div attn_div_of(int d) {
 }
 ATTN_HD int attn_div_by(int n, struct attn_div x) { return (int)(((uint64_t)(uint32_t)n * x.mul) >> x.shift); }
 
-/* What one launch looks like: row (or state) tiles per group and its parts, and how the groups are dealt to the XCDs
- * (attn_place_of). */
+/* What one launch looks like: row (or state) tiles of a sequence and kv head, its parts, and their share of units. */
 struct attn_cross_cut {
-    int tps, nsplit, share, deal;
+    int tps, nsplit, share;
     int rows16; /* blocks of 16 rows per workgroup of the kernel for few rows, 0: tiles of 128 */
     int quads;  /* that kernel's form for four kv heads of a workgroup, a wave each */
     int parts;  /* of a sequence of the call's bounds, about */
     int teams;  /* that kernel: teams of the decode line, 0: whole sequences */
+    int row_teams; /* the kernel of dK and dV: teams of four waves that share a tile of states */
     long grid;
 };
 
@@ -88,28 +88,31 @@ struct attn_cross_args {
     int q_is_len, k_is_len;
     int B, Tq, Tk, Hq, Hkv, g, D; /* g = Hq / Hkv */
     float c, scale; /* scale log2(e), scale */
-    int tps, nsplit, share, deal, tpp;
-    int teams, wgs, Hkv_wg; /* few rows: teams of the decode line, workgroups, groups of kv heads */
-    struct attn_div by_tpp, by_deal, by_nsplit, by_heads, by_hq, by_g; /* tpp, deal, nsplit, Hkv, Hq, g */
-    struct attn_div by_tps, by_B, by_gwg;                              /* tps, B, query heads of a group of kv heads */
+    int tps, nsplit, share, wgs;
+    int teams, Hkv_wg; /* few rows: teams of the decode line, groups of kv heads */
+    int row_teams;     /* dK and dV */
+    struct attn_div by_tps, by_B, by_heads, by_hq, by_g, by_gwg; /* tps, B, Hkv, Hq, g, query heads of a group of kv heads */
     float *pm, *pl, *pacc; /* partial maxima, sums and rows; of gradients: rows in pacc */
 };
 
-/* Where a workgroup is: attn_place_of, and its group as a sequence, a kv head and a part of them (innermost). */
+/* Where a workgroup is. Hardware ids are dealt to the eight XCDs in turn: each takes neighbouring places of the order
+ * [part][kv head][sequence][tile], so that a sequence's tiles, which read the same rows, share its L2, and sequences of
+ * unequal length, which lie next to each other, leave no XCD idle. */
 struct attn_cross_place {
-    int b, u, sp, tile; /* b -1: none */
+    int b, u, sp, tile;
 };
+ATTN_HD int attn_xcd_order(int wg, int n) {
+    const int per = n >> 3, rem = n & 7, x = wg & 7;
+    return (x < rem ? x * (per + 1) : rem * (per + 1) + (x - rem) * per) + (wg >> 3);
+}
 ATTN_HD struct attn_cross_place attn_cross_place_of(const struct attn_cross_args *a, int wg) {
-    const int i = wg >> 3, slot = attn_div_by(i, a->by_tpp);
-    const int piece = (wg & 7) + 8 * slot, group = attn_div_by(piece, a->by_deal);
-    const int bu = attn_div_by(group, a->by_nsplit);
+    const int at = attn_xcd_order(wg, a->wgs), group = attn_div_by(at, a->by_tps);
+    const int us = attn_div_by(group, a->by_B);
     struct attn_cross_place p;
-    p.tile = piece - group * a->deal + a->deal * (i - slot * a->tpp);
-    p.sp = group - bu * a->nsplit;
-    p.b = attn_div_by(bu, a->by_heads);
-    p.u = bu - p.b * a->Hkv;
-    if (p.b >= a->B || p.tile >= a->tps)
-        p.b = -1;
+    p.tile = at - group * a->tps;
+    p.b = group - us * a->B;
+    p.sp = attn_div_by(us, a->by_heads);
+    p.u = us - p.sp * a->Hkv;
     return p;
 }
 
