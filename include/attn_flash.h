@@ -213,8 +213,9 @@ struct attn_spans {
     int32_t T, max;
 };
 
-/* D % 16 == 0, 16 <= D <= 256; scale 0: 1/sqrt(D). Limits: B * Hkv <= 2^20, q.T * Hq and k.T * Hkv <= 2^30. The token
- * strides of all tensors of a call are in [D, ATTN_TOKEN_MAX] elements. */
+/* D % 16 == 0, 16 <= D <= 256; scale 0: 1/sqrt(D). Limits: B * Hkv <= 2^20, q.T * Hq and k.T * Hkv <= 2^30, and, as any
+ * sequence may claim all states, B * Hkv * (k.T / 128 + 8) and B * (Hq * q.max / 16 + 8 Hkv) <= 2^30. The token strides of
+ * all tensors of a call are in [D, ATTN_TOKEN_MAX] elements. */
 #define ATTN_TOKEN_MAX 4194304 /* 2^22 */
 struct attn_cross_call {
     struct attn_spans q, k;
@@ -270,10 +271,11 @@ struct attn_beams {
 };
 
 /* The K best continuations of each entry, best first: score = (x - log sum exp x) + scores, token and parent, the row
- * (b * beams + i) that it continues; [B][K] each. Ties go to the lowest beam, then token. A done beam's only
- * continuation is done_token, at its score; a logit of -inf is none, and a beam whose score is not finite, or that
- * has a NaN or +inf among its logits, has none. Where an entry has fewer than K, the rest is score -inf, token -1 and
- * the entry's first row. The sums of exponentials are taken in fp32, all else in fp64, and the score is rounded once.
+ * (b * beams + i) that it continues; [B][K] each. Ties go to the lowest beam, of its own to the largest logit, then the
+ * lowest token. A done beam's only continuation is done_token, at its score; a logit of -inf is none, and a beam whose
+ * score is not finite, or that has a NaN or +inf among its logits, has none. Where an entry has fewer than K, the rest is
+ * score -inf, token -1 and the entry's first row. The sums of exponentials are taken in fp32, all else in fp64, and the
+ * score is rounded once.
  * scratch: attn_beam_scratch_bytes(c) bytes, ATTN_SCRATCH_ALIGN-aligned; calls that may overlap need one each. */
 size_t attn_beam_scratch_bytes(const struct attn_beams *c);
 void attn_beam_select(const struct attn_beams *c, float *score, int32_t *token, int32_t *parent, void *scratch);

@@ -25,20 +25,21 @@ def select_ref(x, scores, done, done_token, B, beams, K):
     out = np.full((B, K), -np.inf), np.full((B, K), -1), np.repeat(beams * np.arange(B)[:, None], K, 1)
     for b in range(B):
         rows = slice(b * beams, (b + 1) * beams)
-        c = np.full((beams, V), -np.inf)
+        # [beam][its continuations, by logit and token]: a stable sort by score then has the order of ties.
+        c, tok = np.full((beams, min(K, V)), -np.inf), np.zeros((beams, min(K, V)), int)
         for i, r in enumerate(range(rows.start, rows.stop)):
             if not np.isfinite(scores[r]):
                 continue
             if done is not None and done[r]:
-                c[i, done_token] = scores[r]
+                c[i, 0], tok[i, 0] = scores[r], done_token
             elif np.all(np.isfinite(x[r]) | (x[r] == -np.inf)) and np.any(np.isfinite(x[r])):
                 top = x[r].max()
-                c[i] = (x[r] - (top + np.log(np.exp(x[r] - top).sum()))) + float(scores[r])
-        c = c.reshape(-1)
-        best = np.argsort(-c, kind="stable")[:K]
-        best = best[np.isfinite(c[best])]
-        out[0][b, :len(best)], out[1][b, :len(best)] = c[best], best % V
-        out[2][b, :len(best)] = b * beams + best // V
+                tok[i] = np.argsort(-x[r], kind="stable")[:K]
+                c[i] = (x[r, tok[i]] - (top + np.log(np.exp(x[r] - top).sum()))) + float(scores[r])
+        best = np.argsort(-c.reshape(-1), kind="stable")[:K]
+        best = best[np.isfinite(c.reshape(-1)[best])]
+        out[0][b, :len(best)], out[1][b, :len(best)] = c.reshape(-1)[best], tok.reshape(-1)[best]
+        out[2][b, :len(best)] = b * beams + best // c.shape[1]
     return out
 
 

@@ -85,7 +85,9 @@ __device__ __forceinline__ int wg_sum(int x, int *red, int tid) {
 }
 
 // ------------------------------------------------------------------------------------------
-// One chunk of a row: a reference r, its largest x log2(e) rounded, the sum of 2^(x log2(e) - r), and its K largest logits, of equals those at the lowest index.
+// One chunk of a row: its largest logit m, the sum of exp(x - m), and its K largest logits, of equals those at the lowest
+// index. x - m is taken first, for all sizes of x: m log2(e), rounded, is off by more than an exponent of 1 from 2^24 on,
+// and has none at a mask of the type's lowest value.
 // The four waves take neighbouring pieces of it, a step of 4 KB at a time with the next on its way, each lane with a
 // maximum and sum of its own. A wave's threshold is a value that at least K of its lanes have reached (wave_kth), taken
 // anew as the number of steps doubles: some K logits pass it per doubling. They go to LDS; at the end those below the best
@@ -150,7 +152,7 @@ template <typename T> __global__ __launch_bounds__(256, 4) void attn_beam_chunk_
             }
         }
     };
-    float m = kNegInf, ref = 0.f, sum = 0.f; // of this lane: sum of 2^(x log2(e) - ref), ref the rounded m log2(e)
+    float m = kNegInf, sum = 0.f; // of this lane: sum of exp(x - m), 0 while there is no m
     uint32_t least = kOrderedNegInf + 1;
     int taken = 0; // of this wave
     u32x4 v[NV], next[NV];
@@ -165,15 +167,15 @@ template <typename T> __global__ __launch_bounds__(256, 4) void attn_beam_chunk_
 #pragma unroll
             for (int i = 0; i < VEC; i += 2)
                 top = max3f(top, value(v[j], i), value(v[j], i + 1));
+        const float was = m;
         m = fmaxf(m, top);
-        const float to = m == kNegInf ? 0.f : m * kLog2E;
-        sum *= fast_exp2(ref - to);
-        ref = to;
+        const float ref = m == kNegInf ? 0.f : m;
+        sum *= fast_exp2((was - ref) * kLog2E);
 #pragma unroll
         for (int j = 0; j < NV; ++j)
 #pragma unroll
             for (int i = 0; i < VEC; ++i)
-                sum += fast_exp2(fmaf(value(v[j], i), kLog2E, -ref));
+                sum += fast_exp2((value(v[j], i) - ref) * kLog2E);
         if ((n & (n - 1)) == 0)
             least = max(least, wave_kth(ordered(m), kOrderedNegInf, 1u << 20, a.K));
         const float pass = unordered(least);
@@ -197,9 +199,8 @@ template <typename T> __global__ __launch_bounds__(256, 4) void attn_beam_chunk_
         for (int j = 0; j < NV; ++j)
             v[j] = next[j];
     }
-    // A lane without a logit has a sum of 0, and no part in the reference.
-    const float wm = seg_all<true>(m == kNegInf ? kNegInf : ref, true), wuse = wm == kNegInf ? 0.f : wm;
-    sum = seg_all<false>(m == kNegInf ? 0.f : sum * fast_exp2(ref - wuse), true);
+    const float wm = seg_all<true>(m, true), wuse = wm == kNegInf ? 0.f : wm;
+    sum = seg_all<false>(sum * fast_exp2((m - wuse) * kLog2E), true); // of a lane without a logit: 0
     if (lane == 0) {
         redm[w] = wm;
         reds[w] = sum;
@@ -213,7 +214,7 @@ template <typename T> __global__ __launch_bounds__(256, 4) void attn_beam_chunk_
         float s = 0.f;
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-            s += reds[i] * fast_exp2(redm[i] - use);
+            s += reds[i] * fast_exp2((redm[i] - use) * kLog2E);
         a.ms[2 * part] = all;
         a.ms[2 * part + 1] = s;
     }
@@ -279,17 +280,35 @@ template <typename T> __global__ __launch_bounds__(256, 4) void attn_beam_chunk_
 }
 
 // ------------------------------------------------------------------------------------------
-// A batch entry's K best from its beams' chunks, by (x - lse) + score in fp64, of equals those of the lowest beam and
-// index: the threads' own maxima give a threshold that at least K candidates reach, and what reaches it counts how many are
+// A batch entry's K best from its beams' chunks, by (x - lse) + score in fp64, of equals those of the lowest beam, then
+// the largest logit, then the lowest index: the threads' own maxima give a threshold that at least K candidates reach, and what reaches it counts how many are
 // ahead. Bound by latency: one round of loads, two sums over a beam's chunks, a search and a count.
 // ------------------------------------------------------------------------------------------
 constexpr int kBeamFinalRoom = 1024;
+constexpr double kLn2D = 0.693147180559945309417;
+
+// log x of a normal x > 0: x = 2^e f with f in [sqrt(1/2), sqrt(2)], log f = 2 artanh s with s = (f - 1) / (f + 1), whose
+// series s + s^3 / 3 + ... is cut where s^2 <= 0.0295 leaves less than 2^-55. In line: the library's is a call.
+__device__ __forceinline__ double log_of(double x) {
+    double f = __builtin_amdgcn_frexp_mant(x); // in [1/2, 1)
+    int e = __builtin_amdgcn_frexp_exp(x);
+    if (f < 0.707106781186547524401) {
+        f *= 2.0;
+        --e;
+    }
+    const double s = (f - 1.0) / (f + 1.0), t = s * s;
+    double r = 1.0 / 19;
+#pragma unroll
+    for (int i = 17; i >= 1; i -= 2)
+        r = fma(r, t, 1.0 / i);
+    return fma((double)e, kLn2D, 2.0 * s * r);
+}
 
 __global__ __launch_bounds__(256) void attn_beam_select_kernel(const attn_beam_args a) {
     __shared__ double lse[ATTN_BEAMS_MAX], base[ATTN_BEAMS_MAX]; // of a done beam: 0; of one without a continuation: infinite
     __shared__ uint8_t over[ATTN_BEAMS_MAX];
-    __shared__ uint64_t rv[kBeamFinalRoom];
-    __shared__ uint32_t ri[kBeamFinalRoom], redu[4];
+    __shared__ uint64_t rv[kBeamFinalRoom], ri[kBeamFinalRoom];
+    __shared__ uint32_t redu[4];
     __shared__ int redi[4], taken;
     const int b = wg_id_x(), tid = wi_id_x(), lane = tid & 63, w = uniform(tid >> 6);
     const int row0 = b * a.beams;
@@ -311,7 +330,7 @@ __global__ __launch_bounds__(256) void attn_beam_select_kernel(const attn_beam_a
         const float *ms = a.ms + (int64_t)row * a.chunks * 2;
         auto join = [](float &m, double &sum, float m1, double s1) {
             const float both = fmaxf(m, m1), use = both == kNegInf ? 0.f : both;
-            sum = sum * (double)fast_exp2(m - use) + s1 * (double)fast_exp2(m1 - use);
+            sum = sum * (double)fast_exp2((m - use) * kLog2E) + s1 * (double)fast_exp2((m1 - use) * kLog2E);
             m = both;
         };
         float m = kNegInf;
@@ -329,7 +348,7 @@ __global__ __launch_bounds__(256) void attn_beam_select_kernel(const attn_beam_a
         if (done && finite(s))
             l = 0.0;
         else if (finite(s) && finite(m) && finite((float)sum)) // a NaN, an infinity or no logit at all: nothing
-            l = (double)m * 0.693147180559945309417 + log(sum);
+            l = (double)m + log_of(sum);
         if ((tid & 7) == 0) {
             lse[i] = l;
             base[i] = (double)s;
@@ -337,37 +356,40 @@ __global__ __launch_bounds__(256) void attn_beam_select_kernel(const attn_beam_a
         }
     }
     __syncthreads();
-    __syncthreads();
-    // Candidate i's score as an ordered number (0: none) and its place among the entry's continuations.
-    auto candidate = [&](int i, uint64_t key, uint32_t &place) -> uint64_t {
+    // Candidate i's score as an ordered number (0: none), and a number that is larger the further ahead it is among equal
+    // ones: of the lowest beam, then the largest logit, then the lowest token.
+    constexpr uint64_t LOW = ATTN_BEAM_V_MAX - 1;
+    static_assert((LOW & (LOW + 1)) == 0 && LOW < 1u << 20 && ATTN_BEAMS_MAX <= 1 << 8, "60 bits");
+    auto candidate = [&](int i, uint64_t key, uint64_t &tie) -> uint64_t {
         const int beam = i / per;
         const double l = lse[beam];
         if (ordered(l) >= ordered(__builtin_inf()))
             return 0;
+        tie = (uint64_t)(ATTN_BEAMS_MAX - 1 - beam) << 52;
         if (over[beam]) {
-            place = (uint32_t)beam * a.V + a.done_token;
+            tie |= LOW - a.done_token;
             return i == beam * per ? ordered(base[beam]) : 0;
         }
         if (key == 0)
             return 0;
-        place = (uint32_t)beam * a.V + ~(uint32_t)key;
+        tie |= key >> 32 << 20 | (LOW - ~(uint32_t)key);
         return ordered(((double)unordered((uint32_t)(key >> 32)) - l) + base[beam]);
     };
     auto each = [&](auto &&f) __attribute__((always_inline)) {
-        uint32_t place = 0;
+        uint64_t tie = 0;
 #pragma unroll
         for (int r = 0; r < HOLD; ++r)
             if (tid + 256 * r < all) {
-                const uint64_t u = candidate(tid + 256 * r, held[r], place);
-                f(u, place);
+                const uint64_t u = candidate(tid + 256 * r, held[r], tie);
+                f(u, tie);
             }
         for (int i = tid + 256 * HOLD; i < all; i += 256) {
-            const uint64_t u = candidate(i, keys[i], place);
-            f(u, place);
+            const uint64_t u = candidate(i, keys[i], tie);
+            f(u, tie);
         }
     };
     uint64_t top = 0;
-    each([&](uint64_t u, uint32_t) { top = max(top, u); });
+    each([&](uint64_t u, uint64_t) { top = max(top, u); });
     // A threshold of its upper halves, which K threads' upper halves reach.
     const uint32_t kth = wave_kth((uint32_t)(top >> 32), 0, 1u << 16, a.K);
     if (lane == 0)
@@ -375,39 +397,38 @@ __global__ __launch_bounds__(256) void attn_beam_select_kernel(const attn_beam_a
     __syncthreads();
     const uint64_t least = max((uint64_t)max(max(redu[0], redu[1]), max(redu[2], redu[3])) << 32, (uint64_t)1);
     auto collect = [&](auto &&f) {
-        each([&](uint64_t u, uint32_t place) {
-            if (u >= least && f(u, place)) {
+        each([&](uint64_t u, uint64_t tie) {
+            if (u >= least && f(u, tie)) {
                 const int at = atomicAdd(&taken, 1);
                 if (at < kBeamFinalRoom) {
                     rv[at] = u;
-                    ri[at] = place;
+                    ri[at] = tie;
                 }
             }
         });
         __syncthreads();
     };
-    collect([](uint64_t, uint32_t) { return true; });
+    collect([](uint64_t, uint64_t) { return true; });
     int n = taken;
     __syncthreads();
     if (n > kBeamFinalRoom) {
         auto count = [&](auto &&f) {
             int c = 0;
-            each([&](uint64_t u, uint32_t place) { c += u >= least && f(u, place) ? 1 : 0; });
+            each([&](uint64_t u, uint64_t tie) { c += u >= least && f(u, tie) ? 1 : 0; });
             return wg_sum(c, redi, tid);
         };
-        uint64_t v = 0;
-        uint32_t last = 0;
+        uint64_t v = 0, last = 0;
         for (uint64_t bit = 1ull << 63; bit; bit >>= 1)
-            if (count([&](uint64_t u, uint32_t) { return u >= (v | bit); }) >= a.K)
+            if (count([&](uint64_t u, uint64_t) { return u >= (v | bit); }) >= a.K)
                 v |= bit;
-        const int need = a.K - count([&](uint64_t u, uint32_t) { return u > v; });
-        for (uint32_t bit = 0x80000000u; bit; bit >>= 1)
-            if (count([&](uint64_t u, uint32_t i) { return u == v && i < (last | bit); }) < need)
+        const int need = a.K - count([&](uint64_t u, uint64_t) { return u > v; });
+        for (uint64_t bit = 1ull << 59; bit; bit >>= 1)
+            if (count([&](uint64_t u, uint64_t i) { return u == v && i >= (last | bit); }) >= need)
                 last |= bit;
         if (tid == 0)
             taken = 0;
         __syncthreads();
-        collect([&](uint64_t u, uint32_t i) { return u > v || (u == v && i <= last); });
+        collect([&](uint64_t u, uint64_t i) { return u > v || (u == v && i >= last); });
         n = min(taken, kBeamFinalRoom);
     }
     auto put = [&](int r, float score, int token, int parent) {
@@ -418,13 +439,13 @@ __global__ __launch_bounds__(256) void attn_beam_select_kernel(const attn_beam_a
     };
     for (int i = tid; i < n; i += 256) {
         const uint64_t u = rv[i];
-        const uint32_t p = ri[i];
+        const uint64_t p = ri[i];
         int rank = 0;
 #pragma unroll 8
         for (int j = 0; j < n; ++j)
-            rank += rv[j] > u || (rv[j] == u && ri[j] < p) ? 1 : 0;
+            rank += rv[j] > u || (rv[j] == u && ri[j] > p) ? 1 : 0;
         if (rank < a.K)
-            put(rank, (float)unordered(u), (int)(p % (uint32_t)a.V), row0 + (int)(p / (uint32_t)a.V));
+            put(rank, (float)unordered(u), (int)(LOW - (p & LOW)), row0 + ATTN_BEAMS_MAX - 1 - (int)(p >> 52));
     }
     for (int i = n + tid; i < a.K; i += 256)
         put(i, kNegInf, -1, row0);
