@@ -11,10 +11,10 @@ E32 = 2.0 ** -24  # half a step of fp32
 
 class Batch:
     """seqs: (rows, states) of each sequence. Packed, or (room given) padded: each sequence has room[0] rows and room[1]
-    states. What no sequence names is NaN. order: in which order the sequences lie (packed)."""
+    states. What no sequence names is NaN. claim: how many states the call says that there are (0: as many as there are)."""
 
-    def __init__(self, seqs, Hq, Hkv, D, seed, room=None, pad=3, sigma_q=1.0, stride=0, offset=0):
-        self.seqs, self.Hq, self.Hkv, self.D, self.room = seqs, Hq, Hkv, D, room
+    def __init__(self, seqs, Hq, Hkv, D, seed, room=None, claim=0, pad=3, sigma_q=1.0, stride=0, offset=0):
+        self.seqs, self.Hq, self.Hkv, self.D, self.room, self.claim = seqs, Hq, Hkv, D, room, claim
         self.B = len(seqs)
         self.spans = {}
         for x, i, heads in (("q", 0, Hq), ("k", 1, Hkv)):
@@ -121,6 +121,8 @@ def call_of(t, bufs, scale=0.0, max_q=None, max_k=None):
     def spans(x, i, most):
         start, n, T = t.spans[x]
         most = most or max([s[i] for s in t.seqs] + [1])
+        if i and t.claim:
+            T = most = t.claim
         bufs[x + "_start"] = ts.DeviceBuffer.from_array(start)
         if t.room:
             bufs[x + "_len"] = ts.DeviceBuffer.from_array(n)
@@ -145,17 +147,21 @@ def run(t, scale=0.0, grad=True, max_q=None, max_k=None, lse=True):
         r[x] = _rows(bufs[x], s[1], D)
     bufs["lse"] = ts.DeviceBuffer(4 * t.Tq * t.Hq)
     bufs["lse"].fill_bytes(0xFF)
-    bufs["s"] = ts.DeviceBuffer(ts.attn_cross_scratch_bytes(call))
+    guard = 4096  # bytes behind a workspace, which have to stay
+    bufs["s"] = ts.DeviceBuffer(ts.attn_cross_scratch_bytes(call) + guard)
     bufs["s"].fill_bytes(0xFF)
     ts.attn_cross(call, r["q"], r["k"], r["v"], r["o"], bufs["lse"] if lse else None, bufs["s"])
     names = ["o"]
     if grad:
-        bufs["gs"] = ts.DeviceBuffer(ts.attn_cross_grad_scratch_bytes(call))
+        bufs["gs"] = ts.DeviceBuffer(ts.attn_cross_grad_scratch_bytes(call) + guard)
         bufs["gs"].fill_bytes(0xFF)
         ts.attn_cross_grad(call, r["q"], r["k"], r["v"], r["o"], bufs["lse"], r["go"], r["dq"], r["dk"], r["dv"],
                            bufs["gs"])
         names += ["dq", "dk", "dv"]
     ts.synchronize()
+    for x in ("s", "gs"):
+        if x in bufs:
+            assert np.all(bufs[x].download(np.uint8)[-guard:] == 0xFF), x
     out = {}
     for x in names:
         heads, live = (t.Hq, t.live_q) if x in ("o", "dq") else (t.Hkv, t.live_k)
