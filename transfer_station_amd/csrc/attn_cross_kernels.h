@@ -55,17 +55,17 @@ __device__ __forceinline__ uint32_t row_bytes(int rows, int64_t tok, int D) {
     return rows < 1 ? 0u : (uint32_t)(rows - 1) * (uint32_t)(tok * 2) + D * 2;
 }
 
-// ROWS rows of a token tensor into LDS by four waves' LDS-DMA. Wave w writes the KBs whose rows' groups are w mod 4 (at
-// DP = 64 2 w mod 8 and the next), so that a lane's chunk, and with it its offset, is the same in all of them but for the
-// rows' distance. Columns past D, and rows past the last, lie outside the buffer and arrive as zeros.
-template <int DP, int ROWS> struct cross_stage {
-    static constexpr int PW = ROWS * DP / 2048, HALVES = DP == 256 ? 2 : 1; // KBs of a wave; of a group of rows
-    static_assert(PW >= HALVES, "a wave writes whole groups");
-    uint32_t off[HALVES];
+// ROWS rows of a token tensor into LDS by NW waves' LDS-DMA. A wave writes H KBs that hold whole groups of rows, of
+// every NW H in turn, so that a lane's chunks, and with them its offsets, are the same in all turns but for the rows'
+// distance. Columns past D, and rows past the last, lie outside the buffer and arrive as zeros.
+template <int DP, int ROWS, int NW = 4> struct cross_stage {
+    static constexpr int PW = ROWS * DP / (512 * NW), H = DP == 256 ? 2 : DP == 96 ? 3 : 1;
+    static_assert(PW > 0 && PW % H == 0 && H * 512 % (4 * DP) == 0, "whole groups");
+    uint32_t off[H];
     __device__ __forceinline__ void init(int w, int lane, int64_t tok, int D) {
 #pragma unroll
-        for (int p = 0; p < HALVES; ++p) {
-            const int x = (w * HALVES + p) * 1024 + 16 * lane;
+        for (int p = 0; p < H; ++p) {
+            const int x = (w * H + p) * 1024 + 16 * lane;
             const int rg = x / (8 * DP), y = x % (8 * DP);
             const int r = rg * 4 + (y % 256) / 64, c = y / 256 * 4 + ((y % 64 / 16) ^ (rg & 3));
             off[p] = c * 8 < D ? (uint32_t)r * (uint32_t)(tok * 2) + c * 16 : 0x80000000u;
@@ -77,9 +77,8 @@ template <int DP, int ROWS> struct cross_stage {
         const auto r = make_rsrc(first, row_bytes(min(rows, ROWS), tok, D));
 #pragma unroll
         for (int p = 0; p < PW; ++p) {
-            constexpr int H = HALVES;
-            const uint32_t far = (uint32_t)(p / H * (2048 * H / DP)) * (uint32_t)(tok * 2);
-            dma16<0>(r, lds + (w * H + p % H + p / H * 4 * H) * 512, opaque(off[p % H]) + far); // not held in registers
+            const uint32_t far = (uint32_t)(p / H * (NW * H * 512 / DP)) * (uint32_t)(tok * 2);
+            dma16<0>(r, lds + (w * H + p % H + p / H * NW * H) * 512, opaque(off[p % H]) + far); // not held in registers
         }
     }
 };
@@ -154,7 +153,7 @@ constexpr float kCrossSum = 65536.0f;
 //   S^T[key][row] = K . Q^T, O^T[d][row] += V^T . P^T   (v_mfma_f32_32x32x16_bf16)
 // The running maximum is raised only where a lane's sum of p over a tile passes kCrossSum.
 // ------------------------------------------------------------------------------------------
-template <int DP> __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void attn_cross_kernel(const attn_cross_args a) {
+template <int DP> __global__ __launch_bounds__(256, DP <= 96 ? 3 : 2) void attn_cross_kernel(const attn_cross_args a) {
     constexpr int KT = cross_tile_keys(DP), KN = DP / 16, NT = KT / 32;
     // K's tile and V's behind it. Each buffer is a variable of its own: the compiler tells LDS accesses apart by
     // variable, and needs address registers for each.
@@ -690,7 +689,7 @@ __global__ __launch_bounds__(256) void attn_cross_merge_kernel(const attn_cross_
 // K's tile is read both ways. delta = sum dO O is taken on the way in and left for the kernel of dK and dV.
 // ------------------------------------------------------------------------------------------
 template <int DP>
-__global__ __launch_bounds__(256, DP == 64 ? 4 : DP == 128 ? 2 : 1) void attn_cross_dq_kernel(const attn_cross_args a) {
+__global__ __launch_bounds__(256, DP == 64 ? 4 : DP == 96 ? 3 : DP == 128 ? 2 : 1) void attn_cross_dq_kernel(const attn_cross_args a) {
     constexpr int KT = cross_tile_keys(DP), KN = DP / 16, NT = KT / 32;
     constexpr int VO = KT * DP;
     __shared__ __attribute__((aligned(1024))) uint16_t KV0[2 * VO], KV1[2 * VO];
@@ -821,7 +820,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 4 : DP == 128 ? 2 : 1) void attn_cr
 // their sums are joined in LDS at the end.
 // ------------------------------------------------------------------------------------------
 template <int DP, bool DK, bool DV, int TEAMS>
-__global__ __launch_bounds__(256 * TEAMS, TEAMS > 1 ? 1 : DP == 64 ? 3 : DP == 128 || !DK ? 2 : 1)
+__global__ __launch_bounds__(256 * TEAMS, TEAMS > 1 ? 1 : DP == 64 ? 3 : DP <= 128 || !DK ? 2 : 1)
 void attn_cross_dkv_kernel(const attn_cross_args a) {
     constexpr int QT = ATTN_CROSS_STEP, KN = DP / 16, KEYS = ATTN_CROSS_KEYS;
     constexpr int GO = QT * DP; // dO's tile behind Q's
@@ -841,9 +840,13 @@ void attn_cross_dkv_kernel(const attn_cross_args a) {
         return;
     const int t0 = min(sp * cut.per, steps), t1 = min(t0 + cut.per, steps);
     const cross_lane<DP> ln(lane);
-    cross_stage<DP, QT> qs, gs;
-    qs.init(wk, lane, a.q_tok, D);
-    gs.init(wk, lane, a.go_tok, D);
+    // At DP = 96 the tiles are 6 KB, three for each of two waves: the first two load Q's, the others dO's.
+    constexpr int LW = DP == 96 ? 2 : 4;
+    const bool second = LW == 2 && wk >= 2;
+    cross_stage<DP, QT, LW> qs, gs;
+    qs.init(wk % LW, lane, second ? a.go_tok : a.q_tok, D);
+    if constexpr (LW == 4)
+        gs.init(wk, lane, a.go_tok, D);
     auto wait_loads = [] { __builtin_amdgcn_s_waitcnt(waitcnt_vm(0)); };
 
     for (int tile = at.tile; (int64_t)tile * KEYS < kr.n; tile += a.tps) {
@@ -878,8 +881,14 @@ void attn_cross_dkv_kernel(const attn_cross_args a) {
         auto load = [&](uint16_t *to) __attribute__((always_inline)) {
             const int h = u * g + lh, r0 = lt * QT, rows = ls < t1 ? min(qr.n - r0, QT) : 0;
             const int64_t first = qr.at + r0;
-            qs.load(a.q + first * a.q_tok + h * a.q_head, rows, a.q_tok, D, to + team * 2 * GO, wk);
-            gs.load(a.go + first * a.go_tok + h * a.go_head, rows, a.go_tok, D, to + team * 2 * GO + GO, wk);
+            const uint16_t *q = a.q + first * a.q_tok + h * a.q_head, *go = a.go + first * a.go_tok + h * a.go_head;
+            uint16_t *const place = to + team * 2 * GO;
+            if constexpr (LW == 4) {
+                qs.load(q, rows, a.q_tok, D, place, wk);
+                gs.load(go, rows, a.go_tok, D, place + GO, wk);
+            } else {
+                qs.load(second ? go : q, rows, second ? a.go_tok : a.q_tok, D, place + (second ? GO : 0), wk % 2);
+            }
             const int r = opaque(lane) & (QT - 1);
             const float *src = (w & 1 ? a.delta : a.lse) + first * a.Hq + h;
             const float x = src[max(min(r, rows - 1), 0) * a.Hq];
@@ -1034,9 +1043,11 @@ __global__ __launch_bounds__(256) void attn_cross_sum_kernel(const attn_cross_ar
 }
 
 // ---- launchers -------------------------------------------------------------------------------
-// Calls f(std::integral_constant<int, DP>{}) with the tile width for head dim D.
+// Calls f(std::integral_constant<int, DP>{}) with the tile width for head dim D. 96 for what is above 64: eight sequences of
+// up to 1000 rows and 1500 states, 16 heads, D = 80, forward and gradients 281 us, in tiles of 128 340.
 template <typename F> hipError_t with_width(int D, F &&f) {
     return D <= 64    ? f(std::integral_constant<int, 64>{})
+           : D <= 96  ? f(std::integral_constant<int, 96>{})
            : D <= 128 ? f(std::integral_constant<int, 128>{})
                       : f(std::integral_constant<int, 256>{});
 }
@@ -1072,14 +1083,14 @@ extern "C" int attn_hip_launch_cross(const struct attn_cross_args *ap, const str
     const hipError_t e = with_width(a.D, [&](auto W) {
         constexpr int DP = decltype(W)::value;
         auto rows = [&](auto NB, auto NT, auto NWF) {
-            constexpr int kN = decltype(NB)::value, kW = decltype(NWF)::value;
+            constexpr int kN = decltype(NB)::value, kW = decltype(NWF)::value, RP = DP == 96 ? 128 : DP; // bound by HBM
             constexpr bool kT = decltype(NT)::value;
             if (t_plan) {
-                plan_note(grid, block, "attn_cross_rows_kernel<%d, %d, %s, %d> parts=%d share=%d", DP, kN, tf(kT),
+                plan_note(grid, block, "attn_cross_rows_kernel<%d, %d, %s, %d> parts=%d share=%d", RP, kN, tf(kT),
                           kW, a.nsplit, a.share);
                 return hipSuccess;
             }
-            hipLaunchKernelGGL((attn_cross_rows_kernel<DP, kN, kT, kW>), grid, block, 0, st, a);
+            hipLaunchKernelGGL((attn_cross_rows_kernel<RP, kN, kT, kW>), grid, block, 0, st, a);
             return hipGetLastError();
         };
         constexpr std::integral_constant<int, 1> one;
