@@ -90,9 +90,9 @@ static void walk_tiles(const struct attn_cross_args *a, const struct attn_cross_
             int *parts = calloc((size_t)items + 1, sizeof *parts);
             for (int wg = 0; wg < cut->grid; ++wg) {
                 const struct attn_cross_place p = attn_cross_place_of(a, wg);
-                CHECK(p.b >= 0 && p.b < a->B && p.u >= 0 && p.u < a->Hkv && p.sp >= 0 && p.sp < a->nsplit && p.tile >= 0 &&
+                CHECK(p.nth >= 0 && p.nth < a->B && p.u >= 0 && p.u < a->Hkv && p.sp >= 0 && p.sp < a->nsplit && p.tile >= 0 &&
                           p.tile < a->tps, "place of %d", wg);
-                if (p.b != b0 || p.u != u0 || p.sp >= c.live)
+                if (p.nth != b0 || p.u != u0 || p.sp >= c.live)
                     continue;
                 const int t0 = p.sp * c.per < units ? p.sp * c.per : units;
                 const int t1 = t0 + c.per < units ? t0 + c.per : units;

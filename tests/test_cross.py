@@ -44,6 +44,10 @@ CASES = [
     ([(6, 50), (5, 700), (1, 1)], 16, 4, 128, None, 0),
     ([(16, 300)], 1, 1, 256, None, 0),
     ([(7, 150), (2, 400)], 12, 4, 240, None, 0),
+    # the longest of up to 64 sequences first: by their states, equal ones too, and by their rows; one more than 64
+    ([(33 + b % 7 * 9, 13 * b * b % 600 // 3 * 3 + (b == 5) * 500) for b in range(64)], 10, 10, 64, None, 0),
+    ([(30 * b, 280 - 11 * b) for b in range(21)], 16, 16, 32, None, 0),
+    ([(33 + b % 40, 600 - b) for b in range(65)], 8, 8, 64, None, 0),
     # two teams of waves for dK and dV
     ([(4200, 130)], 16, 16, 64, None, 0),
     ([(1500, 70), (300, 200), (0, 20)], 24, 4, 128, None, 0),

@@ -185,10 +185,13 @@ static struct attn_cross_args cross_args(const struct attn_cross_call *c) {
     return a;
 }
 
-static void set_cut(struct attn_cross_args *a, const struct attn_cross_cut *cut) {
+/* walk: how many rows, at most, a tile of this launch walks. */
+static void set_cut(struct attn_cross_args *a, const struct attn_cross_cut *cut, int walk) {
     a->tps = cut->tps, a->nsplit = cut->nsplit, a->share = cut->share, a->wgs = (int)cut->grid;
     a->teams = cut->teams, a->row_teams = cut->row_teams, a->Hkv_wg = cut->quads ? a->Hkv / 4 : a->Hkv;
     a->by_tps = attn_div_of(a->tps), a->by_B = attn_div_of(a->B), a->by_heads = attn_div_of(a->Hkv);
+    a->by_bh = attn_div_of(a->B * a->Hkv);
+    a->by_length = a->B > 1 && a->B <= ATTN_CROSS_RANKED && cut->grid > ATTN_CROSS_AT_ONCE && walk >= ATTN_CROSS_LONG;
     a->by_hq = attn_div_of(a->Hq), a->by_g = attn_div_of(a->g), a->by_gwg = attn_div_of(a->Hq / a->Hkv_wg);
 }
 
@@ -197,11 +200,11 @@ static void cross_run(const char *who, const struct attn_cross_call *c, const st
                       void *scratch) {
     struct attn_cross_args a = cross_args(c);
     const struct attn_cross_cut cut = forward_cut(c);
-    set_cut(&a, &cut);
-    a.q = (const uint16_t *)q->data, a.q_tok = q->token, a.q_head = q->head;
-    a.k = (const uint16_t *)k->data, a.k_tok = k->token, a.k_head = k->head;
-    a.v = (const uint16_t *)v->data, a.v_tok = v->token, a.v_head = v->head;
-    a.o = (uint16_t *)o->data, a.o_tok = o->token, a.o_head = o->head;
+    set_cut(&a, &cut, bound_of(&c->k));
+    a.q = (const uint16_t *)q->data, a.q_tok.n = (int32_t)q->token, a.q_head = q->head;
+    a.k = (const uint16_t *)k->data, a.k_tok.n = (int32_t)k->token, a.k_head = k->head;
+    a.v = (const uint16_t *)v->data, a.v_tok.n = (int32_t)v->token, a.v_head = v->head;
+    a.o = (uint16_t *)o->data, a.o_tok.n = (int32_t)o->token, a.o_head = o->head;
     a.lse = lse;
     /* the scratch of attn_flash: m, l and acc[D] of ATTN_SLOTS partials, each on 256 bytes */
     a.pm = (float *)scratch;
@@ -230,21 +233,21 @@ void attn_cross(const struct attn_cross_call *c, const struct attn_rows *q, cons
 static void grad_run(const char *who, const struct attn_cross_call *c, const struct attn_rows *const *in,
                      const float *lse, const struct attn_rows *const *out, void *scratch) {
     struct attn_cross_args a = cross_args(c);
-    a.q = (const uint16_t *)in[0]->data, a.q_tok = in[0]->token, a.q_head = in[0]->head;
-    a.k = (const uint16_t *)in[1]->data, a.k_tok = in[1]->token, a.k_head = in[1]->head;
-    a.v = (const uint16_t *)in[2]->data, a.v_tok = in[2]->token, a.v_head = in[2]->head;
-    a.o = (uint16_t *)in[3]->data, a.o_tok = in[3]->token, a.o_head = in[3]->head; /* read */
-    a.go = (const uint16_t *)in[4]->data, a.go_tok = in[4]->token, a.go_head = in[4]->head;
-    a.dq = (uint16_t *)out[0]->data, a.dq_tok = out[0]->token, a.dq_head = out[0]->head;
-    a.dk = (uint16_t *)out[1]->data, a.dk_tok = out[1]->token, a.dk_head = out[1]->head;
-    a.dv = (uint16_t *)out[2]->data, a.dv_tok = out[2]->token, a.dv_head = out[2]->head;
+    a.q = (const uint16_t *)in[0]->data, a.q_tok.n = (int32_t)in[0]->token, a.q_head = in[0]->head;
+    a.k = (const uint16_t *)in[1]->data, a.k_tok.n = (int32_t)in[1]->token, a.k_head = in[1]->head;
+    a.v = (const uint16_t *)in[2]->data, a.v_tok.n = (int32_t)in[2]->token, a.v_head = in[2]->head;
+    a.o = (uint16_t *)in[3]->data, a.o_tok.n = (int32_t)in[3]->token, a.o_head = in[3]->head; /* read */
+    a.go = (const uint16_t *)in[4]->data, a.go_tok.n = (int32_t)in[4]->token, a.go_head = in[4]->head;
+    a.dq = (uint16_t *)out[0]->data, a.dq_tok.n = (int32_t)out[0]->token, a.dq_head = out[0]->head;
+    a.dk = (uint16_t *)out[1]->data, a.dk_tok.n = (int32_t)out[1]->token, a.dk_head = out[1]->head;
+    a.dv = (uint16_t *)out[2]->data, a.dv_tok.n = (int32_t)out[2]->token, a.dv_head = out[2]->head;
     a.lse = (float *)(uintptr_t)lse; /* read */
     a.delta = (float *)scratch;
     a.pacc = (float *)((char *)scratch + delta_bytes(c));
     const struct attn_cross_cut dq = dq_cut(c), dkv = dkv_cut(c);
-    set_cut(&a, &dq);
+    set_cut(&a, &dq, bound_of(&c->k));
     cross_hip_check(attn_hip_launch_cross_grad(&a, &dq, 0, bound_of(&c->q), attn_flash_get_stream()), who);
-    set_cut(&a, &dkv);
+    set_cut(&a, &dkv, bound_of(&c->q));
     cross_hip_check(attn_hip_launch_cross_grad(&a, &dkv, 1, bound_of(&c->k), attn_flash_get_stream()), who);
 }
 

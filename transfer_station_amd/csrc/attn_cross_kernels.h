@@ -34,6 +34,34 @@ __device__ __forceinline__ attn_range k_rows(const attn_cross_args &a, int b) {
     return rows_of(a.k_start, a.k_second, a.k_is_len, b, a.Tk);
 }
 
+// The sequence at place nth of the call's: as they come, or by falling length of the rows that a tile has to walk (its
+// states, or with BY_Q its rows), so that no long one is left for the end: each lane counts how many are ahead of its own.
+struct cross_seq {
+    attn_range q, k;
+};
+template <bool BY_Q> __device__ __forceinline__ cross_seq seq_at(const attn_cross_args &a, int nth, int lane) {
+    if (!a.by_length) {
+        int q0 = scalar_i32(a.q_start, nth), q1 = scalar_i32(a.q_second, nth);
+        int k0 = scalar_i32(a.k_start, nth), k1 = scalar_i32(a.k_second, nth);
+        asm("" : "+s"(q0), "+s"(q1), "+s"(k0), "+s"(k1)); // asked for together
+        return cross_seq{attn_range_of(q0, q1, a.q_is_len, a.Tq), attn_range_of(k0, k1, a.k_is_len, a.Tk)};
+    }
+    const int i = min(lane, a.B - 1);
+    const attn_range q = attn_range_of(a.q_start[i], a.q_second[i], a.q_is_len, a.Tq);
+    const attn_range k = attn_range_of(a.k_start[i], a.k_second[i], a.k_is_len, a.Tk);
+    const int len = lane >= a.B ? -1 : BY_Q ? q.n : k.n; // the lanes past the last: behind all sequences
+    int ahead = 0;
+    for (int j = 0; j < a.B; ++j) {
+        const int x = __builtin_amdgcn_readlane(len, j);
+        ahead += x > len || (x == len && j < lane) ? 1 : 0;
+    }
+    const int b = __builtin_ctzll(__builtin_amdgcn_ballot_w64(ahead == nth));
+    auto of = [&](attn_range r) {
+        return attn_range{__builtin_amdgcn_readlane(r.at, b), __builtin_amdgcn_readlane(r.n, b)};
+    };
+    return cross_seq{of(q), of(k)};
+}
+
 __device__ __forceinline__ attn_cut part_of(int total, int share, int nsplit, int step) {
     if (nsplit == 1) // no divisions
         return attn_cut{1, max(total, 1)};
@@ -51,8 +79,8 @@ __device__ __forceinline__ f32x16 mfma32(bf16x8 x, bf16x8 y, f32x16 z) {
 }
 
 // Bytes from a row's first element to the end of `rows` rows, 0 where there are none.
-__device__ __forceinline__ uint32_t row_bytes(int rows, int64_t tok, int D) {
-    return rows < 1 ? 0u : (uint32_t)(rows - 1) * (uint32_t)(tok * 2) + D * 2;
+__device__ __forceinline__ uint32_t row_bytes(int rows, attn_stride tok, int D) {
+    return rows < 1 ? 0u : (uint32_t)(rows - 1) * (uint32_t)(tok.n * 2) + D * 2;
 }
 
 // ROWS rows of a token tensor into LDS by NW waves' LDS-DMA. A wave writes H KBs that hold whole groups of rows, of
@@ -62,22 +90,22 @@ template <int DP, int ROWS, int NW = 4> struct cross_stage {
     static constexpr int PW = ROWS * DP / (512 * NW), H = DP == 256 ? 2 : DP == 96 ? 3 : 1;
     static_assert(PW > 0 && PW % H == 0 && H * 512 % (4 * DP) == 0, "whole groups");
     uint32_t off[H];
-    __device__ __forceinline__ void init(int w, int lane, int64_t tok, int D) {
+    __device__ __forceinline__ void init(int w, int lane, attn_stride tok, int D) {
 #pragma unroll
         for (int p = 0; p < H; ++p) {
             const int x = (w * H + p) * 1024 + 16 * lane;
             const int rg = x / (8 * DP), y = x % (8 * DP);
             const int r = rg * 4 + (y % 256) / 64, c = y / 256 * 4 + ((y % 64 / 16) ^ (rg & 3));
-            off[p] = c * 8 < D ? (uint32_t)r * (uint32_t)(tok * 2) + c * 16 : 0x80000000u;
+            off[p] = c * 8 < D ? (uint32_t)r * (uint32_t)(tok.n * 2) + c * 16 : 0x80000000u;
         }
     }
     // rows: how many there are from `first` on.
-    __device__ __forceinline__ void load(const uint16_t *first, int rows, int64_t tok, int D, uint16_t *lds,
+    __device__ __forceinline__ void load(const uint16_t *first, int rows, attn_stride tok, int D, uint16_t *lds,
                                          int w) const {
         const auto r = make_rsrc(first, row_bytes(min(rows, ROWS), tok, D));
 #pragma unroll
         for (int p = 0; p < PW; ++p) {
-            const uint32_t far = (uint32_t)(p / H * (NW * H * 512 / DP)) * (uint32_t)(tok * 2);
+            const uint32_t far = (uint32_t)(p / H * (NW * H * 512 / DP)) * (uint32_t)(tok.n * 2);
             dma16<0>(r, lds + (w * H + p % H + p / H * NW * H) * 512, opaque(off[p % H]) + far); // not held in registers
         }
     }
@@ -161,9 +189,10 @@ template <int DP> __global__ __launch_bounds__(256, DP <= 96 ? 3 : 2) void attn_
     __shared__ __attribute__((aligned(1024))) uint16_t KV0[2 * VO], KV1[2 * VO];
 
     const attn_cross_place at = attn_cross_place_of(&a, wg_id_x());
-    const int b = at.b, u = at.u, sp = at.sp;
+    const int u = at.u, sp = at.sp;
     const int tid = wi_id_x(), w = uniform(tid >> 6), lane = tid & 63, l32 = lane & 31, hi = lane >> 5;
-    const attn_range qr = q_rows(a, b), kr = k_rows(a, b);
+    const cross_seq seq = seq_at<false>(a, at.nth, lane);
+    const attn_range qr = seq.q, kr = seq.k;
     const attn_cut cut = part_of(kr.n, a.share, a.nsplit, ATTN_CROSS_KEY_STEP);
     if (sp >= cut.live)
         return;
@@ -362,7 +391,7 @@ __global__ __launch_bounds__(256, 2) void attn_cross_rows_kernel(const attn_cros
         ug = attn_div_by(at, a.by_B);
         b = at - ug * a.B;
     }
-    const uint32_t kb2 = (uint32_t)(a.k_tok * 2), vb2 = (uint32_t)(a.v_tok * 2); // bytes from row to row
+    const uint32_t kb2 = (uint32_t)a.k_tok.n * 2, vb2 = (uint32_t)a.v_tok.n * 2; // bytes from row to row
     uint16_t *vt = &Vw[w * VTILE];
     const uint32_t koff = grp * 8 < D ? r16 * kb2 + grp * 16 : 0x80000000u;
     const uint32_t voff = (lane % (DP / 8)) * 8 < D ? (lane / (DP / 8)) * vb2 + (lane % (DP / 8)) * 16 : 0x80000000u;
@@ -413,7 +442,7 @@ __global__ __launch_bounds__(256, 2) void attn_cross_rows_kernel(const attn_cros
                 return n > 0 ? (uint32_t)(n - 1) * step + D * 2 : 0u;
             };
             auto load_k = [&](int tb, frags &f) __attribute__((always_inline)) {
-                const auto r = make_rsrc(kp + (int64_t)min(tb, k1) * a.k_tok, bytes(tb, kb2));
+                const auto r = make_rsrc(kp + min(tb, k1) * a.k_tok, bytes(tb, kb2));
 #pragma unroll
                 for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -422,7 +451,7 @@ __global__ __launch_bounds__(256, 2) void attn_cross_rows_kernel(const attn_cros
                             buf16<NTL>(r, kk * 32 + grp * 8 < D ? koff + 16 * t * kb2 + kk * 64 : 0x80000000u);
             };
             auto load_v = [&](int tb, frags &f) __attribute__((always_inline)) {
-                const auto r = make_rsrc(vp + (int64_t)min(tb, k1) * a.v_tok, bytes(tb, vb2));
+                const auto r = make_rsrc(vp + min(tb, k1) * a.v_tok, bytes(tb, vb2));
 #pragma unroll
                 for (int i = 0; i < NV; ++i)
                     f.v[i] = buf16<NTL>(r, voff + i * (512 / DP) * vb2);
@@ -558,8 +587,8 @@ __global__ __launch_bounds__(256, 2) void attn_cross_rows_kernel(const attn_cros
                         lsum += wgt * red_l[i][NW * team + ww][r];
                     }
                     const int i_tok = attn_div_by(rowb + r, a.by_g), h = u * g + rowb + r - i_tok * g;
-                    const int64_t tok = qr.at + i_tok;
-                    const int64_t slot = tok * a.Hq + h;
+                    const int tok = qr.at + i_tok;
+                    const int64_t slot = (int64_t)tok * a.Hq + h;
                     if (live == 1) {
                         const float inv = lsum > 0.f ? 1.0f / lsum : 0.f;
                         *reinterpret_cast<u32x2 *>(a.o + tok * a.o_tok + h * a.o_head + d) =
@@ -674,7 +703,7 @@ __global__ __launch_bounds__(256) void attn_cross_merge_kernel(const attn_cross_
         }
         if (sg == 0 && row < R && d < a.D && parts > 1) { // one part: written already
             const float inv = sum > 0.f ? 1.0f / sum : 0.f;
-            const int64_t tok = qr.at + i_tok;
+            const int tok = qr.at + i_tok;
             *reinterpret_cast<u32x2 *>(a.o + tok * a.o_tok + h * a.o_head + d) =
                 u32x2{bf16_pair(acc[0] * inv, acc[1] * inv), bf16_pair(acc[2] * inv, acc[3] * inv)};
             if (a.lse && d == 0)
@@ -695,9 +724,10 @@ __global__ __launch_bounds__(256, DP == 64 ? 4 : DP == 96 ? 3 : DP == 128 ? 2 : 
     __shared__ __attribute__((aligned(1024))) uint16_t KV0[2 * VO], KV1[2 * VO];
 
     const attn_cross_place at = attn_cross_place_of(&a, wg_id_x());
-    const int b = at.b, u = at.u, sp = at.sp;
+    const int u = at.u, sp = at.sp;
     const int tid = wi_id_x(), w = uniform(tid >> 6), lane = tid & 63, l32 = lane & 31, hi = lane >> 5;
-    const attn_range qr = q_rows(a, b), kr = k_rows(a, b);
+    const cross_seq seq = seq_at<false>(a, at.nth, lane);
+    const attn_range qr = seq.q, kr = seq.k;
     const attn_cut cut = part_of(kr.n, a.share, a.nsplit, ATTN_CROSS_KEY_STEP);
     if (sp >= cut.live)
         return;
@@ -829,10 +859,11 @@ void attn_cross_dkv_kernel(const attn_cross_args a) {
     __shared__ __attribute__((aligned(16))) float st0[TEAMS * 256], st1[TEAMS * 256]; // lse in log2 units, from 64 on delta
 
     const attn_cross_place at = attn_cross_place_of(&a, wg_id_x());
-    const int b = at.b, u = at.u, sp = at.sp;
+    const int u = at.u, sp = at.sp;
     const int tid = wi_id_x(), w = uniform(tid >> 6), lane = tid & 63, l32 = lane & 31, hi = lane >> 5;
     const int wk = w & 3, team = w >> 2;
-    const attn_range qr = q_rows(a, b), kr = k_rows(a, b);
+    const cross_seq seq = seq_at<true>(a, at.nth, lane);
+    const attn_range qr = seq.q, kr = seq.k;
     const int g = a.g, D = a.D;
     const int per_head = uniform((qr.n + QT - 1) / QT), steps = per_head * g; // of QT rows of one head
     const attn_cut cut = part_of(steps, a.share, a.nsplit, TEAMS);
@@ -853,11 +884,11 @@ void attn_cross_dkv_kernel(const attn_cross_args a) {
         // The wave's rows of K and V, by lane: what lies past the last state or past D is outside the buffer, zeros.
         bf16x8 kf[KN], vf[KN];
         {
-            const int64_t first = kr.at + tile * KEYS + 32 * wk;
+            const int first = kr.at + tile * KEYS + 32 * wk;
             const int rows = min(32, kr.n - tile * KEYS - 32 * wk);
             const auto rk = make_rsrc(a.k + first * a.k_tok + u * a.k_head, row_bytes(rows, a.k_tok, D));
             const auto rv = make_rsrc(a.v + first * a.v_tok + u * a.v_head, row_bytes(rows, a.v_tok, D));
-            const uint32_t ok = l32 * (uint32_t)(a.k_tok * 2) + hi * 16, ov = l32 * (uint32_t)(a.v_tok * 2) + hi * 16;
+            const uint32_t ok = l32 * (uint32_t)(a.k_tok.n * 2) + hi * 16, ov = l32 * (uint32_t)(a.v_tok.n * 2) + hi * 16;
 #pragma unroll
             for (int kk = 0; kk < KN; ++kk) {
                 const bool in = kk * 16 < D; // D % 16 == 0
@@ -880,7 +911,7 @@ void attn_cross_dkv_kernel(const attn_cross_args a) {
         float st; // of one row of that step: lse (even waves) or delta
         auto load = [&](uint16_t *to) __attribute__((always_inline)) {
             const int h = u * g + lh, r0 = lt * QT, rows = ls < t1 ? min(qr.n - r0, QT) : 0;
-            const int64_t first = qr.at + r0;
+            const int first = qr.at + r0;
             const uint16_t *q = a.q + first * a.q_tok + h * a.q_head, *go = a.go + first * a.go_tok + h * a.go_head;
             uint16_t *const place = to + team * 2 * GO;
             if constexpr (LW == 4) {
@@ -890,7 +921,7 @@ void attn_cross_dkv_kernel(const attn_cross_args a) {
                 qs.load(second ? go : q, rows, second ? a.go_tok : a.q_tok, D, place + (second ? GO : 0), wk % 2);
             }
             const int r = opaque(lane) & (QT - 1);
-            const float *src = (w & 1 ? a.delta : a.lse) + first * a.Hq + h;
+            const float *src = (w & 1 ? a.delta : a.lse) + (int64_t)first * a.Hq + h;
             const float x = src[max(min(r, rows - 1), 0) * a.Hq];
             st = w & 1 ? x : r < rows ? x * kLog2e : __builtin_inff();
             ls += TEAMS;
@@ -989,7 +1020,7 @@ void attn_cross_dkv_kernel(const attn_cross_args a) {
         }
         // Taken from the lane anew, so that nothing of it is held through the loop.
         const int ln2 = opaque(lane), hi2 = ln2 >> 5, key = tile * KEYS + 32 * wk + (ln2 & 31);
-        const int64_t tok = kr.at + key;
+        const int tok = kr.at + key;
         if (team == 0 && key < kr.n) {
             if (cut.live == 1) {
                 if (DK)
@@ -997,7 +1028,7 @@ void attn_cross_dkv_kernel(const attn_cross_args a) {
                 if (DV)
                     put_row<DP>(dv, 1.f, a.dv + tok * a.dv_tok + u * a.dv_head, hi2, D);
             } else {
-                float *dst = a.pacc + ((tok * a.Hkv + u) * a.nsplit + sp) * 2 * D;
+                float *dst = a.pacc + (((int64_t)tok * a.Hkv + u) * a.nsplit + sp) * 2 * D;
                 if (DK)
                     put_part<DP>(dk, dst, hi2, D);
                 if (DV)
@@ -1032,7 +1063,7 @@ __global__ __launch_bounds__(256) void attn_cross_sum_kernel(const attn_cross_ar
                 acc[j] += x[j];
         }
         const int i_tok = attn_div_by(row, KV ? a.by_heads : a.by_hq), h = row - i_tok * H;
-        const int64_t tok = first + i_tok;
+        const int tok = first + i_tok;
         const bool v = KV && d >= a.D;
         const float f = v ? 1.f : a.scale;
         uint16_t *dst = !KV ? a.dq + tok * a.dq_tok + h * a.dq_head + d

@@ -52,6 +52,13 @@ ATTN_HD struct attn_cut attn_cut_of(int total, int share, int nsplit, int step) 
 
 #define ATTN_CROSS_STEP 32 /* rows of a step of the kernel of dK and dV */
 
+/* Launches of 2 to 64 sequences (a wave's lanes), of more workgroups than run at once, start the longest first: eight
+ * prompts of 210 to 700 tokens over 2000 to 4001 states 226 -> 216 us, the step of eight by up to 1000 and 1500 268 ->
+ * 245. Tiles that walk few rows are over before it pays (77 states: 3 us lost of 73). */
+#define ATTN_CROSS_RANKED 64
+#define ATTN_CROSS_AT_ONCE 512
+#define ATTN_CROSS_LONG 512
+
 /* n / d for 0 <= n < 2^31 by a product: mul = ceil(2^(31 + l) / d), l = ceil(log2 d), which is below 2^32 and off by
  * less than 2^l, so that the quotient is off by less than n 2^l / (d 2^(31 + l)) < 1 / d. The kernels' divisions by what a
  * call fixes are of this kind: of the compiler's, five take a microsecond before the first load. */
@@ -78,12 +85,20 @@ struct attn_cross_cut {
     long grid;
 };
 
+/* Elements from row to row, at most ATTN_TOKEN_MAX. Its product with a row's number has 64 bits. */
+struct attn_stride {
+    int32_t n;
+};
+#ifdef __cplusplus
+ATTN_HD int64_t operator*(int row, attn_stride s) { return (int64_t)row * s.n; }
+#endif
+
 struct attn_cross_args {
     const uint16_t *q, *k, *v, *go; /* go: dO */
     uint16_t *o, *dq, *dk, *dv;
     float *lse, *delta; /* [Tq][Hq] */
-    int64_t q_tok, q_head, k_tok, k_head, v_tok, v_head, o_tok, o_head, go_tok, go_head;
-    int64_t dq_tok, dq_head, dk_tok, dk_head, dv_tok, dv_head;
+    int64_t q_head, k_head, v_head, o_head, go_head, dq_head, dk_head, dv_head;
+    struct attn_stride q_tok, k_tok, v_tok, o_tok, go_tok, dq_tok, dk_tok, dv_tok;
     const int32_t *q_start, *q_second, *k_start, *k_second; /* second: lengths, or the next starts */
     int q_is_len, k_is_len;
     int B, Tq, Tk, Hq, Hkv, g, D; /* g = Hq / Hkv */
@@ -91,28 +106,35 @@ struct attn_cross_args {
     int tps, nsplit, share, wgs;
     int teams, Hkv_wg; /* few rows: teams of the decode line, groups of kv heads */
     int row_teams;     /* dK and dV */
-    struct attn_div by_tps, by_B, by_heads, by_hq, by_g, by_gwg; /* tps, B, Hkv, Hq, g, query heads of a group of kv heads */
+    int by_length;     /* the tile kernels' sequences come longest first */
+    struct attn_div by_tps, by_B, by_heads, by_bh, by_hq, by_g, by_gwg; /* tps, B, Hkv, B Hkv, Hq, g, heads of a group of kv heads */
     float *pm, *pl, *pacc; /* partial maxima, sums and rows; of gradients: rows in pacc */
 };
 
-/* Where a workgroup is. Hardware ids are dealt to the eight XCDs in turn: each takes neighbouring places of the order
- * [part][kv head][sequence][tile], so that a sequence's tiles, which read the same rows, share its L2, and sequences of
- * unequal length, which lie next to each other, leave no XCD idle. */
-struct attn_cross_place {
-    int b, u, sp, tile;
-};
+/* Place i of n neighbouring places, cut into one run of them for each of the eight XCDs, to which hardware ids are dealt
+ * in turn. */
 ATTN_HD int attn_xcd_order(int wg, int n) {
     const int per = n >> 3, rem = n & 7, x = wg & 7;
     return (x < rem ? x * (per + 1) : rem * (per + 1) + (x - rem) * per) + (wg >> 3);
 }
+
+/* Where a workgroup of the tile kernels is. A sequence's tiles of a kv head and part read the same rows, and share an XCD's
+ * L2; these groups, in the order [part][place of the sequence][kv head], are dealt to the XCDs in turn, so that each
+ * has some of every length, and the first sequences' of all heads first. The last groups, fewer than eight, are cut. */
+struct attn_cross_place {
+    int nth, u, sp, tile; /* nth: the sequence's place among the call's */
+};
 ATTN_HD struct attn_cross_place attn_cross_place_of(const struct attn_cross_args *a, int wg) {
-    const int at = attn_xcd_order(wg, a->wgs), group = attn_div_by(at, a->by_tps);
-    const int us = attn_div_by(group, a->by_B);
+    const int whole = attn_div_by(a->wgs, a->by_tps) & ~7, dealt = whole * a->tps;
+    const int in = wg < dealt, at = in ? wg >> 3 : attn_xcd_order(wg - dealt, a->wgs - dealt);
+    const int k = attn_div_by(at, a->by_tps);
+    int group = in ? k * 8 + (wg & 7) : whole + k;
     struct attn_cross_place p;
-    p.tile = at - group * a->tps;
-    p.b = group - us * a->B;
-    p.sp = attn_div_by(us, a->by_heads);
-    p.u = us - p.sp * a->Hkv;
+    p.tile = at - k * a->tps;
+    p.sp = attn_div_by(group, a->by_bh);
+    group -= p.sp * a->B * a->Hkv;
+    p.nth = attn_div_by(group, a->by_heads);
+    p.u = group - p.nth * a->Hkv;
     return p;
 }
 
