@@ -197,7 +197,8 @@ PLANS = [
     (0, 256, 4, 32, 8, 8, 3000, [("rows_kernel<256, 1, false, 4>", "parts=64 share=1", 256), ("merge_kernel<16, 1>", "", 256)]),
     # more rows: tiles of 128, in parts where they are few
     (0, 128, 1, 32, 8, 9, 3000, [("kernel<128>", "parts=11 share=384", 88), ("merge_kernel<16, 1>", "", 36)]),
-    (0, 80, 8, 16, 16, 1000, 1500, [("kernel<128>", "parts=1 share=1536", 1024)]),
+    (0, 80, 8, 16, 16, 1000, 1500, [("kernel<96>", "parts=1 share=1536", 1024)]),
+    (0, 112, 8, 16, 16, 1000, 1500, [("kernel<128>", "parts=1 share=1536", 1024)]),
     # rows for too many partial slots: no parts
     (0, 64, 70000, 1, 1, 1, 2, [("rows_kernel<64, 1, true, 4>", "parts=1 share=1", 70000)]),
     (1, 64, 3, 8, 8, 37, 50, [("dq_kernel<64>", "parts=1 share=128", 24),
