@@ -50,7 +50,7 @@ CASES = [
     ([(33 + b % 40, 600 - b) for b in range(65)], 8, 8, 64, None, 0),
     # two teams of waves for dK and dV
     ([(4200, 130)], 16, 16, 64, None, 0),
-    ([(2000, 100), (100, 33)], 16, 16, 80, None, 0),
+    ([(2100, 100), (100, 33)], 16, 16, 80, None, 0),
     ([(1500, 70), (300, 200), (0, 20)], 24, 4, 128, None, 0),
     # calls that claim much to read: four kv heads in a workgroup
     ([(1, 900), (1, 130), (1, 2000)], 8, 8, 64, None, 1 << 18),
