@@ -227,7 +227,7 @@ struct attn_cross_call {
  * kv = h / (Hq/Hkv), in bf16; lse[t * Hq + h] = log sum_j exp(scale * Q.K), natural, in fp32 (lse may be NULL). A row
  * whose sequence has no states gets zeros and -inf; rows of no sequence are left as they are. Sequences may share
  * states (their spans may overlap), not rows. P is rounded to bf16 before P.V, as in attn_flash; states that no
- * sequence names are not read, whatever they hold. o must not overlap q, k or v.
+ * sequence names are not read, whatever they hold. o must not overlap q, k or v, nor its heads each other.
  * scratch: attn_cross_scratch_bytes(c) bytes, ATTN_SCRATCH_ALIGN-aligned; calls that may overlap need one each. */
 size_t attn_cross_scratch_bytes(const struct attn_cross_call *c);
 void attn_cross(const struct attn_cross_call *c, const struct attn_rows *q, const struct attn_rows *k,

@@ -59,7 +59,8 @@ def reference(t, scale=0.0, grad=True):
     With e = 2^-8: P and dS enter their products rounded to bf16 (e of each), each result is rounded once (e of it).
     O and dV: off by (e + d) sum P |.| + e |result|, where d is what P is off by before its rounding: a score is off by
     (D + 8) roundings of 2^-24 of sum |q||k|, as is lse, exp2 is good to 2^-21 and enters once per tile and weight.
-    dS = P (dP - delta): delta is made of the rounded O (off by what O is), dP and delta of D products in fp32;
+    dS = P (dP - delta): delta is made of the rounded O (off by what O is), or, of up to 32 states, of P dP in fp32 (off by d
+    of its terms); dP and delta of D products in fp32;
     so dS is off by (e + d) |dS| + P (sum |dO| off(O) + (D + 8) 2^-24 sum |dO| (|V| + |O|)), and dQ and dK by the sums
     of that, times the factors' sizes. Sums over n terms add n 2^-24 of the terms' sizes."""
     scale = scale or t.D ** -0.5
@@ -97,9 +98,11 @@ def reference(t, scale=0.0, grad=True):
             dP = G @ V.T
             dS = P * (dP - (G * O).sum(1, keepdims=True))
             Ga = np.abs(G)
-            ds_off = (E * 1.01 + d) * np.abs(dS) + P * (
-                (Ga * o_off).sum(1, keepdims=True) + (t.D + 8) * E32 * (Ga @ np.abs(V).T + (Ga * np.abs(O)).sum(
-                    1, keepdims=True)))
+            if m <= 32:
+                delta_off = (P * ((d + m * E32) * np.abs(dP) + (t.D + 8) * E32 * (Ga @ np.abs(V).T))).sum(1, keepdims=True)
+            else:
+                delta_off = (Ga * o_off).sum(1, keepdims=True) + (t.D + 8) * E32 * (Ga * np.abs(O)).sum(1, keepdims=True)
+            ds_off = (E * 1.01 + d) * np.abs(dS) + P * (delta_off + (t.D + 8) * E32 * (Ga @ np.abs(V).T))
             dQ = scale * (dS @ K)
             out["dq"][0][rows, h] = dQ
             out["dq"][1][rows, h] = (scale * ((ds_off + m * E32 * np.abs(dS)) @ np.abs(K)) + E * np.abs(dQ) + 1e-30)

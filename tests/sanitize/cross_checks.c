@@ -289,7 +289,7 @@ static void test_calls(void) {
         struct attn_rows r[8];
         static char base[8][16] __attribute__((aligned(16)));
         for (int j = 0; j < 8; ++j)
-            r[j] = (struct attn_rows){base[j], 256, 8};
+            r[j] = (struct attn_rows){base[j], 256, 256};
         const size_t sb = attn_cross_scratch_bytes(&c), gb = attn_cross_grad_scratch_bytes(&c);
         char *scratch = aligned_alloc(64, (sb + 63) / 64 * 64), *grad = aligned_alloc(64, (gb + 63) / 64 * 64);
         attn_cross(&c, &r[0], &r[1], &r[2], &r[3], (float *)base[4], scratch);
@@ -350,7 +350,7 @@ static void test_beams(void) {
             continue;
         /* sizes are multiples of 8: the block ends where the workspace does */
         char *s = aligned_alloc(64, (n + 63) / 64 * 64);
-        attn_beam_select(&c, (float *)base, (int32_t *)base, (int32_t *)base, s);
+        attn_beam_select(&c, (float *)base, (int32_t *)(base + 4), (int32_t *)(base + 8), s);
         free(s);
     }
     for (int page = 16; page <= 256; page *= 2)

@@ -124,6 +124,22 @@ def test_heads_of_one_projection_and_head_major_rows(shape):
     cu.check(t, got, cu.reference(t))
 
 
+@pytest.mark.parametrize("shape", range(2))
+def test_one_head_read_as_many(shape):
+    """A head stride of 0 in what is only read: all kv heads have the first one's K, all heads the first one's dO."""
+    t = cu.Batch(*SHAPES[shape], 21)
+    D = t.D
+    for x, heads in ((t.k, t.Hkv), (t.go, t.Hq)):
+        for h in range(1, heads):
+            x[:, h * D:(h + 1) * D] = x[:, :D]
+    arrays, rows = plain(t)
+    rows.update(k=("k", 0, t.k.shape[1], 0), go=("go", 0, t.go.shape[1], 0))
+    c = Call(t, arrays, rows)
+    c()
+    ts.synchronize()
+    cu.check(t, results(c), cu.reference(t))
+
+
 def test_starts_and_lengths_of_any_kind():
     """What they name is cut to the tensors: the rest is left as it was, and nothing outside is read or written."""
     t = cu.Batch([(30, 50), (1, 20), (4, 3), (2, 100), (3, 40)], 4, 2, 64, 13, room=(30, 100))

@@ -72,7 +72,7 @@ def grad(c="call()", q="r", k="r", v="r", out="o", lse=4096, go="o", dq="x", dk=
     return "ts.attn_cross_grad(%s, %s, %s, %s, %s, %s, %s, %s, %s, %s, %s)" % (c, q, k, v, out, lse, go, dq, dk, dv, s)
 
 
-def select(c="beams()", score=8192, token=4096, parent=4096, s=4096):
+def select(c="beams()", score=8192, token=4096 * 4, parent=4096 * 5, s=4096):
     return "ts.attn_beam_select(%s, %s, %s, %s, %s)" % (c, score, token, parent, s)
 
 
@@ -114,6 +114,9 @@ REFUSED = [
     (cross(k="ts.Rows(4096, 2**22 + 8, 128)"), "k " + ROWS),
     (cross(k="ts.Rows(4096, 1024, -128)"), "k " + ROWS),
     (cross(out="r"), "o must not be q, k or v"),
+    (cross(out="ts.Rows(8192, 1024, 64)"), "heads of o must not overlap"),
+    (grad(dq="ts.Rows(4096 * 9, 1024, 0)"), "heads of dq must not overlap"),
+    (grad(dv="ts.Rows(4096 * 9, 1024, 120)"), "heads of dv must not overlap"),
     (cross(lse=4097), "lse must be"),
     (cross(s="None"), "scratch must be"),
     (cross(s=4128), "scratch must be"),
@@ -146,7 +149,9 @@ REFUSED = [
     (select("beams(scores=None)"), "scores must be"),
     (select("beams(done=4096, done_token=1000)"), "done_token must be"),
     (select("beams(done=4096, done_token=-1)"), "done_token must be"),
-    (select(score=4096), "score must not be scores"),
+    (select(score=4096), "must be four arrays"),
+    (select(token=4096 * 3, parent=4096 * 3), "must be four arrays"),
+    (select(token=8192), "must be four arrays"),
     (select(token="None"), "score, token and parent"),
     (select(parent=4098), "score, token and parent"),
     (select(s=16), "scratch must be"),

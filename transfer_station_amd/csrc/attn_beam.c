@@ -64,8 +64,8 @@ void attn_beam_select(const struct attn_beams *c, float *score, int32_t *token, 
     const struct attn_beam_cut cut = beam_check(who, c);
     if (misaligned(score, 4) || misaligned(token, 4) || misaligned(parent, 4))
         beam_fail(who, "score, token and parent must be device pointers to B * K values");
-    if (score == c->scores)
-        beam_fail(who, "score must not be scores");
+    if (score == c->scores || token == parent || (void *)score == (void *)token || (void *)score == (void *)parent)
+        beam_fail(who, "score, token, parent and scores must be four arrays");
     if (misaligned(scratch, ATTN_SCRATCH_ALIGN))
         beam_fail(who, "scratch must be non-NULL and ATTN_SCRATCH_ALIGN-aligned");
     struct attn_beam_args a;

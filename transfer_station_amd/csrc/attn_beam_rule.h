@@ -34,7 +34,7 @@ struct attn_beam_args {
     int done_token;
     int B, beams, V, K, chunks, steps;
     uint64_t *keys; /* [rows][chunks][K], largest first */
-    float *ms;      /* [rows][chunks][2]: r, the largest x log2(e), and the sum of 2^(x log2(e) - r) */
+    float *ms;      /* [rows][chunks][2]: m, the largest logit, and the sum of exp(x - m) */
     float *score;   /* [B][K] */
     int32_t *token, *parent;
 };

@@ -76,6 +76,15 @@ static void cross_check_rows(const char *who, const char *what, const struct att
     }
 }
 
+/* What a call writes: heads of one row must not share elements. */
+static void cross_check_out(const char *who, const char *what, const struct attn_rows *r, int D, int heads) {
+    cross_check_rows(who, what, r, D);
+    if (heads > 1 && r->head < D) {
+        fprintf(stderr, "%s: the heads of %s must not overlap\n", who, what);
+        abort();
+    }
+}
+
 static int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 /* Parts so that `base` workgroups become up to `target`, which run at once, each of `least` units or more of `total`. */
@@ -220,7 +229,7 @@ void attn_cross(const struct attn_cross_call *c, const struct attn_rows *q, cons
     cross_check_rows(who, "q", q, c->D);
     cross_check_rows(who, "k", k, c->D);
     cross_check_rows(who, "v", v, c->D);
-    cross_check_rows(who, "o", o, c->D);
+    cross_check_out(who, "o", o, c->D, c->Hq);
     if (o->data == q->data || o->data == k->data || o->data == v->data)
         cross_fail(who, "o must not be q, k or v");
     if (lse && misaligned(lse, 4))
@@ -259,8 +268,10 @@ void attn_cross_grad(const struct attn_cross_call *c, const struct attn_rows *q,
     static const char *const names[] = {"q", "k", "v", "o", "d_o", "dq", "dk", "dv"};
     const struct attn_rows *const all[] = {q, k, v, o, d_o, dq, dk, dv};
     cross_check_call(who, c);
-    for (int i = 0; i < 8; ++i)
+    for (int i = 0; i < 5; ++i)
         cross_check_rows(who, names[i], all[i], c->D);
+    for (int i = 5; i < 8; ++i)
+        cross_check_out(who, names[i], all[i], c->D, i == 5 ? c->Hq : c->Hkv);
     for (int i = 5; i < 8; ++i)
         for (int j = 0; j < i; ++j)
             if (all[i]->data == all[j]->data)

@@ -180,6 +180,10 @@ constexpr float kCrossSum = 65536.0f;
 // by LDS-DMA, the next one's beside the products of this one:
 //   S^T[key][row] = K . Q^T, O^T[d][row] += V^T . P^T   (v_mfma_f32_32x32x16_bf16)
 // The running maximum is raised only where a lane's sum of p over a tile passes kCrossSum.
+// Bound by the matrix units and what feeds them: 2 x 4096 rows over 4096 states, 32 heads on 8, D = 128: 519 us, 1060 TFLOP/s
+// where a library product of 8192^3 reaches 1279; the matrix units are at work in 54% of the cycles, the LDS in 27%. At
+// D = 64 287 us (960 TFLOP/s; the exponentials weigh twice as much), 16 heads of 80 209, 2 x 2048 of 16 heads of 256 140. At
+// 77 states (4 x 4096 rows, 10 heads of 64: 19 us) it is bound by the rows' way in and out, 43 MB, and by its start.
 // ------------------------------------------------------------------------------------------
 template <int DP> __global__ __launch_bounds__(256, DP <= 96 ? 3 : 2) void attn_cross_kernel(const attn_cross_args a) {
     constexpr int KT = cross_tile_keys(DP), KN = DP / 16, NT = KT / 32;
@@ -353,7 +357,10 @@ struct cross_units {
 // states, the waves interleaved tiles of 32 states, each with a softmax of its own:
 //   S^T[key][row] = K . Q^T   (v_mfma_f32_16x16x32_bf16, K from memory straight into the operand)
 //   O^T[d][row]  += V^T . P^T (V through a wave-private LDS tile and the transposed read)
-// and joins them in LDS. Bound by HBM. NTL: K and V are read once, past the L2.
+// and joins them in LDS. NTL: K and V are read once, past the L2. NW = 1: the waves take a kv head each, whose
+// rows are read 1 KB of neighbouring heads at a time (rows_cut has the rule). Bound by HBM:
+// 64 tokens over 3277 to 8192 states of 8 heads of 128, 1.55 GB, 231 us (6.7 TB/s), 32 over 4096 at D = 256 161 us; by latency
+// where there is less: 16 times five beams over 750 to 1500 states of 16 heads of 64, 72 MB, 22 us, one over 1500 6 us.
 // ------------------------------------------------------------------------------------------
 template <int DP, int NRB, bool NTL, int NW>
 __global__ __launch_bounds__(256, 2) void attn_cross_rows_kernel(const attn_cross_args a) {
@@ -618,7 +625,7 @@ __global__ __launch_bounds__(256, 2) void attn_cross_rows_kernel(const attn_cros
 
 // Joins the parts of each row: w_s = 2^(m_s - max m), O = sum w_s acc_s / sum w_s l_s, lse the logarithm of the sum. A
 // workgroup takes 256 / (LP SG) rows of one sequence at a time: LP = 2^lglp lanes of four columns each, SG groups of
-// parts. What bounds it is latency: NP parts of a thread are asked for at once.
+// parts. What bounds it is latency: NP parts of a thread are asked for at once (3.6 to 4.8 us a launch).
 template <int NP, int SG>
 __global__ __launch_bounds__(256) void attn_cross_merge_kernel(const attn_cross_args a, int lglp, int tpm) {
     __shared__ __attribute__((aligned(16))) f32x4 accs[SG > 1 ? 256 : 1];
@@ -715,7 +722,11 @@ __global__ __launch_bounds__(256) void attn_cross_merge_kernel(const attn_cross_
 // ------------------------------------------------------------------------------------------
 // dQ. Laid out as the forward kernel: 32 rows of a wave keep Q and dO in registers, tiles of K and V pass through LDS:
 //   S^T[key][row] = K . Q^T, dP^T[key][row] = V . dO^T, dQ^T[d][row] += K^T . dS^T
-// K's tile is read both ways. delta = sum dO O is taken on the way in and left for the kernel of dK and dV.
+// K's tile is read both ways. delta = sum dO O is taken on the way in and left for the kernel of dK and dV. Where a
+// sequence has up to 32 states it is sum P dP instead: O's rounding shifts all of a row's dS alike, and O is the larger beside
+// V - O the fewer states there are (3 states: dQ off by 2.9e-3 in the norm, without 2.4e-3).
+// Six products of the size of S where the forward has four: 724 us at its 4096 x 4096 (1139 TFLOP/s, matrix units 60%), D = 64
+// 386, 16 heads of 80 285, 2 x 2048 of 16 heads of 256 263 (one wave per SIMD: Q, dO and dQ are 256 registers).
 // ------------------------------------------------------------------------------------------
 template <int DP>
 __global__ __launch_bounds__(256, DP == 64 ? 4 : DP == 96 ? 3 : DP == 128 ? 2 : 1) void attn_cross_dq_kernel(const attn_cross_args a) {
@@ -774,13 +785,21 @@ __global__ __launch_bounds__(256, DP == 64 ? 4 : DP == 96 ? 3 : DP == 128 ? 2 : 
         }
         delta = sum_xor32(delta);
         const float lse2 = a.lse[slot] * kLog2e;
-        if (valid && sp == 0 && hi == 0)
-            a.delta[slot] = delta;
         f32x16 o[DP / 32];
 #pragma unroll
         for (int db = 0; db < DP / 32; ++db)
             zero16(o[db]);
 
+        auto products = [&](const uint16_t *kv, int t, f32x16 &s, f32x16 &dp) __attribute__((always_inline)) {
+            zero16(s);
+            zero16(dp);
+#pragma unroll
+            for (int kk = 0; kk < KN; ++kk)
+                s = mfma32(ln.nat(kv, t, kk), qb[kk], s);
+#pragma unroll
+            for (int kk = 0; kk < KN; ++kk)
+                dp = mfma32(ln.nat(kv + VO, t, kk), gb[kk], dp);
+        };
         auto compute = [&](int kb, const uint16_t *kv) __attribute__((always_inline)) {
             if (idle)
                 return;
@@ -789,14 +808,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 4 : DP == 96 ? 3 : DP == 128 ? 2 : 
                 if (t > 0 && kb + 32 * t >= k1)
                     return;
                 f32x16 s, dp;
-                zero16(s);
-                zero16(dp);
-#pragma unroll
-                for (int kk = 0; kk < KN; ++kk)
-                    s = mfma32(ln.nat(kv, t, kk), qb[kk], s);
-#pragma unroll
-                for (int kk = 0; kk < KN; ++kk)
-                    dp = mfma32(ln.nat(kv + VO, t, kk), gb[kk], dp);
+                products(kv, t, s, dp);
                 bf16x8 pk[2];
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
@@ -821,6 +833,18 @@ __global__ __launch_bounds__(256, DP == 64 ? 4 : DP == 96 ? 3 : DP == 128 ? 2 : 
             load(k0, KV0);
         wait_loads();
         __syncthreads();
+        if (kr.n <= 32 && k0 < k1 && !idle) {
+            f32x16 s, dp;
+            products(KV0, 0, s, dp);
+            delta = 0.f;
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                if (8 * (i >> 2) + 4 * hi + (i & 3) < k1)
+                    delta = fmaf(fast_exp2(fmaf(s[i], a.c, -lse2)), dp[i], delta);
+            delta = sum_xor32(delta);
+        }
+        if (valid && sp == 0 && hi == 0)
+            a.delta[slot] = delta;
         auto step = [&](int kb, const uint16_t *kv, uint16_t *next) __attribute__((always_inline)) {
             if (kb + KT < k1)
                 load(kb + KT, next);
@@ -848,6 +872,9 @@ __global__ __launch_bounds__(256, DP == 64 ? 4 : DP == 96 ? 3 : DP == 128 ? 2 : 
 //   S[row][key] = Q . K^T, dP[row][key] = dO . V^T, dV^T[d][key] += dO^T . P, dK^T[d][key] += Q^T . dS
 // Both tiles are read both ways. Two teams of four waves (TEAMS = 2) have the same states and take steps of 32 rows in turn;
 // their sums are joined in LDS at the end.
+// Eight products of that size: 997 us at 4096 x 4096 (1103 TFLOP/s, matrix units 53%; half of a wave's time goes in waits, for
+// operands and at the barrier of each step, with all 256 registers in use), D = 64 615, 16 heads of 80 410. At D = 256 dK and
+// dV are two launches (232 and 184 us for 2 x 2048 of 16 heads on 8): with both, accumulators go to memory, 578 us.
 // ------------------------------------------------------------------------------------------
 template <int DP, bool DK, bool DV, int TEAMS>
 __global__ __launch_bounds__(256 * TEAMS, TEAMS > 1 ? 1 : DP == 64 ? 3 : DP <= 128 || !DK ? 2 : 1)
@@ -1038,7 +1065,7 @@ void attn_cross_dkv_kernel(const attn_cross_args a) {
     }
 }
 
-// Adds the parts of dQ's rows (KV = false), or of dK's and dV's, in order. 256 / LP rows of one sequence at a time.
+// Adds the parts of dQ's rows (KV = false), or of dK's and dV's, in order. 256 / LP rows of one sequence at a time. 5 to 8 us.
 template <bool KV>
 __global__ __launch_bounds__(256) void attn_cross_sum_kernel(const attn_cross_args a, int lglp, int tpm) {
     const int b = uniform(wg_id_x() / tpm), t0 = wg_id_x() - b * tpm, tid = wi_id_x();
@@ -1127,7 +1154,7 @@ extern "C" int attn_hip_launch_cross(const struct attn_cross_args *ap, const str
         constexpr std::integral_constant<int, 1> one;
         constexpr std::integral_constant<int, 2> two;
         constexpr std::integral_constant<int, 4> four;
-                        // Past the L2 where a row tile is the only one of its sequence, which up to D = 128 it always is.
+        // Past the L2 where a row tile is the only one of its sequence, which up to D = 128 it always is.
         if constexpr (DP > 128) {
             if (cut->rows16 == 1)
                 return with_flag(a.tps == 1, [&](auto NT) {
