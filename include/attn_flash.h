@@ -234,8 +234,8 @@ void attn_cross(const struct attn_cross_call *c, const struct attn_rows *q, cons
                 const struct attn_rows *v, const struct attn_rows *o, float *lse, void *scratch);
 
 /* The gradients of q, k and v, in bf16, from that of o (d_o) and what the forward call left in o and lse. dK and dV are
- * summed over the heads of a group. P and dS are rounded to bf16 before their products. States of a sequence without
- * rows get zeros; rows and states of no sequence are left as they are. Here sequences may share neither rows nor
+ * summed over the heads of a group. P and dS are rounded to bf16 before their products, in calls of up to 2^21 scores
+ * (B Hq q.max k.max) in two parts, to 16 bits. States of a sequence without rows get zeros; rows and states of no sequence are left as they are. Here sequences may share neither rows nor
  * states: what two of them claim may hold neither's gradient. dq, dk and dv must overlap none of the other tensors.
  * Sums have a fixed order: the same call gives the same bits.
  * scratch: attn_cross_grad_scratch_bytes(c) bytes: 4 q.T Hq, and, where few sequences leave the GPU unfilled, up to 128

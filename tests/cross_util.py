@@ -15,7 +15,7 @@ class Batch:
 
     def __init__(self, seqs, Hq, Hkv, D, seed, room=None, claim=0, pad=3, sigma_q=1.0, stride=0, offset=0):
         self.seqs, self.Hq, self.Hkv, self.D, self.room, self.claim = seqs, Hq, Hkv, D, room, claim
-        self.B = len(seqs)
+        self.B, self.fine = len(seqs), (False, False)
         self.spans = {}
         for x, i, heads in (("q", 0, Hq), ("k", 1, Hkv)):
             n = [s[i] for s in seqs]
@@ -56,7 +56,8 @@ class Batch:
 def reference(t, scale=0.0, grad=True):
     """{name: (values, bound)} of o, lse, dq, dk and dv, in float64.
 
-    With e = 2^-8: P and dS enter their products rounded to bf16 (e of each), each result is rounded once (e of it).
+    With e = 2^-8: P and dS enter their products rounded to bf16 (e of each; in two parts, e^2 = 2^-16), each result is
+    rounded once (2^-8 of it).
     O and dV: off by (e + d) sum P |.| + e |result|, where d is what P is off by before its rounding: a score is off by
     (D + 8) roundings of 2^-24 of sum |q||k|, as is lse, exp2 is good to 2^-21 and enters once per tile and weight.
     dS = P (dP - delta): delta is made of the rounded O (off by what O is), or, of up to 32 states, of P dP in fp32 (off by d
@@ -102,15 +103,17 @@ def reference(t, scale=0.0, grad=True):
                 delta_off = (P * ((d + m * E32) * np.abs(dP) + (t.D + 8) * E32 * (Ga @ np.abs(V).T))).sum(1, keepdims=True)
             else:
                 delta_off = (Ga * o_off).sum(1, keepdims=True) + (t.D + 8) * E32 * (Ga * np.abs(O)).sum(1, keepdims=True)
-            ds_off = (E * 1.01 + d) * np.abs(dS) + P * (delta_off + (t.D + 8) * E32 * (Ga @ np.abs(V).T))
+            ds_off = d * np.abs(dS) + P * (delta_off + (t.D + 8) * E32 * (Ga @ np.abs(V).T))
+            # e of P and dS in dQ, and in dK and dV
+            eq, ek = (2.0 ** -16 if f else E * 1.01 for f in t.fine)
             dQ = scale * (dS @ K)
             out["dq"][0][rows, h] = dQ
-            out["dq"][1][rows, h] = (scale * ((ds_off + m * E32 * np.abs(dS)) @ np.abs(K)) + E * np.abs(dQ) + 1e-30)
+            out["dq"][1][rows, h] = (scale * ((ds_off + (eq + m * E32) * np.abs(dS)) @ np.abs(K)) + E * np.abs(dQ) + 1e-30)
             n_all = n * g
             out["dk"][0][states, u] += scale * (dS.T @ Q)
-            out["dk"][1][states, u] += scale * ((ds_off + n_all * E32 * np.abs(dS)).T @ np.abs(Q))
+            out["dk"][1][states, u] += scale * ((ds_off + (ek + n_all * E32) * np.abs(dS)).T @ np.abs(Q))
             out["dv"][0][states, u] += P.T @ G
-            out["dv"][1][states, u] += ((E * 1.01 + d + n_all * E32) * P).T @ Ga
+            out["dv"][1][states, u] += ((ek + d + n_all * E32) * P).T @ Ga
         for x in ("dk", "dv"):
             out[x][1][states] += E * np.abs(out[x][0][states]) + 1e-30
     return out
@@ -132,7 +135,11 @@ def call_of(t, bufs, scale=0.0, max_q=None, max_k=None):
             return ts.Spans(bufs[x + "_start"], T, most, bufs[x + "_len"])
         return ts.Spans(bufs[x + "_start"], T, most)
 
-    return ts.CrossCall(spans("q", 0, max_q), spans("k", 1, max_k), t.B, t.Hq, t.Hkv, t.D, scale)
+    call = ts.CrossCall(spans("q", 0, max_q), spans("k", 1, max_k), t.B, t.Hq, t.Hkv, t.D, scale)
+    # Do dQ's kernel, and dK's and dV's, take P and dS in two parts?
+    names = [p[0] for p in ts.attn_cross_plan(call, True)]
+    t.fine = tuple(all(n.endswith("true>") for n in names if x in n) for x in ("_dq_", "_dkv_"))
+    return call
 
 
 def run(t, scale=0.0, grad=True, max_q=None, max_k=None, lse=True):

@@ -48,6 +48,8 @@ CASES = [
     ([(33 + b % 7 * 9, 13 * b * b % 600 // 3 * 3 + (b == 5) * 500) for b in range(64)], 10, 10, 64, None, 0),
     ([(30 * b, 280 - 11 * b) for b in range(21)], 16, 16, 32, None, 0),
     ([(33 + b % 40, 600 - b) for b in range(65)], 8, 8, 64, None, 0),
+    # more scores than are taken in two parts
+    ([(300, 1100)], 8, 8, 80, None, 0),
     # two teams of waves for dK and dV
     ([(4200, 130)], 16, 16, 64, None, 0),
     ([(2100, 100), (100, 33)], 16, 16, 80, None, 0),

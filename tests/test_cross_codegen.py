@@ -67,7 +67,7 @@ def test_tiles_wait_for_their_dma_at_the_end_of_a_step(code):
                 if nxt and nxt[0].startswith("ds_read"):
                     bad.append(i)
         assert not bad, (name, bad)
-    assert n == 16
+    assert n == 25
 
 
 def test_accumulators_stay_in_registers(code):

@@ -206,15 +206,20 @@ PLANS = [
     (0, 112, 8, 16, 16, 1000, 1500, [("kernel<128>", "parts=1 share=1536", 1024)]),
     # rows for too many partial slots: no parts
     (0, 64, 70000, 1, 1, 1, 2, [("rows_kernel<64, 1, true, 4>", "parts=1 share=1", 70000)]),
-    (1, 64, 3, 8, 8, 37, 50, [("dq_kernel<64>", "parts=1 share=128", 24),
-                              ("dkv_kernel<64, true, true, 1>", "parts=1 share=2", 24)]),
-    (1, 64, 4, 10, 10, 4096, 77, [("dq_kernel<64>", "parts=1 share=128", 1280),
-                                  ("dkv_kernel<64, true, true, 2>", "parts=6 share=22", 240), ("sum_kernel<true>", "", 388)]),
-    (1, 128, 2, 32, 8, 4096, 4096, [("dq_kernel<128>", "parts=1 share=4096", 2048),
-                                    ("dkv_kernel<128, true, true, 1>", "parts=1 share=512", 512)]),
-    (1, 256, 1, 4, 2, 100, 9000, [("dq_kernel<256>", "parts=35 share=384", 140), ("sum_kernel<false>", "", 100),
-                                  ("dkv_kernel<256, true, false, 1>", "parts=1 share=8", 142),
-                                  ("dkv_kernel<256, false, true, 1>", "parts=1 share=8", 142)]),
+    (1, 64, 3, 8, 8, 37, 50, [("dq_kernel<64, true>", "parts=1 share=128", 24),
+                              ("dkv_kernel<64, true, true, 1, true>", "parts=1 share=2", 24)]),
+    # up to 2^21 scores P and dS in two parts
+    (1, 64, 1, 4, 4, 1024, 512, [("dq_kernel<64, true>", "parts=2 share=256", 64), ("sum_kernel<false>", "", 256),
+                                 ("dkv_kernel<64, true, true, 1, true>", "parts=16 share=2", 256), ("sum_kernel<true>", "", 256)]),
+    (1, 64, 1, 4, 4, 1024, 513, [("dq_kernel<64, false>", "parts=2 share=384", 64), ("sum_kernel<false>", "", 256),
+                                 ("dkv_kernel<64, true, true, 1, false>", "parts=16 share=2", 320), ("sum_kernel<true>", "", 257)]),
+    (1, 64, 4, 10, 10, 4096, 77, [("dq_kernel<64, false>", "parts=1 share=128", 1280),
+                                  ("dkv_kernel<64, true, true, 2, false>", "parts=6 share=22", 240), ("sum_kernel<true>", "", 388)]),
+    (1, 128, 2, 32, 8, 4096, 4096, [("dq_kernel<128, false>", "parts=1 share=4096", 2048),
+                                    ("dkv_kernel<128, true, true, 1, false>", "parts=1 share=512", 512)]),
+    (1, 256, 1, 4, 2, 100, 9000, [("dq_kernel<256, false>", "parts=35 share=384", 140), ("sum_kernel<false>", "", 100),
+                                  ("dkv_kernel<256, true, false, 1, false>", "parts=1 share=8", 142),
+                                  ("dkv_kernel<256, false, true, 1, false>", "parts=1 share=8", 142)]),
 ]
 
 

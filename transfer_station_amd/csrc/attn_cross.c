@@ -143,10 +143,17 @@ static struct attn_cross_cut forward_cut(const struct attn_cross_call *c) {
                      ATTN_CROSS_KEY_STEP);
 }
 
+static int is_fine(const struct attn_cross_call *c) {
+    return (int64_t)c->B * c->Hq * bound_of(&c->q) * bound_of(&c->k) <= ATTN_CROSS_FINE;
+}
+
 static struct attn_cross_cut dq_cut(const struct attn_cross_call *c) {
     const int64_t R = (int64_t)bound_of(&c->q) * (c->Hq / c->Hkv), groups = (int64_t)c->B * c->Hkv;
-    return cross_cut(groups, (int)ceil_div(R, ATTN_CROSS_ROWS), bound_of(&c->k), 256, c->D <= 128 ? 512 : 256,
-                     ATTN_CROSS_GRAD_FLOATS / ((int64_t)c->q.T * c->Hq * c->D), ATTN_CROSS_KEY_STEP);
+    struct attn_cross_cut cut =
+        cross_cut(groups, (int)ceil_div(R, ATTN_CROSS_ROWS), bound_of(&c->k), 256, c->D <= 128 ? 512 : 256,
+                  ATTN_CROSS_GRAD_FLOATS / ((int64_t)c->q.T * c->Hq * c->D), ATTN_CROSS_KEY_STEP);
+    cut.fine = is_fine(c);
+    return cut;
 }
 
 /* Where tiles of states are no more than the CUs and each has rows enough, eight waves share one, as two teams that take its
@@ -161,6 +168,7 @@ static struct attn_cross_cut dkv_cut(const struct attn_cross_call *c) {
         cross_cut(groups, (int)tps, steps, 2 * row_teams, row_teams > 1 || c->D > 128 ? 256 : 512,
                   ATTN_CROSS_GRAD_FLOATS / ((int64_t)c->k.T * c->Hkv * c->D * 2), row_teams);
     cut.row_teams = row_teams;
+    cut.fine = row_teams == 1 && is_fine(c);
     return cut;
 }
 

@@ -5,7 +5,8 @@
 //   delta = sum_d dO O, dS = P (dO.V - delta), dQ = scale dS.K, dK = scale dS^T.Q, dV = P^T.dO
 //
 // in fp32 but for the operands of the MFMAs: Q, K, V and dO as they are, P and dS rounded to bf16 (half a unit of
-// 2^-8, as much as the outputs' own rounding); outputs are rounded once. Nothing is accumulated by atomics: each
+// 2^-8, as much as the outputs' own rounding), in the gradients of small calls in two parts (FINE, ATTN_CROSS_FINE);
+// outputs are rounded once. Nothing is accumulated by atomics: each
 // output has one workgroup, or parts that are added in order, so that a call gives the same bits every time.
 //
 // Tiles lie in LDS in one layout that serves both ways of reading them without bank conflicts: rows in groups of
@@ -76,6 +77,19 @@ __device__ __forceinline__ float lse_of(float m, float l) { return (m + __builti
 
 __device__ __forceinline__ f32x16 mfma32(bf16x8 x, bf16x8 y, f32x16 z) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, y, z, 0, 0, 0);
+}
+
+// Element i of 16 as a matrix operand's: rounded to bf16, with FINE in two parts, the second what the first leaves (off by
+// 2^-17 of the element).
+template <bool FINE> __device__ __forceinline__ void split(float x, int i, bf16x8 *hi, bf16x8 *lo) {
+    const __bf16 h = (__bf16)x;
+    hi[i >> 3][i & 7] = h;
+    if (FINE)
+        lo[i >> 3][i & 7] = (__bf16)(x - (float)h);
+}
+template <bool FINE> __device__ __forceinline__ f32x16 mfma_fine(bf16x8 x, bf16x8 hi, bf16x8 lo, f32x16 z) {
+    z = mfma32(x, hi, z);
+    return FINE ? mfma32(x, lo, z) : z;
 }
 
 // Bytes from a row's first element to the end of `rows` rows, 0 where there are none.
@@ -728,8 +742,8 @@ __global__ __launch_bounds__(256) void attn_cross_merge_kernel(const attn_cross_
 // Six products of the size of S where the forward has four: 724 us at its 4096 x 4096 (1139 TFLOP/s, matrix units 60%), D = 64
 // 386, 16 heads of 80 285, 2 x 2048 of 16 heads of 256 263 (one wave per SIMD: Q, dO and dQ are 256 registers).
 // ------------------------------------------------------------------------------------------
-template <int DP>
-__global__ __launch_bounds__(256, DP == 64 ? 4 : DP == 96 ? 3 : DP == 128 ? 2 : 1) void attn_cross_dq_kernel(const attn_cross_args a) {
+template <int DP, bool FINE>
+__global__ __launch_bounds__(256, FINE ? 1 : DP == 64 ? 4 : DP == 96 ? 3 : DP == 128 ? 2 : 1) void attn_cross_dq_kernel(const attn_cross_args a) {
     constexpr int KT = cross_tile_keys(DP), KN = DP / 16, NT = KT / 32;
     constexpr int VO = KT * DP;
     __shared__ __attribute__((aligned(1024))) uint16_t KV0[2 * VO], KV1[2 * VO];
@@ -809,7 +823,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 4 : DP == 96 ? 3 : DP == 128 ? 2 : 
                     return;
                 f32x16 s, dp;
                 products(kv, t, s, dp);
-                bf16x8 pk[2];
+                bf16x8 pk[2], lo[2];
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
                     dp[i] = fast_exp2(fmaf(s[i], a.c, -lse2)) * (dp[i] - delta);
@@ -821,12 +835,12 @@ __global__ __launch_bounds__(256, DP == 64 ? 4 : DP == 96 ? 3 : DP == 128 ? 2 : 
                             dp[i] = 0.f;
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
-                    pk[i >> 3][i & 7] = (__bf16)dp[i];
+                    split<FINE>(dp[i], i, pk, lo);
 #pragma unroll
                 for (int cc = 0; cc < 2; ++cc)
 #pragma unroll
                     for (int db = 0; db < DP / 32; ++db)
-                        o[db] = mfma32(ln.tr(kv, 2 * t + cc, db), pk[cc], o[db]);
+                        o[db] = mfma_fine<FINE>(ln.tr(kv, 2 * t + cc, db), pk[cc], lo[cc], o[db]);
             }
         };
         if (k0 < k1)
@@ -876,8 +890,8 @@ __global__ __launch_bounds__(256, DP == 64 ? 4 : DP == 96 ? 3 : DP == 128 ? 2 : 
 // operands and at the barrier of each step, with all 256 registers in use), D = 64 615, 16 heads of 80 410. At D = 256 dK and
 // dV are two launches (232 and 184 us for 2 x 2048 of 16 heads on 8): with both, accumulators go to memory, 578 us.
 // ------------------------------------------------------------------------------------------
-template <int DP, bool DK, bool DV, int TEAMS>
-__global__ __launch_bounds__(256 * TEAMS, TEAMS > 1 ? 1 : DP == 64 ? 3 : DP <= 128 || !DK ? 2 : 1)
+template <int DP, bool DK, bool DV, int TEAMS, bool FINE>
+__global__ __launch_bounds__(256 * TEAMS, TEAMS > 1 || FINE ? 1 : DP == 64 ? 3 : DP <= 128 || !DK ? 2 : 1)
 void attn_cross_dkv_kernel(const attn_cross_args a) {
     constexpr int QT = ATTN_CROSS_STEP, KN = DP / 16, KEYS = ATTN_CROSS_KEYS;
     constexpr int GO = QT * DP; // dO's tile behind Q's
@@ -989,7 +1003,7 @@ void attn_cross_dkv_kernel(const attn_cross_args a) {
                     __builtin_amdgcn_sched_group_barrier(0x008, 3, 0);
                     __builtin_amdgcn_sched_barrier(0);
                 }
-                bf16x8 pk[2], dk8[2];
+                bf16x8 pk[2], dk8[2], plo[2], dlo[2];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const f32x4 l = *reinterpret_cast<const f32x4 *>(sb + 32 * t + 8 * j + 4 * hi);
@@ -997,8 +1011,8 @@ void attn_cross_dkv_kernel(const attn_cross_args a) {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const float p = fast_exp2(fmaf(s[4 * j + i], a.c, -l[i]));
-                        pk[j >> 1][4 * (j & 1) + i] = (__bf16)p;
-                        dk8[j >> 1][4 * (j & 1) + i] = (__bf16)(p * (dp[4 * j + i] - e[i]));
+                        split<FINE>(p, 4 * j + i, pk, plo);
+                        split<FINE>(p * (dp[4 * j + i] - e[i]), 4 * j + i, dk8, dlo);
                     }
                 }
 #pragma unroll
@@ -1006,9 +1020,9 @@ void attn_cross_dkv_kernel(const attn_cross_args a) {
 #pragma unroll
                     for (int db = 0; db < DP / 32; ++db) {
                         if (DV)
-                            dv[db] = mfma32(ln.tr(qg + GO, 2 * t + cc, db), pk[cc], dv[db]);
+                            dv[db] = mfma_fine<FINE>(ln.tr(qg + GO, 2 * t + cc, db), pk[cc], plo[cc], dv[db]);
                         if (DK)
-                            dk[db] = mfma32(ln.tr(qg, 2 * t + cc, db), dk8[cc], dk[db]);
+                            dk[db] = mfma_fine<FINE>(ln.tr(qg, 2 * t + cc, db), dk8[cc], dlo[cc], dk[db]);
                     }
             }
         };
@@ -1203,35 +1217,44 @@ extern "C" int attn_hip_launch_cross_grad(const struct attn_cross_args *ap, cons
     const dim3 grid((unsigned)cut->grid), block(256);
     const hipError_t e = with_width(a.D, [&](auto W) {
         constexpr int DP = decltype(W)::value;
-        if (!kv) {
-            if (t_plan) {
-                plan_note(grid, block, "attn_cross_dq_kernel<%d> parts=%d share=%d", DP, a.nsplit, a.share);
-                return hipSuccess;
-            }
-            hipLaunchKernelGGL((attn_cross_dq_kernel<DP>), grid, block, 0, st, a);
-            return hipGetLastError();
-        }
-        auto dkv = [&](auto K, auto V, auto T) {
-            constexpr bool kK = decltype(K)::value, kV = decltype(V)::value;
+        if (!kv)
+            return with_flag(cut->fine, [&](auto F) {
+                constexpr bool kF = decltype(F)::value;
+                if (t_plan) {
+                    plan_note(grid, block, "attn_cross_dq_kernel<%d, %s> parts=%d share=%d", DP, tf(kF), a.nsplit, a.share);
+                    return hipSuccess;
+                }
+                hipLaunchKernelGGL((attn_cross_dq_kernel<DP, kF>), grid, block, 0, st, a);
+                return hipGetLastError();
+            });
+        auto dkv = [&](auto K, auto V, auto T, auto F) {
+            constexpr bool kK = decltype(K)::value, kV = decltype(V)::value, kF = decltype(F)::value;
             constexpr int kT = decltype(T)::value;
             if (t_plan) {
-                plan_note(grid, dim3(256 * kT), "attn_cross_dkv_kernel<%d, %s, %s, %d> parts=%d share=%d", DP, tf(kK),
-                          tf(kV), kT, a.nsplit, a.share);
+                plan_note(grid, dim3(256 * kT), "attn_cross_dkv_kernel<%d, %s, %s, %d, %s> parts=%d share=%d", DP, tf(kK),
+                          tf(kV), kT, tf(kF), a.nsplit, a.share);
                 return hipSuccess;
             }
-            hipLaunchKernelGGL((attn_cross_dkv_kernel<DP, kK, kV, kT>), grid, dim3(256 * kT), 0, st, a);
+            hipLaunchKernelGGL((attn_cross_dkv_kernel<DP, kK, kV, kT, kF>), grid, dim3(256 * kT), 0, st, a);
             return hipGetLastError();
         };
         constexpr std::true_type yes;
         constexpr std::false_type no;
         constexpr std::integral_constant<int, 1> one;
         constexpr std::integral_constant<int, 2> two;
-        if constexpr (DP > 128) {
-            const hipError_t x = dkv(yes, no, one);
-            return x != hipSuccess ? x : dkv(no, yes, one);
-        } else {
-            return cut->row_teams == 2 ? dkv(yes, yes, two) : dkv(yes, yes, one);
+        if (cut->row_teams == 2) {
+            if constexpr (DP <= 128)
+                return dkv(yes, yes, two, no);
+            return hipErrorInvalidValue;
         }
+        return with_flag(cut->fine, [&](auto F) {
+            if constexpr (DP > 128) {
+                const hipError_t x = dkv(yes, no, one, F);
+                return x != hipSuccess ? x : dkv(no, yes, one, F);
+            } else {
+                return dkv(yes, yes, one, F);
+            }
+        });
     });
     if (e != hipSuccess || a.nsplit == 1)
         return (int)e;

@@ -52,6 +52,13 @@ ATTN_HD struct attn_cut attn_cut_of(int total, int share, int nsplit, int step) 
 
 #define ATTN_CROSS_STEP 32 /* rows of a step of the kernel of dK and dV */
 
+/* Calls of up to this many scores (heads, rows and states as the call bounds them) take P and dS of the gradients in two bf16
+ * parts each, which makes their products as good as fp32's: dQ, dK and dV are off by their own rounding, 1.7e-3 in the norm,
+ * not by 2.4e-3, which single rows and heads pass by a fifth. They wait more than they compute: 512 rows over 512 states, 16
+ * heads of 64 48.5 -> 50.6 us, 8 x 100 over 100 of 128 46.9 -> 45.6, 37 over 50 16.5 -> 17.5; but 4 x 200 over 300 of 96,
+ * 2^22 scores, 54 -> 61. */
+#define ATTN_CROSS_FINE (1L << 21)
+
 /* Launches of 2 to 64 sequences (a wave's lanes), of more workgroups than run at once, start the longest first: eight
  * prompts of 210 to 700 tokens over 2000 to 4001 states 226 -> 216 us, the step of eight by up to 1000 and 1500 268 ->
  * 245. Tiles that walk few rows are over before it pays (77 states: 3 us lost of 73). */
@@ -82,6 +89,7 @@ struct attn_cross_cut {
     int parts;  /* of a sequence of the call's bounds, about */
     int teams;  /* that kernel: teams of the decode line, 0: whole sequences */
     int row_teams; /* the kernel of dK and dV: teams of four waves that share a tile of states */
+    int fine;      /* gradients: P and dS in two parts */
     long grid;
 };
 
