@@ -47,7 +47,7 @@ static struct attn_beam_cut beam_check(const char *who, const struct attn_beams 
         beam_fail(who, "scores must be a device pointer to B * beams floats");
     if (c->done && (c->done_token < 0 || c->done_token >= c->V))
         beam_fail(who, "done_token must be in [0, V)");
-    return attn_beam_cut_of((int64_t)c->B * c->beams, c->V, c->bits / 8);
+    return attn_beam_cut_of((int64_t)c->B * c->beams, c->V, c->bits / 8, c->beams, c->K);
 }
 
 static size_t keys_bytes(const struct attn_beams *c, int chunks) {
