@@ -82,14 +82,15 @@ __device__ __forceinline__ f32x16 mfma32(bf16x8 x, bf16x8 y, f32x16 z) {
 // Element i of 16 as a matrix operand's: rounded to bf16, with FINE in two parts, the second what the first leaves (off by
 // 2^-17 of the element).
 template <bool FINE> __device__ __forceinline__ void split(float x, int i, bf16x8 *hi, bf16x8 *lo) {
-    const __bf16 h = (__bf16)x;
-    hi[i >> 3][i & 7] = h;
-    if (FINE)
-        lo[i >> 3][i & 7] = (__bf16)(x - (float)h);
+    hi[i >> 3][i & 7] = (__bf16)x;
+    if constexpr (FINE)
+        lo[i >> 3][i & 7] = (__bf16)(x - (float)(__bf16)x);
 }
-template <bool FINE> __device__ __forceinline__ f32x16 mfma_fine(bf16x8 x, bf16x8 hi, bf16x8 lo, f32x16 z) {
+template <bool FINE> __device__ __forceinline__ f32x16 mfma_fine(bf16x8 x, const bf16x8 &hi, const bf16x8 &lo, f32x16 z) {
     z = mfma32(x, hi, z);
-    return FINE ? mfma32(x, lo, z) : z;
+    if constexpr (FINE)
+        z = mfma32(x, lo, z);
+    return z;
 }
 
 // Bytes from a row's first element to the end of `rows` rows, 0 where there are none.
@@ -1011,8 +1012,13 @@ void attn_cross_dkv_kernel(const attn_cross_args a) {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const float p = fast_exp2(fmaf(s[4 * j + i], a.c, -l[i]));
-                        split<FINE>(p, 4 * j + i, pk, plo);
-                        split<FINE>(p * (dp[4 * j + i] - e[i]), 4 * j + i, dk8, dlo);
+                        if constexpr (FINE) {
+                            split<FINE>(p, 4 * j + i, pk, plo);
+                            split<FINE>(p * (dp[4 * j + i] - e[i]), 4 * j + i, dk8, dlo);
+                        } else {
+                            pk[j >> 1][4 * (j & 1) + i] = (__bf16)p;
+                            dk8[j >> 1][4 * (j & 1) + i] = (__bf16)(p * (dp[4 * j + i] - e[i]));
+                        }
                     }
                 }
 #pragma unroll
@@ -1020,9 +1026,13 @@ void attn_cross_dkv_kernel(const attn_cross_args a) {
 #pragma unroll
                     for (int db = 0; db < DP / 32; ++db) {
                         if (DV)
-                            dv[db] = mfma_fine<FINE>(ln.tr(qg + GO, 2 * t + cc, db), pk[cc], plo[cc], dv[db]);
+                            dv[db] = mfma32(ln.tr(qg + GO, 2 * t + cc, db), pk[cc], dv[db]);
+                        if constexpr (DV && FINE)
+                            dv[db] = mfma32(ln.tr(qg + GO, 2 * t + cc, db), plo[cc], dv[db]);
                         if (DK)
-                            dk[db] = mfma_fine<FINE>(ln.tr(qg, 2 * t + cc, db), dk8[cc], dlo[cc], dk[db]);
+                            dk[db] = mfma32(ln.tr(qg, 2 * t + cc, db), dk8[cc], dk[db]);
+                        if constexpr (DK && FINE)
+                            dk[db] = mfma32(ln.tr(qg, 2 * t + cc, db), dlo[cc], dk[db]);
                     }
             }
         };
