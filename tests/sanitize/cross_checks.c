@@ -322,6 +322,15 @@ int attn_hip_launch_beam(const struct attn_beam_args *a, int bits, void *stream)
     CHECK(a->chunks >= 1 && a->steps >= 1 && (int64_t)a->chunks * a->steps * 4 * ATTN_BEAM_STEP(bits / 8) >= a->V &&
               (int64_t)(a->chunks - 1) * a->steps * 4 * ATTN_BEAM_STEP(bits / 8) < a->V && rows * a->chunks <= 0x7fffffff,
           "%d chunks of %d steps for %d", a->chunks, a->steps, a->V);
+    /* each logit of an entry's lists belongs to one segment, and a thread holds all that are its */
+    const int lists = a->beams * a->chunks;
+    int seen = 0;
+    for (int s = 0; s < a->segments; ++s) {
+        const int sub = attn_div_by(s, a->by_lists), n = a->K - sub * a->seg;
+        CHECK(sub == s / lists && n > 0, "segment %d", s);
+        seen += n < a->seg ? n : a->seg;
+    }
+    CHECK(seen == lists * a->K && a->segments <= ATTN_BEAM_HELD, "%d of %d logits in %d segments", seen, lists * a->K, a->segments);
     a->keys[0] = 1, a->keys[rows * a->chunks * a->K - 1] = 1;
     a->ms[0] = 1.f, a->ms[rows * a->chunks * 2 - 1] = 1.f;
     return 0;

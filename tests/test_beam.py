@@ -87,7 +87,8 @@ SELECT = [
     (1, 1, 1, 1, 32, 0, 0), (1, 4, 7, 8, 16, 0, 1), (2, 3, 50257, 6, 32, 0, 0), (3, 4, 50257, 8, 16, 0, 1),
     (2, 5, 8192, 64, 16, 0, 0), (1, 16, 2049, 33, 32, 3, 1), (40, 8, 32001, 16, 16, 7, 0),
     (1, 256, 100, 64, 16, 0, 0), (1, 2, 262147, 4, 32, 0, 0), (2, 1, 5, 20, 32, 0, 0), (300, 4, 9000, 8, 32, 0, 0),
-    (1, 3, 1 << 20, 7, 16, 0, 0), (1, 13, 238968, 13, 16, 0, 0),
+    (1, 3, 1 << 20, 7, 16, 0, 0), (1, 13, 238968, 13, 16, 0, 0), (4, 64, 32000, 64, 32, 0, 0), (1, 200, 40000, 64, 16, 0, 0),
+    (2, 256, 5000, 50, 16, 0, 0), (1, 5, 120000, 64, 32, 0, 0),
 ]
 
 

@@ -47,7 +47,7 @@ static struct attn_beam_cut beam_check(const char *who, const struct attn_beams 
         beam_fail(who, "scores must be a device pointer to B * beams floats");
     if (c->done && (c->done_token < 0 || c->done_token >= c->V))
         beam_fail(who, "done_token must be in [0, V)");
-    return attn_beam_cut_of((int64_t)c->B * c->beams, c->V, c->bits / 8, c->beams, c->K);
+    return attn_beam_cut_of((int64_t)c->B * c->beams, c->V, c->bits / 8);
 }
 
 static size_t keys_bytes(const struct attn_beams *c, int chunks) {
@@ -72,6 +72,9 @@ void attn_beam_select(const struct attn_beams *c, float *score, int32_t *token, 
     memset(&a, 0, sizeof a);
     a.logits = c->logits, a.row = c->row, a.scores = c->scores, a.done = c->done, a.done_token = c->done_token;
     a.B = c->B, a.beams = c->beams, a.V = c->V, a.K = c->K, a.chunks = cut.chunks, a.steps = cut.steps;
+    a.seg = attn_beam_segment(c->beams * cut.chunks, c->K);
+    a.segments = c->beams * cut.chunks * ((c->K + a.seg - 1) / a.seg);
+    a.by_lists = attn_div_of(c->beams * cut.chunks), a.by_chunks = attn_div_of(cut.chunks), a.by_K = attn_div_of(c->K);
     a.keys = (uint64_t *)scratch;
     a.ms = (float *)((char *)scratch + keys_bytes(c, a.chunks));
     a.score = score, a.token = token, a.parent = parent;

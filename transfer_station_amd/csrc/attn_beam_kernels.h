@@ -33,13 +33,23 @@ __device__ __forceinline__ bool finite(float x) {
     return (opaque(__builtin_bit_cast(uint32_t, x)) & 0x7f800000u) != 0x7f800000u;
 }
 
-// A value that at least K of the wave's lanes reach (`none` where fewer are above that), and hardly more: from a lane's own
-// value up or down in growing steps until the count passes K, then by halves until it is between K and K + 7.
-__device__ __forceinline__ uint32_t wave_kth(uint32_t x, uint32_t none, uint32_t step, int K) {
-    auto count = [&](uint32_t y) { return (int)__builtin_popcountll(__builtin_amdgcn_ballot_w64(x >= y)); };
+// A value that at least K of the wave's 64 N numbers reach (`none` where fewer are above that), and hardly more: from a
+// lane's largest up or down in growing steps until the count passes K, then by halves until it is between K and K + 7.
+template <int N> __device__ __forceinline__ uint32_t wave_kth(const uint32_t (&x)[N], uint32_t none, uint32_t step, int K) {
+    auto count = [&](uint32_t y) {
+        int n = 0;
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            n += (int)__builtin_popcountll(__builtin_amdgcn_ballot_w64(x[i] >= y));
+        return n;
+    };
     if (count(none + 1) < K)
         return none;
-    uint32_t lo = max((uint32_t)__builtin_amdgcn_readfirstlane((int)x), none + 1), hi = lo; // count(lo) >= K > count(hi)
+    uint32_t first = x[0];
+#pragma unroll
+    for (int i = 1; i < N; ++i)
+        first = max(first, x[i]);
+    uint32_t lo = max((uint32_t)__builtin_amdgcn_readfirstlane((int)first), none + 1), hi = lo; // count(lo) >= K > count(hi)
     if (count(lo) >= K) {
         do {
             lo = hi;
@@ -89,8 +99,9 @@ __device__ __forceinline__ int wg_sum(int x, int *red, int tid) {
 // index. x - m is taken first, for all sizes of x: m log2(e), rounded, is off by more than an exponent of 1 from 2^24 on,
 // and has none at a mask of the type's lowest value.
 // The four waves take neighbouring pieces of it, a step of 4 KB at a time with the next on its way, each lane with a
-// maximum and sum of its own. A wave's threshold is a value that at least K of its lanes have reached (wave_kth), taken
-// anew as the number of steps doubles: some K logits pass it per doubling. They go to LDS; at the end those below the best
+// maximum and sum of its own. A wave's threshold is a value that at least K of its lanes have reached (wave_kth; past K = 32, K of
+// its lanes' halves: the least of 64 lanes is no threshold), taken anew as the number of steps doubles: some K logits pass it
+// per doubling. They go to LDS; at the end those below the best
 // of the four thresholds fall away, and each of the rest counts how many are ahead of it. Where more pass than LDS has room
 // for (equal or ascending logits) the K-th element's value and index are searched for bit by bit, over the chunk in
 // memory. Each logit is read once: 512 rows of 128256 in bf16, 131 MB, 32 us (4.1 TB/s where a copy reaches 4.9; eight
@@ -153,6 +164,7 @@ template <typename T> __global__ __launch_bounds__(256, 4) void attn_beam_chunk_
             }
         }
     };
+    float m0 = kNegInf, m1 = kNegInf; // of every other vector of the lane's
     float m = kNegInf, sum = 0.f; // of this lane: sum of exp(x - m), 0 while there is no m
     uint32_t least = kOrderedNegInf + 1;
     int taken = 0; // of this wave
@@ -162,14 +174,16 @@ template <typename T> __global__ __launch_bounds__(256, 4) void attn_beam_chunk_
     for (int at = begin, n = 1; at < end; at += STEP, ++n) {
         if (at + STEP < end)
             load(at + STEP, next);
-        float top = kNegInf;
+        float half[2] = {kNegInf, kNegInf};
 #pragma unroll
         for (int j = 0; j < NV; ++j)
 #pragma unroll
             for (int i = 0; i < VEC; i += 2)
-                top = max3f(top, value(v[j], i), value(v[j], i + 1));
-        const float was = m;
+                half[j & 1] = max3f(half[j & 1], value(v[j], i), value(v[j], i + 1));
+        const float top = fmaxf(half[0], half[1]), was = m;
+        m0 = fmaxf(m0, half[0]);
         m = fmaxf(m, top);
+        m1 = fmaxf(m1, half[1]);
         const float ref = m == kNegInf ? 0.f : m;
         sum *= fast_exp2((was - ref) * kLog2E);
 #pragma unroll
@@ -178,7 +192,8 @@ template <typename T> __global__ __launch_bounds__(256, 4) void attn_beam_chunk_
             for (int i = 0; i < VEC; ++i)
                 sum += fast_exp2((value(v[j], i) - ref) * kLog2E);
         if ((n & (n - 1)) == 0)
-            least = max(least, wave_kth(ordered(m), kOrderedNegInf, 1u << 20, a.K));
+            least = max(least, a.K <= 32 ? wave_kth<1>({ordered(m)}, kOrderedNegInf, 1u << 20, a.K)
+                                         : wave_kth<2>({ordered(m0), ordered(m1)}, kOrderedNegInf, 1u << 20, a.K));
         const float pass = unordered(least);
         if (__builtin_amdgcn_ballot_w64(top >= pass) != 0)
 #pragma unroll
@@ -282,9 +297,11 @@ template <typename T> __global__ __launch_bounds__(256, 4) void attn_beam_chunk_
 
 // ------------------------------------------------------------------------------------------
 // A batch entry's K best from its beams' chunks, by (x - lse) + score in fp64, of equals those of the lowest beam, then
-// the largest logit, then the lowest index: the threads' own maxima give a threshold that at least K candidates reach, and what reaches it counts how many are
-// ahead. Bound by latency: one round of loads, two sums over a beam's chunks, a search and a count, 6.8 us for 1 to 64
-// entries of 4 to 8 beams.
+// the largest logit, then the lowest index. The chunks' lists of K are cut into segments; a thread holds the first logits of up to
+// eight, and its largest gives, with the others', a threshold that at least K candidates reach. Segments whose first passes it
+// are followed, and what passes counts how many are ahead. Bound by latency: one round of loads, two sums over a beam's chunks,
+// a search and a count, 6 us for 1 to 64 entries of 4 to 8 beams; 13 beams over 238968 tokens, 5070 candidates, 10, and 24 where
+// every candidate was looked at; 4 entries of 64 beams with K = 64 over 32000, 16384 candidates each, 3580 -> 158 with its chunks.
 // ------------------------------------------------------------------------------------------
 constexpr int kBeamFinalRoom = 1024;
 constexpr double kLn2D = 0.693147180559945309417;
@@ -310,20 +327,25 @@ __global__ __launch_bounds__(256) void attn_beam_select_kernel(const attn_beam_a
     __shared__ double lse[ATTN_BEAMS_MAX], base[ATTN_BEAMS_MAX]; // of a done beam: 0; of one without a continuation: infinite
     __shared__ uint8_t over[ATTN_BEAMS_MAX];
     __shared__ uint64_t rv[kBeamFinalRoom], ri[kBeamFinalRoom];
-    __shared__ uint32_t redu[4];
-    __shared__ int redi[4], taken;
-    const int b = wg_id_x(), tid = wi_id_x(), lane = tid & 63, w = uniform(tid >> 6);
+    __shared__ uint32_t tops[256];
+    __shared__ int from[kBeamFinalRoom], redi[4], taken; // from: the segments whose first logits are kept
+    const int b = wg_id_x(), tid = wi_id_x(), lane = tid & 63;
     const int row0 = b * a.beams;
     if (tid == 0)
         taken = 0;
-    // The first candidates are asked for at once; those of a beam without a continuation are anything.
-    constexpr int HOLD = 4;
-    const int per = a.chunks * a.K, all = a.beams * per; // candidates of a beam and of the entry
-    const uint64_t *keys = a.keys + (int64_t)row0 * per;
+    // The segments' first logits are asked for at once; those of a beam without a continuation are anything. Of segment
+    // s, list s mod `lists` and the s / lists-th of its segments.
+    constexpr int HOLD = ATTN_BEAM_HELD / 256;
+    const int lists = a.beams * a.chunks, segments = a.segments;
+    const uint64_t *keys = a.keys + (int64_t)row0 * a.chunks * a.K;
+    auto place = [&](int s) { // of a segment's first logit among the entry's
+        const int sub = attn_div_by(s, a.by_lists);
+        return (s - sub * lists) * a.K + sub * a.seg;
+    };
     uint64_t held[HOLD];
 #pragma unroll
     for (int r = 0; r < HOLD; ++r)
-        held[r] = keys[min(tid + 256 * r, all - 1)];
+        held[r] = keys[place(min(tid + 256 * r, segments - 1))];
     // Eight lanes to a beam, whose chunks they take in turn.
     for (int i = tid >> 3; i < a.beams; i += 32) {
         const int row = row0 + i;
@@ -362,61 +384,89 @@ __global__ __launch_bounds__(256) void attn_beam_select_kernel(const attn_beam_a
     // ones: of the lowest beam, then the largest logit, then the lowest token.
     constexpr uint64_t LOW = ATTN_BEAM_V_MAX - 1;
     static_assert((LOW & (LOW + 1)) == 0 && LOW < 1u << 20 && ATTN_BEAMS_MAX <= 1 << 8, "60 bits");
-    auto candidate = [&](int i, uint64_t key, uint64_t &tie) -> uint64_t {
-        const int beam = i / per;
+    auto beam_of = [&](int i) { return attn_div_by(attn_div_by(i, a.by_K), a.by_chunks); };
+    auto score_of = [&](int i, uint64_t key) -> uint64_t {
+        const int beam = beam_of(i);
         const double l = lse[beam];
         if (ordered(l) >= ordered(__builtin_inf()))
             return 0;
-        tie = (uint64_t)(ATTN_BEAMS_MAX - 1 - beam) << 52;
-        if (over[beam]) {
-            tie |= LOW - a.done_token;
-            return i == beam * per ? ordered(base[beam]) : 0;
-        }
-        if (key == 0)
-            return 0;
-        tie |= key >> 32 << 20 | (LOW - ~(uint32_t)key);
-        return ordered(((double)unordered((uint32_t)(key >> 32)) - l) + base[beam]);
+        if (over[beam])
+            return i == beam * a.chunks * a.K ? ordered(base[beam]) : 0;
+        return key == 0 ? 0 : ordered(((double)unordered((uint32_t)(key >> 32)) - l) + base[beam]);
     };
-    auto each = [&](auto &&f) __attribute__((always_inline)) {
-        uint64_t tie = 0;
+    auto tie_of = [&](int i, uint64_t key) -> uint64_t {
+        const int beam = beam_of(i);
+        const uint64_t own = over[beam] ? LOW - a.done_token : key >> 32 << 20 | (LOW - ~(uint32_t)key);
+        return (uint64_t)(ATTN_BEAMS_MAX - 1 - beam) << 52 | own;
+    };
+    // A threshold of its upper halves, which K threads' largest reach.
+    uint64_t u[HOLD], top = 0;
 #pragma unroll
-        for (int r = 0; r < HOLD; ++r)
-            if (tid + 256 * r < all) {
-                const uint64_t u = candidate(tid + 256 * r, held[r], tie);
-                f(u, tie);
-            }
-        for (int i = tid + 256 * HOLD; i < all; i += 256) {
-            const uint64_t u = candidate(i, keys[i], tie);
-            f(u, tie);
+    for (int r = 0; r < HOLD; ++r) {
+        u[r] = 0;
+        if (256 * r < segments) { // for all threads, or for none
+            u[r] = tid + 256 * r < segments ? score_of(place(tid + 256 * r), held[r]) : 0;
+            top = max(top, u[r]);
         }
-    };
-    uint64_t top = 0;
-    each([&](uint64_t u, uint64_t) { top = max(top, u); });
-    // A threshold of its upper halves, which K threads' upper halves reach.
-    const uint32_t kth = wave_kth((uint32_t)(top >> 32), 0, 1u << 16, a.K);
-    if (lane == 0)
-        redu[w] = kth;
+    }
+    tops[tid] = (uint32_t)(top >> 32);
     __syncthreads();
-    const uint64_t least = max((uint64_t)max(max(redu[0], redu[1]), max(redu[2], redu[3])) << 32, (uint64_t)1);
-    auto collect = [&](auto &&f) {
-        each([&](uint64_t u, uint64_t tie) {
-            if (u >= least && f(u, tie)) {
-                const int at = atomicAdd(&taken, 1);
-                if (at < kBeamFinalRoom) {
-                    rv[at] = u;
-                    ri[at] = tie;
+    const uint32_t kth = wave_kth<4>({tops[lane], tops[lane + 64], tops[lane + 128], tops[lane + 192]}, 0, 1u << 16, a.K);
+    const uint64_t least = max((uint64_t)kth << 32, (uint64_t)1);
+    auto keep = [&](uint64_t v, uint64_t tie) {
+        const int at = atomicAdd(&taken, 1);
+        if (at < kBeamFinalRoom) {
+            rv[at] = v;
+            ri[at] = tie;
+        }
+        return at;
+    };
+#pragma unroll
+    for (int r = 0; r < HOLD; ++r)
+        if (u[r] >= least) {
+            const int s = tid + 256 * r, at = keep(u[r], tie_of(place(s), held[r]));
+            if (at < kBeamFinalRoom)
+                from[at] = s;
+        }
+    if (a.seg > 1) {
+        // Segments whose first logit passes are followed until one does not, four logits at a time.
+        __syncthreads();
+        const int heads = min(taken, kBeamFinalRoom);
+        __syncthreads();
+        for (int h = tid; h < heads; h += 256) {
+            const int s = from[h], first = place(s);
+            const int end = first + min(a.seg, a.K - attn_div_by(s, a.by_lists) * a.seg);
+            bool on = true;
+            for (int i = first + 1; i < end && on; i += 4) {
+                uint64_t next[4];
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    next[q] = keys[min(i + q, end - 1)];
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const uint64_t v = i + q < end && on ? score_of(i + q, next[q]) : 0;
+                    on = v >= least;
+                    if (on)
+                        keep(v, tie_of(i + q, next[q]));
                 }
             }
-        });
-        __syncthreads();
-    };
-    collect([](uint64_t, uint64_t) { return true; });
+        }
+    }
+    __syncthreads();
     int n = taken;
     __syncthreads();
     if (n > kBeamFinalRoom) {
+        // More than there is room for, by far most equal to the K-th: it is searched for bit by bit over all.
+        auto each = [&](auto &&f) __attribute__((always_inline)) {
+            for (int i = tid; i < lists * a.K; i += 256) {
+                const uint64_t key = keys[i], v = score_of(i, key);
+                if (v >= least)
+                    f(v, tie_of(i, key));
+            }
+        };
         auto count = [&](auto &&f) {
             int c = 0;
-            each([&](uint64_t u, uint64_t tie) { c += u >= least && f(u, tie) ? 1 : 0; });
+            each([&](uint64_t v, uint64_t tie) { c += f(v, tie) ? 1 : 0; });
             return wg_sum(c, redi, tid);
         };
         uint64_t v = 0, last = 0;
@@ -430,7 +480,11 @@ __global__ __launch_bounds__(256) void attn_beam_select_kernel(const attn_beam_a
         if (tid == 0)
             taken = 0;
         __syncthreads();
-        collect([&](uint64_t u, uint64_t i) { return u > v || (u == v && i >= last); });
+        each([&](uint64_t x, uint64_t tie) {
+            if (x > v || (x == v && tie >= last))
+                keep(x, tie);
+        });
+        __syncthreads();
         n = min(taken, kBeamFinalRoom);
     }
     auto put = [&](int r, float score, int token, int parent) {
@@ -527,7 +581,7 @@ extern "C" int attn_hip_launch_beam(const struct attn_beam_args *ap, int bits, v
     const hipStream_t st = (hipStream_t)stream;
     const int64_t grid = (int64_t)a.B * a.beams * a.chunks;
     if (grid <= 0 || grid > 0x7fffffff || a.beams > ATTN_BEAMS_MAX || a.K > ATTN_BEAM_K_MAX ||
-        (int64_t)a.chunks * a.steps * 4 * ATTN_BEAM_STEP(bits / 8) < a.V)
+        (int64_t)a.chunks * a.steps * 4 * ATTN_BEAM_STEP(bits / 8) < a.V || a.segments > ATTN_BEAM_HELD)
         return (int)hipErrorInvalidValue;
     const dim3 g((unsigned)grid), block(256);
     if (bits == 16)

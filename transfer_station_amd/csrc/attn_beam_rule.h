@@ -4,6 +4,7 @@
 
 #include <stdint.h>
 
+#include "attn_div.h"
 #include "attn_paged_rule.h"
 
 /* Logits of `size` bytes that a wave takes at a time: 4 KB. */
@@ -14,22 +15,25 @@
  * GPU with longer ones; else four workgroups per CU: 512 rows of 128256 in bf16 38.9 us, with six 42.0, with eight 43.9 (a
  * longer piece of a row has fewer logits that pass its threshold). */
 #define ATTN_BEAM_FILL 1024 /* workgroups */
-/* The second launch looks through an entry's candidates with one workgroup, so that chunks are no more than leave it so many:
- * 13 beams over 238968 tokens 31.2 -> 22.5 us, 2 x 16 over 116230 33.0 -> 25.5; with half as many 22.0 and 24.0, but 16 x 12 over
- * 151936, K = 24, 38 -> 43. */
-#define ATTN_BEAM_CANDIDATES 2048
 struct attn_beam_cut {
     int chunks, steps;
 };
-ATTN_HD struct attn_beam_cut attn_beam_cut_of(int64_t rows, int V, int size, int beams, int K) {
+ATTN_HD struct attn_beam_cut attn_beam_cut_of(int64_t rows, int V, int size) {
     const int64_t most = (V + 4 * ATTN_BEAM_STEP(size) - 1) / (4 * ATTN_BEAM_STEP(size)); /* chunks of one step */
     int64_t chunks = (ATTN_BEAM_FILL + rows - 1) / rows;
-    const int64_t few = ATTN_BEAM_CANDIDATES / (beams * K);
-    chunks = chunks < few ? chunks : few < 1 ? 1 : few;
     chunks = chunks < most ? chunks : most;
     const int64_t steps = (most + chunks - 1) / chunks;
     struct attn_beam_cut c = {(int)((most + steps - 1) / steps), (int)steps};
     return c;
+}
+
+/* The second launch takes the chunks' lists of K in segments, of whose first logits a thread holds up to eight. */
+#define ATTN_BEAM_HELD 2048
+ATTN_HD int attn_beam_segment(int lists, int K) {
+    int seg = 1;
+    while (seg < K && (int64_t)lists * ((K + seg - 1) / seg) > ATTN_BEAM_HELD)
+        ++seg;
+    return seg;
 }
 
 struct attn_beam_args {
@@ -39,6 +43,8 @@ struct attn_beam_args {
     const uint8_t *done;
     int done_token;
     int B, beams, V, K, chunks, steps;
+    int seg, segments; /* logits of a segment, segments of an entry */
+    struct attn_div by_lists, by_chunks, by_K; /* beams * chunks, chunks, K */
     uint64_t *keys; /* [rows][chunks][K], largest first */
     float *ms;      /* [rows][chunks][2]: m, the largest logit, and the sum of exp(x - m) */
     float *score;   /* [B][K] */

@@ -4,6 +4,7 @@
 #ifndef ATTN_CROSS_RULE_H
 #define ATTN_CROSS_RULE_H
 
+#include "attn_div.h"
 #include "attn_paged_rule.h"
 
 /* A sequence's rows of a token tensor of T rows: at .. at + n - 1. Starts and lengths come from device memory:
@@ -65,21 +66,6 @@ ATTN_HD struct attn_cut attn_cut_of(int total, int share, int nsplit, int step) 
 #define ATTN_CROSS_RANKED 64
 #define ATTN_CROSS_AT_ONCE 512
 #define ATTN_CROSS_LONG 512
-
-/* n / d for 0 <= n < 2^31 by a product: mul = ceil(2^(31 + l) / d), l = ceil(log2 d), which is below 2^32 and off by
- * less than 2^l, so that the quotient is off by less than n 2^l / (d 2^(31 + l)) < 1 / d. The kernels' divisions by what a
- * call fixes are of this kind: of the compiler's, five take a microsecond before the first load. */
-struct attn_div {
-    uint32_t mul, shift;
-};
-ATTN_HD struct attn_div attn_div_of(int d) {
-    struct attn_div x = {0, 31};
-    while ((int64_t)1 << (x.shift - 31) < d)
-        ++x.shift;
-    x.mul = (uint32_t)((((uint64_t)1 << x.shift) + (uint64_t)d - 1) / (uint64_t)d);
-    return x;
-}
-ATTN_HD int attn_div_by(int n, struct attn_div x) { return (int)(((uint64_t)(uint32_t)n * x.mul) >> x.shift); }
 
 /* What one launch looks like: row (or state) tiles of a sequence and kv head, its parts, and their share of units. */
 struct attn_cross_cut {
