@@ -888,7 +888,7 @@ __global__ __launch_bounds__(256, FINE ? 1 : DP == 64 ? 4 : DP == 96 ? 3 : DP ==
 // Both tiles are read both ways. Two teams of four waves (TEAMS = 2) have the same states and take steps of 32 rows in turn;
 // their sums are joined in LDS at the end.
 // Eight products of that size: 997 us at 4096 x 4096 (1103 TFLOP/s, matrix units 53%; half of a wave's time goes in waits, for
-// operands and at the barrier of each step, with all 256 registers in use), D = 64 615, 16 heads of 80 410. At D = 256 dK and
+// operands and at the barrier of each step, with all 256 registers in use), D = 64 594, 16 heads of 80 410. At D = 256 dK and
 // dV are two launches (232 and 184 us for 2 x 2048 of 16 heads on 8): with both, accumulators go to memory, 578 us.
 // ------------------------------------------------------------------------------------------
 template <int DP, bool DK, bool DV, int TEAMS, bool FINE>
