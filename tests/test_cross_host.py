@@ -235,6 +235,13 @@ def test_kernel_choice(case):
     assert all(a[1] == b[1] for a, b in zip(got, want))
 
 
+def test_scores_past_64_bits():
+    """8 sequences that may each have 2^30 rows and 2^30 states: 2^63 scores are not few."""
+    c = ts.CrossCall(ts.Spans(4096, 2 ** 30, 2 ** 30), ts.Spans(4096, 2 ** 30, 2 ** 30), 8, 1, 1, 64)
+    names = [p[0] for p in ts.attn_cross_plan(c, True) if "sum" not in p[0]]
+    assert names and all(n.endswith("false>") for n in names), names
+
+
 def test_bounds_past_the_tensor_are_cut():
     """max above T asks for no more workgroups than T rows need."""
     def plan(mq, mk):

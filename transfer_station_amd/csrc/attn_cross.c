@@ -144,7 +144,8 @@ static struct attn_cross_cut forward_cut(const struct attn_cross_call *c) {
 }
 
 static int is_fine(const struct attn_cross_call *c) {
-    return (int64_t)c->B * c->Hq * bound_of(&c->q) * bound_of(&c->k) <= ATTN_CROSS_FINE;
+    const int64_t rows = (int64_t)c->B * c->Hq * bound_of(&c->q); /* the product with the states may pass 64 bits */
+    return rows <= ATTN_CROSS_FINE && rows * bound_of(&c->k) <= ATTN_CROSS_FINE;
 }
 
 static struct attn_cross_cut dq_cut(const struct attn_cross_call *c) {
