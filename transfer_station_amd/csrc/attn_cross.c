@@ -87,6 +87,12 @@ static void cross_check_out(const char *who, const char *what, const struct attn
 
 static int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
+/* Tiles of a sequence and kv head that the launch has workgroups for; these go on to any that are left (tile += tps). */
+static int tiles_at_once(int64_t groups, int64_t tiles) {
+    const int64_t most = ATTN_CROSS_MAX_GRID / groups; /* 15 and more: groups <= 2^20 */
+    return (int)(tiles < most ? tiles : most);
+}
+
 /* Parts so that `base` workgroups become up to `target`, which run at once, each of `least` units or more of `total`. */
 static struct attn_cross_cut cross_cut(int64_t groups, int tps, int64_t total, int64_t least, int64_t target,
                                        int64_t most, int step) {
@@ -139,7 +145,8 @@ static struct attn_cross_cut forward_cut(const struct attn_cross_call *c) {
     const int64_t slots = ATTN_SLOTS / ((int64_t)c->q.T * c->Hq);
     if (R <= 32)
         return rows_cut(c, R, slots);
-    return cross_cut((int64_t)c->B * c->Hkv, (int)ceil_div(R, ATTN_CROSS_ROWS), bound_of(&c->k), 256, 512, slots,
+    const int64_t groups = (int64_t)c->B * c->Hkv;
+    return cross_cut(groups, tiles_at_once(groups, ceil_div(R, ATTN_CROSS_ROWS)), bound_of(&c->k), 256, 512, slots,
                      ATTN_CROSS_KEY_STEP);
 }
 
@@ -151,8 +158,8 @@ static int is_fine(const struct attn_cross_call *c) {
 static struct attn_cross_cut dq_cut(const struct attn_cross_call *c) {
     const int64_t R = (int64_t)bound_of(&c->q) * (c->Hq / c->Hkv), groups = (int64_t)c->B * c->Hkv;
     struct attn_cross_cut cut =
-        cross_cut(groups, (int)ceil_div(R, ATTN_CROSS_ROWS), bound_of(&c->k), 256, c->D <= 128 ? 512 : 256,
-                  ATTN_CROSS_GRAD_FLOATS / ((int64_t)c->q.T * c->Hq * c->D), ATTN_CROSS_KEY_STEP);
+        cross_cut(groups, tiles_at_once(groups, ceil_div(R, ATTN_CROSS_ROWS)), bound_of(&c->k), 256,
+                  c->D <= 128 ? 512 : 256, ATTN_CROSS_GRAD_FLOATS / ((int64_t)c->q.T * c->Hq * c->D), ATTN_CROSS_KEY_STEP);
     cut.fine = is_fine(c);
     return cut;
 }
@@ -166,7 +173,7 @@ static struct attn_cross_cut dkv_cut(const struct attn_cross_call *c) {
     const int64_t steps = ceil_div(bound_of(&c->q), ATTN_CROSS_STEP) * (c->Hq / c->Hkv);
     const int row_teams = c->D <= 128 && groups * tps <= 256 && groups * tps * steps >= 2048 ? 2 : 1;
     struct attn_cross_cut cut =
-        cross_cut(groups, (int)tps, steps, 2 * row_teams, row_teams > 1 || c->D > 128 ? 256 : 512,
+        cross_cut(groups, tiles_at_once(groups, tps), steps, 2 * row_teams, row_teams > 1 || c->D > 128 ? 256 : 512,
                   ATTN_CROSS_GRAD_FLOATS / ((int64_t)c->k.T * c->Hkv * c->D * 2), row_teams);
     cut.row_teams = row_teams;
     cut.fine = row_teams == 1 && is_fine(c);

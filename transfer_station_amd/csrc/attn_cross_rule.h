@@ -47,7 +47,7 @@ ATTN_HD struct attn_cut attn_cut_of(int total, int share, int nsplit, int step) 
 #define ATTN_CROSS_KEY_STEP 128 /* parts of the states are multiples of this */
 #define ATTN_CROSS_MAX_PARTS 64
 #define ATTN_CROSS_TEAMS 256 /* of the kernel for few rows: a workgroup per CU */
-#define ATTN_CROSS_MAX_GRID 0x7fffffffL
+#define ATTN_CROSS_MAX_GRID 0xffffffL /* workgroups of 256 threads: a launch has less than 2^32 work-items */
 /* Floats of partial gradients that a call of attn_cross_grad may take (128 MB). */
 #define ATTN_CROSS_GRAD_FLOATS (1L << 25)
 
