@@ -1,9 +1,16 @@
-"""A launch has less than 2^32 work-items: calls within the documented limits whose tiles are more than that."""
+"""A launch has less than 2^32 work-items: calls within the documented limits whose tiles, or groups, are more than that."""
+import os
+import subprocess
+
 import numpy as np
 import pytest
 
 import cross_util as cu
 import transfer_station_amd as ts
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+ROCM = os.environ.get("ROCM_PATH", "/opt/rocm")
+CSRC = os.path.join(ROOT, "transfer_station_amd", "csrc")
 
 # (B, Hq, Hkv, D, q.T, q.max, k.T, k.max): 2^33 work-items and more for a workgroup of 256 threads per tile
 WIDE = [
@@ -38,3 +45,52 @@ def test_tiles_that_no_workgroup_is_launched_for(rows, states):
     t = cu.Batch(seqs, 1, 1, 16, 31, pad=130000)
     got = cu.run(t, max_q=max(rows, 34), max_k=max(states, 70))
     cu.check(t, got, cu.reference(t))
+
+
+def test_reorder_launches_under_asan_ubsan(tmp_path):
+    exe = str(tmp_path / "reorder_checks")
+    cmd = ["gcc", "-O1", "-g", "-std=gnu11", "-Wall", "-Wextra", "-fsanitize=address,undefined",
+           "-fno-sanitize-recover=all", "-fno-omit-frame-pointer", "-D__HIP_PLATFORM_AMD__=1",
+           "-I" + os.path.join(ROOT, "include"), "-I" + CSRC, "-I" + os.path.join(ROCM, "include"),
+           os.path.join(ROOT, "tests", "sanitize", "reorder_checks.c"), os.path.join(CSRC, "attn_beam.c"), "-o", exe]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    assert r.returncode == 0, r.stdout + r.stderr
+    r = subprocess.run([exe], capture_output=True, text=True, timeout=300)
+    print(r.stdout[-3000:], r.stderr[-3000:])
+    assert r.returncode == 0 and "REORDER_CHECKS OK" in r.stdout
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tables", [0, 1])
+def test_reorder_of_groups_behind_the_first_launch(tables):
+    """2^20 sequences in pairs, 64 or 65 workgroups a pair; a few pairs hold tokens, at the edges of the launches."""
+    assert ts.device_count() >= 1
+    print("pairs", tables, flush=True)
+    B, D, page, n = 1 << 20, 256, 256, 300
+    per = (1 << 24) // 64
+    pairs = [0, 1, 0xffffff // 65 - 1, 0xffffff // 65, per - 1, per, B // 4, B // 2 - 1]
+    rng = np.random.default_rng(3)
+    pages = 4 * len(pairs)
+    data = {x: rng.integers(0, 256, (pages, page, 2 * D), np.uint8) for x in "kv"}
+    table, lens = np.full((B, 2), -1, np.int32), np.zeros(B, np.int32)
+    parent = np.arange(B, dtype=np.int32) ^ 1  # every pair changes places
+    for i, p in enumerate(pairs):
+        lens[2 * p:2 * p + 2] = n
+        table[2 * p:2 * p + 2] = 4 * i + np.arange(4).reshape(2, 2)
+    want_table, want = table.copy(), {x: a.copy() for x, a in data.items()}
+    for p in pairs:
+        a, b = table[2 * p], table[2 * p + 1]
+        if tables:
+            want_table[2 * p, 0], want_table[2 * p + 1, 0] = b[0], a[0]
+        for x in "kv":
+            want[x][a[1], :n - page], want[x][b[1], :n - page] = data[x][b[1], :n - page], data[x][a[1], :n - page]
+    bufs = {x: ts.DeviceBuffer.from_array(a) for x, a in data.items()}
+    with ts.DeviceBuffer.from_array(table) as dt, ts.DeviceBuffer.from_array(lens) as dl, \
+            ts.DeviceBuffer.from_array(parent) as dp:
+        c = ts.KvCache(bufs["k"], bufs["v"], dt, dl, dl, B, 2, pages, page, 1, D, 16)
+        ts.attn_kv_reorder(c, dp, 2, tables)
+        ts.synchronize()
+        assert np.array_equal(dt.download(np.int32).reshape(B, 2), want_table)
+    for x, buf in bufs.items():
+        assert np.array_equal(buf.download(np.uint8).reshape(want[x].shape), want[x]), x
+        buf.free()

@@ -110,7 +110,7 @@ void attn_kv_reorder(const struct attn_kv_cache *c, const int32_t *parent, int b
     a.k = c->k, a.v = c->v, a.ks = c->k_scale, a.vs = c->v_scale;
     a.table = (int32_t *)(uintptr_t)c->table; /* the one call that writes it */
     a.kv_len = c->kv_len, a.parent = parent;
-    a.groups = c->B / beams, a.beams = beams, a.cols = c->table_cols, a.pages = c->pages, a.Hkv = c->Hkv;
+    a.beams = beams, a.cols = c->table_cols, a.pages = c->pages, a.Hkv = c->Hkv;
     while (1 << a.lgp < c->page)
         ++a.lgp;
     a.row = c->bits == ATTN_KV_FP4 ? c->D / 2 : 2 * c->D;
@@ -118,7 +118,11 @@ void attn_kv_reorder(const struct attn_kv_cache *c, const int32_t *parent, int b
     a.data_wgs = (c->Hkv * ((a.row << a.lgp) / 16) + 255) / 256;
     a.scale_wgs = (c->Hkv * ((a.srow << a.lgp) / 16) + 255) / 256;
     a.table_wgs = !tables ? 0 : c->table_cols <= 4096 ? (c->table_cols + 255) / 256 : 16;
-    if ((int64_t)a.groups * (2 * ((int64_t)a.data_wgs + a.scale_wgs) + a.table_wgs) > 0x7fffffff)
-        beam_fail(who, "groups, heads and pages ask for too many workgroups");
-    beam_hip_check(attn_hip_launch_reorder(&a, attn_flash_get_stream()), who);
+    /* Groups past what one launch has workgroups for take further launches. A group has 2^19 workgroups and some at most:
+     * a page of all heads has at most 2^29 elements. */
+    const int groups = c->B / beams, most = ATTN_REORDER_GRID / attn_reorder_wgs(&a);
+    for (a.first = 0; a.first < groups; a.first += a.groups) {
+        a.groups = groups - a.first < most ? groups - a.first : most;
+        beam_hip_check(attn_hip_launch_reorder(&a, attn_flash_get_stream()), who);
+    }
 }

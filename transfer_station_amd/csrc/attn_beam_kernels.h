@@ -515,10 +515,9 @@ __global__ __launch_bounds__(256) void attn_beam_select_kernel(const attn_beam_a
 // beams of 777 tokens, 9.6 for 48 groups of five of 1000 in 4 bits, 8 heads of 128.
 // ------------------------------------------------------------------------------------------
 template <int NB> __global__ __launch_bounds__(256) void attn_kv_reorder_kernel(const attn_reorder_args a) {
-    const int per = 2 * (a.data_wgs + a.scale_wgs) + a.table_wgs;
-    const int g = uniform(wg_id_x() / per), tid = wi_id_x();
+    const int per = attn_reorder_wgs(&a), g = uniform(wg_id_x() / per), tid = wi_id_x();
     int wg = wg_id_x() - g * per;
-    const int first = g * a.beams;
+    const int first = (a.first + g) * a.beams;
     const int64_t most = (int64_t)a.cols << a.lgp;
     const int len = (int)min((int64_t)max(scalar_i32(a.kv_len, first), 0), most);
     const int full = len >> a.lgp, rest = len & ((1 << a.lgp) - 1);
@@ -597,8 +596,8 @@ extern "C" int attn_hip_launch_beam(const struct attn_beam_args *ap, int bits, v
 
 extern "C" int attn_hip_launch_reorder(const struct attn_reorder_args *ap, void *stream) {
     const attn_reorder_args &a = *ap;
-    const int64_t grid = (int64_t)a.groups * (2 * (a.data_wgs + a.scale_wgs) + a.table_wgs);
-    if (grid <= 0 || grid > 0x7fffffff || a.beams < 1 || a.beams > 32)
+    const int64_t grid = (int64_t)a.groups * attn_reorder_wgs(&a);
+    if (grid <= 0 || grid > ATTN_REORDER_GRID || a.beams < 1 || a.beams > ATTN_REORDER_MAX)
         return (int)hipErrorInvalidValue;
     const dim3 g((unsigned)grid), block(256);
     const hipStream_t st = (hipStream_t)stream;

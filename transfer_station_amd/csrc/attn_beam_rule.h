@@ -51,15 +51,23 @@ struct attn_beam_args {
     int32_t *token, *parent;
 };
 
+#define ATTN_REORDER_GRID 0xffffff /* workgroups of 256 threads: a launch has less than 2^32 work-items */
+
 struct attn_reorder_args {
     uint8_t *k, *v, *ks, *vs;
     int32_t *table;
     const int32_t *kv_len, *parent;
-    int groups, beams, cols, pages, lgp, Hkv;
+    int first, groups; /* of this launch */
+    int beams, cols, pages, lgp, Hkv;
     int row, srow;             /* bytes of a row's elements and scales, in one of K and V */
     int data_wgs, scale_wgs;   /* workgroups per group for each of K and V */
     int table_wgs;
 };
+
+/* Workgroups of a group. */
+ATTN_HD int attn_reorder_wgs(const struct attn_reorder_args *a) {
+    return 2 * (a->data_wgs + a->scale_wgs) + a->table_wgs;
+}
 
 /* The parent of a group's member i, as a member of the group: itself where the entry names no other one. */
 ATTN_HD int attn_parent_of(int entry, int first, int i, int beams) {
