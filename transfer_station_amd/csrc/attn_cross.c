@@ -167,16 +167,19 @@ static struct attn_cross_cut dq_cut(const struct attn_cross_call *c) {
 /* Where tiles of states are no more than the CUs and each has rows enough, eight waves share one, as two teams that take its
  * rows in turn: partial gradients cost 8 D bytes per state and part, written and read again. One team -> two: 4096 rows of
  * 40 heads over 77 states, D = 64, 31.5 -> 28.4 us with their sum; 1500 of 16 heads on 4 over 300, D = 128, 42 -> 39; 37
- * rows of 24 heads over 50 states, which keep one, 6.0 -> 8.0. */
+ * rows of 24 heads over 50 states, which keep one, 6.0 -> 8.0. Calls that take P and dS in two parts have one team, and the
+ * parts of two: both gradient kernels of 32 single rows of 64 heads on 8 over 128 states, D = 64, 22.6 us (with the parts of
+ * one team 38.2; 19.8 with two teams, and P and dS in one part), 4 x 2048 rows of 10 heads over 20 37.6 (36.4, 32.5). */
 static struct attn_cross_cut dkv_cut(const struct attn_cross_call *c) {
     const int64_t groups = (int64_t)c->B * c->Hkv, tps = ceil_div(bound_of(&c->k), ATTN_CROSS_KEYS);
     const int64_t steps = ceil_div(bound_of(&c->q), ATTN_CROSS_STEP) * (c->Hq / c->Hkv);
-    const int row_teams = c->D <= 128 && groups * tps <= 256 && groups * tps * steps >= 2048 ? 2 : 1;
+    const int fine = is_fine(c), shared = c->D <= 128 && groups * tps <= 256 && groups * tps * steps >= 2048;
+    const int row_teams = shared && !fine ? 2 : 1;
     struct attn_cross_cut cut =
-        cross_cut(groups, tiles_at_once(groups, tps), steps, 2 * row_teams, row_teams > 1 || c->D > 128 ? 256 : 512,
+        cross_cut(groups, tiles_at_once(groups, tps), steps, shared ? 4 : 2, shared || c->D > 128 ? 256 : 512,
                   ATTN_CROSS_GRAD_FLOATS / ((int64_t)c->k.T * c->Hkv * c->D * 2), row_teams);
     cut.row_teams = row_teams;
-    cut.fine = row_teams == 1 && is_fine(c);
+    cut.fine = fine;
     return cut;
 }
 
