@@ -274,8 +274,10 @@ struct attn_beams {
  * (b * beams + i) that it continues; [B][K] each. Ties go to the lowest beam, of its own to the largest logit, then the
  * lowest token. A done beam's only continuation is done_token, at its score; a logit of -inf is none, and a beam whose
  * score is not finite, or that has a NaN or +inf among its logits, has none. Where an entry has fewer than K, the rest is
- * score -inf, token -1 and the entry's first row. The sums of exponentials are taken in fp32, all else in fp64, and the
- * score is rounded once.
+ * score -inf, token -1 and the entry's first row. The sums of exponentials are taken in fp32, all else in fp64, as
+ * (x - m) - log sum exp(x - m) with the beam's largest logit m, so that logits of any size keep their differences, and the
+ * score is rounded once. A finite logit is a candidate however low: of a beam whose V logits are all the type's lowest
+ * value each scores -log V.
  * scratch: attn_beam_scratch_bytes(c) bytes, ATTN_SCRATCH_ALIGN-aligned; calls that may overlap need one each. */
 size_t attn_beam_scratch_bytes(const struct attn_beams *c);
 void attn_beam_select(const struct attn_beams *c, float *score, int32_t *token, int32_t *parent, void *scratch);

@@ -296,8 +296,9 @@ template <typename T> __global__ __launch_bounds__(256, 4) void attn_beam_chunk_
 }
 
 // ------------------------------------------------------------------------------------------
-// A batch entry's K best from its beams' chunks, by (x - lse) + score in fp64, of equals those of the lowest beam, then
-// the largest logit, then the lowest index. The chunks' lists of K are cut into segments; a thread holds the first logits of up to
+// A batch entry's K best from its beams' chunks, by ((x - m) - log sum exp(x - m)) + score in fp64, m the beam's largest
+// logit (m plus the logarithm would be m alone where m is large), of equals those of the lowest beam, then the largest logit,
+// then the lowest index. The chunks' lists of K are cut into segments; a thread holds the first logits of up to
 // eight, and its largest gives, with the others', a threshold that at least K candidates reach. Segments whose first passes it
 // are followed, and what passes counts how many are ahead. Bound by latency: one round of loads, two sums over a beam's chunks,
 // a search and a count, 6 us for 1 to 64 entries of 4 to 8 beams; 13 beams over 238968 tokens, 5070 candidates, 10, and 24 where
@@ -324,7 +325,8 @@ __device__ __forceinline__ double log_of(double x) {
 }
 
 __global__ __launch_bounds__(256) void attn_beam_select_kernel(const attn_beam_args a) {
-    __shared__ double lse[ATTN_BEAMS_MAX], base[ATTN_BEAMS_MAX]; // of a done beam: 0; of one without a continuation: infinite
+    __shared__ float largest[ATTN_BEAMS_MAX];
+    __shared__ double logs[ATTN_BEAMS_MAX], base[ATTN_BEAMS_MAX]; // of a done beam: 0; of one without a continuation: infinite
     __shared__ uint8_t over[ATTN_BEAMS_MAX];
     __shared__ uint64_t rv[kBeamFinalRoom], ri[kBeamFinalRoom];
     __shared__ uint32_t tops[256];
@@ -372,9 +374,10 @@ __global__ __launch_bounds__(256) void attn_beam_select_kernel(const attn_beam_a
         if (done && finite(s))
             l = 0.0;
         else if (finite(s) && finite(m) && finite((float)sum)) // a NaN, an infinity or no logit at all: nothing
-            l = (double)m + log_of(sum);
+            l = log_of(sum);
         if ((tid & 7) == 0) {
-            lse[i] = l;
+            largest[i] = m;
+            logs[i] = l;
             base[i] = (double)s;
             over[i] = done;
         }
@@ -387,12 +390,12 @@ __global__ __launch_bounds__(256) void attn_beam_select_kernel(const attn_beam_a
     auto beam_of = [&](int i) { return attn_div_by(attn_div_by(i, a.by_K), a.by_chunks); };
     auto score_of = [&](int i, uint64_t key) -> uint64_t {
         const int beam = beam_of(i);
-        const double l = lse[beam];
+        const double l = logs[beam];
         if (ordered(l) >= ordered(__builtin_inf()))
             return 0;
         if (over[beam])
             return i == beam * a.chunks * a.K ? ordered(base[beam]) : 0;
-        return key == 0 ? 0 : ordered(((double)unordered((uint32_t)(key >> 32)) - l) + base[beam]);
+        return key == 0 ? 0 : ordered((((double)unordered((uint32_t)(key >> 32)) - largest[beam]) - l) + base[beam]);
     };
     auto tie_of = [&](int i, uint64_t key) -> uint64_t {
         const int beam = beam_of(i);
