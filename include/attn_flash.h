@@ -198,9 +198,10 @@ int attn_paged_plan(const struct attn_kv_cache *c, int T, int Hq, int causal,
                     const struct attn_scores *scores, int max_q, int max_kv, char *buf, size_t len);
 
 /* ---- Cross attention -----------------------------------------------------------------------------
- * No counterpart in the reference. The attention of an encoder-decoder model, for training and serving: each
- * sequence's rows (a prompt, a target text, a single token, the beams of one input) attend to all of its encoder's
- * states, whose number is another. Batches are ragged: packed one sequence behind the other, or padded. Work is
+ * No counterpart in the reference. The attention of an encoder-decoder model's rows to its encoder's states, for training
+ * and serving: each sequence's rows (a prompt, a target text, a single token, the beams of one input) attend to all of its
+ * states, whose number is another. There is no causal mask, so the gradients are those of cross attention and of an encoder's
+ * own attention, not of a decoder's. Batches are ragged: packed one sequence behind the other, or padded. Work is
  * stream-ordered on the calling thread's stream, nothing is allocated and no device memory is read on the host, so
  * that every call may be captured into a graph and replayed with other lengths.
  */
@@ -226,8 +227,10 @@ struct attn_cross_call {
 /* O[t][h] = sum_j P_j V[j][kv], P = softmax_j(scale * Q[t][h].K[j][kv]) over the states j of row t's sequence,
  * kv = h / (Hq/Hkv), in bf16; lse[t * Hq + h] = log sum_j exp(scale * Q.K), natural, in fp32 (lse may be NULL). A row
  * whose sequence has no states gets zeros and -inf; rows of no sequence are left as they are. Sequences may share
- * states (their spans may overlap), not rows. P is rounded to bf16 before P.V, as in attn_flash; states that no
- * sequence names are not read, whatever they hold. o must not overlap q, k or v, nor its heads each other.
+ * states (their spans may overlap), not rows. With few rows (up to 32 per kv head) each reads them from memory for itself;
+ * as the rows of one sequence they read them once. P is rounded to bf16 before P.V, as in attn_flash; P.V is summed before the
+ * division by the row's sum: elements of V past 2^86 may overflow on the way. States that no sequence names are not read,
+ * whatever they hold. o must not overlap q, k or v, nor its heads each other.
  * scratch: attn_cross_scratch_bytes(c) bytes, ATTN_SCRATCH_ALIGN-aligned; calls that may overlap need one each. */
 size_t attn_cross_scratch_bytes(const struct attn_cross_call *c);
 void attn_cross(const struct attn_cross_call *c, const struct attn_rows *q, const struct attn_rows *k,
@@ -235,9 +238,10 @@ void attn_cross(const struct attn_cross_call *c, const struct attn_rows *q, cons
 
 /* The gradients of q, k and v, in bf16, from that of o (d_o) and what the forward call left in o and lse. dK and dV are
  * summed over the heads of a group. P and dS are rounded to bf16 before their products, in calls of up to 2^21 scores
- * (B Hq q.max k.max) in two parts, to 16 bits. States of a sequence without rows get zeros; rows and states of no sequence are left as they are. Here sequences may share neither rows nor
- * states: what two of them claim may hold neither's gradient. dq, dk and dv must overlap none of the other tensors.
- * Sums have a fixed order: the same call gives the same bits.
+ * (B Hq q.max k.max) in two parts, to 16 bits. States of a sequence without rows get zeros; rows and states of no sequence are
+ * left as they are. Here sequences may share neither rows nor states: what two of them claim may hold neither's gradient. A NaN
+ * or an infinity in a sequence's tensors may reach all of its gradients, from states of probability 0 too. dq, dk and dv must
+ * overlap none of the other tensors. Sums have a fixed order: the same call gives the same bits.
  * scratch: attn_cross_grad_scratch_bytes(c) bytes: 4 q.T Hq, and, where few sequences leave the GPU unfilled, up to 128
  * MB of partial gradients. */
 size_t attn_cross_grad_scratch_bytes(const struct attn_cross_call *c);
@@ -277,13 +281,17 @@ struct attn_beams {
  * score -inf, token -1 and the entry's first row. The sums of exponentials are taken in fp32, all else in fp64, as
  * (x - m) - log sum exp(x - m) with the beam's largest logit m, so that logits of any size keep their differences, and the
  * score is rounded once. A finite logit is a candidate however low: of a beam whose V logits are all the type's lowest
- * value each scores -log V.
+ * value each scores -log V. Two kinds of rows are slow, since what passes has to be searched for bit by bit: those most of
+ * whose logits are one finite value (masked with the lowest value, not with -inf), and large K over many tokens: of 1024 beams
+ * and more in all, K of 64 from some 65536 tokens on in bf16, 48 from 131072, 32 from 524288, in fp32 from half as many; of
+ * fewer beams rows are cut, and may be as much longer.
  * scratch: attn_beam_scratch_bytes(c) bytes, ATTN_SCRATCH_ALIGN-aligned; calls that may overlap need one each. */
 size_t attn_beam_scratch_bytes(const struct attn_beams *c);
 void attn_beam_select(const struct attn_beams *c, float *score, int32_t *token, int32_t *parent, void *scratch);
 
 /* The cache's sequences lie in groups of `beams` neighbours; sequence b continues parent[b] (device, [B], rows as
- * attn_beam_select gives them: members of b's group; any other entry means b itself). All members of a group hold as many
+ * attn_beam_select gives them: members of b's group; any other entry means b itself). beams is at most ATTN_REORDER_MAX:
+ * of a wider search, which attn_beam_select serves, the sequences are the caller's to move. All members of a group hold as many
  * tokens as its first one's kv_len says. Their full pages are shared: with tables, the entries of the parent's row of
  * the table for them replace b's, in place (the one call that writes the table). The tokens of the last, partly filled page
  * are copied into b's own page of that column, with what the 16 bytes at their end hold besides; members must not share

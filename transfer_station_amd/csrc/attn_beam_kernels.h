@@ -102,10 +102,15 @@ __device__ __forceinline__ int wg_sum(int x, int *red, int tid) {
 // maximum and sum of its own. A wave's threshold is a value that at least K of its lanes have reached (wave_kth; past K = 32, K of
 // its lanes' halves: the least of 64 lanes is no threshold), taken anew as the number of steps doubles: some K logits pass it
 // per doubling. They go to LDS; at the end those below the best
-// of the four thresholds fall away, and each of the rest counts how many are ahead of it. Where more pass than LDS has room
-// for (equal or ascending logits) the K-th element's value and index are searched for bit by bit, over the chunk in
-// memory. Each logit is read once: 512 rows of 128256 in bf16, 131 MB, 32 us (4.1 TB/s where a copy reaches 4.9; eight
-// instructions and an exponential, at a quarter of their rate, per logit and lane), four rows of 50257 in fp32 5.4.
+// of the four thresholds fall away, and each of the rest counts how many are ahead of it. Each logit is read once: 512 rows of
+// 128256 in bf16, 131 MB, 32 us (4.1 TB/s where a copy reaches 4.9; eight instructions and an exponential, at a quarter of
+// their rate, per logit and lane), four rows of 50257 in fp32 5.4.
+// Where more pass in one wave than LDS has room for, the K-th element's value and index are searched for bit by bit, up to 66
+// passes over the chunk in memory. That is so for equal and for ascending logits, for pieces of which nearly all have one finite
+// value (64 entries of 8 beams over 128256 in bf16, all but 100 of a row at the lowest value: 5.7 ms, at -inf 32 us), and for
+// large K over many steps, since what has passed stays to the end: of normal logits some K pass per doubling (16 entries of 64
+// beams over 128256 in bf16, 16 steps to a wave: K = 40 76 us, K = 64 11.9 ms; 4 of 64 in fp32, 8 steps: 44 us and 2.9 ms). K = 64
+// is there from 8 steps on, 48 from 16, 40 from 32, 32 from 64.
 // ------------------------------------------------------------------------------------------
 constexpr int kBeamRoom = 256, kBeamBest = 512; // places for a wave's logits, and for those that are ranked
 
