@@ -283,8 +283,8 @@ struct attn_beams {
  * score is rounded once. A finite logit is a candidate however low: of a beam whose V logits are all the type's lowest
  * value each scores -log V. Two kinds of rows are slow, since what passes has to be searched for bit by bit: those most of
  * whose logits are one finite value (masked with the lowest value, not with -inf), and large K over many tokens: of 1024 beams
- * and more in all, K of 64 from some 65536 tokens on in bf16, 48 from 131072, 32 from 524288, in fp32 from half as many; of
- * fewer beams rows are cut, and may be as much longer.
+ * and more in all, K of 64 from some 32000 tokens on in bf16, 48 from 65536, 32 from 128000, 24 from 262144, in fp32 from half as
+ * many; of fewer beams rows are cut, and may be as much longer.
  * scratch: attn_beam_scratch_bytes(c) bytes, ATTN_SCRATCH_ALIGN-aligned; calls that may overlap need one each. */
 size_t attn_beam_scratch_bytes(const struct attn_beams *c);
 void attn_beam_select(const struct attn_beams *c, float *score, int32_t *token, int32_t *parent, void *scratch);

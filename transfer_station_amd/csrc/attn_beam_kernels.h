@@ -109,8 +109,8 @@ __device__ __forceinline__ int wg_sum(int x, int *red, int tid) {
 // passes over the chunk in memory. That is so for equal and for ascending logits, for pieces of which nearly all have one finite
 // value (64 entries of 8 beams over 128256 in bf16, all but 100 of a row at the lowest value: 5.7 ms, at -inf 32 us), and for
 // large K over many steps, since what has passed stays to the end: of normal logits some K pass per doubling (16 entries of 64
-// beams over 128256 in bf16, 16 steps to a wave: K = 40 76 us, K = 64 11.9 ms; 4 of 64 in fp32, 8 steps: 44 us and 2.9 ms). K = 64
-// is there from 8 steps on, 48 from 16, 40 from 32, 32 from 64.
+// beams over 128256 in bf16, 16 steps to a wave: K = 24 67 us, K = 32 5.4 ms, K = 64 11.1; 4 of 64 in fp32, 8 steps: K = 40 44 us,
+// K = 48 1.1 ms, K = 64 2.9). Among 1024 rows some wave is there with K = 64 from 4 steps on, 48 from 8, 32 from 16, 24 from 32.
 // ------------------------------------------------------------------------------------------
 constexpr int kBeamRoom = 256, kBeamBest = 512; // places for a wave's logits, and for those that are ranked
 
